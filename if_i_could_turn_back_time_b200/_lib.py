@@ -13,6 +13,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 
 JQ_F32, JQ_F16, JQ_BF16 = 0, 1, 2
 JQ_FMT_E2M1, JQ_FMT_GF4 = 0, 1
+JQ_KV_INT8, JQ_KV_E4M3 = 0, 1
 
 
 class JqError(RuntimeError):
@@ -33,6 +34,16 @@ class jq_problem(ctypes.Structure):
 class jq_conv(ctypes.Structure):
     _fields_ = [(n, c_int32) for n in ("batch", "channels", "height", "width", "kernel_h", "kernel_w", "stride_h", "stride_w",
                                        "pad_h", "pad_w", "dilation_h", "dilation_w")] + [("stride_x", ctypes.c_int64 * 4)]
+
+
+class jq_kv_cache(ctypes.Structure):
+    _fields_ = [(n, c_void_p) for n in ("keys", "values", "key_scales", "value_scales")] + [
+        (n, c_int32) for n in ("blocks", "kv_heads", "head_dim", "block_size", "fmt", "reserved")]
+
+
+class jq_kv_batch(ctypes.Structure):
+    _fields_ = [(n, c_void_p) for n in ("table", "lengths", "starts")] + [
+        (n, c_int32) for n in ("sequences", "table_width", "table_stride", "tokens", "max_new", "reserved")]
 
 
 _SIGNATURES = {
@@ -71,6 +82,14 @@ _SIGNATURES = {
     "jq_pack_gf4_workspace_bytes": (c_size_t, [c_int]),
     "jq_pack_gf4_workspace_bytes_rows": (c_size_t, [c_int, c_int]),
     "jq_pack_gf4": (c_int, [c_void_p, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_size_t, c_void_p]),
+    "jq_kv_append": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p]),
+    "jq_kv_read": (c_int, [c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_int, c_void_p]),
+    "jq_kv_attend_workspace_bytes": (c_size_t, [c_void_p, c_void_p, c_int]),
+    "jq_kv_attend": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int, ctypes.c_float, c_int, c_void_p, c_void_p, c_int,
+                             c_void_p, c_size_t, c_void_p]),
+    "jq_token_logprobs_workspace_bytes": (c_size_t, [c_int, c_int]),
+    "jq_token_logprobs": (c_int, [c_void_p, ctypes.c_int64, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p, c_int, c_void_p,
+                                  c_void_p, c_void_p, c_size_t, c_void_p]),
     "jq_pack_e2m1_host": (c_int, [c_void_p, c_int, c_int, c_int, c_void_p, c_void_p, c_int]),
     "jq_pack_gf4_host": (c_int, [c_void_p, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p, c_int]),
     "jq_rotate_weights_host": (c_int, [c_void_p, c_int, c_int, c_int, c_int]),

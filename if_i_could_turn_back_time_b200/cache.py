@@ -1,0 +1,189 @@
+"""Key/value cache of 8 bits and attention over it: what a decode step needs between its packed projections.
+
+The reference has no attention (its models are the vision networks and the MLP of
+Python_Jenks_Test/Jenks_Tests/QuantNetworkTest.py); the cache completes a decode step whose matrices are
+``JenksQuantLinear`` layers.  Like the other operators, everything runs on the GPU through the C ABI
+(``jq_kv_append``, ``jq_kv_read``, ``jq_kv_attend`` of include/jq.h, which has the formulas and the order of the codes).
+"""
+from __future__ import annotations
+
+import ctypes
+import math
+from typing import Optional, Tuple
+
+import torch
+
+from . import _lib, ops
+
+_FORMATS = {"int8": _lib.JQ_KV_INT8, "e4m3": _lib.JQ_KV_E4M3}
+BLOCK_SIZES = (16, 32, 64, 128)
+HEAD_DIMS = (64, 128)          # of attend(); append() and read() take every multiple of 32 up to 256
+_Strides = ctypes.c_int64 * 2
+
+
+class KVCache:
+    """A pool of blocks of ``block_size`` tokens for one layer: ``keys`` and ``values`` uint8 [blocks, kv_heads, block_size,
+    head_dim] (codes in the kernels' order: the last two dims only say how many there are), ``key_scales`` and
+    ``value_scales`` fp32 [blocks, kv_heads].  ``KVCache.empty`` makes one; the constructor takes tensors that are there.
+
+    Who owns which block is the caller's: every call takes ``table`` (int32 [sequences, width], the blocks of each
+    sequence in order), ``lengths`` (int32 [sequences], tokens that a sequence holds, the new ones among them) and, where
+    sequences have different numbers of new tokens, ``starts`` (int32 [sequences + 1]: the new tokens of sequence i are
+    the rows starts[i] .. starts[i + 1] - 1; they sit at its end) with ``max_new``, which no sequence's number exceeds.
+    All three stay on the device; a step can be captured in a CUDA graph and replayed with other contents."""
+
+    def __init__(self, keys: torch.Tensor, values: torch.Tensor, key_scales: torch.Tensor, value_scales: torch.Tensor,
+                 fmt: str = "int8"):
+        if fmt not in _FORMATS:
+            raise ValueError(f"unknown cache format {fmt!r}")
+        if keys.dim() != 4 or keys.shape != values.shape or keys.dtype != torch.uint8 or values.dtype != torch.uint8:
+            raise ValueError("keys and values are uint8 tensors of one shape [blocks, kv_heads, block_size, head_dim]")
+        if key_scales.shape != keys.shape[:2] or value_scales.shape != keys.shape[:2] or \
+                key_scales.dtype != torch.float32 or value_scales.dtype != torch.float32:
+            raise ValueError("the scales are fp32 tensors [blocks, kv_heads]")
+        tensors = (keys, values, key_scales, value_scales)
+        if not all(t.is_contiguous() for t in tensors):
+            raise ValueError("the cache's tensors are contiguous")
+        if any(t.device != keys.device for t in tensors):
+            raise ValueError("the cache's tensors are on one device")
+        self.keys, self.values, self.key_scales, self.value_scales, self.fmt = keys, values, key_scales, value_scales, fmt
+        self.blocks, self.kv_heads, self.block_size, self.head_dim = keys.shape
+        if self.blocks == 0 or self.kv_heads == 0:
+            raise ValueError("a cache has at least one block and one head")
+        if self.block_size not in BLOCK_SIZES:
+            raise ValueError(f"block_size must be one of {BLOCK_SIZES}")
+        if self.head_dim % 32 or not 32 <= self.head_dim <= 256:
+            raise ValueError("head_dim must be a multiple of 32 up to 256")
+        self.device = keys.device
+        self._c = _lib.jq_kv_cache(keys.data_ptr(), values.data_ptr(), key_scales.data_ptr(), value_scales.data_ptr(),
+                                   self.blocks, self.kv_heads, self.head_dim, self.block_size, _FORMATS[fmt], 0)
+        self._c_ref = ctypes.byref(self._c)
+
+    @classmethod
+    def empty(cls, blocks: int, kv_heads: int, head_dim: int, *, block_size: int = 64, fmt: str = "int8",
+              device="cuda") -> "KVCache":
+        codes = lambda: torch.full((blocks, kv_heads, block_size, head_dim), 128 if fmt == "int8" else 0,     # noqa: E731
+                                   dtype=torch.uint8, device=device)
+        scales = lambda: torch.ones((blocks, kv_heads), dtype=torch.float32, device=device)                   # noqa: E731
+        return cls(codes(), codes(), scales(), scales(), fmt)
+
+    def nbytes(self) -> int:
+        return sum(t.numel() * t.element_size() for t in (self.keys, self.values, self.key_scales, self.value_scales))
+
+    def _batch(self, table, lengths, starts, tokens, max_new):
+        n = lengths.shape[0]
+        if table.dim() != 2 or lengths.dim() != 1 or table.shape[0] != n:
+            raise RuntimeError(f"table {tuple(table.shape)} and lengths {tuple(lengths.shape)}: [sequences, width] and [sequences]")
+        if table.dtype != torch.int32 or lengths.dtype != torch.int32 or (starts is not None and starts.dtype != torch.int32):
+            raise RuntimeError("table, lengths and starts are int32 tensors")
+        if table.shape[1] == 0:
+            raise RuntimeError("the table has no columns")
+        if table.stride(1) != 1 and table.shape[1] != 1 or not lengths.is_contiguous():
+            raise RuntimeError("the table's rows and the lengths are contiguous")
+        device = self.device
+        if table.device != device or lengths.device != device:
+            raise RuntimeError(f"the cache is on {device}: table, lengths and starts are too")
+        stride = table.stride(0) if n > 1 else table.shape[1]
+        if stride < table.shape[1]:
+            raise RuntimeError("the table's rows lie behind one another")
+        if starts is None:
+            if n and tokens % n:
+                raise RuntimeError(f"{tokens} new tokens of {n} sequences: starts says how many each has")
+            at = None
+        else:
+            if starts.shape != (n + 1,) or not starts.is_contiguous() or starts.device != device:
+                raise RuntimeError(f"starts is a contiguous tensor [{n + 1}] on {device}")
+            at = starts.data_ptr()
+        if max_new is not None and max_new < 0:
+            raise RuntimeError("max_new is a number of tokens")
+        if not self.keys.is_cuda:
+            raise RuntimeError("libjq operators run on CUDA tensors only (there is no CPU path)")
+        return _lib.jq_kv_batch(table.data_ptr(), lengths.data_ptr(), at, n, table.shape[1], stride, tokens,
+                                tokens if max_new is None else max_new, 0)
+
+    def _rows(self, x, heads, what):
+        """[..., heads, head_dim] as rows of one stride: (tensor, strides of a row and of a head)."""
+        if x.dim() < 3 or x.shape[-1] != self.head_dim or (x.shape[-2] != heads if heads else x.shape[-2] % self.kv_heads):
+            raise RuntimeError(f"{what} is {tuple(x.shape)}: [tokens, {heads or 'q_heads'}, {self.head_dim}] "
+                               f"with the cache's {self.kv_heads} key heads")
+        if x.dtype not in ops._DT:
+            raise RuntimeError(f"unsupported dtype {x.dtype}")
+        if x.device != self.device:
+            raise RuntimeError(f"{what} is on {x.device}, the cache on {self.device}")
+        if x.is_neg():
+            x = x.resolve_neg()
+        if x.dim() > 3:
+            x = x.reshape(-1, x.shape[-2], x.shape[-1])
+        if x.stride(2) != 1:
+            x = x.contiguous()
+        return x, _Strides(x.stride(0), x.stride(1))
+
+    def append(self, k: torch.Tensor, v: torch.Tensor, table: torch.Tensor, lengths: torch.Tensor,
+               starts: Optional[torch.Tensor] = None, max_new: Optional[int] = None) -> None:
+        """Quantises the new tokens' ``k`` and ``v`` ([tokens, kv_heads, head_dim], or any leading dims; fp32, fp16 or bf16) into
+        the places that ``table`` and ``lengths`` give them.  A block's scale grows with its largest value, and codes that
+        are there already are rounded to the new one: the result depends on what is appended in one call.  Infinities
+        become the largest code, NaN 0.  A block is appended to by one sequence of a call; shared blocks are full."""
+        k, sk = self._rows(k, self.kv_heads, "k")
+        v, sv = self._rows(v, self.kv_heads, "v")
+        if k.shape != v.shape or k.dtype != v.dtype:
+            raise RuntimeError("k and v have one shape and dtype")
+        batch = self._batch(table, lengths, starts, k.shape[0], max_new)
+        with ops._on(self.device):
+            st = _lib.load().jq_kv_append(self._c_ref, ctypes.byref(batch), k.data_ptr(), v.data_ptr(), sk, sv, ops._DT[k.dtype],
+                                          ops._stream())
+        if st:
+            _lib.check(st, "jq_kv_append")
+
+    def read(self, table: torch.Tensor, lengths: torch.Tensor, last: int,
+             dtype: torch.dtype = torch.float32) -> Tuple[torch.Tensor, torch.Tensor]:
+        """What the codes of every sequence's last ``last`` tokens stand for: keys and values [sequences, last, kv_heads,
+        head_dim], 0 before a sequence's first token."""
+        if dtype not in ops._DT:
+            raise RuntimeError(f"unsupported dtype {dtype}")
+        if last < 0:
+            raise RuntimeError("last is a number of tokens")
+        batch = self._batch(table, lengths, None, 0, None)
+        shape = (lengths.shape[0], last, self.kv_heads, self.head_dim)
+        k, v = torch.empty(shape, dtype=dtype, device=self.device), torch.empty(shape, dtype=dtype, device=self.device)
+        with ops._on(self.device):
+            st = _lib.load().jq_kv_read(self._c_ref, ctypes.byref(batch), last, k.data_ptr(), v.data_ptr(), ops._DT[dtype], ops._stream())
+        if st:
+            _lib.check(st, "jq_kv_read")
+        return k, v
+
+    def attend(self, q: torch.Tensor, table: torch.Tensor, lengths: torch.Tensor, starts: Optional[torch.Tensor] = None,
+               max_new: Optional[int] = None, *, scale: Optional[float] = None, window: int = 0, lse: bool = False):
+        """Causal attention of the new tokens' queries ``q`` ([tokens, q_heads, head_dim], or any leading dims; fp16 or bf16)
+        over the cache, their own keys and values among it (append first).  ``scale`` is 1 / sqrt(head_dim) unless given;
+        with a ``window`` a query sees the last ``window`` tokens up to its own.  A query that sees nothing gets zeros.
+        Returns the outputs in q's shape and dtype, with ``lse`` also fp32 ln(sum(exp(scores))) [tokens, q_heads]."""
+        shape, dtype = q.shape, q.dtype
+        if dtype is not torch.float16 and dtype is not torch.bfloat16:
+            raise RuntimeError(f"unsupported query dtype {dtype}: fp16 or bf16")
+        if self.head_dim not in HEAD_DIMS:
+            raise RuntimeError(f"attend() takes heads of {HEAD_DIMS}, the cache has {self.head_dim}")
+        q, sq = self._rows(q, 0, "q")
+        if scale is None:
+            scale = 1.0 / math.sqrt(self.head_dim)
+        if not 0.0 < scale < 3e38:
+            raise RuntimeError("scale must be above 0")
+        if window < 0:
+            raise RuntimeError("window is a number of tokens, 0 for all")
+        tokens, heads = q.shape[0], q.shape[1]
+        batch = self._batch(table, lengths, starts, tokens, max_new)
+        lib = _lib.load()
+        out = torch.empty((tokens, heads, self.head_dim), dtype=dtype, device=self.device)
+        sums = torch.empty((tokens, heads), dtype=torch.float32, device=self.device) if lse else None
+        with ops._on(self.device):
+            ref = ctypes.byref(batch)
+            own, at, size = ops._parts_workspace(self.device, lib.jq_kv_attend_workspace_bytes(self._c_ref, ref, heads))
+            st = lib.jq_kv_attend(self._c_ref, ref, q.data_ptr(), sq, heads, scale, min(window, 0x7fffffff), out.data_ptr(),
+                                  ops._addr(sums), ops._DT[dtype], at, size, ops._stream())
+            del own
+        if st:
+            _lib.check(st, "jq_kv_attend")
+        if ops._checked:
+            ops.check_status()
+        out = out.view(shape)
+        return (out, sums.view(shape[:-1])) if lse else out

@@ -40,6 +40,11 @@ static inline cudaError_t jq_allow_smem(const void *kernel, int bytes, jq_contex
     return s;
 }
 
+// Workspace of the kernels whose last CTA adds up what the others left (attention over the cache, log probabilities): a status
+// word, at kJqHeader counters that are zero before the first use and that every call leaves at zero, at kJqData partial sums.
+// The places are the same for every call, so that calls of any size can follow one another in one buffer.
+constexpr int kJqHeader = 1024, kJqCounters = 1024, kJqData = kJqHeader + 4 * kJqCounters;
+
 // Number of SMs of the current device (cached per device id).
 int jq_sm_count();
 

@@ -1,0 +1,576 @@
+// Attention over the 8-bit cache, few query rows per key head (single tokens, drafts).
+#include "kv.cuh"
+
+namespace jqkv {
+
+using namespace jqta;
+
+constexpr int kWarps = 4;          // of a CTA; each takes every fourth stage of a segment
+constexpr int kUnit = 64;          // keys: what work is dealt out in
+
+struct AttendArgs {
+    Batch b;
+    const void *q;
+    void *out;
+    float *lse;
+    long long st, sh;              // elements of q between tokens and heads
+    const uint8_t *keys, *values;
+    const float *ks, *vs;
+    int H, G, window, dtype, least;   // least: units that a CTA takes at least
+    float scale;                   // of the scores, times log2(e)
+    int *status;
+    int *counters;                 // one per CTA: parts of the pair that begins in it and is done elsewhere too
+    float *parts;                  // two per CTA: [rows][D] sums, [rows] maxima, [rows] weights
+};
+
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ uint32_t pack_h2(float lo, float hi) {
+    uint32_t r;
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+__device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// A sequence's share of the work: row tiles x key heads pairs of `units` units each, pairs in the order (head, tile).
+struct Share {
+    int row0, n, len, lo, units, tiles;
+    long long total;
+};
+template <int ROWS>
+__device__ __forceinline__ Share share_of(const AttendArgs &p, int i) {
+    Share s;
+    s.n = p.b.count(i, s.row0);
+    s.len = p.b.length(i);
+    const int first = s.len - s.n;
+    s.lo = p.window > 0 ? max(0, first - p.window + 1) : 0;
+    s.lo -= s.lo % kUnit;
+    s.units = max(1, (s.len - s.lo + kUnit - 1) / kUnit);      // (a row that sees nothing has its zeros written too)
+    s.tiles = (int)(((long long)s.n * p.G + ROWS - 1) / ROWS);
+    s.total = (long long)s.tiles * p.H * s.units;
+    return s;
+}
+
+// ROWS: 8 (rows 8 to 15 of the matrix instruction's tile are not there), 16 or 32 query rows (query, head of the group) at once.
+template <int D, bool E4M3, int ROWS>
+__global__ void __launch_bounds__(kWarps * 32) attend_kernel(const __grid_constant__ AttendArgs p) {
+    constexpr int MT = ROWS > 16 ? ROWS / 16 : 1;              // tiles of 16 rows
+    constexpr bool TWO = ROWS > 8;                             // rows 8 to 15 are there
+    constexpr int C = D / 32;                                  // chunks of a group
+    constexpr int KEYS = D <= 128 ? 32 : 16;                   // keys of a stage
+    constexpr int NG = KEYS / 16;
+    constexpr int kStageBytes = KEYS * D * 2;
+    constexpr int NS = 24576 / kStageBytes;                    // stages of a warp's ring: 24 KB, two CTAs on an SM
+    constexpr int TR = MT * 16;                                // rows of a tile
+    constexpr int kPart = TR * D + 2 * TR;                     // floats of a part
+    extern __shared__ __align__(128) unsigned char smem[];
+    __shared__ __align__(8) uint64_t bars[kWarps * NS];
+    __shared__ int s_err, s_seq, s_last;
+    __shared__ long long s_sum[kWarps], s_off;
+    __shared__ float s_m[kWarps][TR], s_l[kWarps][TR];
+
+    const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31, g = lane >> 2, tq = lane & 3;
+    unsigned char *const ring = smem + warp * 24576;
+    const uint32_t ring_u = smem_u32(ring), bar0 = smem_u32(&bars[warp * NS]);
+    if (lane == 0)
+        for (int s = 0; s < NS; ++s) mbar_init(bar0 + 8 * s, 1);
+    if (tid == 0) s_err = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    fence_async_smem();
+
+    // ---- this CTA's units: [lo, hi) of all, the same number for every CTA up to one
+    const int per = (p.b.S + kWarps * 32 - 1) / (kWarps * 32), i0 = min(p.b.S, tid * per), i1 = min(p.b.S, i0 + per);
+    long long mine = 0;
+    for (int i = i0; i < i1; ++i) mine += share_of<ROWS>(p, i).total;
+    long long before = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const long long v = __shfl_up_sync(0xffffffffu, before, o);
+        if (lane >= o) before += v;
+    }
+    if (lane == 31) s_sum[warp] = before;
+    __syncthreads();
+    long long total = 0;
+    for (int w = 0; w < kWarps; ++w) {
+        if (w == warp) before += total - mine;
+        total += s_sum[w];
+    }
+    if (total == 0) return;
+    const long long fit = (total + p.least - 1) / p.least;
+    const int W = fit < (long long)gridDim.x ? (int)fit : (int)gridDim.x;
+    if ((int)blockIdx.x >= W) return;
+    long long cur = total * blockIdx.x / W;
+    const long long hi = total * (blockIdx.x + 1) / W;
+    if (cur >= before && cur < before + mine) {                // (one thread's sequences hold the first unit)
+        long long at = before;
+        for (int i = i0; i < i1; ++i) {
+            const long long t = share_of<ROWS>(p, i).total;
+            if (cur < at + t) {
+                s_seq = i;
+                s_off = at;
+                break;
+            }
+            at += t;
+        }
+    }
+    __syncthreads();
+    int seq = s_seq;
+    long long seq_at = s_off;
+    Share sh = share_of<ROWS>(p, seq);
+
+    uint32_t phases = 0;                                       // parity of each stage's next completion
+    while (cur < hi) {
+        while (cur >= seq_at + sh.total) {
+            seq_at += sh.total;
+            sh = share_of<ROWS>(p, ++seq);
+        }
+        const long long in_seq = cur - seq_at;
+        const int pair = (int)(in_seq / sh.units), u0 = (int)(in_seq % sh.units);
+        const int u1 = (int)min((long long)sh.units, u0 + (hi - cur));
+        const int h = pair / sh.tiles, tile = pair % sh.tiles;
+        const int k0 = sh.lo + u0 * kUnit, k1 = min(sh.len, sh.lo + u1 * kUnit);
+        const int stages = k1 > k0 ? (k1 - k0 + KEYS - 1) / KEYS : 0;
+        const int own = stages > warp ? (stages - warp + kWarps - 1) / kWarps : 0;      // stages of this warp
+        const int r0 = tile * TR, rows = min(TR, sh.n * p.G - r0);
+
+        // ---- the warp's stages, 32 of them at a time: lane l has the blocks and scales of the l-th
+        int id[NG];
+        float kc[NG], vl[NG], vi[NG];
+        auto look_up = [&](int first) {
+            const int st = first + lane;
+            const int key = k0 + (warp + st * kWarps) * KEYS;
+#pragma unroll
+            for (int n = 0; n < NG; ++n) {
+                id[n] = -1;
+                if (st < own && key + 16 * n < k1) id[n] = p.b.block(seq, key + 16 * n);
+            }
+        };
+        auto scales = [&]() {
+#pragma unroll
+            for (int n = 0; n < NG; ++n) {
+                const size_t at = (size_t)max(id[n], 0) * p.H + h;
+                const float v = id[n] >= 0 ? p.vs[at] : 1.f;
+                kc[n] = id[n] >= 0 ? p.ks[at] * p.scale : 0.f;
+                vl[n] = log2f(v);
+                vi[n] = __fdividef(1.f, v);
+            }
+        };
+        auto issue = [&](int st, int slot) {                   // all lanes; stage `st` of the warp, within the 32 looked up
+            int ids[NG];
+#pragma unroll
+            for (int n = 0; n < NG; ++n) ids[n] = __shfl_sync(0xffffffffu, id[n], st & 31);
+            if (lane == 0) {
+                const int key = k0 + (warp + st * kWarps) * KEYS;
+                const uint32_t bar = bar0 + 8 * slot, dst = ring_u + slot * kStageBytes;
+                uint32_t bytes = 0;
+#pragma unroll
+                for (int n = 0; n < NG; ++n) bytes += ids[n] >= 0 ? 32 * D : 0;
+                mbar_expect_tx(bar, bytes);
+                const bool whole = NG == 1 || (ids[0] >= 0 && ids[NG - 1] >= 0 && p.b.T >= KEYS);
+                if (whole) {
+                    const size_t at = (((size_t)ids[0] * p.H + h) * p.b.T + key % p.b.T) * D;
+                    if (ids[0] >= 0) {
+                        bulk_g2s(dst, p.keys + at, KEYS * D, bar);
+                        bulk_g2s(dst + KEYS * D, p.values + at, KEYS * D, bar);
+                    }
+                } else {
+#pragma unroll
+                    for (int n = 0; n < NG; ++n) {
+                        if (ids[n] < 0) continue;
+                        const size_t at = (((size_t)ids[n] * p.H + h) * p.b.T + (key + 16 * n) % p.b.T) * D;
+                        bulk_g2s(dst + n * 16 * D, p.keys + at, 16 * D, bar);
+                        bulk_g2s(dst + KEYS * D + n * 16 * D, p.values + at, 16 * D, bar);
+                    }
+                }
+            }
+        };
+        look_up(0);
+#pragma unroll
+        for (int s = 0; s < NS; ++s)
+            if (s < own) issue(s, s);
+        scales();
+
+        // ---- queries: rows as the A operand, each divided by a power of two that brings it into fp16's range
+        uint32_t qa[MT][C][2][4];
+        float qs[MT][2];                                       // what the scores of the lane's rows are multiplied by
+        int pos[MT][2];                                        // positions of its rows; -1: no such row
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                const int r = mt * 16 + half * 8 + g;
+                const bool there = r < rows && (half == 0 || TWO);
+                const int j = (r0 + r) / p.G, hq = h * p.G + (r0 + r) % p.G;
+                pos[mt][half] = there ? sh.len - sh.n + j : -1;
+                float amax = 0.f;
+                uint4 raw[C];
+#pragma unroll
+                for (int c = 0; c < C; ++c) {
+                    raw[c] = make_uint4(0, 0, 0, 0);
+                    if (there) {
+                        const unsigned short *at = reinterpret_cast<const unsigned short *>(p.q) + (sh.row0 + j) * p.st + hq * p.sh + c * 32 + tq * 8;
+                        if ((reinterpret_cast<uintptr_t>(at) & 15u) == 0) {
+                            raw[c] = *reinterpret_cast<const uint4 *>(at);
+                        } else {
+                            unsigned short *e = reinterpret_cast<unsigned short *>(&raw[c]);
+#pragma unroll
+                            for (int k = 0; k < 8; ++k) e[k] = at[k];
+                        }
+                    }
+                }
+                auto value = [&](uint32_t w, int hi_half) -> float {
+                    const unsigned short u = (unsigned short)(hi_half ? w >> 16 : w & 0xffffu);
+                    return p.dtype == JQ_F16 ? __half2float(__ushort_as_half(u)) : __uint_as_float((uint32_t)u << 16);
+                };
+#pragma unroll
+                for (int c = 0; c < C; ++c) {
+                    const uint32_t w[4] = {raw[c].x, raw[c].y, raw[c].z, raw[c].w};
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) amax = fmaxf(amax, fmaxf(fabsf(value(w[k], 0)), fabsf(value(w[k], 1))));
+                }
+                amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+                amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+                const int e = act_exponent(amax, false);
+                const float down = __uint_as_float((uint32_t)(127 - e) << 23);
+                qs[mt][half] = __uint_as_float((uint32_t)(127 + e) << 23);
+#pragma unroll
+                for (int c = 0; c < C; ++c) {
+                    const uint32_t w[4] = {raw[c].x, raw[c].y, raw[c].z, raw[c].w};
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)                // word k: values 2k, 2k + 1 = step k / 2, register 0 or 2 (+ half)
+                        qa[mt][c][k >> 1][(k & 1) * 2 + half] = pack_h2(value(w[k], 0) * down, value(w[k], 1) * down);
+                }
+            }
+
+        float o[MT][D / 8][4], M[MT][2], l[MT][2];
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) {
+            M[mt][0] = M[mt][1] = -INFINITY;
+            l[mt][0] = l[mt][1] = 0.f;
+#pragma unroll
+            for (int n = 0; n < D / 8; ++n) o[mt][n][0] = o[mt][n][1] = o[mt][n][2] = o[mt][n][3] = 0.f;
+        }
+        // the queries' least and largest positions: keys between them and the window's edges are looked at one by one
+        const int pos_first = sh.len - sh.n + r0 / p.G, pos_last = sh.len - sh.n + (r0 + rows - 1) / p.G;
+
+        int slot = 0;
+        for (int st = 0; st < own; ++st) {
+            const int sl = st & 31;
+            const int key = k0 + (warp + st * kWarps) * KEYS;
+            mbar_wait(bar0 + 8 * slot, phases >> slot & 1, &s_err);
+            phases ^= 1u << slot;
+            const uint32_t base = ring_u + slot * kStageBytes;
+            float kcs[NG], vls[NG], vis[NG];
+            bool there[NG];
+#pragma unroll
+            for (int n = 0; n < NG; ++n) {
+                kcs[n] = __shfl_sync(0xffffffffu, kc[n], sl);
+                vls[n] = __shfl_sync(0xffffffffu, vl[n], sl);
+                vis[n] = __shfl_sync(0xffffffffu, vi[n], sl);
+                there[n] = __shfl_sync(0xffffffffu, id[n], sl) >= 0;
+            }
+            float s[MT][NG][2][4];
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                for (int n = 0; n < NG; ++n)
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) s[mt][n][j][0] = s[mt][n][j][1] = s[mt][n][j][2] = s[mt][n][j][3] = 0.f;
+#pragma unroll
+            for (int c = 0; c < C; ++c)
+#pragma unroll
+                for (int n = 0; n < NG; ++n) {
+                    const uint4 w = lds128(base + n * 16 * D + c * 512 + lane * 16);
+                    uint32_t b[4][2];
+                    codes_to_h4<E4M3>(w.x, b[0][0], b[0][1]);
+                    codes_to_h4<E4M3>(w.y, b[1][0], b[1][1]);
+                    codes_to_h4<E4M3>(w.z, b[2][0], b[2][1]);
+                    codes_to_h4<E4M3>(w.w, b[3][0], b[3][1]);
+#pragma unroll
+                    for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                        for (int j = 0; j < 2; ++j) {
+                            mma16816(s[mt][n][j], qa[mt][c][0], b[2 * j][0], b[2 * j][1]);
+                            mma16816(s[mt][n][j], qa[mt][c][1], b[2 * j + 1][0], b[2 * j + 1][1]);
+                        }
+                }
+            // t = log2(weight of the key times its block's value scale); the sums are formed relative to the largest t
+            const bool masked = key + KEYS - 1 > pos_first || (p.window > 0 && key <= pos_last - p.window) || !there[0] || !there[NG - 1];
+            uint32_t pa[MT][NG][4];
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt) {
+                float alpha[2] = {1.f, 1.f};
+#pragma unroll
+                for (int half = 0; half < (TWO ? 2 : 1); ++half) {
+                    float m = M[mt][half];
+#pragma unroll
+                    for (int n = 0; n < NG; ++n) {
+                        const float f = kcs[n] * qs[mt][half];
+#pragma unroll
+                        for (int j = 0; j < 2; ++j)
+#pragma unroll
+                            for (int k = 0; k < 2; ++k) {
+                                float &t = s[mt][n][j][half * 2 + k];
+                                t = fmaf(t, f, vls[n]);
+                                if (masked) {
+                                    const int kp = key + n * 16 + 4 * tq + 2 * j + k;
+                                    if (kp > pos[mt][half] || (p.window > 0 && kp <= pos[mt][half] - p.window) || !there[n]) t = -INFINITY;
+                                }
+                                m = fmaxf(m, t);
+                            }
+                    }
+                    m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
+                    m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
+                    const float ref = m == -INFINITY ? 0.f : m;          // (nothing seen yet: every weight is 0)
+                    alpha[half] = ex2(M[mt][half] - ref);
+                    M[mt][half] = m;
+                    float sum = 0.f;
+#pragma unroll
+                    for (int n = 0; n < NG; ++n) {
+                        float part = 0.f;
+#pragma unroll
+                        for (int j = 0; j < 2; ++j)
+#pragma unroll
+                            for (int k = 0; k < 2; ++k) {
+                                float &t = s[mt][n][j][half * 2 + k];
+                                t = ex2(t - ref);
+                                part += t;
+                            }
+                        sum = fmaf(part, vis[n], sum);
+                    }
+                    l[mt][half] = fmaf(l[mt][half], alpha[half], sum);
+                }
+#pragma unroll
+                for (int n = 0; n < NG; ++n)
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) {
+                        pa[mt][n][2 * j] = pack_h2(s[mt][n][j][0], s[mt][n][j][1]);
+                        pa[mt][n][2 * j + 1] = TWO ? pack_h2(s[mt][n][j][2], s[mt][n][j][3]) : 0u;
+                    }
+                if (__any_sync(0xffffffffu, alpha[0] != 1.f || alpha[1] != 1.f)) {
+#pragma unroll
+                    for (int n = 0; n < D / 8; ++n) {
+                        o[mt][n][0] *= alpha[0];
+                        o[mt][n][1] *= alpha[0];
+                        if (TWO) {
+                            o[mt][n][2] *= alpha[1];
+                            o[mt][n][3] *= alpha[1];
+                        }
+                    }
+                }
+            }
+#pragma unroll
+            for (int n = 0; n < NG; ++n) {
+                // e4m3 has a NaN, and places behind a sequence's end, or of a block that is not there, may hold anything
+                uint32_t keep = 0xffffffffu;
+                if (E4M3) {
+                    const int left = there[n] ? sh.len - (key + n * 16 + 4 * tq) : 0;
+                    keep = left >= 4 ? 0xffffffffu : (left <= 0 ? 0u : (1u << 8 * left) - 1u);
+                }
+#pragma unroll
+                for (int c = 0; c < C; ++c) {
+                    const uint4 w = lds128(base + KEYS * D + n * 16 * D + c * 512 + lane * 16);
+                    const uint32_t word[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+                    for (int dt = 0; dt < 4; ++dt) {
+                        uint32_t b0, b1;
+                        codes_to_h4<E4M3>(E4M3 ? word[dt] & keep : word[dt], b0, b1);
+#pragma unroll
+                        for (int mt = 0; mt < MT; ++mt) mma16816(o[mt][c * 4 + dt], pa[mt][n], b0, b1);
+                    }
+                }
+            }
+            __syncwarp();                                      // every lane has read the stage
+            if (sl == 31 && st + 1 < own) {                    // (the stages in flight keep their codes; their scales are looked up anew)
+                look_up(st + 1);
+                scales();
+            }
+            if (st + NS < own) {
+                if ((st + NS) / 32 == (st + 1) / 32) {
+                    issue(st + NS, slot);
+                } else {                                       // its block lies in the next 32: looked up for it alone
+                    int keep_id[NG];
+#pragma unroll
+                    for (int n = 0; n < NG; ++n) keep_id[n] = id[n];
+                    look_up((st + NS) & ~31);
+                    issue(st + NS, slot);
+#pragma unroll
+                    for (int n = 0; n < NG; ++n) id[n] = keep_id[n];
+                }
+            }
+            if (++slot == NS) slot = 0;
+        }
+        // (stages are dealt to slots from slot 0 in every segment; all copies of this one have been waited for)
+
+        // ---- the four warps' sums become one
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+            for (int half = 0; half < (TWO ? 2 : 1); ++half) {
+                float v = l[mt][half];
+                v += __shfl_xor_sync(0xffffffffu, v, 1);
+                v += __shfl_xor_sync(0xffffffffu, v, 2);
+                const int r = mt * 16 + half * 8 + g;
+                if (tq == 0) {
+                    s_m[warp][r] = M[mt][half];
+                    s_l[warp][r] = v;
+                }
+                float *dst = reinterpret_cast<float *>(ring) + (size_t)r * D;
+#pragma unroll
+                for (int n = 0; n < D / 8; ++n)                // columns rotated by the row, so that rows do not meet in a bank
+                    *reinterpret_cast<float2 *>(dst + ((n * 8 + 2 * tq + 8 * (r & 7)) & (D - 1))) =
+                        make_float2(o[mt][n][half * 2], o[mt][n][half * 2 + 1]);
+            }
+        __syncthreads();
+        const long long pair_at = seq_at + (long long)pair * sh.units, pair_end = pair_at + sh.units;
+        const bool all = u0 == 0 && u1 == sh.units;
+        const int w0 = all ? 0 : (int)(((pair_at + 1) * W - 1) / total), w1 = all ? 0 : (int)((pair_end * W - 1) / total);
+        float *part = p.parts + (size_t)(2 * blockIdx.x + (u0 == 0 ? 1 : 0)) * kPart;
+        auto finish = [&](int r, int d, float4 v, float m, float lsum) {      // outputs of four values of a row
+            const int j = (r0 + r) / p.G, hq = h * p.G + (r0 + r) % p.G;
+            const float inv = lsum > 0.f ? 1.f / lsum : (lsum == 0.f ? 0.f : lsum);
+            const size_t at = ((size_t)(sh.row0 + j) * p.H * p.G + hq) * D + d;
+            const float a = v.x * inv, b = v.y * inv, c = v.z * inv, e = v.w * inv;
+            if (p.dtype == JQ_F16) {
+                *reinterpret_cast<uint2 *>(reinterpret_cast<__half *>(p.out) + at) = make_uint2(pack_h2(a, b), pack_h2(c, e));
+            } else {
+                const __nv_bfloat162 x = __floats2bfloat162_rn(a, b), y = __floats2bfloat162_rn(c, e);
+                *reinterpret_cast<uint2 *>(reinterpret_cast<__nv_bfloat16 *>(p.out) + at) =
+                    make_uint2(*reinterpret_cast<const uint32_t *>(&x), *reinterpret_cast<const uint32_t *>(&y));
+            }
+            if (d == 0 && p.lse) p.lse[(size_t)(sh.row0 + j) * p.H * p.G + hq] = lsum > 0.f ? (m + log2f(lsum)) * kLn2 : (lsum == 0.f ? -INFINITY : lsum);
+        };
+        for (int e = tid; e < rows * (D / 4); e += kWarps * 32) {
+            const int r = e / (D / 4), d = e % (D / 4) * 4;
+            float m = s_m[0][r];
+#pragma unroll
+            for (int w = 1; w < kWarps; ++w) m = fmaxf(m, s_m[w][r]);
+            const float ref = m == -INFINITY ? 0.f : m;
+            float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+            float lsum = 0.f;
+#pragma unroll
+            for (int w = 0; w < kWarps; ++w) {
+                const float f = ex2(s_m[w][r] - ref);
+                const float4 x = *reinterpret_cast<const float4 *>(smem + w * 24576 + ((size_t)r * D + ((d + 8 * (r & 7)) & (D - 1))) * 4);
+                lsum = fmaf(s_l[w][r], f, lsum);
+                v.x = fmaf(x.x, f, v.x); v.y = fmaf(x.y, f, v.y); v.z = fmaf(x.z, f, v.z); v.w = fmaf(x.w, f, v.w);
+            }
+            if (all) {
+                finish(r, d, v, m, lsum);
+            } else {
+                *reinterpret_cast<float4 *>(part + (size_t)r * D + d) = v;
+                if (d == 0) {
+                    part[TR * D + r] = m;
+                    part[TR * D + TR + r] = lsum;
+                }
+            }
+        }
+        if (!all) {
+            // the last of the pair's CTAs to get here adds the parts, in their order
+            __threadfence();
+            __syncthreads();
+            if (tid == 0) {
+                const int n = atomicAdd(p.counters + w0, 1);
+                s_last = n == w1 - w0;
+                if (s_last) p.counters[w0] = 0;
+            }
+            __syncthreads();
+            if (s_last) {
+                __threadfence();
+                for (int e = tid; e < rows * (D / 4); e += kWarps * 32) {
+                    const int r = e / (D / 4), d = e % (D / 4) * 4;
+                    float m = -INFINITY, lsum = 0.f;
+                    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+                    for (int w = w0; w <= w1; ++w) {
+                        const float *x = p.parts + (size_t)(2 * w + (w == w0 ? 1 : 0)) * kPart;
+                        const float mw = __ldcg(x + TR * D + r);
+                        const float4 y = __ldcg(reinterpret_cast<const float4 *>(x + (size_t)r * D + d));
+                        const float lw = __ldcg(x + TR * D + TR + r);
+                        const float top = fmaxf(m, mw), ref = top == -INFINITY ? 0.f : top;
+                        const float a = ex2(m - ref), b = ex2(mw - ref);
+                        v.x = fmaf(v.x, a, y.x * b); v.y = fmaf(v.y, a, y.y * b); v.z = fmaf(v.z, a, y.z * b); v.w = fmaf(v.w, a, y.w * b);
+                        lsum = fmaf(lsum, a, lw * b);
+                        m = top;
+                    }
+                    finish(r, d, v, m, lsum);
+                }
+            }
+        }
+        fence_async_smem();                                    // the ring was written to by threads; copies land in it next
+        __syncthreads();
+        cur += u1 - u0;
+    }
+    if (s_err) {                                               // a wait gave up: copies in flight land before the shared memory goes away
+        for (int i = 0; i < 400; ++i) __nanosleep(256);
+        if (tid == 0) atomicExch(p.status, s_err);
+    }
+}
+
+constexpr int kSmem = kWarps * 24576;
+
+static int grid_of() { return 2 * jq_sm_count() < kJqCounters ? 2 * jq_sm_count() : kJqCounters; }
+
+typedef void (*attend_fn)(const AttendArgs);
+template <int D>
+static attend_fn pick(bool e4m3, int rows) {
+    if (e4m3) return rows == 8 ? attend_kernel<D, true, 8> : (rows == 16 ? attend_kernel<D, true, 16> : attend_kernel<D, true, 32>);
+    return rows == 8 ? attend_kernel<D, false, 8> : (rows == 16 ? attend_kernel<D, false, 16> : attend_kernel<D, false, 32>);
+}
+
+int check_cache(const jq_kv_cache *c, const jq_kv_batch *s);
+Batch batch_of(const jq_kv_cache *c, const jq_kv_batch *s);
+int most_new(const jq_kv_batch *s);
+
+}  // namespace jqkv
+
+using namespace jqkv;
+
+extern "C" size_t jq_kv_attend_workspace_bytes(const jq_kv_cache *c, const jq_kv_batch *s, int q_heads) {
+    if (check_cache(c, s) || q_heads <= 0) return 0;
+    const size_t grid = (size_t)grid_of();
+    return kJqData + 2 * grid * (32 * (size_t)c->head_dim + 64) * 4;
+}
+
+extern "C" int jq_kv_attend(const jq_kv_cache *c, const jq_kv_batch *s, const void *q, const int64_t *stride_q, int q_heads,
+                            float scale, int window, void *out, float *lse_or_null, int dtype, void *workspace,
+                            size_t workspace_bytes, jq_stream_t stream) {
+    const int bad = check_cache(c, s);
+    if (bad) return bad;
+    if (dtype != JQ_F16 && dtype != JQ_BF16) return JQ_ERR_BAD_DTYPE;
+    if (q_heads <= 0 || q_heads % c->kv_heads || window < 0 || !(scale > 0.f) || scale > 3e38f) return JQ_ERR_BAD_SHAPE;
+    if (c->head_dim != 64 && c->head_dim != 128) return JQ_ERR_UNSUPPORTED;
+    if (s->sequences == 0 || s->tokens == 0) return JQ_OK;
+    if (!q || !out || !stride_q || !workspace) return JQ_ERR_NULL_PTR;
+    if ((reinterpret_cast<uintptr_t>(q) & 1u) || !jq_aligned16(out) || (reinterpret_cast<uintptr_t>(lse_or_null) & 3u) ||
+        (reinterpret_cast<uintptr_t>(workspace) & 127u))
+        return JQ_ERR_BAD_ALIGN;
+    if (workspace_bytes < jq_kv_attend_workspace_bytes(c, s, q_heads)) return JQ_ERR_WORKSPACE;
+    AttendArgs a{};
+    a.b = batch_of(c, s);
+    a.q = q; a.out = out; a.lse = lse_or_null;
+    a.st = stride_q[0]; a.sh = stride_q[1];
+    a.keys = reinterpret_cast<const uint8_t *>(c->keys); a.values = reinterpret_cast<const uint8_t *>(c->values);
+    a.ks = c->key_scales; a.vs = c->value_scales;
+    a.H = c->kv_heads; a.G = q_heads / c->kv_heads; a.window = window; a.dtype = dtype;
+    a.scale = scale * kLog2e;
+    a.least = 2;
+    const int grid = grid_of();
+    unsigned char *ws = reinterpret_cast<unsigned char *>(workspace);
+    a.status = reinterpret_cast<int *>(ws);
+    a.counters = reinterpret_cast<int *>(ws + kJqHeader);
+    a.parts = reinterpret_cast<float *>(ws + kJqData);
+    const long long rows = (long long)most_new(s) * a.G;
+    const int tile = rows <= 8 ? 8 : (rows <= 16 ? 16 : 32);
+    const bool e4m3 = c->fmt == JQ_KV_E4M3;
+    const attend_fn kern = c->head_dim == 64 ? pick<64>(e4m3, tile) : pick<128>(e4m3, tile);
+    static jq_contexts done[2][2][3];
+    JQ_CUDA_TRY(jq_allow_smem(reinterpret_cast<const void *>(kern), kSmem, done[c->head_dim == 128][e4m3][tile == 8 ? 0 : tile / 16]));
+    kern<<<grid, kWarps * 32, kSmem, reinterpret_cast<cudaStream_t>(stream)>>>(a);
+    return jq_launch_status();
+}

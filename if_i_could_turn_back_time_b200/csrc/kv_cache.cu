@@ -1,0 +1,289 @@
+// Writing into the 8-bit key/value cache and reading it back.
+#include "kv.cuh"
+
+namespace jqkv {
+
+struct AppendArgs {
+    Batch b;
+    const void *x[2];                 // keys, values
+    long long st[2], sh[2];           // elements between tokens and heads
+    uint8_t *codes[2];
+    float *scales[2];
+    int H, D, touched, vec;
+};
+
+template <class T>
+__device__ __forceinline__ void load8(const T *p, bool vec, float (&v)[8]) {
+    if (sizeof(T) == 2 && vec) {
+        const uint4 u = *reinterpret_cast<const uint4 *>(p);
+        const T *e = reinterpret_cast<const T *>(&u);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = (float)e[i];
+    } else if (vec) {
+        const float4 a = reinterpret_cast<const float4 *>(p)[0], b = reinterpret_cast<const float4 *>(p)[1];
+        v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = (float)p[i];
+    }
+}
+
+// The code of x at this scale: the quotient, rounded to fp32 and then to the format's nearest value, ties to even.  Infinities are
+// the largest codes, NaN is 0 (a block's one scale cannot hold either).
+template <bool E4M3>
+__device__ __forceinline__ uint32_t encode(float x, float scale) {
+    const float top = E4M3 ? kTopE4m3 : kTopInt8;
+    float q = __fdiv_rn(x, scale);
+    q = q != q ? 0.f : fminf(fmaxf(q, -top), top);
+    if (!E4M3) return (uint32_t)(__float2int_rn(q) + 128);
+    uint16_t r;
+    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(0.f), "f"(q));
+    return r & 0xffu;
+}
+template <bool E4M3>
+__device__ __forceinline__ float decode(uint32_t code) {
+    uint32_t lo, hi;
+    codes_to_h4<E4M3>(code, lo, hi);
+    return __half2float(__ushort_as_half((unsigned short)(lo & 0xffffu)));
+}
+
+// One CTA per block that receives tokens, head, and keys or values: the maximum of the new tokens, the block's scale, then the codes.
+template <class T, bool E4M3>
+__global__ void __launch_bounds__(256) append_kernel(const __grid_constant__ AppendArgs p) {
+    __shared__ float red[8];
+    const int i = blockIdx.x / p.touched, h = blockIdx.y, what = blockIdx.z, BT = p.b.T, D = p.D;
+    int row0;
+    const int n = p.b.count(i, row0), len = p.b.length(i);
+    const int first = len - n;
+    const int blk = (first > 0 ? first / BT : 0) + (int)(blockIdx.x % p.touched);
+    const int t0 = max(first, blk * BT), t1 = min(len, (blk + 1) * BT);
+    if (n == 0 || t0 >= t1) return;
+    const int id = p.b.block(i, t0);
+    if (id < 0) return;
+    const T *x = reinterpret_cast<const T *>(p.x[what]) + (long long)row0 * p.st[what] + h * p.sh[what];
+    uint8_t *codes = p.codes[what] + ((size_t)id * p.H + h) * BT * D;
+    float *scale_at = p.scales[what] + (size_t)id * p.H + h;
+    const int per = D / 8;
+    float m = 0.f;
+    for (int e = threadIdx.x; e < (t1 - t0) * per; e += 256) {
+        float v[8];
+        load8(x + (t0 + e / per - first) * p.st[what] + e % per * 8, p.vec, v);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) m = fabsf(v[k]) <= 3.402823466e38f ? fmaxf(m, fabsf(v[k])) : m;
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = m;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < 8; ++w) m = fmaxf(m, red[w]);
+    const int held = t0 - blk * BT, end = t1 - blk * BT;         // places of the block: [0, held) old, [held, end) new
+    const float old = held > 0 ? *scale_at : 0.f;
+    const float scale = fmaxf(old, __fdiv_rn(fmaxf(m, kLeastMax), E4M3 ? kTopE4m3 : kTopInt8));
+    const bool grown = held > 0 && scale > old;
+    __syncthreads();
+    if (threadIdx.x == 0) *scale_at = scale;
+    const int g0 = (grown ? 0 : held) / 16, g1 = (end + 15) / 16;
+    for (int e = threadIdx.x + g0 * D; e < g1 * D; e += 256) {        // pieces of 16 bytes, D of them in a group of 16 tokens
+        const int group = e / D, c = e % D / 32, g = e % 32 / 4, t = e % 4;
+        uint4 *at = reinterpret_cast<uint4 *>(codes) + e;
+        uint4 w = *at;
+        uint32_t *word = &w.x;
+        if (what == 0) {
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                const int token = group * 16 + 4 * (g >> 1) + (g & 1) + 2 * j;
+                if (token >= held && token < end) {
+                    float v[8];
+                    load8(x + (blk * BT + token - first) * p.st[0] + c * 32 + t * 8, p.vec, v);
+#pragma unroll
+                    for (int k = 0; k < 2; ++k)
+                        word[2 * j + k] = encode<E4M3>(v[4 * k], scale) | encode<E4M3>(v[4 * k + 1], scale) << 8 |
+                                          encode<E4M3>(v[4 * k + 2], scale) << 16 | encode<E4M3>(v[4 * k + 3], scale) << 24;
+                } else if (grown && token < held) {
+#pragma unroll
+                    for (int k = 0; k < 2; ++k) {
+                        uint32_t u = 0;
+#pragma unroll
+                        for (int b = 0; b < 4; ++b)
+                            u |= encode<E4M3>(__fmul_rn(decode<E4M3>(word[2 * j + k] >> 8 * b & 255), old), scale) << 8 * b;
+                        word[2 * j + k] = u;
+                    }
+                }
+            }
+        } else {
+#pragma unroll
+            for (int b = 0; b < 4; ++b) {
+                const int token = group * 16 + 4 * t + b;
+                const bool fresh = token >= held && token < end;
+                if (!fresh && !(grown && token < held)) continue;
+                const T *row = x + (blk * BT + token - first) * p.st[1] + c * 32 + g;
+#pragma unroll
+                for (int dt = 0; dt < 4; ++dt) {
+                    const uint32_t was = word[dt] >> 8 * b & 255;
+                    const uint32_t is = fresh ? encode<E4M3>((float)row[dt * 8], scale)
+                                              : encode<E4M3>(__fmul_rn(decode<E4M3>(was), old), scale);
+                    word[dt] ^= (was ^ is) << 8 * b;
+                }
+            }
+        }
+        *at = w;
+    }
+}
+
+struct ReadArgs {
+    Batch b;
+    const uint8_t *codes[2];
+    const float *scales[2];
+    void *out[2];
+    int H, D, last, groups, dtype;
+};
+
+// A warp per group of 16 tokens and head: what the codes stand for, in the order of a user's tensors.
+template <bool E4M3>
+__global__ void __launch_bounds__(256) read_kernel(const __grid_constant__ ReadArgs p) {
+    const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    const long long job = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
+    const int h = (int)(job % p.H), what = blockIdx.y;
+    const long long k = job / p.H;
+    const int i = (int)(k / p.groups);
+    if (i >= p.b.S) return;
+    const int begin = p.b.length(i) - p.last;                                 // (below 0: places before the first token read as 0)
+    const int group = (begin >= 0 ? begin / 16 : -((15 - begin) / 16)) + (int)(k % p.groups);
+    const int base = group * 16 - begin;                                      // place of the group's first token in the output
+    if (base >= p.last) return;
+    const int id = group >= 0 ? p.b.block(i, group * 16) : -1;
+    const float scale = id >= 0 ? p.scales[what][(size_t)id * p.H + h] : 0.f;
+    const uint4 *at = reinterpret_cast<const uint4 *>(p.codes[what] + (((size_t)max(id, 0) * p.H + h) * p.b.T + (group >= 0 ? group * 16 % p.b.T : 0)) * p.D);
+    const size_t row = (size_t)p.H * p.D;
+    const size_t out0 = (size_t)i * p.last * row + (size_t)h * p.D;
+    for (int c = 0; c < p.D / 32; ++c) {
+        const uint4 w = id >= 0 ? at[c * 32 + lane] : make_uint4(0, 0, 0, 0);
+        const uint32_t word[4] = {w.x, w.y, w.z, w.w};
+        float v[16];
+#pragma unroll
+        for (int k4 = 0; k4 < 4; ++k4) {
+            uint32_t lo, hi;
+            codes_to_h4<E4M3>(word[k4], lo, hi);
+            const float2 a = __half22float2(*reinterpret_cast<const __half2 *>(&lo)), b = __half22float2(*reinterpret_cast<const __half2 *>(&hi));
+            v[4 * k4] = a.x; v[4 * k4 + 1] = a.y; v[4 * k4 + 2] = b.x; v[4 * k4 + 3] = b.y;
+        }
+#pragma unroll
+        for (int e = 0; e < 16; ++e) v[e] = id >= 0 ? __fmul_rn(v[e], scale) : 0.f;
+        if (what == 0) {
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                const int place = base + 4 * (g >> 1) + (g & 1) + 2 * j;
+                if (place < 0 || place >= p.last) continue;
+                const size_t o = out0 + place * row + c * 32 + t * 8;
+                if (p.dtype == JQ_F32) {
+                    float4 *q = reinterpret_cast<float4 *>(reinterpret_cast<float *>(p.out[0]) + o);
+                    q[0] = make_float4(v[8 * j], v[8 * j + 1], v[8 * j + 2], v[8 * j + 3]);
+                    q[1] = make_float4(v[8 * j + 4], v[8 * j + 5], v[8 * j + 6], v[8 * j + 7]);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) jq::store_out(p.out[0], o + e, v[8 * j + e], p.dtype);
+                }
+            }
+        } else {
+#pragma unroll
+            for (int b = 0; b < 4; ++b) {
+                const int place = base + 4 * t + b;
+                if (place < 0 || place >= p.last) continue;
+#pragma unroll
+                for (int dt = 0; dt < 4; ++dt) jq::store_out(p.out[1], out0 + place * row + c * 32 + dt * 8 + g, v[4 * dt + b], p.dtype);
+            }
+        }
+    }
+}
+
+// What every entry asks of a cache and its sequences; JQ_OK or the refusal.
+int check_cache(const jq_kv_cache *c, const jq_kv_batch *s) {
+    if (!c || !s || !c->keys || !c->values || !c->key_scales || !c->value_scales) return JQ_ERR_NULL_PTR;
+    if (s->sequences != 0 && (!s->table || !s->lengths)) return JQ_ERR_NULL_PTR;
+    if (c->fmt != JQ_KV_INT8 && c->fmt != JQ_KV_E4M3) return JQ_ERR_BAD_DTYPE;
+    if (c->blocks <= 0 || c->kv_heads <= 0 || c->kv_heads > 65535 || c->head_dim <= 0 || c->head_dim % 32 || c->head_dim > 256 ||
+        (c->block_size != 16 && c->block_size != 32 && c->block_size != 64 && c->block_size != 128))
+        return JQ_ERR_BAD_SHAPE;
+    if (s->sequences < 0 || s->table_width <= 0 || s->table_stride < s->table_width || s->tokens < 0 ||
+        (long long)s->table_width * c->block_size > 0x7fffff00LL)
+        return JQ_ERR_BAD_SHAPE;
+    if (!s->starts && s->sequences && s->tokens % s->sequences) return JQ_ERR_BAD_SHAPE;
+    if (!jq_aligned16(c->keys) || !jq_aligned16(c->values) || (reinterpret_cast<uintptr_t>(c->key_scales) & 3u) ||
+        (reinterpret_cast<uintptr_t>(c->value_scales) & 3u) || (reinterpret_cast<uintptr_t>(s->table) & 3u) ||
+        (reinterpret_cast<uintptr_t>(s->lengths) & 3u) || (reinterpret_cast<uintptr_t>(s->starts) & 3u))
+        return JQ_ERR_BAD_ALIGN;
+    return JQ_OK;
+}
+
+Batch batch_of(const jq_kv_cache *c, const jq_kv_batch *s) {
+    Batch b{};
+    b.table = s->table; b.lengths = s->lengths; b.starts = s->starts;
+    b.S = s->sequences; b.width = s->table_width; b.table_stride = s->table_stride; b.tokens = s->tokens;
+    b.each = s->sequences ? s->tokens / s->sequences : 0;
+    b.T = c->block_size; b.blocks = c->blocks;
+    return b;
+}
+
+// Most new tokens of a sequence: what the caller says, at most all of them.
+int most_new(const jq_kv_batch *s) {
+    if (!s->starts) return s->sequences ? s->tokens / s->sequences : 0;
+    return s->max_new > 0 && s->max_new < s->tokens ? s->max_new : s->tokens;
+}
+
+}  // namespace jqkv
+
+using namespace jqkv;
+
+extern "C" int jq_kv_append(const jq_kv_cache *c, const jq_kv_batch *s, const void *k, const void *v, const int64_t *stride_k,
+                            const int64_t *stride_v, int dtype, jq_stream_t stream) {
+    const int bad = check_cache(c, s);
+    if (bad) return bad;
+    if (dtype < 0 || dtype > 2) return JQ_ERR_BAD_DTYPE;
+    if (s->sequences == 0 || s->tokens == 0) return JQ_OK;
+    if (!k || !v || !stride_k || !stride_v) return JQ_ERR_NULL_PTR;
+    const unsigned esz = dtype == JQ_F32 ? 4 : 2;
+    if ((reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) & (esz - 1)) return JQ_ERR_BAD_ALIGN;
+    AppendArgs a{};
+    a.b = batch_of(c, s);
+    a.x[0] = k; a.x[1] = v;
+    a.st[0] = stride_k[0]; a.sh[0] = stride_k[1]; a.st[1] = stride_v[0]; a.sh[1] = stride_v[1];
+    a.codes[0] = reinterpret_cast<uint8_t *>(c->keys); a.codes[1] = reinterpret_cast<uint8_t *>(c->values);
+    a.scales[0] = c->key_scales; a.scales[1] = c->value_scales;
+    a.H = c->kv_heads; a.D = c->head_dim;
+    const long long most = most_new(s);
+    a.touched = (int)((most + c->block_size - 2) / c->block_size + 1);
+    if (a.touched > s->table_width) a.touched = s->table_width;
+    const long long piece = 16 / esz;
+    a.vec = ((reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) & 15u) == 0 &&
+            (a.st[0] | a.sh[0] | a.st[1] | a.sh[1]) % piece == 0;
+    const long long grid = (long long)a.touched * s->sequences;
+    if (grid > 0x7fffffffLL) return JQ_ERR_BAD_SHAPE;
+    const dim3 blocks((unsigned)grid, (unsigned)c->kv_heads, 2);
+    const cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+    const bool e = c->fmt == JQ_KV_E4M3;
+    if (dtype == JQ_F32) (e ? append_kernel<float, true> : append_kernel<float, false>)<<<blocks, 256, 0, st>>>(a);
+    else if (dtype == JQ_F16) (e ? append_kernel<__half, true> : append_kernel<__half, false>)<<<blocks, 256, 0, st>>>(a);
+    else (e ? append_kernel<__nv_bfloat16, true> : append_kernel<__nv_bfloat16, false>)<<<blocks, 256, 0, st>>>(a);
+    return jq_launch_status();
+}
+
+extern "C" int jq_kv_read(const jq_kv_cache *c, const jq_kv_batch *s, int last, void *k, void *v, int dtype, jq_stream_t stream) {
+    const int bad = check_cache(c, s);
+    if (bad) return bad;
+    if (dtype < 0 || dtype > 2) return JQ_ERR_BAD_DTYPE;
+    if (last < 0) return JQ_ERR_BAD_SHAPE;
+    if (s->sequences == 0 || last == 0) return JQ_OK;
+    if (!k || !v) return JQ_ERR_NULL_PTR;
+    if (!jq_aligned16(k) || !jq_aligned16(v)) return JQ_ERR_BAD_ALIGN;
+    ReadArgs a{};
+    a.b = batch_of(c, s);
+    a.codes[0] = reinterpret_cast<const uint8_t *>(c->keys); a.codes[1] = reinterpret_cast<const uint8_t *>(c->values);
+    a.scales[0] = c->key_scales; a.scales[1] = c->value_scales;
+    a.out[0] = k; a.out[1] = v;
+    a.H = c->kv_heads; a.D = c->head_dim; a.last = last; a.groups = last / 16 + 2; a.dtype = dtype;
+    const long long jobs = (long long)a.groups * s->sequences * c->kv_heads, grid = (jobs + 7) / 8;
+    if (grid > 0x7fffffffLL) return JQ_ERR_BAD_SHAPE;
+    (c->fmt == JQ_KV_E4M3 ? read_kernel<true> : read_kernel<false>)<<<dim3((unsigned)grid, 2), 256, 0, reinterpret_cast<cudaStream_t>(stream)>>>(a);
+    return jq_launch_status();
+}

@@ -9,7 +9,7 @@ from __future__ import annotations
 import ctypes
 import threading
 import warnings
-from typing import List, Optional, Sequence
+from typing import List, NamedTuple, Optional, Sequence
 
 import numpy as np
 import torch
@@ -176,7 +176,8 @@ def _workspace(device, nbytes: int, kind: str = "gemv") -> torch.Tensor:
 def reserve_workspace(device, nbytes: int, kind: str = "ta") -> None:
     """Allocate this thread's scratch for (device, current stream, kernel family) ahead of time, e.g. before a
     CUDA-graph capture or a region that must not allocate: kind "gemv" = split-K partial sums of the row loops,
-    "ta" = prepared activations and status word of the TMA-fed kernels."""
+    "ta" = prepared activations and status word of the TMA-fed kernels, "parts" = partial sums of attention over the
+    cache and of token log probabilities."""
     _workspace(torch.device(device), nbytes, kind)
 
 
@@ -187,12 +188,25 @@ def check_status(raise_on_error: bool = True) -> int:
     written; every later call keeps the word until it is read here."""
     lib = _lib.load()
     worst = 0
-    ws = _ws_cache().get((torch.cuda.current_device(), torch.cuda.current_stream().cuda_stream, "ta"))
-    if ws is not None:
-        worst = min(worst, lib.jq_ta_status(_ptr(ws), 1, _stream()))
+    for kind in ("ta", "parts"):
+        ws = _ws_cache().get((torch.cuda.current_device(), torch.cuda.current_stream().cuda_stream, kind))
+        if ws is not None:
+            worst = min(worst, lib.jq_ta_status(_ptr(ws), 1, _stream()))
     if worst and raise_on_error:
         raise _lib.JqError(worst, "device status")
     return worst
+
+
+def _parts_workspace(device, nbytes: int):
+    """(tensor to keep, address, size) of the scratch of a call whose last CTA adds up what the others left: this thread's and
+    stream's "parts" buffer, or, while a graph is captured, zeros of the call's own from the graph's pool (graphs that were
+    captured on one stream may replay on several).  The kernels leave the counters in it as they found them, at zero."""
+    if _capturing(_stream()):
+        t = torch.empty(nbytes, dtype=torch.uint8, device=device)
+        t[:8192].zero_()
+    else:
+        t = _workspace(device, nbytes, "parts")
+    return t, t.data_ptr(), t.numel()
 
 
 _ta_workspace_bytes = {}       # (K, rows) -> bytes
@@ -437,6 +451,59 @@ def linear(x: torch.Tensor, pw: PackedWeight, bias: Optional[torch.Tensor] = Non
     y = _linear_rows(x2, pw.qweight, pw.scales, pw.codebook, bias, pw.spec.fmt_id, pw.N, pw.K, pw.spec.group_size,
                      pw.spec.had_block, out_id)
     return y if flat else y.reshape(*x.shape[:-1], pw.N)
+
+
+class TokenLogprobs(NamedTuple):
+    """What ``token_logprobs`` returns; the leading dims are those of the logits."""
+    logprob: torch.Tensor                 # fp32 [...]: of the given tokens
+    entropy: torch.Tensor                 # fp32 [...], in nats
+    top_logprobs: torch.Tensor            # fp32 [..., top], falling
+    top_tokens: torch.Tensor              # int64 [..., top]
+
+
+def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0) -> TokenLogprobs:
+    """Log probabilities of ``tokens`` (int64 [...]) under ``logits`` ([..., vocab]; fp32, fp16 or bf16, any row stride), the
+    entropy of every row and its ``top`` (up to 32) strongest tokens, the lowest index first among equals.  One pass
+    over the logits, sums in fp32.  Masked logits may be -inf or the type's lowest value; a row of nothing but -inf has
+    log probabilities -inf and entropy 0, a row with a NaN or +inf has NaN.  A negative token stands for none and gives
+    0, a token that the vocabulary does not have gives NaN.
+
+    Replaces the log-softmax of an evaluation loop's loss (the reference's TestNetwork,
+    Python_Jenks_Test/Jenks_Tests/QuantNetworkTest.py:227-243)."""
+    if logits.dim() < 1 or logits.shape[-1] == 0:
+        raise RuntimeError("logits have at least one token")
+    vocab, lead = logits.shape[-1], logits.shape[:-1]
+    if logits.dtype not in _DT:
+        raise RuntimeError(f"unsupported logits dtype {logits.dtype}")
+    if tokens.shape != lead or tokens.dtype != torch.int64:
+        raise RuntimeError(f"tokens {tuple(tokens.shape)} {tokens.dtype}: int64 of the logits' leading dims {tuple(lead)}")
+    if not 0 <= top <= 32 or top > vocab:
+        raise RuntimeError(f"top is {top}: 0 to 32 of the {vocab} tokens")
+    _need_cuda(logits, tokens)
+    if tokens.device != logits.device:
+        raise RuntimeError(f"tokens are on {tokens.device}, logits on {logits.device}")
+    if logits.is_neg():
+        logits = logits.resolve_neg()
+    x = logits if logits.dim() == 2 else logits.reshape(-1, vocab)
+    if x.stride(1) != 1 and vocab > 1:
+        x = x.contiguous()
+    if not tokens.is_contiguous():
+        tokens = tokens.contiguous()
+    lib = _lib.load()
+    rows, device = x.shape[0], x.device
+    f = torch.empty(rows * (2 + top), dtype=torch.float32, device=device)
+    logprob, entropy, tops = f[:rows], f[rows:2 * rows], f[2 * rows:]
+    top_tokens = torch.empty((rows, top), dtype=torch.int64, device=device)
+    with _on(device):
+        need = lib.jq_token_logprobs_workspace_bytes(rows, vocab)
+        own, at, size = _parts_workspace(device, need) if need else (None, None, 0)
+        st = lib.jq_token_logprobs(x.data_ptr(), x.stride(0), rows, vocab, _DT[x.dtype], tokens.data_ptr(), logprob.data_ptr(),
+                                   entropy.data_ptr(), top, tops.data_ptr() if top else None,
+                                   top_tokens.data_ptr() if top else None, at, size, _stream())
+        del own
+    if st:
+        _lib.check(st, "jq_token_logprobs")
+    return TokenLogprobs(logprob.view(lead), entropy.view(lead), tops.view(*lead, top), top_tokens.view(*lead, top))
 
 
 class GroupedGemv:

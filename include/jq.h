@@ -325,6 +325,80 @@ size_t jq_pack_gf4_workspace_bytes_rows(int N, int K);
 int jq_pack_gf4(const float *W, int N, int K, int g, void *qweight, void *scales_or_null,
                 void *codebook, void *workspace, size_t workspace_bytes, jq_stream_t stream);
 
+/* ---- the key/value cache of 8 bits and attention over it ----
+ * What stands between the packed q/k/v and o projections of a decode step; the reference has no attention (its models are
+ * the vision networks and the MLP of Python_Jenks_Test/Jenks_Tests/QuantNetworkTest.py).
+ * The pool holds `blocks` blocks of block_size tokens (16, 32, 64 or 128).  keys and values are uint8
+ * [blocks, kv_heads, block_size * head_dim], 16-byte aligned, head_dim a multiple of 32 up to 256; a block and head has one fp32 scale
+ * for its keys and one for its values ([blocks, kv_heads]), always positive.  A code stands for value(code) * scale,
+ *   JQ_KV_INT8: value = code - 128, -127 .. 127;   JQ_KV_E4M3: value of the e4m3 number, -448 .. 448 and never NaN.
+ * Codes lie in the order in which a warp's matrix instructions read them: groups of 16 tokens (16 * head_dim bytes), in a
+ * group chunks of 32 values (512 bytes), in a chunk 32 places (g, t), g = 0..7, t = 0..3, of 16 bytes at (4 g + t) * 16:
+ *   keys:   values 8t .. 8t+7 of token k, then of token k + 2, k = 4 (g / 2) + g % 2;
+ *   values: tokens 4t .. 4t+3 of value g, then of g + 8, g + 16, g + 24. */
+#define JQ_KV_INT8 0
+#define JQ_KV_E4M3 1
+typedef struct jq_kv_cache {
+    void *keys, *values;
+    float *key_scales, *value_scales;
+    int32_t blocks, kv_heads, head_dim, block_size, fmt;
+    int32_t reserved;      /* must be 0 */
+} jq_kv_cache;
+/* The sequences of a call.  The arrays are on the device and the host does not look at them: token t of sequence i lies in block
+ * table[i * table_stride + t / block_size]; the sequence holds lengths[i] tokens (at most table_width * block_size are
+ * looked at), of which the last n are new: the rows starts[i] .. starts[i + 1] - 1 of the call's tensors, or, where starts
+ * is NULL, rows i n .. (i + 1) n - 1 with n = tokens / sequences.  max_new: no sequence has more new tokens
+ * (0: not known); it only sizes launches, and new tokens beyond it may be left out.  A table entry that names no block of the pool
+ * is not followed: what would lie there is neither read (it counts as masked) nor written.  So is a sequence whose starts name no
+ * rows of the call (a < 0, b > tokens, b <= a): it has no new tokens. */
+typedef struct jq_kv_batch {
+    const int32_t *table, *lengths, *starts;
+    int32_t sequences, table_width, table_stride, tokens, max_new;
+    int32_t reserved;      /* must be 0 */
+} jq_kv_batch;
+
+/* Quantises the new tokens' keys and values, [tokens, kv_heads, head_dim] of dtype (F32, F16 or BF16; stride_k and stride_v: elements
+ * between tokens and between heads, the values of a head are adjacent), into their places.  For a block that holds m of its
+ * sequence's tokens already, with top = 127 or 448:
+ *   a = max |x| over the block's new tokens and the head's values, infinities and NaN left out, at least 2^-60;
+ *   scale' = max(m ? scale : 0, a / top);
+ *   codes that are there, where scale' > scale: round(value(code) * scale / scale'); new: round(x / scale'),
+ * fp32 quotients rounded to the nearest code, ties to even; an infinity becomes the largest code, NaN becomes 0.  What a block holds
+ * beyond the sequence's end is not defined.  A block takes new tokens of one sequence in a call.  One launch. */
+int jq_kv_append(const jq_kv_cache *cache, const jq_kv_batch *batch, const void *k, const void *v, const int64_t *stride_k,
+                 const int64_t *stride_v, int dtype, jq_stream_t stream);
+/* The last `last` tokens of every sequence as value(code) * scale, [sequences, last, kv_heads, head_dim] of dtype, 16-byte
+ * aligned; 0 before a sequence's first token. */
+int jq_kv_read(const jq_kv_cache *cache, const jq_kv_batch *batch, int last, void *k, void *v, int dtype, jq_stream_t stream);
+/* Causal attention of the new tokens' queries over the cache, their own keys and values among it (append them first): a query at
+ * position p = length - n + j sees the keys max(0, p - window + 1) .. p (window 0: 0 .. p),
+ *   out = sum softmax(scale * q.k) v,   lse = ln sum exp(scale * q.k)   (fp32 [tokens, q_heads], or NULL);
+ * a query that sees nothing gets 0 and -infinity.  q is [tokens, q_heads, head_dim] F16 or BF16 (strides as above), out the same shape,
+ * contiguous and 16-byte aligned; query head h reads key head h / (q_heads / kv_heads).  head_dim 64 or 128.  scale > 0.
+ * A row of q is brought into fp16's range by a power of two and rounded to fp16 (exact for F16, and for BF16 except
+ * values 2^-29 of the row's largest and less); codes are exact in fp16; weights relative to the row's largest are rounded to fp16
+ * for the second product; scores, maxima and sums are fp32.  The split of a long cache over CTAs is by its length and
+ * the device alone and the parts are added in their order: results repeat bit for bit.
+ * workspace: jq_kv_attend_workspace_bytes, 128-byte aligned, zero before its first use, one per stream.  Its first int is a status word
+ * like that of jq_gemm_ta's workspace (jq_ta_status reads it).  Allocates nothing; may be captured in a graph. */
+size_t jq_kv_attend_workspace_bytes(const jq_kv_cache *cache, const jq_kv_batch *batch, int q_heads);
+int jq_kv_attend(const jq_kv_cache *cache, const jq_kv_batch *batch, const void *q, const int64_t *stride_q, int q_heads,
+                 float scale, int window, void *out, float *lse_or_null, int dtype, void *workspace,
+                 size_t workspace_bytes, jq_stream_t stream);
+
+/* Rows of logits [rows, vocab] of dtype, row_stride elements apart: for each row the log probability of its token, the entropy
+ * (NULL: none) and the `top` (0 to 32) strongest tokens in falling order, the lowest index first among equals, with
+ * their log probabilities.  One pass over the row, sums in fp32.  Masked logits may be -infinity or the type's lowest value; a row
+ * that has nothing else than -infinity has log probabilities -infinity and entropy 0; a row with a NaN or +infinity has
+ * NaN.  A token below 0 stands for none (0 is stored), one at vocab or above gives NaN.  workspace (128-byte aligned, zero
+ * before its first use, one per stream; jq_token_logprobs_workspace_bytes, which may be 0) may be the one of
+ * jq_kv_attend.  The reference's counterpart is the loss of its evaluation loop
+ * (Python_Jenks_Test/Jenks_Tests/QuantNetworkTest.py:227-243). */
+size_t jq_token_logprobs_workspace_bytes(int rows, int vocab);
+int jq_token_logprobs(const void *logits, int64_t row_stride, int rows, int vocab, int dtype, const int64_t *tokens,
+                      float *logprob, float *entropy_or_null, int top, float *top_logprob_or_null,
+                      int64_t *top_token_or_null, void *workspace, size_t workspace_bytes, jq_stream_t stream);
+
 /* ---- host-side packers (CPU, multi-threaded; one-off, not the hot path) ----
  * Replace the grid/scale construction of QuantLinear.__init__
  * (Quantization_Experiments/layers.py:22-26) for the packed formats.  All
