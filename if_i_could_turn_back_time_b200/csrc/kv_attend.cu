@@ -1,5 +1,5 @@
 // Attention over the 8-bit cache, few query rows per key head (single tokens, drafts).
-#include "kv.cuh"
+#include "kv_attend.cuh"
 
 namespace jqkv {
 
@@ -8,31 +8,6 @@ using namespace jqta;
 constexpr int kWarps = 4;          // of a CTA; each takes every fourth stage of a segment
 constexpr int kUnit = 64;          // keys: what work is dealt out in
 
-struct AttendArgs {
-    Batch b;
-    const void *q;
-    void *out;
-    float *lse;
-    long long st, sh;              // elements of q between tokens and heads
-    const uint8_t *keys, *values;
-    const float *ks, *vs;
-    int H, G, window, dtype, least;   // least: units that a CTA takes at least
-    float scale;                   // of the scores, times log2(e)
-    int *status;
-    int *counters;                 // one per CTA: parts of the pair that begins in it and is done elsewhere too
-    float *parts;                  // two per CTA: [rows][D] sums, [rows] maxima, [rows] weights
-};
-
-__device__ __forceinline__ float ex2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-__device__ __forceinline__ uint32_t pack_h2(float lo, float hi) {
-    uint32_t r;
-    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
-    return r;
-}
 __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
@@ -434,17 +409,9 @@ __global__ void __launch_bounds__(kWarps * 32) attend_kernel(const __grid_consta
         float *part = p.parts + (size_t)(2 * blockIdx.x + (u0 == 0 ? 1 : 0)) * kPart;
         auto finish = [&](int r, int d, float4 v, float m, float lsum) {      // outputs of four values of a row
             const int j = (r0 + r) / p.G, hq = h * p.G + (r0 + r) % p.G;
-            const float inv = lsum > 0.f ? 1.f / lsum : (lsum == 0.f ? 0.f : lsum);
             const size_t at = ((size_t)(sh.row0 + j) * p.H * p.G + hq) * D + d;
-            const float a = v.x * inv, b = v.y * inv, c = v.z * inv, e = v.w * inv;
-            if (p.dtype == JQ_F16) {
-                *reinterpret_cast<uint2 *>(reinterpret_cast<__half *>(p.out) + at) = make_uint2(pack_h2(a, b), pack_h2(c, e));
-            } else {
-                const __nv_bfloat162 x = __floats2bfloat162_rn(a, b), y = __floats2bfloat162_rn(c, e);
-                *reinterpret_cast<uint2 *>(reinterpret_cast<__nv_bfloat16 *>(p.out) + at) =
-                    make_uint2(*reinterpret_cast<const uint32_t *>(&x), *reinterpret_cast<const uint32_t *>(&y));
-            }
-            if (d == 0 && p.lse) p.lse[(size_t)(sh.row0 + j) * p.H * p.G + hq] = lsum > 0.f ? (m + log2f(lsum)) * kLn2 : (lsum == 0.f ? -INFINITY : lsum);
+            store4(p, at, v, inverse(lsum));
+            if (d == 0 && p.lse) p.lse[at / D] = lse_of(m, lsum);
         };
         for (int e = tid; e < rows * (D / 4); e += kWarps * 32) {
             const int r = e / (D / 4), d = e % (D / 4) * 4;
@@ -489,14 +456,8 @@ __global__ void __launch_bounds__(kWarps * 32) attend_kernel(const __grid_consta
                     float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
                     for (int w = w0; w <= w1; ++w) {
                         const float *x = p.parts + (size_t)(2 * w + (w == w0 ? 1 : 0)) * kPart;
-                        const float mw = __ldcg(x + TR * D + r);
-                        const float4 y = __ldcg(reinterpret_cast<const float4 *>(x + (size_t)r * D + d));
-                        const float lw = __ldcg(x + TR * D + TR + r);
-                        const float top = fmaxf(m, mw), ref = top == -INFINITY ? 0.f : top;
-                        const float a = ex2(m - ref), b = ex2(mw - ref);
-                        v.x = fmaf(v.x, a, y.x * b); v.y = fmaf(v.y, a, y.y * b); v.z = fmaf(v.z, a, y.z * b); v.w = fmaf(v.w, a, y.w * b);
-                        lsum = fmaf(lsum, a, lw * b);
-                        m = top;
+                        add_part(m, lsum, v, __ldcg(x + TR * D + r), __ldcg(x + TR * D + TR + r),
+                                 __ldcg(reinterpret_cast<const float4 *>(x + (size_t)r * D + d)));
                     }
                     finish(r, d, v, m, lsum);
                 }
@@ -513,6 +474,7 @@ __global__ void __launch_bounds__(kWarps * 32) attend_kernel(const __grid_consta
 }
 
 constexpr int kSmem = kWarps * 24576;
+constexpr int kFewRows = 32;       // query rows of a key head up to which attend_kernel is used
 
 static int grid_of() { return 2 * jq_sm_count() < kJqCounters ? 2 * jq_sm_count() : kJqCounters; }
 
@@ -533,8 +495,8 @@ using namespace jqkv;
 
 extern "C" size_t jq_kv_attend_workspace_bytes(const jq_kv_cache *c, const jq_kv_batch *s, int q_heads) {
     if (check_cache(c, s) || q_heads <= 0) return 0;
-    const size_t grid = (size_t)grid_of();
-    return kJqData + 2 * grid * (32 * (size_t)c->head_dim + 64) * 4;
+    if ((long long)most_new(s) * (q_heads / c->kv_heads) > kFewRows) return kJqData + prompt_workspace(c->head_dim);
+    return kJqData + 2 * (size_t)grid_of() * (32 * (size_t)c->head_dim + 64) * 4;
 }
 
 extern "C" int jq_kv_attend(const jq_kv_cache *c, const jq_kv_batch *s, const void *q, const int64_t *stride_q, int q_heads,
@@ -560,14 +522,18 @@ extern "C" int jq_kv_attend(const jq_kv_cache *c, const jq_kv_batch *s, const vo
     a.H = c->kv_heads; a.G = q_heads / c->kv_heads; a.window = window; a.dtype = dtype;
     a.scale = scale * kLog2e;
     a.least = 2;
-    const int grid = grid_of();
     unsigned char *ws = reinterpret_cast<unsigned char *>(workspace);
     a.status = reinterpret_cast<int *>(ws);
     a.counters = reinterpret_cast<int *>(ws + kJqHeader);
     a.parts = reinterpret_cast<float *>(ws + kJqData);
     const long long rows = (long long)most_new(s) * a.G;
+    const int grid = grid_of();
     const int tile = rows <= 8 ? 8 : (rows <= 16 ? 16 : 32);
     const bool e4m3 = c->fmt == JQ_KV_E4M3;
+    if (rows > kFewRows) {
+        a.least = 8;
+        return prompt_launch(a, c->head_dim, e4m3, reinterpret_cast<cudaStream_t>(stream));
+    }
     const attend_fn kern = c->head_dim == 64 ? pick<64>(e4m3, tile) : pick<128>(e4m3, tile);
     static jq_contexts done[2][2][3];
     JQ_CUDA_TRY(jq_allow_smem(reinterpret_cast<const void *>(kern), kSmem, done[c->head_dim == 128][e4m3][tile == 8 ? 0 : tile / 16]));
