@@ -508,6 +508,7 @@ extern "C" int jq_kv_attend(const jq_kv_cache *c, const jq_kv_batch *s, const vo
     if (q_heads <= 0 || q_heads % c->kv_heads || window < 0 || !(scale > 0.f) || scale > 3e38f) return JQ_ERR_BAD_SHAPE;
     if (c->head_dim != 64 && c->head_dim != 128) return JQ_ERR_UNSUPPORTED;
     if (s->sequences == 0 || s->tokens == 0) return JQ_OK;
+    if ((long long)most_new(s) * (q_heads / c->kv_heads) > (1 << 30)) return JQ_ERR_BAD_SHAPE;
     if (!q || !out || !stride_q || !workspace) return JQ_ERR_NULL_PTR;
     if ((reinterpret_cast<uintptr_t>(q) & 1u) || !jq_aligned16(out) || (reinterpret_cast<uintptr_t>(lse_or_null) & 3u) ||
         (reinterpret_cast<uintptr_t>(workspace) & 127u))

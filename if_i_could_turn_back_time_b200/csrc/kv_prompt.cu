@@ -1,7 +1,7 @@
 // Attention over the 8-bit cache, many query rows per key head (prompts and parts of prompts): tcgen05.
 //
 // A CTA has 256 rows (query, head of the group) of a key head as two tiles of 128 and walks along the keys in tiles of
-// 64.  Four warps turn a tile's codes into fp16 operands in shared memory, once for both row tiles; one warp issues S = Q K^T and O += P V
+// 64.  Four warps turn a tile's codes into fp16 operands in shared memory, once for both row tiles; a warp for each row tile issues S = Q K^T and O += P V
 // (M = 128, N = 64 and N = D, accumulators in tensor memory); four warps for each row tile, a thread per row, turn
 // scores into weights, which go back to tensor memory as the A operand of the second product.  Block scales never touch the
 // operands: a key block's scale multiplies its columns of S in fp32, a value block's goes into the exponent,
@@ -15,9 +15,10 @@ using namespace jqta;
 
 namespace prompt {
 
-constexpr int kThreads = 512;      // warps 0-3 and 4-7: the two row tiles, 8-11: codes to operands, 12: matrix instructions
+constexpr int kThreads = 768;      // warps 0-15: weights, 16-19: codes to operands, 20 and 21: matrix instructions, 22: segments
 constexpr int kRows = kPromptRows, kKeys = 64;
 constexpr int kStages = 4;         // of the rings of key and value operands
+constexpr int kSegments = 32;      // planned at once
 constexpr int kScaleSlots = 8;     // tiles whose scales are kept: at most five are in use (four operands ahead of the scores)
 constexpr int kQTmem = 64;         // values of a query row in tensor memory; the others, at D = 128, lie in shared memory
 
@@ -41,17 +42,31 @@ __device__ __forceinline__ void mma_f16_ss(uint32_t elected, uint32_t d_tmem, ui
                  ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(elected) : "memory");
 }
 
-// (s0, s1) * f + add + shift, two values at once, rounded after each step
-__device__ __forceinline__ float2 exponents(uint32_t s0, uint32_t s1, float f, float add, float shift) {
-    float2 r;
-    asm("{ .reg .b64 s, f, a, t; mov.b64 s, {%2, %3}; mov.b64 f, {%4, %4}; mov.b64 a, {%5, %5}; mov.b64 t, {%6, %6};\n"
-        "  fma.rn.f32x2 s, s, f, a; add.rn.f32x2 s, s, t; mov.b64 {%0, %1}, s; }"
-        : "=f"(r.x), "=f"(r.y) : "r"(s0), "r"(s1), "f"(f), "f"(add), "f"(shift));
+// Two fp32 values in a register pair
+__device__ __forceinline__ uint64_t pair2(float a, float b) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
     return r;
 }
-__device__ __forceinline__ void add2(float2 &a, float2 b) {
-    asm("{ .reg .b64 x, y; mov.b64 x, {%0, %1}; mov.b64 y, {%2, %3}; add.rn.f32x2 x, x, y; mov.b64 {%0, %1}, x; }"
-        : "+f"(a.x), "+f"(a.y) : "f"(b.x), "f"(b.y));
+__device__ __forceinline__ uint64_t pair2(uint32_t a, uint32_t b) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "r"(a), "r"(b));
+    return r;
+}
+__device__ __forceinline__ float2 unpair2(uint64_t x) {
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(x));
+    return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
 }
 
 // Keys that the rows of a tile see, rounded down to a unit at their beginning.
@@ -100,18 +115,27 @@ struct Walk {
         cur += u1 - u0;
         return true;
     }
-    __device__ __forceinline__ int rows(const AttendArgs &p) const { return (int)min((long long)kRows, (long long)n * p.G - (long long)tile * kRows); }
-    __device__ __forceinline__ int key0() const { return range.lo + u0 * kKeys; }
+};
+
+// A segment, as the planning warp hands it to the others.
+struct Segment {
+    int tiles, key0, hi;           // key tiles, first key, end of the keys that its rows see
+    int seq, head, row0, n, len;   // row0, n: the sequence's rows of the call's tensors
+    int flat0, rows;               // first of the rows (query, head of the group) among the sequence's, and how many
+    int all, w0, w1, slot;         // the whole of a pair, or a part: CTAs that have one, and the place of this one's
 };
 
 template <int D, bool E4M3>
 __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_constant__ AttendArgs p) {
     using S = Shape<D>;
+    constexpr int H = D / 2;                                 // values of a row that a thread loads, scales and stores
     extern __shared__ __align__(128) unsigned char smem[];
-    __shared__ __align__(8) uint64_t bars[4 * kStages + 2 * 5 + kScaleSlots];
-    __shared__ float s_scales[kScaleSlots][4][4];            // [.][group]: factor of the scores (negative: not there), log2(vs), 1 / vs
+    __shared__ __align__(8) uint64_t bars[4 * kStages + 2 * 5];
+    __shared__ __align__(16) float s_scales[kScaleSlots][4][4];    // [.][group]: factor of the scores (negative: not there), log2(vs), 1 / vs
+    __shared__ float s_top[2][2][kRows];                     // [parity][half][row]
+    __shared__ Segment s_seg[kSegments];
     __shared__ long long s_sum[8], s_at;
-    __shared__ int s_err, s_seq, s_tile, s_last;
+    __shared__ int s_err, s_seq, s_tile, s_last, s_count;
     __shared__ uint32_t s_tmem;
 
     const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
@@ -125,7 +149,6 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
     auto sfree = [&](int w) { return b0 + 8 * (4 * kStages + 4 + w); };
     auto pfull = [&](int w) { return b0 + 8 * (4 * kStages + 6 + w); };
     auto odone = [&](int w) { return b0 + 8 * (4 * kStages + 8 + w); };
-    auto scales_full = [&](int s) { return b0 + 8 * (4 * kStages + 10 + s); };
 
     // ---- this CTA's units: a group of threads for each sequence, tiles in turn over its threads
     const int spread = p.b.S >= 256 ? 1 : 256 / p.b.S, per = (p.b.S + 255) / 256;
@@ -167,17 +190,16 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
         for (int s = 0; s < kStages; ++s) {
             mbar_init(kfull(s), 4);
             mbar_init(vfull(s), 4);
-            mbar_init(kfree(s), 1);
-            mbar_init(vfree(s), 1);
+            mbar_init(kfree(s), 2);
+            mbar_init(vfree(s), 2);
         }
         for (int w = 0; w < 2; ++w) {
-            mbar_init(qfull(w), 4);
+            mbar_init(qfull(w), 8);
             mbar_init(sfull(w), 1);
-            mbar_init(sfree(w), 4);
-            mbar_init(pfull(w), 4);
+            mbar_init(sfree(w), 8);
+            mbar_init(pfull(w), 8);
             mbar_init(odone(w), 1);
         }
-        for (int s = 0; s < kScaleSlots; ++s) mbar_init(scales_full(s), 4);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         fence_async_smem();
     }
@@ -191,17 +213,15 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
     const long long fit = (total + p.least - 1) / p.least;
     const int W = fit < (long long)gridDim.x ? (int)fit : (int)gridDim.x;
     if ((int)blockIdx.x >= W) return;
-    Walk walk;
-    walk.cur = total * blockIdx.x / W;
-    walk.end = total * (blockIdx.x + 1) / W;
-    if (tid < 256 && walk.cur >= before && walk.cur < before + mine) {
+    const long long cur = total * blockIdx.x / W;
+    if (tid < 256 && cur >= before && cur < before + mine) {
         long long at = before;
         for (int i = 0; i < my_seqs; ++i) {
             int row0;
             const int n = p.b.count(my_seq + i, row0), len = p.b.length(my_seq + i), tiles = tiles_of(p, n);
             for (int t = my_tile; t < min(my_tiles, tiles); ++t) {
                 const long long u = (long long)range_of(p, len, n, t).units * p.H;
-                if (walk.cur >= at && walk.cur < at + u) {
+                if (cur >= at && cur < at + u) {
                     s_seq = my_seq + i;
                     s_tile = t;
                     s_at = at;
@@ -210,7 +230,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
             }
         }
     }
-    if (warp == 12) {
+    if (warp == 20) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&s_tmem)), "r"(512) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
         tc_fence_before();
@@ -218,11 +238,6 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = s_tmem;
-    walk.seq = s_seq;
-    walk.tile = s_tile;
-    walk.at = s_at;
-    walk.sequence(p);
-    walk.range = range_of(p, walk.len, walk.n, walk.tile);
     volatile int *err = &s_err;
     auto wait = [&](uint32_t bar, uint32_t parity) {          // (converged again behind it: what follows is often the whole warp's)
         mbar_wait(bar, parity, err);
@@ -230,71 +245,87 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
     };
     unsigned char *const kring = smem, *const vring = smem + kStages * S::kKBytes, *const qmem = vring + kStages * S::vBytes;
 
-    // Registers: 512 x 128 at launch = 256 x 160 + 128 x 112 + 128 x 80
-    if (warp < 8) {
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 160;");
-        // =============================== scores to weights: a thread per row ===============================
-        const int w = warp >> 2, r = tid & 127;
-        const uint32_t mine_t = tmem + w * kColTile + ((uint32_t)(warp & 3) << 21);      // this warp's 32 lanes of its tile
+    // The next segment, in batches that the planning warp fills.  How often a warp gets to a barrier goes by the segments alone, so that
+    // the barriers are met even after a wait that gave up.
+    int seg = kSegments, segs = kSegments;
+    auto batch_sync = [&]() { asm volatile("bar.sync 10, 736;" ::: "memory"); };
+    auto next_segment = [&]() -> const Segment * {
+        if (seg == segs) {
+            if (segs < kSegments) return nullptr;          // (the last batch is not full)
+            batch_sync();                                  // every warp is done with the batch before
+            batch_sync();                                  // the next one is there
+            segs = s_count;
+            seg = 0;
+            if (segs == 0) return nullptr;
+        }
+        return &s_seg[seg++];
+    };
+    // Registers: 768 x 80 at launch = 512 x 80 + 128 x 96 + 128 x 64
+    if (warp < 16) {
+        // ============ scores to weights: two threads per row, each with 32 of a tile's 64 keys and half of the row's values ============
+        const int w = warp >> 3, half = warp >> 2 & 1, r = (warp & 3) * 32 + lane, row = w * 128 + r;
+        const int pair_bar = 1 + w * 4 + (warp & 3);                                     // the two warps that have the same rows
+        const uint32_t mine_t = tmem + w * kColTile + ((uint32_t)(warp & 3) << 21);      // their 32 lanes of tensor memory
+        auto pair_sync = [&]() { asm volatile("bar.sync %0, 64;" ::"r"(pair_bar) : "memory"); };
         uint32_t it = 0;                                   // tiles of this row tile so far
         int slot = 0;                                      // of the scales
-        uint32_t slot_par = 0;
-        while (walk.next(p)) {
-            const int tiles = walk.u1 - walk.u0, rows = walk.rows(p);
+        while (const Segment *sg = next_segment()) {
+            const int tiles = sg->tiles, rows = sg->rows;
             const bool active = w == 0 || rows > 128;
-            const long long flat = (long long)walk.tile * kRows + w * 128 + r;           // row among the sequence's
-            const bool there = w * 128 + r < rows;
-            const int j = there ? (int)(flat / p.G) : 0, hq = walk.head * p.G + (there ? (int)(flat % p.G) : 0);
-            const int pos = there ? walk.len - walk.n + j : -1;
+            const bool there = row < rows;
+            const int fr = sg->flat0 + (there ? row : 0), j = fr / p.G, hq = sg->head * p.G + fr % p.G;
             float ref = -INFINITY, l = 0.f, qs = 0.f;
             if (active) {
-                // the query row, divided by a power of two that brings it into fp16's range
-                const unsigned short *at = reinterpret_cast<const unsigned short *>(p.q) + (walk.row0 + j) * p.st + hq * p.sh;
-                const bool vec = (reinterpret_cast<uintptr_t>(at) & 15u) == 0;
-                auto load = [&](int c) -> uint4 {
-                    uint4 u = make_uint4(0, 0, 0, 0);
-                    if (there) {
-                        if (vec) {
-                            u = reinterpret_cast<const uint4 *>(at)[c];
-                        } else {
-                            unsigned short *e = reinterpret_cast<unsigned short *>(&u);
+                // half of the query row, divided by a power of two that brings the row into fp16's range
+                // (a row that is not there reads the tile's first; nothing comes of it)
+                const unsigned short *at = reinterpret_cast<const unsigned short *>(p.q) + (sg->row0 + j) * p.st + hq * p.sh + half * H;
+                uint4 raw[H / 8];
+                if ((p.st | p.sh) % 8 == 0 && (reinterpret_cast<uintptr_t>(p.q) & 15u) == 0) {
 #pragma unroll
-                            for (int k = 0; k < 8; ++k) e[k] = at[c * 8 + k];
-                        }
+                    for (int c = 0; c < H / 8; ++c) raw[c] = __ldg(reinterpret_cast<const uint4 *>(at) + c);
+                } else {
+#pragma unroll
+                    for (int c = 0; c < H / 8; ++c) {
+                        uint32_t x[4];
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) x[k] = at[c * 8 + 2 * k] | (uint32_t)at[c * 8 + 2 * k + 1] << 16;
+                        raw[c] = make_uint4(x[0], x[1], x[2], x[3]);
                     }
-                    return u;
-                };
+                }
                 auto value = [&](uint32_t x, int hi_half) -> float {
                     const unsigned short u = (unsigned short)(hi_half ? x >> 16 : x & 0xffffu);
                     return p.dtype == JQ_F16 ? __half2float(__ushort_as_half(u)) : __uint_as_float((uint32_t)u << 16);
                 };
                 float amax = 0.f;
 #pragma unroll
-                for (int c = 0; c < D / 8; ++c) {
-                    const uint4 u = load(c);
-                    const uint32_t x[4] = {u.x, u.y, u.z, u.w};
+                for (int c = 0; c < H / 8; ++c) {
+                    const uint32_t x[4] = {raw[c].x, raw[c].y, raw[c].z, raw[c].w};
 #pragma unroll
                     for (int k = 0; k < 4; ++k) amax = fmaxf(amax, fmaxf(fabsf(value(x[k], 0)), fabsf(value(x[k], 1))));
                 }
+                s_top[1][half][row] = amax;
+                pair_sync();
+                amax = fmaxf(amax, s_top[1][half ^ 1][row]);
+                pair_sync();
                 const int e = act_exponent(amax, false);
                 const float down = __uint_as_float((uint32_t)(127 - e) << 23);
                 qs = __uint_as_float((uint32_t)(127 + e) << 23);
 #pragma unroll
-                for (int c4 = 0; c4 < D / 32; ++c4) {
+                for (int c4 = 0; c4 < H / 32; ++c4) {
                     uint32_t h[16];
 #pragma unroll
                     for (int c = 0; c < 4; ++c) {
-                        const uint4 u = load(c4 * 4 + c);
+                        const uint4 u = raw[c4 * 4 + c];
                         const uint32_t x[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
                         for (int k = 0; k < 4; ++k) h[c * 4 + k] = pack_h2(value(x[k], 0) * down, value(x[k], 1) * down);
                     }
-                    if (c4 * 32 < kQTmem) {
-                        tmem_st16(mine_t + kColQ + c4 * 16, h);
+                    if (D <= kQTmem || half == 0) {
+                        tmem_st16(mine_t + kColQ + half * (H / 2) + c4 * 16, h);
                     } else {
 #pragma unroll
                         for (int c = 0; c < 4; ++c)
-                            *reinterpret_cast<uint4 *>(qmem + w * S::qBytes + ((c4 - kQTmem / 32) * 4 + c) * 2048 + r * 16) =
+                            *reinterpret_cast<uint4 *>(qmem + w * S::qBytes + (c4 * 4 + c) * 2048 + r * 16) =
                                 make_uint4(h[c * 4], h[c * 4 + 1], h[c * 4 + 2], h[c * 4 + 3]);
                     }
                 }
@@ -304,40 +335,41 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
                 __syncwarp();
                 if (lane == 0) mbar_arrive(qfull(w));
             }
-            int key = walk.key0();
-            for (int i = 0; i < tiles; ++i, key += kKeys) {
+            // columns of the thread that its row sees, counted from its first
+            int last = (there ? sg->len - sg->n + j : -1) - sg->key0 - half * 32;
+            for (int i = 0; i < tiles; ++i, last -= kKeys) {
                 if (active) {
-                    wait(scales_full(slot), slot_par);
                     wait(sfull(w), it & 1);
                     tc_fence_after();
-                    uint32_t s[64];
-                    tmem_ld32(mine_t + kColS, *reinterpret_cast<uint32_t(*)[32]>(s));
-                    tmem_ld32(mine_t + kColS + 32, *reinterpret_cast<uint32_t(*)[32]>(s + 32));
+                    uint32_t s[32];
+                    tmem_ld32(mine_t + kColS + half * 32, s);
+                    const float4 sc0 = *reinterpret_cast<const float4 *>(s_scales[slot][half * 2]),
+                                 sc1 = *reinterpret_cast<const float4 *>(s_scales[slot][half * 2 + 1]);
+                    const int first = p.window > 0 ? last - p.window + 1 : 0;
+                    const bool edge = last < 31 || first > 0 || sc0.x < 0.f || sc1.x < 0.f;
                     tmem_wait_ld();
                     tc_fence_before();
                     __syncwarp();
                     if (lane == 0) mbar_arrive(sfree(w));
-                    float4 sc[4];
-#pragma unroll
-                    for (int n = 0; n < 4; ++n) sc[n] = *reinterpret_cast<const float4 *>(s_scales[slot][n]);
-                    const int last = pos - key, first = p.window > 0 ? last - p.window + 1 : -1;     // columns that the row sees
-                    const bool edge = last < kKeys - 1 || first > 0 || sc[0].x < 0.f || sc[1].x < 0.f || sc[2].x < 0.f || sc[3].x < 0.f;
                     if (__any_sync(0xffffffffu, edge)) {
 #pragma unroll
-                        for (int c = 0; c < 64; ++c)
-                            if (c > last || c < first || sc[c >> 4].x < 0.f) s[c] = 0xff800000u;
+                        for (int c = 0; c < 32; ++c)
+                            if (c > last || c < first || (c < 16 ? sc0.x : sc1.x) < 0.f) s[c] = 0xff800000u;
                     }
-                    float top = -INFINITY, f[4];
+                    float m0 = __uint_as_float(s[0]), m1 = __uint_as_float(s[16]);
 #pragma unroll
-                    for (int n = 0; n < 4; ++n) {
-                        float m = __uint_as_float(s[16 * n]);
-#pragma unroll
-                        for (int c = 1; c < 16; ++c) m = fmaxf(m, __uint_as_float(s[16 * n + c]));
-                        f[n] = fabsf(sc[n].x) * qs;
-                        top = fmaxf(top, fmaf(m, f[n], sc[n].y));
+                    for (int c = 1; c < 16; ++c) {
+                        m0 = fmaxf(m0, __uint_as_float(s[c]));
+                        m1 = fmaxf(m1, __uint_as_float(s[16 + c]));
                     }
+                    const float f0 = fabsf(sc0.x) * qs, f1 = fabsf(sc1.x) * qs;
+                    float top = fmaxf(fmaf(m0, f0, sc0.y), fmaf(m1, f1, sc1.y));
+                    float(*const tops)[kRows] = s_top[it & 1];
+                    tops[half][row] = top;
+                    pair_sync();
+                    top = fmaxf(top, tops[half ^ 1][row]);           // (NaN is neither's maximum, and comes back in the sums)
                     if (i == 0) {
-                        ref = top;
+                        ref = fmaxf(top, -INFINITY);
                     } else if (__any_sync(0xffffffffu, top > ref + 8.f)) {
                         const float to = top > ref + 8.f ? top : ref;
                         const float a = to == -INFINITY ? 1.f : ex2(ref - to);
@@ -346,77 +378,89 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
                         wait(odone(w), (it & 1) ^ 1);
                         tc_fence_after();
 #pragma unroll
-                        for (int c = 0; c < D / 32; ++c) {
-                            uint32_t o[32];
-                            tmem_ld32(mine_t + c * 32, o);
+                        for (int c = 0; c < H / 16; ++c) {
+                            uint32_t o[16];
+                            tmem_ld16(mine_t + half * H + c * 16, o);
                             tmem_wait_ld();
 #pragma unroll
-                            for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * a);
-                            tmem_st16(mine_t + c * 32, *reinterpret_cast<uint32_t(*)[16]>(o));
-                            tmem_st16(mine_t + c * 32 + 16, *reinterpret_cast<uint32_t(*)[16]>(o + 16));
+                            for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * a);
+                            tmem_st16(mine_t + half * H + c * 16, o);
                         }
                         tmem_wait_st();
                     }
-                    const float base = ref == -INFINITY ? 0.f : ref;
-                    wait(odone(w), (it & 1) ^ 1);                        // the weights of the tile before have been used
+                    const float base = ref == -INFINITY ? 0.f : -ref;
+                    const uint64_t base2 = pair2(base, base);
+                    // (asked here, needed behind the exponentials: whether the weights of the tile before have been used)
+                    const bool used = mbar_try(odone(w), (it & 1) ^ 1);
                     uint32_t h[16];
 #pragma unroll
-                    for (int n = 0; n < 4; ++n) {
+                    for (int n = 0; n < 2; ++n) {
                         // (the exponent as the maximum was formed, then the difference: both at once would leave the rounding of
                         // a large exponent in the weight)
-                        float2 sum = make_float2(0.f, 0.f);
+                        const float f = n ? f1 : f0, add = n ? sc1.y : sc0.y;
+                        const uint64_t f2 = pair2(f, f), a2 = pair2(add, add);
+                        uint64_t sum = 0;
 #pragma unroll
                         for (int c = 0; c < 16; c += 2) {
-                            const float2 e = exponents(s[16 * n + c], s[16 * n + c + 1], f[n], sc[n].y, -base);
-                            const float2 a = make_float2(ex2(e.x), ex2(e.y));
-                            add2(sum, a);
-                            h[8 * (n & 1) + c / 2] = pack_h2(a.x, a.y);
+                            const float2 e = unpair2(add2(fma2(pair2(s[16 * n + c], s[16 * n + c + 1]), f2, a2), base2));
+                            const float x = ex2(e.x), y = ex2(e.y);
+                            sum = add2(sum, pair2(x, y));
+                            h[8 * n + c / 2] = pack_h2(x, y);
                         }
-                        l = fmaf(sum.x + sum.y, sc[n].z, l);
-                        if (n & 1) tmem_st16(mine_t + kColP + 8 * (n - 1), h);
+                        const float2 sums = unpair2(sum);
+                        l = fmaf(sums.x + sums.y, n ? sc1.z : sc0.z, l);
                     }
+                    if (!__all_sync(0xffffffffu, used)) wait(odone(w), (it & 1) ^ 1);
+                    tc_fence_after();
+                    tmem_st16(mine_t + kColP + half * 16, h);
                     tmem_wait_st();
                     tc_fence_before();
                     __syncwarp();
                     if (lane == 0) mbar_arrive(pfull(w));
                     ++it;
                 }
-                if (++slot == kScaleSlots) { slot = 0; slot_par ^= 1; }
+                if (++slot == kScaleSlots) slot = 0;
             }
             // ---- outputs, or a part of them
-            const bool all = walk.u0 == 0 && walk.u1 == walk.range.units;
-            const long long pair_at = walk.at + (long long)walk.head * walk.range.units, pair_end = pair_at + walk.range.units;
-            const int w0 = all ? 0 : (int)(((pair_at + 1) * W - 1) / total), w1 = all ? 0 : (int)((pair_end * W - 1) / total);
-            float *part = p.parts + (size_t)(2 * blockIdx.x + (walk.u0 == 0 ? 1 : 0)) * S::part;
-            const size_t out_at = ((size_t)(walk.row0 + j) * p.H * p.G + hq) * D;
+            const bool all = sg->all != 0;
+            float *part = p.parts + (size_t)sg->slot * S::part;
             if (active) {
+                pair_sync();
+                s_top[0][half][row] = l;
+                pair_sync();
+                l += s_top[0][half ^ 1][row];
+                pair_sync();
+                const size_t out_at = ((size_t)(sg->row0 + j) * p.H * p.G + hq) * D + half * H;
+                if (there && half == 0) {
+                    if (!all) {
+                        part[kRows * D + row] = ref;
+                        part[kRows * D + kRows + row] = l;
+                    } else if (p.lse) {
+                        p.lse[out_at / D] = lse_of(ref, l);
+                    }
+                }
+                const float inv = inverse(l);
                 wait(odone(w), (it & 1) ^ 1);
                 tc_fence_after();
-                const float inv = inverse(l);
-                if (all && there && p.lse) p.lse[out_at / D] = lse_of(ref, l);
-                if (!all && there) {
-                    part[kRows * D + w * 128 + r] = ref;
-                    part[kRows * D + kRows + w * 128 + r] = l;
-                }
 #pragma unroll
-                for (int c = 0; c < D / 32; ++c) {
-                    uint32_t o[32];
-                    tmem_ld32(mine_t + c * 32, o);
+                for (int c = 0; c < H / 16; ++c) {
+                    uint32_t o[16];
+                    tmem_ld16(mine_t + half * H + c * 16, o);
                     tmem_wait_ld();
                     if (there) {
 #pragma unroll
-                    for (int k = 0; k < 32; k += 8) {
-                        float v[8];
+                        for (int k = 0; k < 16; k += 8) {
+                            float v[8];
 #pragma unroll
-                        for (int x = 0; x < 8; ++x) v[x] = __uint_as_float(o[k + x]);
-                        if (all) {
-                            store8(p, out_at + c * 32 + k, v, inv);
-                        } else {
-                            float4 *dst = reinterpret_cast<float4 *>(part + (size_t)(w * 128 + r) * D + c * 32 + k);
-                            dst[0] = make_float4(v[0], v[1], v[2], v[3]);
-                            dst[1] = make_float4(v[4], v[5], v[6], v[7]);
+                            for (int x = 0; x < 8; ++x) v[x] = __uint_as_float(o[k + x]);
+                            if (all) {
+                                store8(p, out_at + c * 16 + k, v, inv);
+                            } else {
+                                float4 *dst = reinterpret_cast<float4 *>(part + (size_t)row * D + half * H + c * 16 + k);
+                                dst[0] = make_float4(v[0], v[1], v[2], v[3]);
+                                dst[1] = make_float4(v[4], v[5], v[6], v[7]);
+                            }
                         }
-                    }
                     }
                     __syncwarp();
                 }
@@ -424,55 +468,56 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
             }
             if (!all) {
                 // the last of the pair's CTAs to get here adds the parts, in their order
+                const int w0 = sg->w0, w1 = sg->w1;
                 __threadfence();
-                asm volatile("bar.sync 1, 256;" ::: "memory");
+                asm volatile("bar.sync 9, 512;" ::: "memory");
                 if (tid == 0) {
                     const int n = atomicAdd(p.counters + w0, 1);
                     s_last = n == w1 - w0;
                     if (s_last) p.counters[w0] = 0;
                 }
-                asm volatile("bar.sync 1, 256;" ::: "memory");
+                asm volatile("bar.sync 9, 512;" ::: "memory");
                 if (s_last) {
                     __threadfence();
-                    for (int e = tid; e < rows * (D / 4); e += 256) {
-                        const int row = e / (D / 4), d = e % (D / 4) * 4;
+                    for (int e = tid; e < rows * (D / 4); e += 512) {
+                        const int k = e / (D / 4), d = e % (D / 4) * 4;
                         float m = -INFINITY, lsum = 0.f;
                         float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-                        for (int k = w0; k <= w1; ++k) {
-                            const float *x = p.parts + (size_t)(2 * k + (k == w0 ? 1 : 0)) * S::part;
-                            add_part(m, lsum, v, __ldcg(x + kRows * D + row), __ldcg(x + kRows * D + kRows + row),
-                                     __ldcg(reinterpret_cast<const float4 *>(x + (size_t)row * D + d)));
+                        for (int x = w0; x <= w1; ++x) {
+                            const float *y = p.parts + (size_t)(2 * x + (x == w0 ? 1 : 0)) * S::part;
+                            add_part(m, lsum, v, __ldcg(y + kRows * D + k), __ldcg(y + kRows * D + kRows + k),
+                                     __ldcg(reinterpret_cast<const float4 *>(y + (size_t)k * D + d)));
                         }
-                        const long long fr = (long long)walk.tile * kRows + row;
-                        const size_t o = ((size_t)(walk.row0 + fr / p.G) * p.H * p.G + walk.head * p.G + fr % p.G) * D;
+                        const int f = sg->flat0 + k;
+                        const size_t o = ((size_t)(sg->row0 + f / p.G) * p.H * p.G + sg->head * p.G + f % p.G) * D;
                         store4(p, o + d, v, inverse(lsum));
                         if (d == 0 && p.lse) p.lse[o / D] = lse_of(m, lsum);
                     }
                 }
-                asm volatile("bar.sync 1, 256;" ::: "memory");           // (s_last is read before the next segment writes it)
+                asm volatile("bar.sync 9, 512;" ::: "memory");           // (s_last is read before the next segment writes it)
             }
         }
-    } else if (warp < 12) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 112;");
+    } else if (warp < 20) {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 96;");
         // =============================== codes to operands: a warp per 16 keys of a tile ===============================
-        const int cw = warp - 8, g = lane >> 2, t = lane & 3;
+        const int cw = warp - 16, g = lane >> 2, t = lane & 3;
         constexpr int C = D / 32;
         int st = 0, slot = 0;
         uint32_t par = 1;                                  // (the first round finds every stage free)
         const uint32_t none = E4M3 ? 0u : 0x80808080u;     // code of 0
-        while (walk.next(p)) {
-            const int tiles = walk.u1 - walk.u0, key0 = walk.key0() + 16 * cw;
+        while (const Segment *sg = next_segment()) {
+            const int tiles = sg->tiles, key0 = sg->key0 + 16 * cw, hi = sg->hi, head = sg->head, len = sg->len, seq = sg->seq;
             int id = -1;
             float kc = -1.f, vl = 0.f, vi = 1.f;
             auto look_up = [&](int first) {                // lane l: block and scales of tile first + l
                 const int k = key0 + (first + lane) * kKeys;
                 id = -1;
-                if (first + lane < tiles && k < walk.range.hi) id = p.b.block(walk.seq, k);
+                if (first + lane < tiles && k < hi) id = p.b.block(seq, k);
                 kc = -1.f;
                 vl = 0.f;
                 vi = 1.f;
                 if (id >= 0) {
-                    const size_t at = (size_t)id * p.H + walk.head;
+                    const size_t at = (size_t)id * p.H + head;
                     const float v = p.vs[at];
                     kc = p.ks[at] * p.scale;
                     vl = log2f(v);
@@ -483,7 +528,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
             auto load = [&](const uint8_t *codes, int tile, uint4 (&x)[C]) {     // (ids of the 32 tiles that `tile` is one of)
                 const int b = __shfl_sync(0xffffffffu, id, tile & 31);
                 const int k = key0 + tile * kKeys;
-                const uint4 *at = reinterpret_cast<const uint4 *>(codes + (((size_t)max(b, 0) * p.H + walk.head) * p.b.T + k % p.b.T) * D) + lane;
+                const uint4 *at = reinterpret_cast<const uint4 *>(codes + (((size_t)max(b, 0) * p.H + head) * p.b.T + k % p.b.T) * D) + lane;
 #pragma unroll
                 for (int c = 0; c < C; ++c) x[c] = b >= 0 ? __ldg(at + c * 32) : make_uint4(none, none, none, none);
             };
@@ -496,10 +541,8 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
                 if (i + 1 < tiles && ((i + 1) & 31) == 0) look_up(i + 1);
                 wait(kfree(st), par);
                 unsigned char *kd = kring + st * S::kKBytes + t * S::kLbo + (16 * cw + 4 * (g >> 1) + (g & 1)) * 16;
-                if (lane == 0) {
-                    *reinterpret_cast<float4 *>(s_scales[slot][cw]) = make_float4(kc_i, vl_i, vi_i, 0.f);
-                    mbar_arrive(scales_full(slot));
-                }
+                // (in shared memory before the operand is announced: who waits for the scores made of it finds them there)
+                if (lane == 0) *reinterpret_cast<float4 *>(s_scales[slot][cw]) = make_float4(kc_i, vl_i, vi_i, 0.f);
 #pragma unroll
                 for (int c = 0; c < C; ++c) {
                     uint4 a, b;
@@ -518,7 +561,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
                 unsigned char *vd = vring + st * S::vBytes + (2 * cw + (t >> 1)) * S::vLbo + g * 16 + (t & 1) * 8;
                 uint32_t keep = 0xffffffffu;               // e4m3 has a NaN, and places behind the sequence's end may hold anything
                 if (E4M3) {
-                    const int left = walk.len - (key0 + i * kKeys + 4 * t);
+                    const int left = len - (key0 + i * kKeys + 4 * t);
                     keep = left >= 4 ? 0xffffffffu : (left <= 0 ? 0u : (1u << 8 * left) - 1u);
                 }
 #pragma unroll
@@ -540,67 +583,99 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
             }
         }
     } else {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
-        if (warp == 12) {
-        // =============================== matrix instructions ===============================
-        // (the warp runs converged, see mma_f16_ts)
-        const uint32_t elected = elect_one();
-        const uint64_t kdesc = smem_desc(smem_u32(kring), S::kLbo, 128), vdesc = smem_desc(smem_u32(vring), S::vLbo, 128),
-                       qdesc = smem_desc(smem_u32(qmem), 2048, 128);
-        constexpr uint32_t idesc_s = idesc_f16(128, kKeys), idesc_o = idesc_f16(128, D);
-        int ks = 0, vs = 0;
-        uint32_t kpar = 0, vpar = 0, qpar[2] = {0, 0}, it[2] = {0, 0};          // it: scores of the row tile so far
-        auto scores = [&](int w) {
-            wait(sfree(w), (it[w] & 1) ^ 1);
-            tc_fence_after();
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+        if (warp < 22) {
+            // =============================== matrix instructions: a warp for each row tile ===============================
+            // (One warp for both took 1080 clocks for a tile of each, waits and issue one after another, where the tensor core
+            // needs 580.  The warp runs converged, see mma_f16_ts.)
+            const int w = warp - 20;
+            const uint32_t elected = elect_one();
             const uint32_t t0 = tmem + w * kColTile;
-            const uint64_t b = kdesc + (uint64_t)(ks * (S::kKBytes >> 4));
+            const uint64_t kdesc = smem_desc(smem_u32(kring), S::kLbo, 128), vdesc = smem_desc(smem_u32(vring), S::vLbo, 128),
+                           qdesc = smem_desc(smem_u32(qmem + w * S::qBytes), 2048, 128);
+            constexpr uint32_t idesc_s = idesc_f16(128, kKeys), idesc_o = idesc_f16(128, D);
+            int ks = 0, vs = 0;
+            uint32_t kpar = 0, vpar = 0, qpar = 0, spar = 1, opar = 0;
+            auto next_k = [&]() { if (++ks == kStages) { ks = 0; kpar ^= 1; } };
+            auto next_v = [&]() { if (++vs == kStages) { vs = 0; vpar ^= 1; } };
+            auto scores = [&]() {
+                wait(kfull(ks), kpar);
+                wait(sfree(w), spar);
+                spar ^= 1;
+                tc_fence_after();
+                const uint64_t b = kdesc + (uint64_t)(ks * (S::kKBytes >> 4));
 #pragma unroll
-            for (int k = 0; k < D / 16; ++k) {
-                if (k < kQTmem / 16) mma_f16_ts(elected, t0 + kColS, t0 + kColQ + 8 * k, b + (uint64_t)(k * (2 * S::kLbo >> 4)), idesc_s, k > 0);
-                else mma_f16_ss(elected, t0 + kColS, qdesc + (uint64_t)((w * S::qBytes + (k - kQTmem / 16) * 4096) >> 4),
-                                b + (uint64_t)(k * (2 * S::kLbo >> 4)), idesc_s, 1);
-            }
-            mma_commit(elected, sfull(w));
-            ++it[w];
-        };
-        uint32_t ot[2] = {0, 0};                           // outputs of the row tile so far
-        while (walk.next(p)) {
-            const int tiles = walk.u1 - walk.u0, both = walk.rows(p) > 128 ? 2 : 1;
-            for (int w = 0; w < both; ++w) {
-                wait(qfull(w), qpar[w]);
-                qpar[w] ^= 1;
-            }
-            tc_fence_after();
-            auto step = [&](int i, int w) {                // scores of tile i + 1, then outputs of tile i
-                if (i + 1 < tiles) {
-                    if (w == 0) wait(kfull(ks), kpar);
-                    scores(w);
-                    if (w == both - 1) {
-                        mma_commit(elected, kfree(ks));
-                        if (++ks == kStages) { ks = 0; kpar ^= 1; }
-                    }
+                for (int k = 0; k < D / 16; ++k) {
+                    if (k < kQTmem / 16) mma_f16_ts(elected, t0 + kColS, t0 + kColQ + 8 * k, b + (uint64_t)(k * (2 * S::kLbo >> 4)), idesc_s, k > 0);
+                    else mma_f16_ss(elected, t0 + kColS, qdesc + (uint64_t)((k - kQTmem / 16) * (4096 >> 4)),
+                                    b + (uint64_t)(k * (2 * S::kLbo >> 4)), idesc_s, 1);
                 }
-                if (i >= 0) {
-                    if (w == 0) wait(vfull(vs), vpar);
-                    wait(pfull(w), ot[w] & 1);
-                    ++ot[w];
+                mma_commit(elected, sfull(w));
+                mma_commit(elected, kfree(ks));
+                next_k();
+            };
+            while (const Segment *sg = next_segment()) {
+                const int tiles = sg->tiles, rows = sg->rows;
+                if (w == 1 && rows <= 128) {       // the operands are the other tile's alone
+                    for (int i = 0; i < tiles; ++i) {
+                        wait(kfull(ks), kpar);
+                        if (lane == 0) mbar_arrive(kfree(ks));
+                        next_k();
+                        wait(vfull(vs), vpar);
+                        if (lane == 0) mbar_arrive(vfree(vs));
+                        next_v();
+                    }
+                    continue;
+                }
+                wait(qfull(w), qpar);
+                qpar ^= 1;
+                scores();
+                for (int i = 0; i < tiles; ++i) {
+                    if (i + 1 < tiles) scores();
+                    wait(vfull(vs), vpar);
+                    wait(pfull(w), opar);
+                    opar ^= 1;
                     tc_fence_after();
-                    const uint32_t t0 = tmem + w * kColTile;
                     const uint64_t b = vdesc + (uint64_t)(vs * (S::vBytes >> 4));
 #pragma unroll
                     for (int k = 0; k < kKeys / 16; ++k)
                         mma_f16_ts(elected, t0, t0 + kColP + 8 * k, b + (uint64_t)(k * (2 * S::vLbo >> 4)), idesc_o, i > 0 || k > 0);
                     mma_commit(elected, odone(w));
-                    if (w == both - 1) {
-                        mma_commit(elected, vfree(vs));
-                        if (++vs == kStages) { vs = 0; vpar ^= 1; }
-                    }
+                    mma_commit(elected, vfree(vs));
+                    next_v();
                 }
-            };
-            for (int i = -1; i < tiles; ++i)
-                for (int w = 0; w < both; ++w) step(i, w);
-        }
+            }
+        } else if (warp == 22) {
+            // =============================== segments ===============================
+            Walk walk;
+            walk.cur = cur;
+            walk.end = total * (blockIdx.x + 1) / W;
+            walk.seq = s_seq;
+            walk.tile = s_tile;
+            walk.at = s_at;
+            walk.sequence(p);
+            walk.range = range_of(p, walk.len, walk.n, walk.tile);
+            int count;
+            do {
+                batch_sync();
+                for (count = 0; count < kSegments && walk.next(p); ++count) {
+                    if (lane) continue;
+                    Segment &s = s_seg[count];
+                    s.tiles = walk.u1 - walk.u0;
+                    s.key0 = walk.range.lo + walk.u0 * kKeys;
+                    s.hi = walk.range.hi;
+                    s.seq = walk.seq; s.head = walk.head; s.row0 = walk.row0; s.n = walk.n; s.len = walk.len;
+                    s.flat0 = walk.tile * kRows;
+                    s.rows = min(kRows, walk.n * p.G - s.flat0);
+                    s.all = walk.u0 == 0 && walk.u1 == walk.range.units;
+                    const long long pair_at = walk.at + (long long)walk.head * walk.range.units, pair_end = pair_at + walk.range.units;
+                    s.w0 = s.all ? 0 : (int)(((pair_at + 1) * W - 1) / total);
+                    s.w1 = s.all ? 0 : (int)((pair_end * W - 1) / total);
+                    s.slot = 2 * blockIdx.x + (walk.u0 == 0 ? 1 : 0);
+                }
+                if (lane == 0) s_count = count;
+                batch_sync();
+            } while (count == kSegments);
         }
     }
 
@@ -611,7 +686,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
     tc_fence_before();
     __syncthreads();
     if (tid == 0 && s_err) atomicExch(p.status, s_err);
-    if (warp == 12) {
+    if (warp == 20) {
         tc_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
     }
