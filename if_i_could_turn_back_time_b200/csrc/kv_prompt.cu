@@ -19,6 +19,7 @@ constexpr int kThreads = 768;      // warps 0-15: weights, 16-19: codes to opera
 constexpr int kRows = kPromptRows, kKeys = 64;
 constexpr int kStages = 4;         // of the rings of key and value operands
 constexpr int kSegments = 32;      // planned at once
+constexpr int kPairCost = 6;       // what a pair costs besides its key tiles, in units of one: queries, outputs, hand-over
 constexpr int kScaleSlots = 8;     // tiles whose scales are kept: at most five are in use (four operands ahead of the scores)
 constexpr int kQTmem = 64;         // values of a query row in tensor memory; the others, at D = 128, lie in shared memory
 
@@ -42,6 +43,11 @@ __device__ __forceinline__ void mma_f16_ss(uint32_t elected, uint32_t d_tmem, ui
                  ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(elected) : "memory");
 }
 
+__device__ __forceinline__ float max3(float a, uint32_t b, uint32_t c) {
+    float r;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(__uint_as_float(b)), "f"(__uint_as_float(c)));
+    return r;
+}
 // Two fp32 values in a register pair
 __device__ __forceinline__ uint64_t pair2(float a, float b) {
     uint64_t r;
@@ -71,49 +77,70 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
 
 // Keys that the rows of a tile see, rounded down to a unit at their beginning.
 struct Range {
-    int lo, hi, units;
+    int lo, hi, units;             // units: kPairCost and the key tiles
 };
 __device__ __forceinline__ Range range_of(const AttendArgs &p, int len, int n, int tile) {
     const int first = len - n;
-    const int q0 = (int)((long long)tile * kRows / p.G), q1 = (int)min((long long)n - 1, ((long long)(tile + 1) * kRows - 1) / p.G);
+    const int q0 = (int)((uint32_t)tile * kRows / (uint32_t)p.G), q1 = min(n - 1, (int)(((uint32_t)(tile + 1) * kRows - 1) / (uint32_t)p.G));
     Range r;
     r.hi = max(0, min(len, first + q1 + 1));
     r.lo = p.window > 0 ? max(0, first + q0 - p.window + 1) : 0;
     r.lo = min(r.lo, r.hi) & ~(kKeys - 1);
-    r.units = max(1, (r.hi - r.lo + kKeys - 1) / kKeys);
+    r.units = kPairCost + max(1, (r.hi - r.lo + kKeys - 1) / kKeys);
     return r;
 }
-__device__ __forceinline__ int tiles_of(const AttendArgs &p, int n) { return (int)(((long long)n * p.G + kRows - 1) / kRows); }
+// (n * G is at most 2^30 where max_new is what it says; a longer sequence has its first 2^30 rows)
+__device__ __forceinline__ int tiles_of(const AttendArgs &p, int n) { return (int)((min((long long)n * p.G, 1LL << 30) + kRows - 1) / kRows); }
+
+// Whole quotients; most operands have 32 bits, whose division is short.
+__device__ __forceinline__ long long quotient(long long a, long long b) {
+    return ((a | b) >> 32) == 0 ? (long long)((uint32_t)a / (uint32_t)b) : a / b;
+}
+// `total` units dealt to W CTAs: the first `extra` have one more than the others.
+struct Shares {
+    long long base;
+    int extra;
+    __device__ __forceinline__ Shares(long long total, int W) : base(quotient(total, W)), extra((int)(total - base * W)) {}
+    __device__ __forceinline__ long long first(int w) const { return base * w + min(w, extra); }
+    __device__ __forceinline__ int owner(long long unit) const {
+        const long long longer = extra * (base + 1);
+        return unit < longer ? (int)quotient(unit, base + 1) : extra + (int)quotient(unit - longer, base);
+    }
+};
 
 // The segments of a CTA: units in the order (sequence, row tile, key head, unit), cut evenly.
 struct Walk {
     long long cur, end, at;        // at: first unit of (seq, tile)
     int seq, tile, n, len, row0, tiles;
     Range range;
-    // of the segment
-    int head, u0, u1;
+    int head, u0, u1;              // of the segment: key head, key tiles
     __device__ __forceinline__ void sequence(const AttendArgs &p) {
         n = p.b.count(seq, row0);
         len = p.b.length(seq);
         tiles = tiles_of(p, n);
     }
     __device__ __forceinline__ bool next(const AttendArgs &p) {
-        if (cur >= end) return false;
-        while (tiles == 0 || cur >= at + (long long)range.units * p.H) {
-            if (tiles) at += (long long)range.units * p.H;
-            if (++tile >= tiles) {
-                ++seq;
-                tile = 0;
-                sequence(p);
+        while (cur < end) {
+            while (tiles == 0 || cur >= at + (long long)range.units * p.H) {
+                if (tiles) at += (long long)range.units * p.H;
+                if (++tile >= tiles) {
+                    ++seq;
+                    tile = 0;
+                    sequence(p);
+                }
+                if (tiles) range = range_of(p, len, n, tile);
             }
-            if (tiles) range = range_of(p, len, n, tile);
+            const long long in = cur - at;
+            head = (int)quotient(in, range.units);
+            u0 = (int)(in - (long long)head * range.units);
+            u1 = (int)min((long long)range.units, u0 + (end - cur));
+            cur += u1 - u0;
+            // from here on in key tiles: the first units of a pair stand for none
+            u0 = max(0, u0 - kPairCost);
+            u1 -= kPairCost;
+            if (u1 > u0) return true;
         }
-        const long long in = cur - at;
-        head = (int)(in / range.units);
-        u0 = (int)(in % range.units);
-        u1 = (int)min((long long)range.units, u0 + (end - cur));
-        cur += u1 - u0;
-        return true;
+        return false;
     }
 };
 
@@ -210,10 +237,11 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
         total += s_sum[w];
     }
     if (total == 0) return;
-    const long long fit = (total + p.least - 1) / p.least;
+    const long long fit = quotient(total + p.least - 1, p.least);
     const int W = fit < (long long)gridDim.x ? (int)fit : (int)gridDim.x;
     if ((int)blockIdx.x >= W) return;
-    const long long cur = total * blockIdx.x / W;
+    const Shares shares(total, W);
+    const long long cur = shares.first(blockIdx.x);
     if (tid < 256 && cur >= before && cur < before + mine) {
         long long at = before;
         for (int i = 0; i < my_seqs; ++i) {
@@ -337,9 +365,10 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
             }
             // columns of the thread that its row sees, counted from its first
             int last = (there ? sg->len - sg->n + j : -1) - sg->key0 - half * 32;
+            bool ready = false;                            // the next scores are there
             for (int i = 0; i < tiles; ++i, last -= kKeys) {
                 if (active) {
-                    wait(sfull(w), it & 1);
+                    if (!__all_sync(0xffffffffu, ready)) wait(sfull(w), it & 1);
                     tc_fence_after();
                     uint32_t s[32];
                     tmem_ld32(mine_t + kColS + half * 32, s);
@@ -356,11 +385,11 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
                         for (int c = 0; c < 32; ++c)
                             if (c > last || c < first || (c < 16 ? sc0.x : sc1.x) < 0.f) s[c] = 0xff800000u;
                     }
-                    float m0 = __uint_as_float(s[0]), m1 = __uint_as_float(s[16]);
+                    float m0 = fmaxf(__uint_as_float(s[0]), __uint_as_float(s[1])), m1 = fmaxf(__uint_as_float(s[16]), __uint_as_float(s[17]));
 #pragma unroll
-                    for (int c = 1; c < 16; ++c) {
-                        m0 = fmaxf(m0, __uint_as_float(s[c]));
-                        m1 = fmaxf(m1, __uint_as_float(s[16 + c]));
+                    for (int c = 2; c < 16; c += 2) {
+                        m0 = max3(m0, s[c], s[c + 1]);
+                        m1 = max3(m1, s[16 + c], s[17 + c]);
                     }
                     const float f0 = fabsf(sc0.x) * qs, f1 = fabsf(sc1.x) * qs;
                     float top = fmaxf(fmaf(m0, f0, sc0.y), fmaf(m1, f1, sc1.y));
@@ -391,7 +420,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
                     const float base = ref == -INFINITY ? 0.f : -ref;
                     const uint64_t base2 = pair2(base, base);
                     // (asked here, needed behind the exponentials: whether the weights of the tile before have been used)
-                    const bool used = mbar_try(odone(w), (it & 1) ^ 1);
+                    const bool used = mbar_test(odone(w), (it & 1) ^ 1);
                     uint32_t h[16];
 #pragma unroll
                     for (int n = 0; n < 2; ++n) {
@@ -413,6 +442,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
                     if (!__all_sync(0xffffffffu, used)) wait(odone(w), (it & 1) ^ 1);
                     tc_fence_after();
                     tmem_st16(mine_t + kColP + half * 16, h);
+                    ready = mbar_test(sfull(w), (it & 1) ^ 1);
                     tmem_wait_st();
                     tc_fence_before();
                     __syncwarp();
@@ -455,10 +485,10 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
                             for (int x = 0; x < 8; ++x) v[x] = __uint_as_float(o[k + x]);
                             if (all) {
                                 store8(p, out_at + c * 16 + k, v, inv);
-                            } else {
-                                float4 *dst = reinterpret_cast<float4 *>(part + (size_t)row * D + half * H + c * 16 + k);
+                            } else {                       // [four values][row]: a warp's rows are adjacent
+                                float4 *dst = reinterpret_cast<float4 *>(part) + (half * H + c * 16 + k) / 4 * kRows + row;
                                 dst[0] = make_float4(v[0], v[1], v[2], v[3]);
-                                dst[1] = make_float4(v[4], v[5], v[6], v[7]);
+                                dst[kRows] = make_float4(v[4], v[5], v[6], v[7]);
                             }
                         }
                     }
@@ -479,19 +509,34 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
                 asm volatile("bar.sync 9, 512;" ::: "memory");
                 if (s_last) {
                     __threadfence();
-                    for (int e = tid; e < rows * (D / 4); e += 512) {
-                        const int k = e / (D / 4), d = e % (D / 4) * 4;
+                    if (there) {
+                        auto of = [&](int x) { return p.parts + (size_t)(2 * x + (x == w0 ? 1 : 0)) * S::part; };
                         float m = -INFINITY, lsum = 0.f;
-                        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-                        for (int x = w0; x <= w1; ++x) {
-                            const float *y = p.parts + (size_t)(2 * x + (x == w0 ? 1 : 0)) * S::part;
-                            add_part(m, lsum, v, __ldcg(y + kRows * D + k), __ldcg(y + kRows * D + kRows + k),
-                                     __ldcg(reinterpret_cast<const float4 *>(y + (size_t)k * D + d)));
+                        for (int x = w0; x <= w1; ++x) m = fmaxf(m, __ldcg(of(x) + kRows * D + row));
+                        const float base = m == -INFINITY ? 0.f : m;
+                        for (int x = w0; x <= w1; ++x)
+                            lsum = fmaf(__ldcg(of(x) + kRows * D + kRows + row), ex2(__ldcg(of(x) + kRows * D + row) - base), lsum);
+                        const float f = inverse(lsum);
+                        const size_t o = ((size_t)(sg->row0 + j) * p.H * p.G + hq) * D + half * H;
+                        if (half == 0 && p.lse) p.lse[o / D] = lse_of(m, lsum);
+#pragma unroll 1
+                        for (int c = 0; c < H; c += 16) {
+                            float v[16];
+#pragma unroll
+                            for (int k = 0; k < 16; ++k) v[k] = 0.f;
+                            for (int x = w0; x <= w1; ++x) {
+                                const float4 *y = reinterpret_cast<const float4 *>(of(x)) + (half * H + c) / 4 * kRows + row;
+                                const float a = ex2(__ldcg(of(x) + kRows * D + row) - base);
+#pragma unroll
+                                for (int k = 0; k < 4; ++k) {
+                                    const float4 u = __ldcg(y + k * kRows);
+                                    v[4 * k] = fmaf(u.x, a, v[4 * k]); v[4 * k + 1] = fmaf(u.y, a, v[4 * k + 1]);
+                                    v[4 * k + 2] = fmaf(u.z, a, v[4 * k + 2]); v[4 * k + 3] = fmaf(u.w, a, v[4 * k + 3]);
+                                }
+                            }
+#pragma unroll
+                            for (int k = 0; k < 16; k += 8) store8(p, o + c + k, *reinterpret_cast<const float(*)[8]>(v + k), f);
                         }
-                        const int f = sg->flat0 + k;
-                        const size_t o = ((size_t)(sg->row0 + f / p.G) * p.H * p.G + sg->head * p.G + f % p.G) * D;
-                        store4(p, o + d, v, inverse(lsum));
-                        if (d == 0 && p.lse) p.lse[o / D] = lse_of(m, lsum);
                     }
                 }
                 asm volatile("bar.sync 9, 512;" ::: "memory");           // (s_last is read before the next segment writes it)
@@ -649,7 +694,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
             // =============================== segments ===============================
             Walk walk;
             walk.cur = cur;
-            walk.end = total * (blockIdx.x + 1) / W;
+            walk.end = shares.first(blockIdx.x + 1);
             walk.seq = s_seq;
             walk.tile = s_tile;
             walk.at = s_at;
@@ -666,11 +711,11 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
                     s.hi = walk.range.hi;
                     s.seq = walk.seq; s.head = walk.head; s.row0 = walk.row0; s.n = walk.n; s.len = walk.len;
                     s.flat0 = walk.tile * kRows;
-                    s.rows = min(kRows, walk.n * p.G - s.flat0);
-                    s.all = walk.u0 == 0 && walk.u1 == walk.range.units;
+                    s.rows = (int)min((long long)kRows, (long long)walk.n * p.G - s.flat0);
+                    s.all = walk.u0 == 0 && walk.u1 == walk.range.units - kPairCost;
                     const long long pair_at = walk.at + (long long)walk.head * walk.range.units, pair_end = pair_at + walk.range.units;
-                    s.w0 = s.all ? 0 : (int)(((pair_at + 1) * W - 1) / total);
-                    s.w1 = s.all ? 0 : (int)((pair_end * W - 1) / total);
+                    s.w0 = s.all ? 0 : shares.owner(pair_at + kPairCost);
+                    s.w1 = s.all ? 0 : shares.owner(pair_end - 1);
                     s.slot = 2 * blockIdx.x + (walk.u0 == 0 ? 1 : 0);
                 }
                 if (lane == 0) s_count = count;

@@ -25,7 +25,14 @@ __device__ __forceinline__ bool mbar_try(uint32_t bar, uint32_t parity) {
                  : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
     return ok != 0;
 }
-// The same, suspended by the hardware for up to about a microsecond: a waiting warp that polls takes issue slots (some
+// Whether the phase is over, without waiting at all (a try may be held up by the hardware).
+__device__ __forceinline__ bool mbar_test(uint32_t bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile("{ .reg .pred p; mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2; selp.u32 %0, 1, 0, p; }"
+                 : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
+    return ok != 0;
+}
+// A try, suspended by the hardware for up to about a microsecond: a waiting warp that polls takes issue slots (some
 // ten instructions every 50 clocks) from the decode warps beside it.
 __device__ __forceinline__ bool mbar_try_suspended(uint32_t bar, uint32_t parity) {
     uint32_t ok;
