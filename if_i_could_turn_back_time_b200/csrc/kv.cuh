@@ -46,7 +46,7 @@ __device__ __forceinline__ void codes_to_h4(uint32_t w, uint32_t &lo, uint32_t &
 struct Batch {
     const int32_t *table, *lengths, *starts;
     int S, width, table_stride, tokens, each;      // each: new tokens of every sequence where starts is null
-    int T, blocks;
+    int T, shift, blocks;                          // tokens of a block: T = 2^shift
 
     __device__ __forceinline__ int length(int i) const {
         const int n = lengths[i];
@@ -64,7 +64,7 @@ struct Batch {
     }
     // Block of a sequence's position, -1 where the table does not name one of the pool.
     __device__ __forceinline__ int block(int i, int position) const {
-        const int id = table[(size_t)i * table_stride + position / T];
+        const int id = table[(size_t)i * table_stride + (position >> shift)];
         return (unsigned)id < (unsigned)blocks ? id : -1;
     }
 };

@@ -25,7 +25,7 @@ __device__ __forceinline__ Share share_of(const AttendArgs &p, int i) {
     s.len = p.b.length(i);
     const int first = s.len - s.n;
     s.lo = p.window > 0 ? max(0, first - p.window + 1) : 0;
-    s.lo -= s.lo % kUnit;
+    s.lo &= ~(kUnit - 1);
     s.units = max(1, (s.len - s.lo + kUnit - 1) / kUnit);      // (a row that sees nothing has its zeros written too)
     s.tiles = (int)(((long long)s.n * p.G + ROWS - 1) / ROWS);
     s.total = (long long)s.tiles * p.H * s.units;
@@ -149,7 +149,7 @@ __global__ void __launch_bounds__(kWarps * 32) attend_kernel(const __grid_consta
                 mbar_expect_tx(bar, bytes);
                 const bool whole = NG == 1 || (ids[0] >= 0 && ids[NG - 1] >= 0 && p.b.T >= KEYS);
                 if (whole) {
-                    const size_t at = (((size_t)ids[0] * p.H + h) * p.b.T + key % p.b.T) * D;
+                    const size_t at = (((size_t)ids[0] * p.H + h) * p.b.T + (key & (p.b.T - 1))) * D;
                     if (ids[0] >= 0) {
                         bulk_g2s(dst, p.keys + at, KEYS * D, bar);
                         bulk_g2s(dst + KEYS * D, p.values + at, KEYS * D, bar);
@@ -158,7 +158,7 @@ __global__ void __launch_bounds__(kWarps * 32) attend_kernel(const __grid_consta
 #pragma unroll
                     for (int n = 0; n < NG; ++n) {
                         if (ids[n] < 0) continue;
-                        const size_t at = (((size_t)ids[n] * p.H + h) * p.b.T + (key + 16 * n) % p.b.T) * D;
+                        const size_t at = (((size_t)ids[n] * p.H + h) * p.b.T + ((key + 16 * n) & (p.b.T - 1))) * D;
                         bulk_g2s(dst + n * 16 * D, p.keys + at, 16 * D, bar);
                         bulk_g2s(dst + KEYS * D + n * 16 * D, p.values + at, 16 * D, bar);
                     }

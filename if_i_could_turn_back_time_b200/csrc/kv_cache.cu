@@ -55,7 +55,7 @@ __global__ void __launch_bounds__(256) append_kernel(const __grid_constant__ App
     int row0;
     const int n = p.b.count(i, row0), len = p.b.length(i);
     const int first = len - n;
-    const int blk = (first > 0 ? first / BT : 0) + (int)(blockIdx.x % p.touched);
+    const int blk = (first > 0 ? first >> p.b.shift : 0) + (int)(blockIdx.x % p.touched);
     const int t0 = max(first, blk * BT), t1 = min(len, (blk + 1) * BT);
     if (n == 0 || t0 >= t1) return;
     const int id = p.b.block(i, t0);
@@ -154,7 +154,7 @@ __global__ void __launch_bounds__(256) read_kernel(const __grid_constant__ ReadA
     if (base >= p.last) return;
     const int id = group >= 0 ? p.b.block(i, group * 16) : -1;
     const float scale = id >= 0 ? p.scales[what][(size_t)id * p.H + h] : 0.f;
-    const uint4 *at = reinterpret_cast<const uint4 *>(p.codes[what] + (((size_t)max(id, 0) * p.H + h) * p.b.T + (group >= 0 ? group * 16 % p.b.T : 0)) * p.D);
+    const uint4 *at = reinterpret_cast<const uint4 *>(p.codes[what] + (((size_t)max(id, 0) * p.H + h) * p.b.T + (group >= 0 ? group * 16 & (p.b.T - 1) : 0)) * p.D);
     const size_t row = (size_t)p.H * p.D;
     const size_t out0 = (size_t)i * p.last * row + (size_t)h * p.D;
     for (int c = 0; c < p.D / 32; ++c) {
@@ -222,6 +222,7 @@ Batch batch_of(const jq_kv_cache *c, const jq_kv_batch *s) {
     b.S = s->sequences; b.width = s->table_width; b.table_stride = s->table_stride; b.tokens = s->tokens;
     b.each = s->sequences ? s->tokens / s->sequences : 0;
     b.T = c->block_size; b.blocks = c->blocks;
+    while (1 << b.shift < b.T) ++b.shift;
     return b;
 }
 

@@ -418,20 +418,26 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
                         tmem_wait_st();
                     }
                     const float base = ref == -INFINITY ? 0.f : -ref;
-                    const uint64_t base2 = pair2(base, base);
+                    float g0 = f0, g1 = f1, add0 = sc0.y + base, add1 = sc1.y + base;
+                    if (fabsf(base) > 8192.f) {
+                        // exponents so large that the rounding of log2(vs) - ref would show in the weights: formed as the maximum was,
+                        // then the difference
+#pragma unroll
+                        for (int c = 0; c < 32; ++c) s[c] = __float_as_uint(fmaf(__uint_as_float(s[c]), c < 16 ? f0 : f1, c < 16 ? sc0.y : sc1.y));
+                        g0 = g1 = 1.f;
+                        add0 = add1 = base;
+                    }
+                    __syncwarp();
                     // (asked here, needed behind the exponentials: whether the weights of the tile before have been used)
                     const bool used = mbar_test(odone(w), (it & 1) ^ 1);
                     uint32_t h[16];
 #pragma unroll
                     for (int n = 0; n < 2; ++n) {
-                        // (the exponent as the maximum was formed, then the difference: both at once would leave the rounding of
-                        // a large exponent in the weight)
-                        const float f = n ? f1 : f0, add = n ? sc1.y : sc0.y;
-                        const uint64_t f2 = pair2(f, f), a2 = pair2(add, add);
+                        const uint64_t f2 = n ? pair2(g1, g1) : pair2(g0, g0), a2 = n ? pair2(add1, add1) : pair2(add0, add0);
                         uint64_t sum = 0;
 #pragma unroll
                         for (int c = 0; c < 16; c += 2) {
-                            const float2 e = unpair2(add2(fma2(pair2(s[16 * n + c], s[16 * n + c + 1]), f2, a2), base2));
+                            const float2 e = unpair2(fma2(pair2(s[16 * n + c], s[16 * n + c + 1]), f2, a2));
                             const float x = ex2(e.x), y = ex2(e.y);
                             sum = add2(sum, pair2(x, y));
                             h[8 * n + c / 2] = pack_h2(x, y);
@@ -573,7 +579,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
             auto load = [&](const uint8_t *codes, int tile, uint4 (&x)[C]) {     // (ids of the 32 tiles that `tile` is one of)
                 const int b = __shfl_sync(0xffffffffu, id, tile & 31);
                 const int k = key0 + tile * kKeys;
-                const uint4 *at = reinterpret_cast<const uint4 *>(codes + (((size_t)max(b, 0) * p.H + head) * p.b.T + k % p.b.T) * D) + lane;
+                const uint4 *at = reinterpret_cast<const uint4 *>(codes + (((size_t)max(b, 0) * p.H + head) * p.b.T + (k & (p.b.T - 1))) * D) + lane;
 #pragma unroll
                 for (int c = 0; c < C; ++c) x[c] = b >= 0 ? __ldg(at + c * 32) : make_uint4(none, none, none, none);
             };
