@@ -7,10 +7,18 @@ using namespace jqta;
 
 constexpr int kWarps = 4;          // of a CTA; each takes every fourth stage of a segment
 constexpr int kUnit = 64;          // keys: what work is dealt out in
+constexpr int kRing = 16384;       // bytes of a warp's ring: two stages of 32 keys at D = 128, three CTAs on an SM
 
 __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// A matrix of 8 x 8 fp16 values, two of a row in a lane (row lane / 4), the other way round.
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
+    uint32_t r;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
+    return r;
 }
 
 // A sequence's share of the work: row tiles x key heads pairs of `units` units each, pairs in the order (head, tile).
@@ -32,18 +40,19 @@ __device__ __forceinline__ Share share_of(const AttendArgs &p, int i) {
     return s;
 }
 
-// ROWS: 8 (rows 8 to 15 of the matrix instruction's tile are not there), 16 or 32 query rows (query, head of the group) at once.
-template <int D, bool E4M3, int ROWS>
-__global__ void __launch_bounds__(kWarps * 32) attend_kernel(const __grid_constant__ AttendArgs p) {
-    constexpr int MT = ROWS > 16 ? ROWS / 16 : 1;              // tiles of 16 rows
-    constexpr bool TWO = ROWS > 8;                             // rows 8 to 15 are there
+// NT: tiles of 8 query rows (query, head of the group).  Both products have the cache as their 16-row operand, so that 8 query rows cost
+// one instruction for 16 keys x 16 values: S^T = K Q^T, O^T = V^T P^T.  A lane has the scores of the keys (g, 0) and (g, 1) of a
+// group (see kv.cuh) for the rows 2t and 2t + 1; packed to fp16 and transposed by movmatrix they are the second product's B operand.
+template <int D, bool E4M3, int NT>
+__global__ void __launch_bounds__(kWarps * 32, NT == 4 ? 2 : 3) attend_kernel(const __grid_constant__ AttendArgs p) {
     constexpr int C = D / 32;                                  // chunks of a group
-    constexpr int KEYS = D <= 128 ? 32 : 16;                   // keys of a stage
-    constexpr int NG = KEYS / 16;
+    constexpr int KEYS = 32, NG = KEYS / 16;                   // keys and groups of a stage
     constexpr int kStageBytes = KEYS * D * 2;
-    constexpr int NS = 24576 / kStageBytes;                    // stages of a warp's ring: 24 KB, two CTAs on an SM
-    constexpr int TR = MT * 16;                                // rows of a tile
+    constexpr int NS = kRing / kStageBytes;                    // stages of a warp's ring
+    constexpr int TR = NT * 8;                                 // rows of a tile
     constexpr int kPart = TR * D + 2 * TR;                     // floats of a part
+    constexpr int kPitch = D + 4;                              // floats of a row on its way to the other warps: rows 2t, 2t + 2, .. in different banks
+    static_assert(TR * kPitch * 4 <= kRing || NT == 4, "a warp's sums take the place of its ring");
     extern __shared__ __align__(128) unsigned char smem[];
     __shared__ __align__(8) uint64_t bars[kWarps * NS];
     __shared__ int s_err, s_seq, s_last;
@@ -51,7 +60,8 @@ __global__ void __launch_bounds__(kWarps * 32) attend_kernel(const __grid_consta
     __shared__ float s_m[kWarps][TR], s_l[kWarps][TR];
 
     const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31, g = lane >> 2, tq = lane & 3;
-    unsigned char *const ring = smem + warp * 24576;
+    constexpr int kOwn = TR * kPitch * 4 > kRing ? TR * kPitch * 4 : kRing;
+    unsigned char *const ring = smem + warp * kOwn;
     const uint32_t ring_u = smem_u32(ring), bar0 = smem_u32(&bars[warp * NS]);
     if (lane == 0)
         for (int s = 0; s < NS; ++s) mbar_init(bar0 + 8 * s, 1);
@@ -62,7 +72,7 @@ __global__ void __launch_bounds__(kWarps * 32) attend_kernel(const __grid_consta
     // ---- this CTA's units: [lo, hi) of all, the same number for every CTA up to one
     const int per = (p.b.S + kWarps * 32 - 1) / (kWarps * 32), i0 = min(p.b.S, tid * per), i1 = min(p.b.S, i0 + per);
     long long mine = 0;
-    for (int i = i0; i < i1; ++i) mine += share_of<ROWS>(p, i).total;
+    for (int i = i0; i < i1; ++i) mine += share_of<TR>(p, i).total;
     long long before = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -72,20 +82,22 @@ __global__ void __launch_bounds__(kWarps * 32) attend_kernel(const __grid_consta
     if (lane == 31) s_sum[warp] = before;
     __syncthreads();
     long long total = 0;
+#pragma unroll
     for (int w = 0; w < kWarps; ++w) {
         if (w == warp) before += total - mine;
         total += s_sum[w];
     }
     if (total == 0) return;
-    const long long fit = (total + p.least - 1) / p.least;
+    const long long fit = quotient(total + p.least - 1, p.least);
     const int W = fit < (long long)gridDim.x ? (int)fit : (int)gridDim.x;
     if ((int)blockIdx.x >= W) return;
-    long long cur = total * blockIdx.x / W;
-    const long long hi = total * (blockIdx.x + 1) / W;
+    const Shares shares(total, W);
+    long long cur = shares.first(blockIdx.x);
+    const long long hi = shares.first(blockIdx.x + 1);
     if (cur >= before && cur < before + mine) {                // (one thread's sequences hold the first unit)
         long long at = before;
         for (int i = i0; i < i1; ++i) {
-            const long long t = share_of<ROWS>(p, i).total;
+            const long long t = share_of<TR>(p, i).total;
             if (cur < at + t) {
                 s_seq = i;
                 s_off = at;
@@ -97,18 +109,18 @@ __global__ void __launch_bounds__(kWarps * 32) attend_kernel(const __grid_consta
     __syncthreads();
     int seq = s_seq;
     long long seq_at = s_off;
-    Share sh = share_of<ROWS>(p, seq);
+    Share sh = share_of<TR>(p, seq);
 
     uint32_t phases = 0;                                       // parity of each stage's next completion
     while (cur < hi) {
         while (cur >= seq_at + sh.total) {
             seq_at += sh.total;
-            sh = share_of<ROWS>(p, ++seq);
+            sh = share_of<TR>(p, ++seq);
         }
         const long long in_seq = cur - seq_at;
-        const int pair = (int)(in_seq / sh.units), u0 = (int)(in_seq % sh.units);
+        const int pair = (int)quotient(in_seq, sh.units), u0 = (int)(in_seq - (long long)pair * sh.units);
         const int u1 = (int)min((long long)sh.units, u0 + (hi - cur));
-        const int h = pair / sh.tiles, tile = pair % sh.tiles;
+        const int h = sh.tiles == 1 ? pair : pair / sh.tiles, tile = sh.tiles == 1 ? 0 : pair % sh.tiles;
         const int k0 = sh.lo + u0 * kUnit, k1 = min(sh.len, sh.lo + u1 * kUnit);
         const int stages = k1 > k0 ? (k1 - k0 + KEYS - 1) / KEYS : 0;
         const int own = stages > warp ? (stages - warp + kWarps - 1) / kWarps : 0;      // stages of this warp
@@ -147,13 +159,10 @@ __global__ void __launch_bounds__(kWarps * 32) attend_kernel(const __grid_consta
 #pragma unroll
                 for (int n = 0; n < NG; ++n) bytes += ids[n] >= 0 ? 32 * D : 0;
                 mbar_expect_tx(bar, bytes);
-                const bool whole = NG == 1 || (ids[0] >= 0 && ids[NG - 1] >= 0 && p.b.T >= KEYS);
-                if (whole) {
+                if (ids[0] >= 0 && ids[1] >= 0 && p.b.T >= KEYS) {
                     const size_t at = (((size_t)ids[0] * p.H + h) * p.b.T + (key & (p.b.T - 1))) * D;
-                    if (ids[0] >= 0) {
-                        bulk_g2s(dst, p.keys + at, KEYS * D, bar);
-                        bulk_g2s(dst + KEYS * D, p.values + at, KEYS * D, bar);
-                    }
+                    bulk_g2s(dst, p.keys + at, KEYS * D, bar);
+                    bulk_g2s(dst + KEYS * D, p.values + at, KEYS * D, bar);
                 } else {
 #pragma unroll
                     for (int n = 0; n < NG; ++n) {
@@ -166,70 +175,71 @@ __global__ void __launch_bounds__(kWarps * 32) attend_kernel(const __grid_consta
             }
         };
         look_up(0);
+        // ---- queries, row g of each tile as the B operand, divided by a power of two that brings the row into fp16's range
+        uint4 raw[NT][C];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+            const int r = nt * 8 + g, fr = r0 + (r < rows ? r : 0);                    // (a row that is not there reads the tile's first)
+            const unsigned short *at = reinterpret_cast<const unsigned short *>(p.q) + (sh.row0 + fr / p.G) * p.st + (h * p.G + fr % p.G) * p.sh + tq * 8;
+            if ((p.st | p.sh) % 8 == 0 && (reinterpret_cast<uintptr_t>(p.q) & 15u) == 0) {
+#pragma unroll
+                for (int c = 0; c < C; ++c) raw[nt][c] = __ldg(reinterpret_cast<const uint4 *>(at + c * 32));
+            } else {
+#pragma unroll
+                for (int c = 0; c < C; ++c) {
+                    uint32_t x[4];
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) x[k] = at[c * 32 + 2 * k] | (uint32_t)at[c * 32 + 2 * k + 1] << 16;
+                    raw[nt][c] = make_uint4(x[0], x[1], x[2], x[3]);
+                }
+            }
+        }
 #pragma unroll
         for (int s = 0; s < NS; ++s)
             if (s < own) issue(s, s);
         scales();
-
-        // ---- queries: rows as the A operand, each divided by a power of two that brings it into fp16's range
-        uint32_t qa[MT][C][2][4];
-        float qs[MT][2];                                       // what the scores of the lane's rows are multiplied by
-        int pos[MT][2];                                        // positions of its rows; -1: no such row
+        uint32_t qb[NT][C][2][2];
+        float qs[NT][2];                                       // what the scores of the rows 2t and 2t + 1 are multiplied by
+        int pos[NT][2];                                        // their positions; -1: no such row
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt)
+        for (int nt = 0; nt < NT; ++nt) {
+            auto value = [&](uint32_t w, int hi_half) -> float {
+                const unsigned short u = (unsigned short)(hi_half ? w >> 16 : w & 0xffffu);
+                return p.dtype == JQ_F16 ? __half2float(__ushort_as_half(u)) : __uint_as_float((uint32_t)u << 16);
+            };
+            float amax = 0.f;
 #pragma unroll
-            for (int half = 0; half < 2; ++half) {
-                const int r = mt * 16 + half * 8 + g;
-                const bool there = r < rows && (half == 0 || TWO);
-                const int j = (r0 + r) / p.G, hq = h * p.G + (r0 + r) % p.G;
-                pos[mt][half] = there ? sh.len - sh.n + j : -1;
-                float amax = 0.f;
-                uint4 raw[C];
+            for (int c = 0; c < C; ++c) {
+                const uint32_t w[4] = {raw[nt][c].x, raw[nt][c].y, raw[nt][c].z, raw[nt][c].w};
 #pragma unroll
-                for (int c = 0; c < C; ++c) {
-                    raw[c] = make_uint4(0, 0, 0, 0);
-                    if (there) {
-                        const unsigned short *at = reinterpret_cast<const unsigned short *>(p.q) + (sh.row0 + j) * p.st + hq * p.sh + c * 32 + tq * 8;
-                        if ((reinterpret_cast<uintptr_t>(at) & 15u) == 0) {
-                            raw[c] = *reinterpret_cast<const uint4 *>(at);
-                        } else {
-                            unsigned short *e = reinterpret_cast<unsigned short *>(&raw[c]);
-#pragma unroll
-                            for (int k = 0; k < 8; ++k) e[k] = at[k];
-                        }
-                    }
-                }
-                auto value = [&](uint32_t w, int hi_half) -> float {
-                    const unsigned short u = (unsigned short)(hi_half ? w >> 16 : w & 0xffffu);
-                    return p.dtype == JQ_F16 ? __half2float(__ushort_as_half(u)) : __uint_as_float((uint32_t)u << 16);
-                };
-#pragma unroll
-                for (int c = 0; c < C; ++c) {
-                    const uint32_t w[4] = {raw[c].x, raw[c].y, raw[c].z, raw[c].w};
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) amax = fmaxf(amax, fmaxf(fabsf(value(w[k], 0)), fabsf(value(w[k], 1))));
-                }
-                amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
-                amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
-                const int e = act_exponent(amax, false);
-                const float down = __uint_as_float((uint32_t)(127 - e) << 23);
-                qs[mt][half] = __uint_as_float((uint32_t)(127 + e) << 23);
-#pragma unroll
-                for (int c = 0; c < C; ++c) {
-                    const uint32_t w[4] = {raw[c].x, raw[c].y, raw[c].z, raw[c].w};
-#pragma unroll
-                    for (int k = 0; k < 4; ++k)                // word k: values 2k, 2k + 1 = step k / 2, register 0 or 2 (+ half)
-                        qa[mt][c][k >> 1][(k & 1) * 2 + half] = pack_h2(value(w[k], 0) * down, value(w[k], 1) * down);
-                }
+                for (int k = 0; k < 4; ++k) amax = fmaxf(amax, fmaxf(fabsf(value(w[k], 0)), fabsf(value(w[k], 1))));
             }
+            amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+            amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+            const int e = act_exponent(amax, false);
+            const float down = __uint_as_float((uint32_t)(127 - e) << 23);
+#pragma unroll
+            for (int c = 0; c < C; ++c) {
+                const uint32_t w[4] = {raw[nt][c].x, raw[nt][c].y, raw[nt][c].z, raw[nt][c].w};
+#pragma unroll
+                for (int k = 0; k < 4; ++k)                    // word k: values 2k, 2k + 1 = step k / 2, register k % 2
+                    qb[nt][c][k >> 1][k & 1] = pack_h2(value(w[k], 0) * down, value(w[k], 1) * down);
+            }
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                const int r = nt * 8 + 2 * tq + k, ee = __shfl_sync(0xffffffffu, e, (2 * tq + k) * 4);
+                qs[nt][k] = __uint_as_float((uint32_t)(127 + ee) << 23);
+                pos[nt][k] = r < rows ? sh.len - sh.n + (r0 + r) / p.G : -1;
+            }
+        }
 
-        float o[MT][D / 8][4], M[MT][2], l[MT][2];
+        float o[NT][D / 16][4], M[NT][2], l[NT][2];            // o: values 16 i + g and 16 i + g + 8 of the rows 2t, 2t + 1
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt) {
-            M[mt][0] = M[mt][1] = -INFINITY;
-            l[mt][0] = l[mt][1] = 0.f;
+        for (int nt = 0; nt < NT; ++nt) {
+            M[nt][0] = M[nt][1] = -INFINITY;
+            l[nt][0] = l[nt][1] = 0.f;
 #pragma unroll
-            for (int n = 0; n < D / 8; ++n) o[mt][n][0] = o[mt][n][1] = o[mt][n][2] = o[mt][n][3] = 0.f;
+            for (int n = 0; n < D / 16; ++n) o[nt][n][0] = o[nt][n][1] = o[nt][n][2] = o[nt][n][3] = 0.f;
         }
         // the queries' least and largest positions: keys between them and the window's edges are looked at one by one
         const int pos_first = sh.len - sh.n + r0 / p.G, pos_last = sh.len - sh.n + (r0 + rows - 1) / p.G;
@@ -239,8 +249,9 @@ __global__ void __launch_bounds__(kWarps * 32) attend_kernel(const __grid_consta
             const int sl = st & 31;
             const int key = k0 + (warp + st * kWarps) * KEYS;
             mbar_wait(bar0 + 8 * slot, phases >> slot & 1, &s_err);
+            __syncwarp();
             phases ^= 1u << slot;
-            const uint32_t base = ring_u + slot * kStageBytes;
+            const uint32_t base = ring_u + slot * kStageBytes + lane * 16;
             float kcs[NG], vls[NG], vis[NG];
             bool there[NG];
 #pragma unroll
@@ -250,93 +261,77 @@ __global__ void __launch_bounds__(kWarps * 32) attend_kernel(const __grid_consta
                 vis[n] = __shfl_sync(0xffffffffu, vi[n], sl);
                 there[n] = __shfl_sync(0xffffffffu, id[n], sl) >= 0;
             }
-            float s[MT][NG][2][4];
+            float s[NT][NG][4];
 #pragma unroll
-            for (int mt = 0; mt < MT; ++mt)
+            for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                for (int n = 0; n < NG; ++n)
-#pragma unroll
-                    for (int j = 0; j < 2; ++j) s[mt][n][j][0] = s[mt][n][j][1] = s[mt][n][j][2] = s[mt][n][j][3] = 0.f;
+                for (int n = 0; n < NG; ++n) s[nt][n][0] = s[nt][n][1] = s[nt][n][2] = s[nt][n][3] = 0.f;
 #pragma unroll
             for (int c = 0; c < C; ++c)
 #pragma unroll
                 for (int n = 0; n < NG; ++n) {
-                    const uint4 w = lds128(base + n * 16 * D + c * 512 + lane * 16);
-                    uint32_t b[4][2];
-                    codes_to_h4<E4M3>(w.x, b[0][0], b[0][1]);
-                    codes_to_h4<E4M3>(w.y, b[1][0], b[1][1]);
-                    codes_to_h4<E4M3>(w.z, b[2][0], b[2][1]);
-                    codes_to_h4<E4M3>(w.w, b[3][0], b[3][1]);
+                    const uint4 w = lds128(base + n * 16 * D + c * 512);
+                    uint32_t a[2][4];                          // the two steps of 16 values
+                    codes_to_h4<E4M3>(w.x, a[0][0], a[0][2]);
+                    codes_to_h4<E4M3>(w.y, a[1][0], a[1][2]);
+                    codes_to_h4<E4M3>(w.z, a[0][1], a[0][3]);
+                    codes_to_h4<E4M3>(w.w, a[1][1], a[1][3]);
 #pragma unroll
-                    for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-                        for (int j = 0; j < 2; ++j) {
-                            mma16816(s[mt][n][j], qa[mt][c][0], b[2 * j][0], b[2 * j][1]);
-                            mma16816(s[mt][n][j], qa[mt][c][1], b[2 * j + 1][0], b[2 * j + 1][1]);
-                        }
+                    for (int nt = 0; nt < NT; ++nt) {
+                        mma16816(s[nt][n], a[0], qb[nt][c][0][0], qb[nt][c][0][1]);
+                        mma16816(s[nt][n], a[1], qb[nt][c][1][0], qb[nt][c][1][1]);
+                    }
                 }
             // t = log2(weight of the key times its block's value scale); the sums are formed relative to the largest t
             const bool masked = key + KEYS - 1 > pos_first || (p.window > 0 && key <= pos_last - p.window) || !there[0] || !there[NG - 1];
-            uint32_t pa[MT][NG][4];
+            uint32_t pb[NT][NG][2];
 #pragma unroll
-            for (int mt = 0; mt < MT; ++mt) {
-                float alpha[2] = {1.f, 1.f};
+            for (int nt = 0; nt < NT; ++nt) {
+                float alpha[2];
 #pragma unroll
-                for (int half = 0; half < (TWO ? 2 : 1); ++half) {
-                    float m = M[mt][half];
+                for (int k = 0; k < 2; ++k) {                  // row 2t + k; element 2 j + k: key (g, j)
+                    float m = M[nt][k];
 #pragma unroll
                     for (int n = 0; n < NG; ++n) {
-                        const float f = kcs[n] * qs[mt][half];
+                        const float f = kcs[n] * qs[nt][k];
 #pragma unroll
-                        for (int j = 0; j < 2; ++j)
-#pragma unroll
-                            for (int k = 0; k < 2; ++k) {
-                                float &t = s[mt][n][j][half * 2 + k];
-                                t = fmaf(t, f, vls[n]);
-                                if (masked) {
-                                    const int kp = key + n * 16 + 4 * tq + 2 * j + k;
-                                    if (kp > pos[mt][half] || (p.window > 0 && kp <= pos[mt][half] - p.window) || !there[n]) t = -INFINITY;
-                                }
-                                m = fmaxf(m, t);
+                        for (int j = 0; j < 2; ++j) {
+                            float &t = s[nt][n][2 * j + k];
+                            t = fmaf(t, f, vls[n]);
+                            if (masked) {
+                                const int kp = key + n * 16 + 4 * (g >> 1) + (g & 1) + 2 * j;
+                                if (kp > pos[nt][k] || (p.window > 0 && kp <= pos[nt][k] - p.window) || !there[n]) t = -INFINITY;
                             }
+                            m = fmaxf(m, t);
+                        }
                     }
-                    m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
-                    m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
+                    m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 4));
+                    m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
+                    m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
                     const float ref = m == -INFINITY ? 0.f : m;          // (nothing seen yet: every weight is 0)
-                    alpha[half] = ex2(M[mt][half] - ref);
-                    M[mt][half] = m;
+                    alpha[k] = ex2(M[nt][k] - ref);
+                    M[nt][k] = m;
                     float sum = 0.f;
 #pragma unroll
                     for (int n = 0; n < NG; ++n) {
-                        float part = 0.f;
-#pragma unroll
-                        for (int j = 0; j < 2; ++j)
-#pragma unroll
-                            for (int k = 0; k < 2; ++k) {
-                                float &t = s[mt][n][j][half * 2 + k];
-                                t = ex2(t - ref);
-                                part += t;
-                            }
-                        sum = fmaf(part, vis[n], sum);
+                        float &t0 = s[nt][n][k], &t1 = s[nt][n][2 + k];
+                        t0 = ex2(t0 - ref);
+                        t1 = ex2(t1 - ref);
+                        sum = fmaf(t0 + t1, vis[n], sum);
                     }
-                    l[mt][half] = fmaf(l[mt][half], alpha[half], sum);
+                    l[nt][k] = fmaf(l[nt][k], alpha[k], sum);
                 }
 #pragma unroll
                 for (int n = 0; n < NG; ++n)
 #pragma unroll
-                    for (int j = 0; j < 2; ++j) {
-                        pa[mt][n][2 * j] = pack_h2(s[mt][n][j][0], s[mt][n][j][1]);
-                        pa[mt][n][2 * j + 1] = TWO ? pack_h2(s[mt][n][j][2], s[mt][n][j][3]) : 0u;
-                    }
+                    for (int j = 0; j < 2; ++j) pb[nt][n][j] = transpose8x8(pack_h2(s[nt][n][2 * j], s[nt][n][2 * j + 1]));
                 if (__any_sync(0xffffffffu, alpha[0] != 1.f || alpha[1] != 1.f)) {
 #pragma unroll
-                    for (int n = 0; n < D / 8; ++n) {
-                        o[mt][n][0] *= alpha[0];
-                        o[mt][n][1] *= alpha[0];
-                        if (TWO) {
-                            o[mt][n][2] *= alpha[1];
-                            o[mt][n][3] *= alpha[1];
-                        }
+                    for (int n = 0; n < D / 16; ++n) {
+                        o[nt][n][0] *= alpha[0];
+                        o[nt][n][1] *= alpha[1];
+                        o[nt][n][2] *= alpha[0];
+                        o[nt][n][3] *= alpha[1];
                     }
                 }
             }
@@ -350,14 +345,17 @@ __global__ void __launch_bounds__(kWarps * 32) attend_kernel(const __grid_consta
                 }
 #pragma unroll
                 for (int c = 0; c < C; ++c) {
-                    const uint4 w = lds128(base + KEYS * D + n * 16 * D + c * 512 + lane * 16);
-                    const uint32_t word[4] = {w.x, w.y, w.z, w.w};
+                    uint4 w = lds128(base + KEYS * D + n * 16 * D + c * 512);
+                    if (E4M3) { w.x &= keep; w.y &= keep; w.z &= keep; w.w &= keep; }
+                    uint32_t a[2][4];                          // values g, g + 8 and g + 16, g + 24 of the chunk
+                    codes_to_h4<E4M3>(w.x, a[0][0], a[0][2]);
+                    codes_to_h4<E4M3>(w.y, a[0][1], a[0][3]);
+                    codes_to_h4<E4M3>(w.z, a[1][0], a[1][2]);
+                    codes_to_h4<E4M3>(w.w, a[1][1], a[1][3]);
 #pragma unroll
-                    for (int dt = 0; dt < 4; ++dt) {
-                        uint32_t b0, b1;
-                        codes_to_h4<E4M3>(E4M3 ? word[dt] & keep : word[dt], b0, b1);
-#pragma unroll
-                        for (int mt = 0; mt < MT; ++mt) mma16816(o[mt][c * 4 + dt], pa[mt][n], b0, b1);
+                    for (int nt = 0; nt < NT; ++nt) {
+                        mma16816(o[nt][c * 2], a[0], pb[nt][n][0], pb[nt][n][1]);
+                        mma16816(o[nt][c * 2 + 1], a[1], pb[nt][n][0], pb[nt][n][1]);
                     }
                 }
             }
@@ -385,31 +383,33 @@ __global__ void __launch_bounds__(kWarps * 32) attend_kernel(const __grid_consta
 
         // ---- the four warps' sums become one
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt)
+        for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-            for (int half = 0; half < (TWO ? 2 : 1); ++half) {
-                float v = l[mt][half];
-                v += __shfl_xor_sync(0xffffffffu, v, 1);
-                v += __shfl_xor_sync(0xffffffffu, v, 2);
-                const int r = mt * 16 + half * 8 + g;
-                if (tq == 0) {
-                    s_m[warp][r] = M[mt][half];
+            for (int k = 0; k < 2; ++k) {
+                float v = l[nt][k];
+                v += __shfl_xor_sync(0xffffffffu, v, 4);
+                v += __shfl_xor_sync(0xffffffffu, v, 8);
+                v += __shfl_xor_sync(0xffffffffu, v, 16);
+                const int r = nt * 8 + 2 * tq + k;
+                if (g == 0) {
+                    s_m[warp][r] = M[nt][k];
                     s_l[warp][r] = v;
                 }
-                float *dst = reinterpret_cast<float *>(ring) + (size_t)r * D;
+                float *dst = reinterpret_cast<float *>(ring) + r * kPitch + g;
 #pragma unroll
-                for (int n = 0; n < D / 8; ++n)                // columns rotated by the row, so that rows do not meet in a bank
-                    *reinterpret_cast<float2 *>(dst + ((n * 8 + 2 * tq + 8 * (r & 7)) & (D - 1))) =
-                        make_float2(o[mt][n][half * 2], o[mt][n][half * 2 + 1]);
+                for (int n = 0; n < D / 16; ++n) {
+                    dst[n * 16] = o[nt][n][k];
+                    dst[n * 16 + 8] = o[nt][n][2 + k];
+                }
             }
         __syncthreads();
-        const long long pair_at = seq_at + (long long)pair * sh.units, pair_end = pair_at + sh.units;
+        const long long pair_at = seq_at + (long long)pair * sh.units;
         const bool all = u0 == 0 && u1 == sh.units;
-        const int w0 = all ? 0 : (int)(((pair_at + 1) * W - 1) / total), w1 = all ? 0 : (int)((pair_end * W - 1) / total);
+        const int w0 = all ? 0 : shares.owner(pair_at), w1 = all ? 0 : shares.owner(pair_at + sh.units - 1);
         float *part = p.parts + (size_t)(2 * blockIdx.x + (u0 == 0 ? 1 : 0)) * kPart;
         auto finish = [&](int r, int d, float4 v, float m, float lsum) {      // outputs of four values of a row
-            const int j = (r0 + r) / p.G, hq = h * p.G + (r0 + r) % p.G;
-            const size_t at = ((size_t)(sh.row0 + j) * p.H * p.G + hq) * D + d;
+            const int fr = r0 + r;
+            const size_t at = ((size_t)(sh.row0 + fr / p.G) * p.H * p.G + h * p.G + fr % p.G) * D + d;
             store4(p, at, v, inverse(lsum));
             if (d == 0 && p.lse) p.lse[at / D] = lse_of(m, lsum);
         };
@@ -424,14 +424,14 @@ __global__ void __launch_bounds__(kWarps * 32) attend_kernel(const __grid_consta
 #pragma unroll
             for (int w = 0; w < kWarps; ++w) {
                 const float f = ex2(s_m[w][r] - ref);
-                const float4 x = *reinterpret_cast<const float4 *>(smem + w * 24576 + ((size_t)r * D + ((d + 8 * (r & 7)) & (D - 1))) * 4);
+                const float4 x = *reinterpret_cast<const float4 *>(smem + w * kOwn + (r * kPitch + d) * 4);
                 lsum = fmaf(s_l[w][r], f, lsum);
                 v.x = fmaf(x.x, f, v.x); v.y = fmaf(x.y, f, v.y); v.z = fmaf(x.z, f, v.z); v.w = fmaf(x.w, f, v.w);
             }
             if (all) {
                 finish(r, d, v, m, lsum);
             } else {
-                *reinterpret_cast<float4 *>(part + (size_t)r * D + d) = v;
+                *reinterpret_cast<float4 *>(part + r * D + d) = v;
                 if (d == 0) {
                     part[TR * D + r] = m;
                     part[TR * D + TR + r] = lsum;
@@ -454,10 +454,11 @@ __global__ void __launch_bounds__(kWarps * 32) attend_kernel(const __grid_consta
                     const int r = e / (D / 4), d = e % (D / 4) * 4;
                     float m = -INFINITY, lsum = 0.f;
                     float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
                     for (int w = w0; w <= w1; ++w) {
                         const float *x = p.parts + (size_t)(2 * w + (w == w0 ? 1 : 0)) * kPart;
                         add_part(m, lsum, v, __ldcg(x + TR * D + r), __ldcg(x + TR * D + TR + r),
-                                 __ldcg(reinterpret_cast<const float4 *>(x + (size_t)r * D + d)));
+                                 __ldcg(reinterpret_cast<const float4 *>(x + r * D + d)));
                     }
                     finish(r, d, v, m, lsum);
                 }
@@ -473,17 +474,27 @@ __global__ void __launch_bounds__(kWarps * 32) attend_kernel(const __grid_consta
     }
 }
 
-constexpr int kSmem = kWarps * 24576;
-constexpr int kFewRows = 32;       // query rows of a key head up to which attend_kernel is used
-
-static int grid_of() { return 2 * jq_sm_count() < kJqCounters ? 2 * jq_sm_count() : kJqCounters; }
+// CTAs on an SM, and dynamic shared memory of one: rings, or the sums that take their place where those are longer.
+static int ctas_of(int tile) { return tile == 32 ? 2 : 3; }
+static int smem_of(int tile, int D) {
+    const int sums = tile * (D + 4) * 4;
+    return kWarps * (sums > kRing ? sums : kRing);
+}
+static int grid_of(int tile) {
+    const int n = ctas_of(tile) * jq_sm_count();
+    return n < kJqCounters ? n : kJqCounters;
+}
+// Query rows of a tile, by those that a key head has in a call.
+static int tile_of(long long rows) { return rows <= 8 ? 8 : (rows <= 16 ? 16 : 32); }
 
 typedef void (*attend_fn)(const AttendArgs);
 template <int D>
-static attend_fn pick(bool e4m3, int rows) {
-    if (e4m3) return rows == 8 ? attend_kernel<D, true, 8> : (rows == 16 ? attend_kernel<D, true, 16> : attend_kernel<D, true, 32>);
-    return rows == 8 ? attend_kernel<D, false, 8> : (rows == 16 ? attend_kernel<D, false, 16> : attend_kernel<D, false, 32>);
+static attend_fn pick(bool e4m3, int tile) {
+    if (e4m3) return tile == 8 ? attend_kernel<D, true, 1> : (tile == 16 ? attend_kernel<D, true, 2> : attend_kernel<D, true, 4>);
+    return tile == 8 ? attend_kernel<D, false, 1> : (tile == 16 ? attend_kernel<D, false, 2> : attend_kernel<D, false, 4>);
 }
+
+constexpr int kFewRows = 32;       // query rows of a key head up to which attend_kernel is used
 
 int check_cache(const jq_kv_cache *c, const jq_kv_batch *s);
 Batch batch_of(const jq_kv_cache *c, const jq_kv_batch *s);
@@ -495,8 +506,10 @@ using namespace jqkv;
 
 extern "C" size_t jq_kv_attend_workspace_bytes(const jq_kv_cache *c, const jq_kv_batch *s, int q_heads) {
     if (check_cache(c, s) || q_heads <= 0) return 0;
-    if ((long long)most_new(s) * (q_heads / c->kv_heads) > kFewRows) return kJqData + prompt_workspace(c->head_dim);
-    return kJqData + 2 * (size_t)grid_of() * (32 * (size_t)c->head_dim + 64) * 4;
+    const long long rows = (long long)most_new(s) * (q_heads / c->kv_heads);
+    if (rows > kFewRows) return kJqData + prompt_workspace(c->head_dim);
+    const int tile = tile_of(rows);
+    return kJqData + 2 * (size_t)grid_of(tile) * tile * (c->head_dim + 2) * 4;
 }
 
 extern "C" int jq_kv_attend(const jq_kv_cache *c, const jq_kv_batch *s, const void *q, const int64_t *stride_q, int q_heads,
@@ -528,16 +541,15 @@ extern "C" int jq_kv_attend(const jq_kv_cache *c, const jq_kv_batch *s, const vo
     a.counters = reinterpret_cast<int *>(ws + kJqHeader);
     a.parts = reinterpret_cast<float *>(ws + kJqData);
     const long long rows = (long long)most_new(s) * a.G;
-    const int grid = grid_of();
-    const int tile = rows <= 8 ? 8 : (rows <= 16 ? 16 : 32);
     const bool e4m3 = c->fmt == JQ_KV_E4M3;
     if (rows > kFewRows) {
         a.least = 8;
         return prompt_launch(a, c->head_dim, e4m3, reinterpret_cast<cudaStream_t>(stream));
     }
+    const int tile = tile_of(rows), smem = smem_of(tile, c->head_dim);
     const attend_fn kern = c->head_dim == 64 ? pick<64>(e4m3, tile) : pick<128>(e4m3, tile);
     static jq_contexts done[2][2][3];
-    JQ_CUDA_TRY(jq_allow_smem(reinterpret_cast<const void *>(kern), kSmem, done[c->head_dim == 128][e4m3][tile == 8 ? 0 : tile / 16]));
-    kern<<<grid, kWarps * 32, kSmem, reinterpret_cast<cudaStream_t>(stream)>>>(a);
+    JQ_CUDA_TRY(jq_allow_smem(reinterpret_cast<const void *>(kern), smem, done[c->head_dim == 128][e4m3][tile / 16]));
+    kern<<<grid_of(tile), kWarps * 32, smem, reinterpret_cast<cudaStream_t>(stream)>>>(a);
     return jq_launch_status();
 }

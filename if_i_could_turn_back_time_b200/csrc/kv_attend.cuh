@@ -57,6 +57,22 @@ __device__ __forceinline__ void add_part(float &m, float &l, float4 &v, float mw
     m = top;
 }
 
+// Whole quotients; most operands have 32 bits, whose division is short.
+__device__ __forceinline__ long long quotient(long long a, long long b) {
+    return ((a | b) >> 32) == 0 ? (long long)((uint32_t)a / (uint32_t)b) : a / b;
+}
+// `total` units dealt to W CTAs: the first `extra` have one more than the others.
+struct Shares {
+    long long base;
+    int extra;
+    __device__ __forceinline__ Shares(long long total, int W) : base(quotient(total, W)), extra((int)(total - base * W)) {}
+    __device__ __forceinline__ long long first(int w) const { return base * w + min(w, extra); }
+    __device__ __forceinline__ int owner(long long unit) const {
+        const long long longer = extra * (base + 1);
+        return unit < longer ? (int)quotient(unit, base + 1) : extra + (int)quotient(unit - longer, base);
+    }
+};
+
 // Prompts (kv_prompt.cu): rows of a CTA, CTAs, bytes of their parts, launch.
 constexpr int kPromptRows = 256;
 static inline int prompt_grid() { return jq_sm_count() < kJqCounters ? jq_sm_count() : kJqCounters; }

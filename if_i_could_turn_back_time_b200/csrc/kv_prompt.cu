@@ -92,22 +92,6 @@ __device__ __forceinline__ Range range_of(const AttendArgs &p, int len, int n, i
 // (n * G is at most 2^30 where max_new is what it says; a longer sequence has its first 2^30 rows)
 __device__ __forceinline__ int tiles_of(const AttendArgs &p, int n) { return (int)((min((long long)n * p.G, 1LL << 30) + kRows - 1) / kRows); }
 
-// Whole quotients; most operands have 32 bits, whose division is short.
-__device__ __forceinline__ long long quotient(long long a, long long b) {
-    return ((a | b) >> 32) == 0 ? (long long)((uint32_t)a / (uint32_t)b) : a / b;
-}
-// `total` units dealt to W CTAs: the first `extra` have one more than the others.
-struct Shares {
-    long long base;
-    int extra;
-    __device__ __forceinline__ Shares(long long total, int W) : base(quotient(total, W)), extra((int)(total - base * W)) {}
-    __device__ __forceinline__ long long first(int w) const { return base * w + min(w, extra); }
-    __device__ __forceinline__ int owner(long long unit) const {
-        const long long longer = extra * (base + 1);
-        return unit < longer ? (int)quotient(unit, base + 1) : extra + (int)quotient(unit - longer, base);
-    }
-};
-
 // The segments of a CTA: units in the order (sequence, row tile, key head, unit), cut evenly.
 struct Walk {
     long long cur, end, at;        // at: first unit of (seq, tile)
