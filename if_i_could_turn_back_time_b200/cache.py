@@ -7,8 +7,8 @@ Python_Jenks_Test/Jenks_Tests/QuantNetworkTest.py); the cache completes a decode
 """
 from __future__ import annotations
 
-import ctypes
 import math
+import struct
 from typing import Optional, Tuple
 
 import torch
@@ -18,7 +18,8 @@ from . import _lib, ops
 _FORMATS = {"int8": _lib.JQ_KV_INT8, "e4m3": _lib.JQ_KV_E4M3}
 BLOCK_SIZES = (16, 32, 64, 128)
 HEAD_DIMS = (64, 128)          # of attend(); append() and read() take every multiple of 32 up to 256
-_Strides = ctypes.c_int64 * 2
+_pack_strides = struct.Struct("=qq").pack              # int64_t[2]
+_pack_batch = struct.Struct("=QQQiiiiii").pack         # jq_kv_batch
 
 
 class KVCache:
@@ -55,9 +56,11 @@ class KVCache:
         if self.head_dim % 32 or not 32 <= self.head_dim <= 256:
             raise ValueError("head_dim must be a multiple of 32 up to 256")
         self.device = keys.device
-        self._c = _lib.jq_kv_cache(keys.data_ptr(), values.data_ptr(), key_scales.data_ptr(), value_scales.data_ptr(),
-                                   self.blocks, self.kv_heads, self.head_dim, self.block_size, _FORMATS[fmt], 0)
-        self._c_ref = ctypes.byref(self._c)
+        self._cuda = keys.is_cuda
+        # (the structure of jq.h as bytes; the fields do not change)
+        self._c = bytes(_lib.jq_kv_cache(keys.data_ptr(), values.data_ptr(), key_scales.data_ptr(), value_scales.data_ptr(),
+                                         self.blocks, self.kv_heads, self.head_dim, self.block_size, _FORMATS[fmt], 0))
+        self._need = {}                # (tokens of a sequence at most, query heads) -> bytes of workspace
 
     @classmethod
     def empty(cls, blocks: int, kv_heads: int, head_dim: int, *, block_size: int = 64, fmt: str = "int8",
@@ -70,41 +73,46 @@ class KVCache:
     def nbytes(self) -> int:
         return sum(t.numel() * t.element_size() for t in (self.keys, self.values, self.key_scales, self.value_scales))
 
-    def _batch(self, table, lengths, starts, tokens, max_new):
-        n = lengths.shape[0]
-        if table.dim() != 2 or lengths.dim() != 1 or table.shape[0] != n:
+    def _batch(self, table, lengths, starts, tokens, max_new) -> bytes:
+        """jq_kv_batch of a call, its arguments looked over."""
+        n, width = table.shape if table.dim() == 2 else (-1, 0)
+        if lengths.shape != (n,):
             raise RuntimeError(f"table {tuple(table.shape)} and lengths {tuple(lengths.shape)}: [sequences, width] and [sequences]")
-        if table.dtype != torch.int32 or lengths.dtype != torch.int32 or (starts is not None and starts.dtype != torch.int32):
+        if table.dtype is not torch.int32 or lengths.dtype is not torch.int32 or (starts is not None and starts.dtype is not torch.int32):
             raise RuntimeError("table, lengths and starts are int32 tensors")
-        if table.shape[1] == 0:
+        if width == 0:
             raise RuntimeError("the table has no columns")
-        if table.stride(1) != 1 and table.shape[1] != 1 or not lengths.is_contiguous():
+        row, column = table.stride()
+        if column != 1 and width != 1 or not lengths.is_contiguous():
             raise RuntimeError("the table's rows and the lengths are contiguous")
         device = self.device
         if table.device != device or lengths.device != device:
             raise RuntimeError(f"the cache is on {device}: table, lengths and starts are too")
-        stride = table.stride(0) if n > 1 else table.shape[1]
-        if stride < table.shape[1]:
+        if n <= 1:
+            row = width
+        elif row < width:
             raise RuntimeError("the table's rows lie behind one another")
+        at = 0
         if starts is None:
             if n and tokens % n:
                 raise RuntimeError(f"{tokens} new tokens of {n} sequences: starts says how many each has")
-            at = None
         else:
             if starts.shape != (n + 1,) or not starts.is_contiguous() or starts.device != device:
                 raise RuntimeError(f"starts is a contiguous tensor [{n + 1}] on {device}")
             at = starts.data_ptr()
-        if max_new is not None and max_new < 0:
+        if max_new is None:
+            max_new = tokens
+        elif max_new < 0:
             raise RuntimeError("max_new is a number of tokens")
-        if not self.keys.is_cuda:
+        if not self._cuda:
             raise RuntimeError("libjq operators run on CUDA tensors only (there is no CPU path)")
-        return _lib.jq_kv_batch(table.data_ptr(), lengths.data_ptr(), at, n, table.shape[1], stride, tokens,
-                                tokens if max_new is None else max_new, 0)
+        return _pack_batch(table.data_ptr(), lengths.data_ptr(), at, n, width, row, tokens, max_new, 0)
 
     def _rows(self, x, heads, what):
-        """[..., heads, head_dim] as rows of one stride: (tensor, strides of a row and of a head)."""
-        if x.dim() < 3 or x.shape[-1] != self.head_dim or (x.shape[-2] != heads if heads else x.shape[-2] % self.kv_heads):
-            raise RuntimeError(f"{what} is {tuple(x.shape)}: [tokens, {heads or 'q_heads'}, {self.head_dim}] "
+        """[..., heads, head_dim] as rows of one stride: (tensor [tokens, heads, head_dim], strides of a row and of a head)."""
+        shape = x.shape
+        if len(shape) < 3 or shape[-1] != self.head_dim or (shape[-2] != heads if heads else shape[-2] % self.kv_heads):
+            raise RuntimeError(f"{what} is {tuple(shape)}: [tokens, {heads or 'q_heads'}, {self.head_dim}] "
                                f"with the cache's {self.kv_heads} key heads")
         if x.dtype not in ops._DT:
             raise RuntimeError(f"unsupported dtype {x.dtype}")
@@ -112,11 +120,13 @@ class KVCache:
             raise RuntimeError(f"{what} is on {x.device}, the cache on {self.device}")
         if x.is_neg():
             x = x.resolve_neg()
-        if x.dim() > 3:
-            x = x.reshape(-1, x.shape[-2], x.shape[-1])
-        if x.stride(2) != 1:
+        if len(shape) > 3:
+            x = x.reshape(-1, shape[-2], shape[-1])
+        row, head, one = x.stride()
+        if one != 1:
             x = x.contiguous()
-        return x, _Strides(x.stride(0), x.stride(1))
+            row, head, one = x.stride()
+        return x, _pack_strides(row, head)
 
     def append(self, k: torch.Tensor, v: torch.Tensor, table: torch.Tensor, lengths: torch.Tensor,
                starts: Optional[torch.Tensor] = None, max_new: Optional[int] = None) -> None:
@@ -130,7 +140,7 @@ class KVCache:
             raise RuntimeError("k and v have one shape and dtype")
         batch = self._batch(table, lengths, starts, k.shape[0], max_new)
         with ops._on(self.device):
-            st = _lib.load().jq_kv_append(self._c_ref, ctypes.byref(batch), k.data_ptr(), v.data_ptr(), sk, sv, ops._DT[k.dtype],
+            st = _lib.load().jq_kv_append(self._c, batch, k.data_ptr(), v.data_ptr(), sk, sv, ops._DT[k.dtype],
                                           ops._stream())
         if st:
             _lib.check(st, "jq_kv_append")
@@ -144,10 +154,9 @@ class KVCache:
         if last < 0:
             raise RuntimeError("last is a number of tokens")
         batch = self._batch(table, lengths, None, 0, None)
-        shape = (lengths.shape[0], last, self.kv_heads, self.head_dim)
-        k, v = torch.empty(shape, dtype=dtype, device=self.device), torch.empty(shape, dtype=dtype, device=self.device)
+        k, v = torch.empty((2, lengths.shape[0], last, self.kv_heads, self.head_dim), dtype=dtype, device=self.device).unbind()
         with ops._on(self.device):
-            st = _lib.load().jq_kv_read(self._c_ref, ctypes.byref(batch), last, k.data_ptr(), v.data_ptr(), ops._DT[dtype], ops._stream())
+            st = _lib.load().jq_kv_read(self._c, batch, last, k.data_ptr(), v.data_ptr(), ops._DT[dtype], ops._stream())
         if st:
             _lib.check(st, "jq_kv_read")
         return k, v
@@ -163,27 +172,36 @@ class KVCache:
             raise RuntimeError(f"unsupported query dtype {dtype}: fp16 or bf16")
         if self.head_dim not in HEAD_DIMS:
             raise RuntimeError(f"attend() takes heads of {HEAD_DIMS}, the cache has {self.head_dim}")
-        q, sq = self._rows(q, 0, "q")
+        x, strides = self._rows(q, 0, "q")
         if scale is None:
             scale = 1.0 / math.sqrt(self.head_dim)
-        if not 0.0 < scale < 3e38:
+        elif not 0.0 < scale < 3e38:
             raise RuntimeError("scale must be above 0")
         if window < 0:
             raise RuntimeError("window is a number of tokens, 0 for all")
-        tokens, heads = q.shape[0], q.shape[1]
+        heads = shape[-2]
+        tokens = x.shape[0]
         batch = self._batch(table, lengths, starts, tokens, max_new)
         lib = _lib.load()
-        out = torch.empty((tokens, heads, self.head_dim), dtype=dtype, device=self.device)
-        sums = torch.empty((tokens, heads), dtype=torch.float32, device=self.device) if lse else None
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
+        sums = torch.empty(shape[:-1], dtype=torch.float32, device=self.device) if lse else None
+        if starts is None:
+            most = tokens // max(1, lengths.shape[0])
+        else:
+            most = tokens if not max_new else min(max_new, tokens)
         with ops._on(self.device):
-            ref = ctypes.byref(batch)
-            own, at, size = ops._parts_workspace(self.device, lib.jq_kv_attend_workspace_bytes(self._c_ref, ref, heads))
-            st = lib.jq_kv_attend(self._c_ref, ref, q.data_ptr(), sq, heads, scale, min(window, 0x7fffffff), out.data_ptr(),
-                                  ops._addr(sums), ops._DT[dtype], at, size, ops._stream())
+            need = self._need.get((most, heads))
+            if need is None:
+                if len(self._need) >= 1024:
+                    self._need.clear()
+                need = self._need[most, heads] = lib.jq_kv_attend_workspace_bytes(self._c, batch, heads)
+            stream = ops._stream()
+            own, at, size = ops._parts_workspace(self.device, need, stream)
+            st = lib.jq_kv_attend(self._c, batch, x.data_ptr(), strides, heads, scale, min(window, 0x7fffffff), out.data_ptr(),
+                                  ops._addr(sums), ops._DT[dtype], at, size, stream)
             del own
         if st:
             _lib.check(st, "jq_kv_attend")
         if ops._checked:
             ops.check_status()
-        out = out.view(shape)
-        return (out, sums.view(shape[:-1])) if lse else out
+        return (out, sums) if lse else out

@@ -5,7 +5,8 @@ namespace jqkv {
 
 using namespace jqta;
 
-constexpr int kWarps = 4;          // of a CTA; each takes every fourth stage of a segment
+constexpr int kFewParts = 8;       // of a pair: up to here they are added as they are read
+constexpr int kNear = 16;          // units
 constexpr int kUnit = 64;          // keys: what work is dealt out in
 constexpr int kRing = 16384;       // bytes of a warp's ring: two stages of 32 keys at D = 128, three CTAs on an SM
 
@@ -13,6 +14,9 @@ __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], 
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
+
+// Warps of a CTA: four, two or three CTAs on an SM, so that one's beginning and end fall into the others' loops; or all of an SM's.
+__host__ __device__ constexpr int warps_of(int NT, bool wide) { return wide ? (NT > 2 ? 8 : 12) : 4; }
 
 // A matrix of 8 x 8 fp16 values, two of a row in a lane (row lane / 4), the other way round.
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
@@ -40,11 +44,76 @@ __device__ __forceinline__ Share share_of(const AttendArgs &p, int i) {
     return s;
 }
 
+// The parts of a pair, of the CTAs w0 .. w1, added in their order; outputs.  Parts of many CTAs: their factors first, a warp per row, so that
+// the loads of the sums need not wait for one another.  (Not inlined: its registers are not the main loop's.)
+template <int D, int TR, int THREADS>
+__device__ __noinline__ void add_parts(const AttendArgs &p, float *factor, float *s_m, float *s_l, int w0, int w1, int rows, int r0, int row0, int h) {
+    constexpr int kPart = TR * D + 2 * TR;
+    const int tid = threadIdx.x, lane = tid & 31, parts = w1 - w0 + 1;
+    auto of = [&](int w) { return p.parts + (size_t)(2 * w + (w == w0 ? 1 : 0)) * kPart; };
+    auto finish = [&](int r, int d, const float4 &v, float m, float l) {
+        const int fr = r0 + r;
+        const size_t at = ((size_t)(row0 + fr / p.G) * p.H * p.G + h * p.G + fr % p.G) * D + d;
+        store4(p, at, v, inverse(l));
+        if (d == 0 && p.lse) p.lse[at / D] = lse_of(m, l);
+    };
+    if (parts <= kFewParts) {
+        for (int e = tid; e < rows * (D / 4); e += THREADS) {
+            const int r = e / (D / 4), d = e % (D / 4) * 4;
+            float m = -INFINITY, l = 0.f;
+            float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+            for (int w = w0; w <= w1; ++w) {
+                const float *x = of(w);
+                add_part(m, l, v, __ldcg(x + TR * D + r), __ldcg(x + TR * D + TR + r), __ldcg(reinterpret_cast<const float4 *>(x + r * D + d)));
+            }
+            finish(r, d, v, m, l);
+        }
+        return;
+    }
+    for (int r = tid >> 5; r < rows; r += THREADS / 32) {
+        float m = -INFINITY, l = 0.f;
+        for (int x = lane; x < parts; x += 32) m = fmaxf(m, __ldcg(of(w0 + x) + TR * D + r));
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+        const float ref = m == -INFINITY ? 0.f : m;
+        for (int x = lane; x < parts; x += 32) {
+            const float f = ex2(__ldcg(of(w0 + x) + TR * D + r) - ref);
+            factor[x * TR + r] = f;                        // [part][row], in place of the rings
+            l = fmaf(__ldcg(of(w0 + x) + TR * D + TR + r), f, l);
+        }
+        l = jq::warp_sum(l);
+        if (lane == 0) {
+            s_m[r] = m;
+            s_l[r] = l;
+        }
+    }
+    __syncthreads();
+    for (int e = tid; e < rows * (D / 4); e += THREADS) {
+        const int r = e / (D / 4), d = e % (D / 4) * 4;
+        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int x0 = 0; x0 < parts; x0 += 16) {
+            float4 y[16];
+#pragma unroll
+            for (int x = 0; x < 16; ++x)
+                if (x0 + x < parts) y[x] = __ldcg(reinterpret_cast<const float4 *>(of(w0 + x0 + x) + r * D + d));
+#pragma unroll
+            for (int x = 0; x < 16; ++x) {
+                if (x0 + x >= parts) break;
+                const float f = factor[(x0 + x) * TR + r];
+                v.x = fmaf(y[x].x, f, v.x); v.y = fmaf(y[x].y, f, v.y); v.z = fmaf(y[x].z, f, v.z); v.w = fmaf(y[x].w, f, v.w);
+            }
+        }
+        finish(r, d, v, s_m[r], s_l[r]);
+    }
+}
+
 // NT: tiles of 8 query rows (query, head of the group).  Both products have the cache as their 16-row operand, so that 8 query rows cost
 // one instruction for 16 keys x 16 values: S^T = K Q^T, O^T = V^T P^T.  A lane has the scores of the keys (g, 0) and (g, 1) of a
 // group (see kv.cuh) for the rows 2t and 2t + 1; packed to fp16 and transposed by movmatrix they are the second product's B operand.
-template <int D, bool E4M3, int NT>
-__global__ void __launch_bounds__(kWarps * 32, NT == 4 ? 2 : 3) attend_kernel(const __grid_constant__ AttendArgs p) {
+template <int D, bool E4M3, int NT, bool WIDE>
+__global__ void __launch_bounds__(warps_of(NT, WIDE) * 32, WIDE ? 1 : (NT > 2 ? 2 : 3)) attend_kernel(const __grid_constant__ AttendArgs p) {
+    constexpr int kWarps = warps_of(NT, WIDE);                 // each takes every kWarps-th stage of a segment
     constexpr int C = D / 32;                                  // chunks of a group
     constexpr int KEYS = 32, NG = KEYS / 16;                   // keys and groups of a stage
     constexpr int kStageBytes = KEYS * D * 2;
@@ -57,6 +126,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 4 ? 2 : 3) attend_kernel(co
     __shared__ __align__(8) uint64_t bars[kWarps * NS];
     __shared__ int s_err, s_seq, s_last;
     __shared__ long long s_sum[kWarps], s_off;
+    __shared__ Share s_share;
     __shared__ float s_m[kWarps][TR], s_l[kWarps][TR];
 
     const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31, g = lane >> 2, tq = lane & 3;
@@ -92,24 +162,27 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 4 ? 2 : 3) attend_kernel(co
     const int W = fit < (long long)gridDim.x ? (int)fit : (int)gridDim.x;
     if ((int)blockIdx.x >= W) return;
     const Shares shares(total, W);
-    long long cur = shares.first(blockIdx.x);
+    const long long lo = shares.first(blockIdx.x);
+    long long cur = lo;
+    const long long near = shares.base > 2 * kNear ? kNear : shares.base / 2;
     const long long hi = shares.first(blockIdx.x + 1);
     if (cur >= before && cur < before + mine) {                // (one thread's sequences hold the first unit)
         long long at = before;
         for (int i = i0; i < i1; ++i) {
-            const long long t = share_of<TR>(p, i).total;
-            if (cur < at + t) {
+            const Share s = share_of<TR>(p, i);
+            if (cur < at + s.total) {
                 s_seq = i;
                 s_off = at;
+                s_share = s;
                 break;
             }
-            at += t;
+            at += s.total;
         }
     }
     __syncthreads();
     int seq = s_seq;
     long long seq_at = s_off;
-    Share sh = share_of<TR>(p, seq);
+    Share sh = s_share;
 
     uint32_t phases = 0;                                       // parity of each stage's next completion
     while (cur < hi) {
@@ -117,9 +190,18 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 4 ? 2 : 3) attend_kernel(co
             seq_at += sh.total;
             sh = share_of<TR>(p, ++seq);
         }
-        const long long in_seq = cur - seq_at;
-        const int pair = (int)quotient(in_seq, sh.units), u0 = (int)(in_seq - (long long)pair * sh.units);
-        const int u1 = (int)min((long long)sh.units, u0 + (hi - cur));
+        const int pair = (int)quotient(cur - seq_at, sh.units);
+        const long long pair_at = seq_at + (long long)pair * sh.units, pair_end = pair_at + sh.units;
+        // A boundary between two CTAs that is near a pair's begin or end is taken to lie there: a few units more for one of them are
+        // less than a further segment.
+        auto snap = [&](long long b) {
+            const long long off = b - pair_at, rest = pair_end - b;
+            return off <= near && off <= rest ? pair_at : (rest <= near ? pair_end : b);
+        };
+        const long long from = cur == lo ? snap(cur) : cur, to = hi < pair_end ? snap(hi) : pair_end;
+        cur = pair_end;
+        if (to <= from) continue;
+        const int u0 = (int)(from - pair_at), u1 = (int)(to - pair_at);
         const int h = sh.tiles == 1 ? pair : pair / sh.tiles, tile = sh.tiles == 1 ? 0 : pair % sh.tiles;
         const int k0 = sh.lo + u0 * kUnit, k1 = min(sh.len, sh.lo + u1 * kUnit);
         const int stages = k1 > k0 ? (k1 - k0 + KEYS - 1) / KEYS : 0;
@@ -381,7 +463,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 4 ? 2 : 3) attend_kernel(co
         }
         // (stages are dealt to slots from slot 0 in every segment; all copies of this one have been waited for)
 
-        // ---- the four warps' sums become one
+        // ---- the warps' sums become one
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -403,9 +485,14 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 4 ? 2 : 3) attend_kernel(co
                 }
             }
         __syncthreads();
-        const long long pair_at = seq_at + (long long)pair * sh.units;
         const bool all = u0 == 0 && u1 == sh.units;
-        const int w0 = all ? 0 : shares.owner(pair_at), w1 = all ? 0 : shares.owner(pair_at + sh.units - 1);
+        int w0 = 0, w1 = 0;                                    // CTAs that have a part of the pair
+        if (!all) {
+            w0 = shares.owner(pair_at);
+            w1 = shares.owner(pair_end - 1);
+            if (w0 < w1 && snap(shares.first(w0 + 1)) == pair_at) ++w0;
+            if (w0 < w1 && snap(shares.first(w1)) == pair_end) --w1;
+        }
         float *part = p.parts + (size_t)(2 * blockIdx.x + (u0 == 0 ? 1 : 0)) * kPart;
         auto finish = [&](int r, int d, float4 v, float m, float lsum) {      // outputs of four values of a row
             const int fr = r0 + r;
@@ -450,23 +537,11 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 4 ? 2 : 3) attend_kernel(co
             __syncthreads();
             if (s_last) {
                 __threadfence();
-                for (int e = tid; e < rows * (D / 4); e += kWarps * 32) {
-                    const int r = e / (D / 4), d = e % (D / 4) * 4;
-                    float m = -INFINITY, lsum = 0.f;
-                    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-                    for (int w = w0; w <= w1; ++w) {
-                        const float *x = p.parts + (size_t)(2 * w + (w == w0 ? 1 : 0)) * kPart;
-                        add_part(m, lsum, v, __ldcg(x + TR * D + r), __ldcg(x + TR * D + TR + r),
-                                 __ldcg(reinterpret_cast<const float4 *>(x + r * D + d)));
-                    }
-                    finish(r, d, v, m, lsum);
-                }
+                add_parts<D, TR, kWarps * 32>(p, reinterpret_cast<float *>(smem), s_m[0], s_l[0], w0, w1, rows, r0, sh.row0, h);
             }
         }
         fence_async_smem();                                    // the ring was written to by threads; copies land in it next
         __syncthreads();
-        cur += u1 - u0;
     }
     if (s_err) {                                               // a wait gave up: copies in flight land before the shared memory goes away
         for (int i = 0; i < 400; ++i) __nanosleep(256);
@@ -474,27 +549,32 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 4 ? 2 : 3) attend_kernel(co
     }
 }
 
-// CTAs on an SM, and dynamic shared memory of one: rings, or the sums that take their place where those are longer.
-static int ctas_of(int tile) { return tile == 32 ? 2 : 3; }
-static int smem_of(int tile, int D) {
-    const int sums = tile * (D + 4) * 4;
-    return kWarps * (sums > kRing ? sums : kRing);
+// Dynamic shared memory of a CTA: rings, or the sums that take their place where those are longer.
+static int smem_of(int NT, bool wide, int D) {
+    const int sums = NT * 8 * (D + 4) * 4;
+    return warps_of(NT, wide) * (sums > kRing ? sums : kRing);
 }
-static int grid_of(int tile) {
-    const int n = ctas_of(tile) * jq_sm_count();
+static int grid_of(int NT, bool wide) {
+    const int n = (wide ? 1 : (NT > 2 ? 2 : 3)) * jq_sm_count();
     return n < kJqCounters ? n : kJqCounters;
 }
-// Query rows of a tile, by those that a key head has in a call.
-static int tile_of(long long rows) { return rows <= 8 ? 8 : (rows <= 16 ? 16 : 32); }
-
-typedef void (*attend_fn)(const AttendArgs);
-template <int D>
-static attend_fn pick(bool e4m3, int tile) {
-    if (e4m3) return tile == 8 ? attend_kernel<D, true, 1> : (tile == 16 ? attend_kernel<D, true, 2> : attend_kernel<D, true, 4>);
-    return tile == 8 ? attend_kernel<D, false, 1> : (tile == 16 ? attend_kernel<D, false, 2> : attend_kernel<D, false, 4>);
-}
+// Tiles of 8 query rows, by the rows that a key head has in a call.
+static int tiles_of_rows(long long rows) { return rows <= 8 ? 1 : (rows <= 16 ? 2 : (rows <= 24 ? 3 : 4)); }
+// With fewer pairs (sequence, key head, tile of rows) than SMs every pair is cut anyway, and what counts is how many parts come of it.
+static bool wide_of(long long pairs) { return 8 * pairs <= jq_sm_count(); }
 
 constexpr int kFewRows = 32;       // query rows of a key head up to which attend_kernel is used
+constexpr int kLeastUnits = 6, kLeastWide = 6;     // units that a CTA takes at least: a stage for each warp
+
+typedef void (*attend_fn)(const AttendArgs);
+template <int D, bool E4M3, int NT>
+static attend_fn pick(bool wide) { return wide ? attend_kernel<D, E4M3, NT, true> : attend_kernel<D, E4M3, NT, false>; }
+template <int D, bool E4M3>
+static attend_fn pick(int NT, bool wide) {
+    return NT == 1 ? pick<D, E4M3, 1>(wide) : (NT == 2 ? pick<D, E4M3, 2>(wide) : (NT == 3 ? pick<D, E4M3, 3>(wide) : pick<D, E4M3, 4>(wide)));
+}
+template <int D>
+static attend_fn pick(bool e4m3, int NT, bool wide) { return e4m3 ? pick<D, true>(NT, wide) : pick<D, false>(NT, wide); }
 
 int check_cache(const jq_kv_cache *c, const jq_kv_batch *s);
 Batch batch_of(const jq_kv_cache *c, const jq_kv_batch *s);
@@ -508,8 +588,8 @@ extern "C" size_t jq_kv_attend_workspace_bytes(const jq_kv_cache *c, const jq_kv
     if (check_cache(c, s) || q_heads <= 0) return 0;
     const long long rows = (long long)most_new(s) * (q_heads / c->kv_heads);
     if (rows > kFewRows) return kJqData + prompt_workspace(c->head_dim);
-    const int tile = tile_of(rows);
-    return kJqData + 2 * (size_t)grid_of(tile) * tile * (c->head_dim + 2) * 4;
+    const int NT = tiles_of_rows(rows);
+    return kJqData + 2 * (size_t)grid_of(NT, false) * NT * 8 * (c->head_dim + 2) * 4;        // (enough for wide CTAs, of which there are fewer)
 }
 
 extern "C" int jq_kv_attend(const jq_kv_cache *c, const jq_kv_batch *s, const void *q, const int64_t *stride_q, int q_heads,
@@ -535,7 +615,6 @@ extern "C" int jq_kv_attend(const jq_kv_cache *c, const jq_kv_batch *s, const vo
     a.ks = c->key_scales; a.vs = c->value_scales;
     a.H = c->kv_heads; a.G = q_heads / c->kv_heads; a.window = window; a.dtype = dtype;
     a.scale = scale * kLog2e;
-    a.least = 2;
     unsigned char *ws = reinterpret_cast<unsigned char *>(workspace);
     a.status = reinterpret_cast<int *>(ws);
     a.counters = reinterpret_cast<int *>(ws + kJqHeader);
@@ -546,10 +625,13 @@ extern "C" int jq_kv_attend(const jq_kv_cache *c, const jq_kv_batch *s, const vo
         a.least = 8;
         return prompt_launch(a, c->head_dim, e4m3, reinterpret_cast<cudaStream_t>(stream));
     }
-    const int tile = tile_of(rows), smem = smem_of(tile, c->head_dim);
-    const attend_fn kern = c->head_dim == 64 ? pick<64>(e4m3, tile) : pick<128>(e4m3, tile);
-    static jq_contexts done[2][2][3];
-    JQ_CUDA_TRY(jq_allow_smem(reinterpret_cast<const void *>(kern), smem, done[c->head_dim == 128][e4m3][tile / 16]));
-    kern<<<grid_of(tile), kWarps * 32, smem, reinterpret_cast<cudaStream_t>(stream)>>>(a);
+    const int NT = tiles_of_rows(rows);
+    const bool wide = wide_of((long long)s->sequences * c->kv_heads);
+    const int smem = smem_of(NT, wide, c->head_dim);
+    const attend_fn kern = c->head_dim == 64 ? pick<64>(e4m3, NT, wide) : pick<128>(e4m3, NT, wide);
+    static jq_contexts done[2][2][4][2];
+    JQ_CUDA_TRY(jq_allow_smem(reinterpret_cast<const void *>(kern), smem, done[c->head_dim == 128][e4m3][NT - 1][wide]));
+    a.least = wide ? kLeastWide : kLeastUnits;
+    kern<<<grid_of(NT, wide), warps_of(NT, wide) * 32, smem, reinterpret_cast<cudaStream_t>(stream)>>>(a);
     return jq_launch_status();
 }

@@ -197,15 +197,18 @@ def check_status(raise_on_error: bool = True) -> int:
     return worst
 
 
-def _parts_workspace(device, nbytes: int):
-    """(tensor to keep, address, size) of the scratch of a call whose last CTA adds up what the others left: this thread's and
-    stream's "parts" buffer, or, while a graph is captured, zeros of the call's own from the graph's pool (graphs that were
-    captured on one stream may replay on several).  The kernels leave the counters in it as they found them, at zero."""
-    if _capturing(_stream()):
+def _parts_workspace(device, nbytes: int, stream: int):
+    """(tensor to keep, address, size) of the scratch of a call on the current stream whose last CTA adds up what the others
+    left: this thread's and stream's "parts" buffer, or, while a graph is captured, zeros of the call's own from the graph's
+    pool (graphs that were captured on one stream may replay on several).  The kernels leave the counters in it as they
+    found them, at zero."""
+    if _capturing(stream):
         t = torch.empty(nbytes, dtype=torch.uint8, device=device)
         t[:8192].zero_()
     else:
-        t = _workspace(device, nbytes, "parts")
+        t = _ws_cache().get((device.index, stream, "parts"))
+        if t is None or t.numel() < nbytes:
+            t = _workspace(device, nbytes, "parts")
     return t, t.data_ptr(), t.numel()
 
 
@@ -461,6 +464,9 @@ class TokenLogprobs(NamedTuple):
     top_tokens: torch.Tensor              # int64 [..., top]
 
 
+_logprobs_workspace_bytes = {}        # (rows, vocabulary, device) -> bytes
+
+
 def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0) -> TokenLogprobs:
     """Log probabilities of ``tokens`` (int64 [...]) under ``logits`` ([..., vocab]; fp32, fp16 or bf16, any row stride), the
     entropy of every row and its ``top`` (up to 32) strongest tokens, the lowest index first among equals.  One pass
@@ -470,40 +476,51 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0) -> 
 
     Replaces the log-softmax of an evaluation loop's loss (the reference's TestNetwork,
     Python_Jenks_Test/Jenks_Tests/QuantNetworkTest.py:227-243)."""
-    if logits.dim() < 1 or logits.shape[-1] == 0:
+    shape, dtype = logits.shape, logits.dtype
+    if not shape or shape[-1] == 0:
         raise RuntimeError("logits have at least one token")
-    vocab, lead = logits.shape[-1], logits.shape[:-1]
-    if logits.dtype not in _DT:
-        raise RuntimeError(f"unsupported logits dtype {logits.dtype}")
-    if tokens.shape != lead or tokens.dtype != torch.int64:
+    vocab, lead = shape[-1], shape[:-1]
+    if dtype not in _DT:
+        raise RuntimeError(f"unsupported logits dtype {dtype}")
+    if tokens.shape != lead or tokens.dtype is not torch.int64:
         raise RuntimeError(f"tokens {tuple(tokens.shape)} {tokens.dtype}: int64 of the logits' leading dims {tuple(lead)}")
     if not 0 <= top <= 32 or top > vocab:
         raise RuntimeError(f"top is {top}: 0 to 32 of the {vocab} tokens")
     _need_cuda(logits, tokens)
-    if tokens.device != logits.device:
-        raise RuntimeError(f"tokens are on {tokens.device}, logits on {logits.device}")
+    device = logits.device
+    if tokens.device != device:
+        raise RuntimeError(f"tokens are on {tokens.device}, logits on {device}")
     if logits.is_neg():
         logits = logits.resolve_neg()
-    x = logits if logits.dim() == 2 else logits.reshape(-1, vocab)
-    if x.stride(1) != 1 and vocab > 1:
+    x = logits if len(shape) == 2 else logits.reshape(-1, vocab)
+    row, one = x.stride()
+    if one != 1 and vocab > 1:
         x = x.contiguous()
+        row = vocab
     if not tokens.is_contiguous():
         tokens = tokens.contiguous()
     lib = _lib.load()
-    rows, device = x.shape[0], x.device
-    f = torch.empty(rows * (2 + top), dtype=torch.float32, device=device)
-    logprob, entropy, tops = f[:rows], f[rows:2 * rows], f[2 * rows:]
-    top_tokens = torch.empty((rows, top), dtype=torch.int64, device=device)
+    rows = x.shape[0]
+    logprob = torch.empty_like(tokens, dtype=torch.float32)
+    entropy = torch.empty_like(logprob)
+    top_tokens = torch.empty((*lead, top), dtype=torch.int64, device=device)
+    top_logprobs = torch.empty_like(top_tokens, dtype=torch.float32)
     with _on(device):
-        need = lib.jq_token_logprobs_workspace_bytes(rows, vocab)
-        own, at, size = _parts_workspace(device, need) if need else (None, None, 0)
-        st = lib.jq_token_logprobs(x.data_ptr(), x.stride(0), rows, vocab, _DT[x.dtype], tokens.data_ptr(), logprob.data_ptr(),
-                                   entropy.data_ptr(), top, tops.data_ptr() if top else None,
-                                   top_tokens.data_ptr() if top else None, at, size, _stream())
+        stream = _stream()
+        key = (rows, vocab, device.index)
+        need = _logprobs_workspace_bytes.get(key)
+        if need is None:
+            if len(_logprobs_workspace_bytes) >= 4096:
+                _logprobs_workspace_bytes.clear()
+            need = _logprobs_workspace_bytes[key] = lib.jq_token_logprobs_workspace_bytes(rows, vocab)
+        own, at, size = _parts_workspace(device, need, stream) if need else (None, None, 0)
+        st = lib.jq_token_logprobs(x.data_ptr(), row, rows, vocab, _DT[dtype], tokens.data_ptr(), logprob.data_ptr(),
+                                   entropy.data_ptr(), top, top_logprobs.data_ptr() if top else None,
+                                   top_tokens.data_ptr() if top else None, at, size, stream)
         del own
     if st:
         _lib.check(st, "jq_token_logprobs")
-    return TokenLogprobs(logprob.view(lead), entropy.view(lead), tops.view(*lead, top), top_tokens.view(*lead, top))
+    return TokenLogprobs(logprob, entropy, top_logprobs, top_tokens)
 
 
 class GroupedGemv:
