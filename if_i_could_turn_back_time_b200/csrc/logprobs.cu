@@ -6,6 +6,7 @@ namespace jqlp {
 constexpr int kThreads = 256, kWarps = kThreads / 32;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr uint32_t kFull = 0xffffffffu;
+constexpr int kCandidates = 1024;              // keys that are ranked at most
 
 struct Args {
     const void *x;
@@ -86,154 +87,386 @@ struct Sums {
     }
 };
 
-template <class T> __device__ __forceinline__ float as_float(T x) { return (float)x; }
+// Two values at once (fp32 pairs): d = x - m, w = e^d, l += w, u += w d
+struct Pairs {
+    uint64_t l, u;
+};
+__device__ __forceinline__ uint64_t pair2(float a, float b) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ float2 unpair2(uint64_t x) {
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(x));
+    return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
 
-template <class T, bool TOP>
-__global__ void __launch_bounds__(kThreads) logprobs_kernel(const __grid_constant__ Args p) {
-    constexpr int V = 16 / sizeof(T);                      // elements of a load
-    constexpr int L = 4;                                   // loads of a step
-    __shared__ Sums s_sums[kWarps];
-    __shared__ unsigned long long s_lists[TOP ? kWarps : 1][32];
-    __shared__ int s_last;
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int row = blockIdx.x / p.parts, part = blockIdx.x % p.parts;
-    const T *x = reinterpret_cast<const T *>(p.x) + (long long)row * p.stride;
-    const int begin = min(p.vocab, part * p.chunk), end = min(p.vocab, begin + p.chunk);
-
-    Sums s{-INFINITY, 0.f, 0.f};
-    unsigned long long list = 0;                           // (below every key)
-    float least = -INFINITY;                               // the k-th value of this warp's list, and its index
-    uint32_t least_at = 0xffffffffu;
-
-    auto take = [&](const float (&v)[V], uint32_t at, int count) {       // `count` values from index `at` on; warp-uniform flow where TOP
-        float top = -INFINITY;
+// 16 bytes of logits
+template <class T> struct Vec;
+template <> struct Vec<float> {
+    static constexpr int V = 4;
+    static __device__ __forceinline__ void values(const uint4 &r, float (&v)[4]) {
+        v[0] = __uint_as_float(r.x); v[1] = __uint_as_float(r.y); v[2] = __uint_as_float(r.z); v[3] = __uint_as_float(r.w);
+    }
+};
+template <> struct Vec<__half> {
+    static constexpr int V = 8;
+    static __device__ __forceinline__ void values(const uint4 &r, float (&v)[8]) {
+        const uint32_t w[4] = {r.x, r.y, r.z, r.w};
 #pragma unroll
-        for (int e = 0; e < V; ++e) top = fmaxf(top, v[e]);
-        if (top > s.m) s.to(top);
-        const float m = s.m == -INFINITY ? 0.f : s.m;
-#pragma unroll
-        for (int e = 0; e < V; ++e) {
-            const float d = v[e] - m, w = ex2(d * kLog2e);
-            s.l += w;
-            s.u = fmaf(w, fmaxf(d, -1e30f), s.u);          // (0 times -infinity is 0)
+        for (int i = 0; i < 4; ++i) {
+            const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&w[i]));
+            v[2 * i] = f.x;
+            v[2 * i + 1] = f.y;
         }
-        if (TOP) {
-            const bool better = count > 0 && (top > least || (top == least && at < least_at));
-            if (__any_sync(kFull, better)) {
+    }
+};
+template <> struct Vec<__nv_bfloat16> {
+    static constexpr int V = 8;
+    static __device__ __forceinline__ void values(const uint4 &r, float (&v)[8]) {
+        const uint32_t w[4] = {r.x, r.y, r.z, r.w};
 #pragma unroll
-                for (int e = 0; e < V; ++e) {
-                    const unsigned long long bar = __shfl_sync(kFull, list, p.k - 1);
-                    unsigned long long key = e < count ? key_of(v[e], at + e) : 0;
-                    if (key <= bar) key = 0;
-                    unsigned hits = __ballot_sync(kFull, key != 0);
-                    if (__popc(hits) > 6) {
-                        list = merge_sorted(list, sort_warp(key, lane), lane);
-                    } else {
-                        while (hits) {
-                            list = insert(list, __shfl_sync(kFull, key, __ffs(hits) - 1), lane);
-                            hits &= hits - 1;
-                        }
-                    }
-                }
-                const unsigned long long bar = __shfl_sync(kFull, list, p.k - 1);
-                if (bar) {
-                    least = value_of(bar);
-                    least_at = ~(uint32_t)bar;
-                }
+        for (int i = 0; i < 4; ++i) {
+            v[2 * i] = __uint_as_float(w[i] << 16);
+            v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+        }
+    }
+};
+
+__device__ __forceinline__ uint32_t ordered(float x) {      // larger values, larger numbers; NaN is not asked for
+    const uint32_t u = __float_as_uint(x + 0.f);
+    return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
+}
+
+// A part of a row: its elements, and how threads take them: those before the first 16-byte boundary and behind the last one by one,
+// by the first warp's lanes; the others 16 bytes at a time, thread by thread.
+template <class T>
+struct Part {
+    static constexpr int V = Vec<T>::V;
+    const T *x;
+    int begin, head, body, tail0, end;
+    __device__ __forceinline__ Part(const T *row, int b, int e) : x(row), begin(b), end(e) {
+        head = min((int)((16 - (reinterpret_cast<uintptr_t>(row + b) & 15u)) % 16 / sizeof(T)), e - b);
+        body = (e - b - head) / V;
+        tail0 = b + head + body * V;
+    }
+    __device__ __forceinline__ int single(int tid) const {   // index of the thread's single element, -1: none
+        return tid < head ? begin + tid : (tid < head + end - tail0 ? tail0 + tid - head : -1);
+    }
+    __device__ __forceinline__ const uint4 *vectors() const { return reinterpret_cast<const uint4 *>(x + begin + head); }
+    __device__ __forceinline__ int index(int vector) const { return begin + head + vector * V; }
+};
+
+// The k largest keys of the part, the plain way: every warp keeps a sorted list.  Any number of equal values; used where the candidates of
+// the quick way (below) are too many.
+template <class T>
+__device__ __noinline__ void scan_lists(const Part<T> part, int k, unsigned long long (*lists)[32], unsigned long long *out) {
+    constexpr int V = Part<T>::V;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    unsigned long long list = 0, bar = 0;
+    auto take = [&](unsigned long long key) {
+        if (key <= bar) key = 0;
+        unsigned hits = __ballot_sync(kFull, key != 0);
+        if (!hits) return;
+        if (__popc(hits) > 6) {
+            list = merge_sorted(list, sort_warp(key, lane), lane);
+        } else {
+            while (hits) {
+                list = insert(list, __shfl_sync(kFull, key, __ffs(hits) - 1), lane);
+                hits &= hits - 1;
             }
         }
+        bar = __shfl_sync(kFull, list, k - 1);
     };
-
-    // values before the first 16-byte boundary and behind the last are taken one by one (a thread has at most one of them)
-    const int head = min((int)((16 - (reinterpret_cast<uintptr_t>(x + begin) & 15u)) % 16 / sizeof(T)), end - begin);
-    const int body = (end - begin - head) / V, tail0 = begin + head + body * V;
     if (warp == 0) {
-        float v[V];
-#pragma unroll
-        for (int e = 0; e < V; ++e) v[e] = -INFINITY;
-        const int at = lane < head ? begin + lane : tail0 + lane - head;
-        const bool there = lane < head + (end - tail0);
-        if (there) v[0] = as_float(x[at]);
-        take(v, at, there ? 1 : 0);
+        const int at = part.single(lane);
+        take(at >= 0 ? key_of((float)part.x[at], at) : 0);
     }
-    const uint4 *xb = reinterpret_cast<const uint4 *>(x + begin + head);
-    for (int i0 = warp * 32; i0 < body; i0 += kThreads * L) {
+    for (int i0 = warp * 32; i0 < part.body; i0 += kThreads) {
+        const int i = i0 + lane;
+        float v[V];
+        if (i < part.body) Vec<T>::values(part.vectors()[i], v);
+#pragma unroll
+        for (int e = 0; e < V; ++e) take(i < part.body ? key_of(v[e], part.index(i) + e) : 0);
+    }
+    lists[warp][lane] = list;
+    __syncthreads();
+    if (warp == 0) {
+        for (int w = 1; w < kWarps; ++w) list = merge_sorted(list, lists[w][lane], lane);
+        out[lane] = list;
+    }
+    __syncthreads();
+}
+
+// The 32 largest of `count` different keys in falling order, 0 behind them: a key's place is the number of keys above it.
+__device__ __forceinline__ void rank_keys(const unsigned long long *keys, int count, unsigned long long *out) {
+    if (threadIdx.x < 32) out[threadIdx.x] = 0;
+    __syncthreads();
+    for (int i = threadIdx.x; i < count; i += kThreads) {
+        const unsigned long long mine = keys[i];
+        int above = 0;
+#pragma unroll 8
+        for (int j = 0; j < count; ++j) above += keys[j] > mine;
+        if (above < 32) out[above] = mine;
+    }
+    __syncthreads();
+}
+
+// Top tokens the quick way.  A thread knows the largest of its elements.  With j = ceil(k / 8), the j-th largest of a warp's 32 such
+// values, and the least of these over the 8 warps, is a bound that at least 8 j >= k elements of the part reach; it is raised by halving
+// while k threads' largest values reach it.  Only the elements of those threads are looked at again, and what reaches the bound
+// (little more than k of random values) is ranked.
+template <class T, bool TOP>
+__global__ void __launch_bounds__(kThreads) logprobs_kernel(const __grid_constant__ Args p) {
+    constexpr int V = Vec<T>::V;
+    constexpr int L = 32 / V;                              // loads of a step: 32 elements a thread
+    __shared__ float s_l[kWarps], s_u[kWarps];
+    __shared__ uint32_t s_top[kWarps], s_bar[kWarps];
+    __shared__ unsigned long long s_keys[TOP ? kCandidates : 1], s_list[32];
+    __shared__ int s_count, s_threads, s_last;
+    __shared__ unsigned char s_hot[TOP ? kThreads : 1];
+    static_assert(!TOP || kCandidates >= kWarps * 32, "the lists of scan_lists lie there too");
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int row = blockIdx.x / p.parts, at_part = blockIdx.x % p.parts;
+    const T *x = reinterpret_cast<const T *>(p.x) + (long long)row * p.stride;
+    const int begin = min(p.vocab, at_part * p.chunk);
+    const Part<T> part(x, begin, min(p.vocab, begin + p.chunk));
+
+    // ---- one pass: m, the largest value so far; l and u, sums of e^(x - m) and e^(x - m) (x - m)
+    Sums s{-INFINITY, 0.f, 0.f};
+    auto take = [&](const float (&v)[V]) {
+        float top = v[0];
+#pragma unroll
+        for (int e = 1; e < V; ++e) top = fmaxf(top, v[e]);
+        if (top > s.m) s.to(top);
+        const float m = s.m == -INFINITY ? 0.f : -s.m;
+        const uint64_t m2 = pair2(m, m), scale = pair2(kLog2e, kLog2e);
+        uint64_t l = pair2(s.l, 0.f), u = pair2(s.u, 0.f);
+#pragma unroll
+        for (int e = 0; e < V; e += 2) {
+            const uint64_t d = add2(pair2(v[e], v[e + 1]), m2);
+            const float2 y = unpair2(mul2(d, scale)), f = unpair2(d);
+            const uint64_t w = pair2(ex2(y.x), ex2(y.y));
+            l = add2(l, w);
+            u = fma2(w, pair2(fmaxf(f.x, -1e30f), fmaxf(f.y, -1e30f)), u);       // (0 times -infinity is 0)
+        }
+        const float2 a = unpair2(l), b = unpair2(u);
+        s.l = a.x + a.y;
+        s.u = b.x + b.y;
+    };
+    const uint4 *const xb = part.vectors();
+    for (int i0 = tid; i0 < part.body; i0 += kThreads * L) {
         uint4 raw[L];
 #pragma unroll
-        for (int j = 0; j < L; ++j) {
-            const int i = i0 + j * kThreads + lane;
-            if (i < body) raw[j] = __ldcs(xb + i);
-        }
+        for (int j = 0; j < L; ++j)
+            if (i0 + j * kThreads < part.body) raw[j] = __ldg(xb + i0 + j * kThreads);
 #pragma unroll
-        for (int j = 0; j < L; ++j) {
-            const int i = i0 + j * kThreads + lane;
-            if (i0 + j * kThreads >= body) break;
-            float v[V];
-            const T *e = reinterpret_cast<const T *>(&raw[j]);
+        for (int j = 0; j < L; ++j)
+            if (i0 + j * kThreads < part.body) {
+                float v[V];
+                Vec<T>::values(raw[j], v);
+                take(v);
+            }
+    }
+    const int single = part.single(tid);
+    if (single >= 0) {
+        float v[V];
 #pragma unroll
-            for (int k = 0; k < V; ++k) v[k] = i < body ? as_float(e[k]) : -INFINITY;
-            take(v, (uint32_t)(begin + head + i * V), i < body ? V : 0);
-        }
+        for (int e = 1; e < V; ++e) v[e] = -INFINITY;
+        v[0] = (float)x[single];
+        take(v);
     }
 
-    // ---- the block's sums and list
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1)
-        s.add(Sums{__shfl_xor_sync(kFull, s.m, o), __shfl_xor_sync(kFull, s.l, o), __shfl_xor_sync(kFull, s.u, o)});
-    if (lane == 0) s_sums[warp] = s;
-    if (TOP) s_lists[warp][lane] = list;
-    __syncthreads();
-    if (warp != 0) return;                                 // (what is left is one warp's work)
-    s = s_sums[0];
-    for (int w = 1; w < kWarps; ++w) s.add(s_sums[w]);
-    if (TOP)
-        for (int w = 1; w < kWarps; ++w) list = merge_sorted(list, s_lists[w][lane], lane);
-    if (p.parts > 1) {
-        const size_t mine = (size_t)row * p.parts + part;
-        if (lane == 0) {
-            p.sums[mine * 3] = s.m;
-            p.sums[mine * 3 + 1] = s.l;
-            p.sums[mine * 3 + 2] = s.u;
+    // ---- the block's largest value, and the bound
+    uint32_t mine = ordered(s.m);
+    const uint32_t warp_top = __reduce_max_sync(kFull, mine);
+    if (lane == 0) s_top[warp] = warp_top;
+    if (TOP) {
+        uint32_t left = mine, bar = warp_top;
+        for (int j = (p.k + kWarps - 1) / kWarps; j > 1; --j) {                   // (one lane of those that have the largest leaves)
+            const unsigned has = __ballot_sync(kFull, left == bar);
+            if (lane == __ffs(has) - 1) left = 0;
+            bar = __reduce_max_sync(kFull, left);
         }
-        if (TOP) p.lists[mine * 32 + lane] = list;
-        __threadfence();
-        __syncwarp();
-        if (lane == 0) {
+        if (lane == 0) s_bar[warp] = bar;
+        if (tid == 0) s_count = s_threads = 0;
+    }
+    __syncthreads();
+    uint32_t top = s_top[0], bar = s_bar[0];
+#pragma unroll
+    for (int w = 1; w < kWarps; ++w) {
+        top = max(top, s_top[w]);
+        if (TOP) bar = min(bar, s_bar[w]);
+    }
+    s.to(value_of((unsigned long long)top << 32));
+    float l = jq::warp_sum(s.l), u = jq::warp_sum(s.u);
+    if (lane == 0) {
+        s_l[warp] = l;
+        s_u[warp] = u;
+    }
+    if (TOP) {
+        auto offer = [&](float v, int at) {
+            const unsigned long long key = key_of(v, at);
+            if ((uint32_t)(key >> 32) < bar) return;
+            const int i = atomicAdd(&s_count, 1);
+            if (i < kCandidates) s_keys[i] = key;
+        };
+        // a better bound by halving: as many threads as may be reach it, as long as these are at least k
+        uint32_t high = top;
+        int threads = __syncthreads_count(mine >= bar);
+        for (int i = 0; i < 16 && bar < high && threads > p.k + 8; ++i) {
+            const uint32_t mid = bar + (high - bar + 1) / 2;
+            const int c = __syncthreads_count(mine >= mid);
+            if (c >= p.k) {
+                bar = mid;
+                threads = c;
+            } else {
+                high = mid - 1;
+            }
+        }
+        if (mine >= bar) {
+            s_hot[atomicAdd(&s_threads, 1)] = (unsigned char)tid;
+            if (single >= 0) offer((float)x[single], single);
+        }
+        __syncthreads();
+        // their vectors, by all threads
+        const int rounds = (part.body + kThreads - 1) / kThreads;
+        for (int q = tid; q < threads * rounds; q += kThreads) {
+            const int i = s_hot[q % threads] + q / threads * kThreads;
+            if (i >= part.body) continue;
+            float v[V];
+            Vec<T>::values(__ldg(xb + i), v);
+            float most = v[0];
+#pragma unroll
+            for (int e = 1; e < V; ++e) most = fmaxf(most, v[e]);
+            if (ordered(most) < bar) continue;
+#pragma unroll
+            for (int e = 0; e < V; ++e) offer(v[e], part.index(i) + e);
+        }
+    }
+    __syncthreads();
+    float m = s.m;
+    l = u = 0.f;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+        l += s_l[w];
+        u += s_u[w];
+    }
+    if (TOP) {
+        const int count = s_count;
+        if (count <= kCandidates) rank_keys(s_keys, count, s_list);
+        else scan_lists(part, p.k, reinterpret_cast<unsigned long long(*)[32]>(s_keys), s_list);
+    }
+    if (p.parts > 1) {
+        // the row's last part adds all of them, in an order that does not depend on which it is
+        const size_t first = (size_t)row * p.parts, own = first + at_part;
+        if (tid == 0) {
+            p.sums[own * 3] = m;
+            p.sums[own * 3 + 1] = l;
+            p.sums[own * 3 + 2] = u;
+        }
+        if (TOP && tid < 32) p.lists[own * 32 + tid] = s_list[tid];
+        if (tid < 32) __threadfence();
+        __syncthreads();
+        if (tid == 0) {
             s_last = atomicAdd(p.counters + row, 1) == p.parts - 1;
             if (s_last) p.counters[row] = 0;
+            s_count = 0;
         }
-        __syncwarp();
+        __syncthreads();
         if (!s_last) return;
         __threadfence();
-        // the row's last part adds all of them, in their order
-        const size_t first = (size_t)row * p.parts;
+        float pm = -INFINITY, pl = 0.f, pu = 0.f;
+        unsigned long long least = 0;                      // the largest of the parts' k-th keys: k keys reach it
         s = Sums{-INFINITY, 0.f, 0.f};
-        list = 0;
-        for (int w = 0; w < p.parts; ++w) {
-            const float *o = p.sums + (first + w) * 3;
-            s.add(Sums{__ldcg(o), __ldcg(o + 1), __ldcg(o + 2)});
-            if (TOP) list = merge_sorted(list, __ldcg(p.lists + (first + w) * 32 + lane), lane);
+        for (int i = tid; i < p.parts; i += kThreads) {
+            const float *o = p.sums + (first + i) * 3;
+            pm = __ldcg(o);
+            pl = __ldcg(o + 1);
+            pu = __ldcg(o + 2);
+            s.add(Sums{pm, pl, pu});
+            if (TOP) least = max64(least, __ldcg(p.lists + (first + i) * 32 + p.k - 1));
         }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) {
+            s.add(Sums{__shfl_xor_sync(kFull, s.m, o), __shfl_xor_sync(kFull, s.l, o), __shfl_xor_sync(kFull, s.u, o)});
+            if (TOP) least = max64(least, __shfl_xor_sync(kFull, least, o));
+        }
+        __shared__ Sums s_sums[kWarps];
+        __shared__ unsigned long long s_least[kWarps];
+        if (lane == 0) {
+            s_sums[warp] = s;
+            s_least[warp] = least;
+        }
+        __syncthreads();
+        s = s_sums[0];
+#pragma unroll
+        for (int w = 1; w < kWarps; ++w) {
+            s.add(s_sums[w]);
+            if (TOP) least = max64(least, s_least[w]);
+        }
+        if (TOP) {
+            least = max64(least, s_least[0]);
+            for (int i = tid; i < p.parts * 32; i += kThreads) {
+                const unsigned long long key = __ldcg(p.lists + first * 32 + i);
+                if (!key || key < least) continue;
+                const int c = atomicAdd(&s_count, 1);
+                if (c < kCandidates) s_keys[c] = key;
+            }
+            __syncthreads();
+            const int count = s_count;
+            if (count <= kCandidates) {
+                rank_keys(s_keys, count, s_list);
+            } else if (warp == 0) {                        // (many parts whose lists lie between one another)
+                unsigned long long list = 0;
+                for (int i = 0; i < p.parts; ++i) list = merge_sorted(list, __ldcg(p.lists + (first + i) * 32 + lane), lane);
+                s_list[lane] = list;
+                __syncwarp();
+            }
+        }
+        m = s.m;
+        l = s.l;
+        u = s.u;
     }
-    const float log_l = logf(s.l);
-    auto logprob = [&](float v) { return s.m == -INFINITY ? (s.l == 0.f ? -INFINITY : s.l) : v - s.m - log_l; };
+    if (warp != 0) return;
+    const float log_l = logf(l);
+    auto logprob = [&](float v) { return m == -INFINITY ? (l == 0.f ? -INFINITY : l) : v - m - log_l; };
     if (lane == 0) {
         const long long token = p.tokens[row];
-        p.logprob[row] = token < 0 ? 0.f : (token >= p.vocab ? __int_as_float(0x7fffffff) : logprob(as_float(x[token])));
-        if (p.entropy) p.entropy[row] = s.m == -INFINITY && s.l == 0.f ? 0.f : log_l - s.u / s.l;
+        p.logprob[row] = token < 0 ? 0.f : (token >= p.vocab ? __int_as_float(0x7fffffff) : logprob((float)x[token]));
+        if (p.entropy) p.entropy[row] = m == -INFINITY && l == 0.f ? 0.f : log_l - u / l;
     }
     if (TOP && lane < p.k) {
-        p.top_logprob[(size_t)row * p.k + lane] = logprob(value_of(list));
-        p.top_token[(size_t)row * p.k + lane] = (long long)(uint32_t)~(uint32_t)list;
+        const unsigned long long key = s_list[lane];
+        p.top_logprob[(size_t)row * p.k + lane] = logprob(value_of(key));
+        p.top_token[(size_t)row * p.k + lane] = (long long)(uint32_t)~(uint32_t)key;
     }
 }
 
-// Parts of a row: one where the rows fill the chip by themselves.
+constexpr int kStep = 2048;                    // elements that a part has at least
+
+// Parts of a row: as many as fill the chip where there are few rows, one where the rows fill it by themselves.  (Halves that would fill a
+// partly empty last wave cost more than it: 2047 rows of 32003 bf16 33 us whole, 46 us in halves; 1024 of 131072 fp32 108 and 115.)
 static int parts_of(int rows, int vocab) {
     const int fill = 4 * jq_sm_count() < kJqCounters ? 4 * jq_sm_count() : kJqCounters;
-    const int steps = (vocab + 2047) / 2048;
-    int parts = rows >= fill ? 1 : fill / rows;
-    return parts < steps ? parts : steps;
+    const int most = (vocab + kStep - 1) / kStep, parts = rows >= fill ? 1 : fill / rows;
+    return parts < most ? parts : most;
 }
 
 }  // namespace jqlp
@@ -267,7 +500,7 @@ extern "C" int jq_token_logprobs(const void *logits, int64_t row_stride, int row
     a.logprob = logprob; a.entropy = entropy_or_null; a.top_logprob = top_logprob_or_null;
     a.top_token = reinterpret_cast<long long *>(top_token_or_null);
     a.rows = rows; a.vocab = vocab; a.k = top; a.parts = parts_of(rows, vocab);
-    a.chunk = ((vocab + a.parts - 1) / a.parts + 2047) / 2048 * 2048;
+    a.chunk = ((vocab + a.parts - 1) / a.parts + 511) / 512 * 512;
     unsigned char *ws = reinterpret_cast<unsigned char *>(workspace);
     if (a.parts > 1) {
         a.counters = reinterpret_cast<int *>(ws + kJqHeader);

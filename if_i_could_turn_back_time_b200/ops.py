@@ -197,6 +197,9 @@ def check_status(raise_on_error: bool = True) -> int:
     return worst
 
 
+_PARTS_DATA = 1024 + 4 * 1024        # status word and counters of such a buffer, which start at zero; behind them partial sums
+
+
 def _parts_workspace(device, nbytes: int, stream: int):
     """(tensor to keep, address, size) of the scratch of a call on the current stream whose last CTA adds up what the others
     left: this thread's and stream's "parts" buffer, or, while a graph is captured, zeros of the call's own from the graph's
@@ -204,7 +207,7 @@ def _parts_workspace(device, nbytes: int, stream: int):
     found them, at zero."""
     if _capturing(stream):
         t = torch.empty(nbytes, dtype=torch.uint8, device=device)
-        t[:8192].zero_()
+        t[:_PARTS_DATA].zero_()
     else:
         t = _ws_cache().get((device.index, stream, "parts"))
         if t is None or t.numel() < nbytes:
