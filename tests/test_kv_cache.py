@@ -379,6 +379,57 @@ def test_append_and_read_bit_for_bit(case, values):
 
 
 @gpu
+@pytest.mark.parametrize("fmt", ["int8", "e4m3"])
+def test_quotients_near_the_middle_of_two_codes(fmt):
+    """Values at and beside every boundary between two codes, for scales of many mantissas: the kernel's product with the
+    reciprocal has to end where the quotient does."""
+    H, D, T = 64, 128, 128
+    cache = jq.KVCache.empty(1, H, D, block_size=T, fmt=fmt, device=DEV)
+    gen = torch.Generator().manual_seed(2)
+    grid = oracle.e4m3_values()[:127] if fmt == "e4m3" else np.arange(128.0)
+    middle = (grid[1:] + grid[:-1]) / 2
+    x = torch.empty(T, H, D)
+    for h in range(H):
+        top = np.float32(np.exp(torch.randn((), generator=gen).item() * 20))
+        scale = np.float32(top / oracle.TOP[fmt])
+        near = (middle * float(scale)).astype(np.float32)
+        steps = torch.randint(-6, 7, (T, D), generator=gen).numpy().astype(np.int32)
+        pick = torch.randint(0, len(near), (T, D), generator=gen).numpy()
+        x[:, h] = torch.from_numpy((near[pick].view(np.int32) + steps).view(np.float32) * np.sign(steps + 0.5).astype(np.float32)).clamp(-float(top), float(top))
+        x[0, h, 0] = float(top)
+    table, lens = torch.zeros(1, 1, dtype=torch.int32, device=DEV), torch.tensor([T], dtype=torch.int32, device=DEV)
+    cache.append(x.to(DEV), -x.to(DEV), table, lens)
+    got = cache.keys.cpu().numpy().reshape(H, T * D), cache.values.cpu().numpy().reshape(H, T * D)
+    for h in range(H):
+        for what, codes, sign in (("keys", got[0], 1), ("values", got[1], -1)):
+            want, _ = oracle.append_block(np.zeros((T, D), np.uint8), 0, 0, sign * x[:, h].numpy(), fmt)
+            assert np.array_equal(codes[h][oracle.places(T, D, what)], want)
+
+
+@gpu
+def test_more_prompts_than_are_planned_at_once():
+    """2500 short prompts: over 32 segments for every CTA of the prompt kernel; and more new tokens than max_new names (tokens beyond it
+    may be left out by append, and nothing else happens)."""
+    S, H, D, T, new = 2500, 2, 64, 64, 33
+    lengths = [new + i % 32 for i in range(S)]
+    cache, table, dense = _filled(lengths, H, D, T, "int8", 5)
+    q = torch.randn(S * new, H, D, generator=torch.Generator().manual_seed(6)).half().to(DEV)
+    table, lens = table.to(DEV), torch.tensor(lengths, dtype=torch.int32, device=DEV)
+    got = cache.attend(q, table, lens)
+    for i in range(0, S, 83):
+        _check_attend(q[i * new:(i + 1) * new], got[i * new:(i + 1) * new], None, {k: [v[i]] for k, v in dense.items()}, [lengths[i]], [new], 0)
+    assert torch.isfinite(got).all()
+    starts = _starts([new] * S).to(DEV)
+    for few in (1, 3, 40):                                     # any max_new gives every query its output
+        assert torch.isfinite(cache.attend(q, table, lens, starts, max_new=few)).all()
+    keys = cache.keys.clone()
+    k = torch.randn(S * new, H, D, device=DEV)
+    cache.append(k, k, table, lens, starts, max_new=5)
+    changed = (cache.keys != keys).view(cache.blocks, -1).any(1)
+    assert changed.any() and ops.check_status(raise_on_error=False) == 0
+
+
+@gpu
 def test_append_writes_nothing_where_the_table_names_nothing():
     cache, table, _ = _filled([100, 60], 2, 64, 16, "int8", 3)
     keys, scales = cache.keys.clone(), cache.key_scales.clone()
