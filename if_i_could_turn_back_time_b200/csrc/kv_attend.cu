@@ -5,8 +5,7 @@ namespace jqkv {
 
 using namespace jqta;
 
-constexpr int kFewParts = 8;       // of a pair: up to here they are added as they are read
-constexpr int kNear = 16;          // units
+constexpr int kNear = 16;          // units: how far a boundary between CTAs moves to a pair's begin or end, at most half a CTA's share (see snap)
 constexpr int kUnit = 64;          // keys: what work is dealt out in
 constexpr int kRing = 16384;       // bytes of a warp's ring: two stages of 32 keys at D = 128, three CTAs on an SM
 
@@ -44,67 +43,23 @@ __device__ __forceinline__ Share share_of(const AttendArgs &p, int i) {
     return s;
 }
 
-// The parts of a pair, of the CTAs w0 .. w1, added in their order; outputs.  Parts of many CTAs: their factors first, a warp per row, so that
-// the loads of the sums need not wait for one another.  (Not inlined: its registers are not the main loop's.)
+// The parts of a pair, of the CTAs w0 .. w1, added in their order; outputs.  (Not inlined: its registers are not the main loop's.  Forming all
+// factors first, so that the loads of the sums wait for nothing, took as long for 3 to 55 parts.)
 template <int D, int TR, int THREADS>
-__device__ __noinline__ void add_parts(const AttendArgs &p, float *factor, float *s_m, float *s_l, int w0, int w1, int rows, int r0, int row0, int h) {
+__device__ __noinline__ void add_parts(const AttendArgs &p, int w0, int w1, int rows, int r0, int row0, int h) {
     constexpr int kPart = TR * D + 2 * TR;
-    const int tid = threadIdx.x, lane = tid & 31, parts = w1 - w0 + 1;
-    auto of = [&](int w) { return p.parts + (size_t)(2 * w + (w == w0 ? 1 : 0)) * kPart; };
-    auto finish = [&](int r, int d, const float4 &v, float m, float l) {
-        const int fr = r0 + r;
+    for (int e = threadIdx.x; e < rows * (D / 4); e += THREADS) {
+        const int r = e / (D / 4), d = e % (D / 4) * 4, fr = r0 + r;
+        float m = -INFINITY, l = 0.f;
+        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+        for (int w = w0; w <= w1; ++w) {
+            const float *x = p.parts + (size_t)(2 * w + (w == w0 ? 1 : 0)) * kPart;
+            add_part(m, l, v, __ldcg(x + TR * D + r), __ldcg(x + TR * D + TR + r), __ldcg(reinterpret_cast<const float4 *>(x + r * D + d)));
+        }
         const size_t at = ((size_t)(row0 + fr / p.G) * p.H * p.G + h * p.G + fr % p.G) * D + d;
         store4(p, at, v, inverse(l));
         if (d == 0 && p.lse) p.lse[at / D] = lse_of(m, l);
-    };
-    if (parts <= kFewParts) {
-        for (int e = tid; e < rows * (D / 4); e += THREADS) {
-            const int r = e / (D / 4), d = e % (D / 4) * 4;
-            float m = -INFINITY, l = 0.f;
-            float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-            for (int w = w0; w <= w1; ++w) {
-                const float *x = of(w);
-                add_part(m, l, v, __ldcg(x + TR * D + r), __ldcg(x + TR * D + TR + r), __ldcg(reinterpret_cast<const float4 *>(x + r * D + d)));
-            }
-            finish(r, d, v, m, l);
-        }
-        return;
-    }
-    for (int r = tid >> 5; r < rows; r += THREADS / 32) {
-        float m = -INFINITY, l = 0.f;
-        for (int x = lane; x < parts; x += 32) m = fmaxf(m, __ldcg(of(w0 + x) + TR * D + r));
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-        const float ref = m == -INFINITY ? 0.f : m;
-        for (int x = lane; x < parts; x += 32) {
-            const float f = ex2(__ldcg(of(w0 + x) + TR * D + r) - ref);
-            factor[x * TR + r] = f;                        // [part][row], in place of the rings
-            l = fmaf(__ldcg(of(w0 + x) + TR * D + TR + r), f, l);
-        }
-        l = jq::warp_sum(l);
-        if (lane == 0) {
-            s_m[r] = m;
-            s_l[r] = l;
-        }
-    }
-    __syncthreads();
-    for (int e = tid; e < rows * (D / 4); e += THREADS) {
-        const int r = e / (D / 4), d = e % (D / 4) * 4;
-        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-        for (int x0 = 0; x0 < parts; x0 += 16) {
-            float4 y[16];
-#pragma unroll
-            for (int x = 0; x < 16; ++x)
-                if (x0 + x < parts) y[x] = __ldcg(reinterpret_cast<const float4 *>(of(w0 + x0 + x) + r * D + d));
-#pragma unroll
-            for (int x = 0; x < 16; ++x) {
-                if (x0 + x >= parts) break;
-                const float f = factor[(x0 + x) * TR + r];
-                v.x = fmaf(y[x].x, f, v.x); v.y = fmaf(y[x].y, f, v.y); v.z = fmaf(y[x].z, f, v.z); v.w = fmaf(y[x].w, f, v.w);
-            }
-        }
-        finish(r, d, v, s_m[r], s_l[r]);
     }
 }
 
@@ -193,7 +148,8 @@ __global__ void __launch_bounds__(warps_of(NT, WIDE) * 32, WIDE ? 1 : (NT > 2 ? 
         const int pair = (int)quotient(cur - seq_at, sh.units);
         const long long pair_at = seq_at + (long long)pair * sh.units, pair_end = pair_at + sh.units;
         // A boundary between two CTAs that is near a pair's begin or end is taken to lie there: a few units more for one of them are
-        // less than a further segment.
+        // less than a further segment (one row of 517 tokens, 32 heads: 9.7 us, 15.9 with boundaries as they fall; 64 sequences of
+        // 257 to 8191 tokens, 8 key heads: 100 and 107).
         auto snap = [&](long long b) {
             const long long off = b - pair_at, rest = pair_end - b;
             return off <= near && off <= rest ? pair_at : (rest <= near ? pair_end : b);
@@ -537,7 +493,7 @@ __global__ void __launch_bounds__(warps_of(NT, WIDE) * 32, WIDE ? 1 : (NT > 2 ? 
             __syncthreads();
             if (s_last) {
                 __threadfence();
-                add_parts<D, TR, kWarps * 32>(p, reinterpret_cast<float *>(smem), s_m[0], s_l[0], w0, w1, rows, r0, sh.row0, h);
+                add_parts<D, TR, kWarps * 32>(p, w0, w1, rows, r0, sh.row0, h);
             }
         }
         fence_async_smem();                                    // the ring was written to by threads; copies land in it next
@@ -560,18 +516,28 @@ static int grid_of(int NT, bool wide) {
 }
 // Tiles of 8 query rows, by the rows that a key head has in a call.
 static int tiles_of_rows(long long rows) { return rows <= 8 ? 1 : (rows <= 16 ? 2 : (rows <= 24 ? 3 : 4)); }
-// With fewer pairs (sequence, key head, tile of rows) than SMs every pair is cut anyway, and what counts is how many parts come of it.
-static bool wide_of(long long pairs) { return 8 * pairs <= jq_sm_count(); }
-
-constexpr int kFewRows = 32;       // query rows of a key head up to which attend_kernel is used
-constexpr int kLeastUnits = 6, kLeastWide = 6;     // units that a CTA takes at least: a stage for each warp
+// Few pairs (sequence, key head) are cut into many parts, one for a CTA, and added by the last of them: CTAs of all an SM's warps leave a third
+// as many parts.  us, wide / narrow, 64 query and 8 key heads of 128: 131071 tokens 61 / 70, eight sequences of 16000 54 / 61, four
+// new tokens behind 16000 48 / 70.  With about as many pairs as SMs narrow CTAs hide one another's begin and end: 16 sequences of up to
+// 4000 tokens, 3 to 5 new, 8 key heads of 64: 51 / 36.
+static bool wide_of(long long pairs) { return 2 * pairs <= jq_sm_count(); }
+// Query rows of a key head up to which attend_kernel is used, the kernel for prompts from there on.  us, attend_kernel / prompt_kernel, 64
+// query and 8 key heads:
+//     rows                              16         24         32         40         64
+//     16 sequences of 2000, D = 128     45 / 54    43 / 55    70 / 53    90 / 54    91 / 54
+//     1 of 16384, D = 128               30 / 44               49 / 48               70 / 48
+//     64 of 1000, D = 64                39 / 91               50 / 89    91 / 92    94 / 91
+static long long few_rows(int D) { return D == 64 ? 32 : 24; }
+// Units that a CTA takes at least, about a stage for each warp: one row of 517 tokens, 32 heads: 9.7 us, 10.2 with two units, 16 with twelve.
+constexpr int kLeast = 6;
 
 typedef void (*attend_fn)(const AttendArgs);
 template <int D, bool E4M3, int NT>
 static attend_fn pick(bool wide) { return wide ? attend_kernel<D, E4M3, NT, true> : attend_kernel<D, E4M3, NT, false>; }
 template <int D, bool E4M3>
 static attend_fn pick(int NT, bool wide) {
-    return NT == 1 ? pick<D, E4M3, 1>(wide) : (NT == 2 ? pick<D, E4M3, 2>(wide) : (NT == 3 ? pick<D, E4M3, 3>(wide) : pick<D, E4M3, 4>(wide)));
+    if (NT == 4) return pick<64, E4M3, 4>(wide);           // (no more than 24 rows at D = 128, see few_rows)
+    return NT == 1 ? pick<D, E4M3, 1>(wide) : (NT == 2 ? pick<D, E4M3, 2>(wide) : pick<D, E4M3, 3>(wide));
 }
 template <int D>
 static attend_fn pick(bool e4m3, int NT, bool wide) { return e4m3 ? pick<D, true>(NT, wide) : pick<D, false>(NT, wide); }
@@ -587,7 +553,7 @@ using namespace jqkv;
 extern "C" size_t jq_kv_attend_workspace_bytes(const jq_kv_cache *c, const jq_kv_batch *s, int q_heads) {
     if (check_cache(c, s) || q_heads <= 0) return 0;
     const long long rows = (long long)most_new(s) * (q_heads / c->kv_heads);
-    if (rows > kFewRows) return kJqData + prompt_workspace(c->head_dim);
+    if (rows > few_rows(c->head_dim)) return kJqData + prompt_workspace(c->head_dim);
     const int NT = tiles_of_rows(rows);
     return kJqData + 2 * (size_t)grid_of(NT, false) * NT * 8 * (c->head_dim + 2) * 4;        // (enough for wide CTAs, of which there are fewer)
 }
@@ -613,7 +579,9 @@ extern "C" int jq_kv_attend(const jq_kv_cache *c, const jq_kv_batch *s, const vo
     a.st = stride_q[0]; a.sh = stride_q[1];
     a.keys = reinterpret_cast<const uint8_t *>(c->keys); a.values = reinterpret_cast<const uint8_t *>(c->values);
     a.ks = c->key_scales; a.vs = c->value_scales;
-    a.H = c->kv_heads; a.G = q_heads / c->kv_heads; a.window = window; a.dtype = dtype;
+    a.H = c->kv_heads; a.G = q_heads / c->kv_heads;
+    a.window = (long long)window >= (long long)s->table_width * c->block_size ? 0 : window;      // (no sequence is longer)
+    a.dtype = dtype;
     a.scale = scale * kLog2e;
     unsigned char *ws = reinterpret_cast<unsigned char *>(workspace);
     a.status = reinterpret_cast<int *>(ws);
@@ -621,7 +589,7 @@ extern "C" int jq_kv_attend(const jq_kv_cache *c, const jq_kv_batch *s, const vo
     a.parts = reinterpret_cast<float *>(ws + kJqData);
     const long long rows = (long long)most_new(s) * a.G;
     const bool e4m3 = c->fmt == JQ_KV_E4M3;
-    if (rows > kFewRows) {
+    if (rows > few_rows(c->head_dim)) {
         a.least = 8;
         return prompt_launch(a, c->head_dim, e4m3, reinterpret_cast<cudaStream_t>(stream));
     }
@@ -631,7 +599,7 @@ extern "C" int jq_kv_attend(const jq_kv_cache *c, const jq_kv_batch *s, const vo
     const attend_fn kern = c->head_dim == 64 ? pick<64>(e4m3, NT, wide) : pick<128>(e4m3, NT, wide);
     static jq_contexts done[2][2][4][2];
     JQ_CUDA_TRY(jq_allow_smem(reinterpret_cast<const void *>(kern), smem, done[c->head_dim == 128][e4m3][NT - 1][wide]));
-    a.least = wide ? kLeastWide : kLeastUnits;
+    a.least = kLeast;
     kern<<<grid_of(NT, wide), warps_of(NT, wide) * 32, smem, reinterpret_cast<cudaStream_t>(stream)>>>(a);
     return jq_launch_status();
 }
