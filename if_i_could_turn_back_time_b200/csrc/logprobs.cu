@@ -230,8 +230,8 @@ __device__ __forceinline__ void rank_keys(const unsigned long long *keys, int co
 
 // Top tokens the quick way.  A thread knows the largest of its elements.  With j = ceil(k / 8), the j-th largest of a warp's 32 such
 // values, and the least of these over the 8 warps, is a bound that at least 8 j >= k elements of the part reach; it is raised by halving
-// while k threads' largest values reach it.  Only the elements of those threads are looked at again, and what reaches the bound
-// (little more than k of random values) is ranked.
+// while k threads' largest values reach it.  Only those threads look again, nearly always at the one 16-byte piece that had their largest, and
+// what reaches the bound (little more than k of random values) is ranked.
 template <class T, bool TOP>
 __global__ void __launch_bounds__(kThreads) logprobs_kernel(const __grid_constant__ Args p) {
     constexpr int V = Vec<T>::V;
@@ -250,11 +250,21 @@ __global__ void __launch_bounds__(kThreads) logprobs_kernel(const __grid_constan
 
     // ---- one pass: m, the largest value so far; l and u, sums of e^(x - m) and e^(x - m) (x - m)
     Sums s{-INFINITY, 0.f, 0.f};
-    auto take = [&](const float (&v)[V]) {
+    float second = -INFINITY;                              // the largest value outside the piece that has the largest, and that piece
+    int piece = -1;
+    auto take = [&](const float (&v)[V], int i) {
         float top = v[0];
 #pragma unroll
         for (int e = 1; e < V; ++e) top = fmaxf(top, v[e]);
-        if (top > s.m) s.to(top);
+        if (top > s.m) {
+            if (TOP) {
+                second = s.m;
+                piece = i;
+            }
+            s.to(top);
+        } else if (TOP) {
+            second = fmaxf(second, top);
+        }
         const float m = s.m == -INFINITY ? 0.f : -s.m;
         const uint64_t m2 = pair2(m, m), scale = pair2(kLog2e, kLog2e);
         uint64_t l = pair2(s.l, 0.f), u = pair2(s.u, 0.f);
@@ -281,7 +291,7 @@ __global__ void __launch_bounds__(kThreads) logprobs_kernel(const __grid_constan
             if (i0 + j * kThreads < part.body) {
                 float v[V];
                 Vec<T>::values(raw[j], v);
-                take(v);
+                take(v, i0 + j * kThreads);
             }
     }
     const int single = part.single(tid);
@@ -290,7 +300,7 @@ __global__ void __launch_bounds__(kThreads) logprobs_kernel(const __grid_constan
 #pragma unroll
         for (int e = 1; e < V; ++e) v[e] = -INFINITY;
         v[0] = (float)x[single];
-        take(v);
+        take(v, -1);                                       // (a single value is always looked at again by itself)
     }
 
     // ---- the block's largest value, and the bound
@@ -340,24 +350,27 @@ __global__ void __launch_bounds__(kThreads) logprobs_kernel(const __grid_constan
                 high = mid - 1;
             }
         }
-        if (mine >= bar) {
-            s_hot[atomicAdd(&s_threads, 1)] = (unsigned char)tid;
-            if (single >= 0) offer((float)x[single], single);
-        }
-        __syncthreads();
-        // their vectors, by all threads
-        const int rounds = (part.body + kThreads - 1) / kThreads;
-        for (int q = tid; q < threads * rounds; q += kThreads) {
-            const int i = s_hot[q % threads] + q / threads * kThreads;
-            if (i >= part.body) continue;
+        // what reaches it: a thread whose other pieces do not looks at one piece again; the others' pieces go to all threads
+        auto look = [&](int i) {
             float v[V];
             Vec<T>::values(__ldg(xb + i), v);
             float most = v[0];
 #pragma unroll
             for (int e = 1; e < V; ++e) most = fmaxf(most, v[e]);
-            if (ordered(most) < bar) continue;
+            if (ordered(most) < bar) return;
 #pragma unroll
             for (int e = 0; e < V; ++e) offer(v[e], part.index(i) + e);
+        };
+        if (mine >= bar) {
+            if (ordered(second) >= bar) s_hot[atomicAdd(&s_threads, 1)] = (unsigned char)tid;
+            else if (piece >= 0) look(piece);
+            if (single >= 0) offer((float)x[single], single);
+        }
+        __syncthreads();
+        const int hot = s_threads, rounds = (part.body + kThreads - 1) / kThreads;
+        for (int q = tid; q < hot * rounds; q += kThreads) {
+            const int i = s_hot[q % hot] + q / hot * kThreads;
+            if (i < part.body) look(i);
         }
     }
     __syncthreads();
