@@ -16,7 +16,7 @@ struct AttendArgs {
     float scale;                   // of the scores, times log2(e)
     int *status;
     int *counters;                 // one per CTA: parts of the pair that begins in it and is done elsewhere too
-    float *parts;                  // two per CTA: [rows][D] sums, [rows] maxima, [rows] weights
+    float *parts;                  // two per CTA: sums, [rows] maxima, [rows] weights (each kernel has an order of its own)
 };
 
 __device__ __forceinline__ float ex2(float x) {

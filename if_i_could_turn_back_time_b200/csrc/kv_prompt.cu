@@ -1,12 +1,16 @@
 // Attention over the 8-bit cache, many query rows per key head (prompts and parts of prompts): tcgen05.
 //
-// A CTA has 256 rows (query, head of the group) of a key head as two tiles of 128 and walks along the keys in tiles of
-// 64.  Four warps turn a tile's codes into fp16 operands in shared memory, once for both row tiles; a warp for each row tile issues S = Q K^T and O += P V
-// (M = 128, N = 64 and N = D, accumulators in tensor memory); four warps for each row tile, a thread per row, turn
-// scores into weights, which go back to tensor memory as the A operand of the second product.  Block scales never touch the
-// operands: a key block's scale multiplies its columns of S in fp32, a value block's goes into the exponent,
+// A CTA has 256 rows (query, head of the group) of a key head as two tiles of 128 and walks along the keys in tiles of 64.
+// Four warps turn a tile's codes into fp16 operands in shared memory, once for both row tiles; a warp for each row tile issues
+// S = Q K^T and O += P V (M = 128, N = 64 and N = D, accumulators in tensor memory); sixteen warps, two threads per row,
+// turn scores into weights, which go back to tensor memory as the A operand of the second product; one plans.  Block scales
+// never touch the operands: a key block's scale multiplies its columns of S in fp32, a value block's goes into the exponent,
 //   t = s ks scale log2(e) + log2(vs),  p = 2^(t - ref),  O = sum p v_code,  l = sum p / vs,  out = O / l,
 // and O is only rescaled when a row's maximum has grown by more than 2^8 over its reference (p fits fp16 up to 2^16).
+//
+// 1024 tokens behind 15360 cached ones, 64 query and 8 key heads of 128: 530 us, 1000 TFLOP/s; a prompt of 2048 tokens, 32 heads: 80 us.
+// A step of 64 keys takes about 2100 clocks, of which the tensor core needs 1150 and the exponentials' unit 1024; the rest is the
+// latency of a row's chain scores -> maxima -> weights -> tensor memory (one thread per row: 664 us; four warps a tile).
 #include "kv_attend.cuh"
 
 namespace jqkv {

@@ -1,4 +1,7 @@
 // Log probabilities of given tokens, entropies and the strongest alternatives of rows of logits, in one pass over the row.
+//
+// Bound by reading the logits where there are many: 1024 rows of 131072 fp32, 537 MB: 94 us, 5.7 TB/s; 2047 rows of 32003 bf16, 131 MB: 33 us, 4 TB/s (2.3
+// waves of CTAs).  64 rows of 131072 with 20 alternatives take 16 us, 3 of them reading: the rest are barriers and the join of nine parts a row.
 #include "common.cuh"
 
 namespace jqlp {
@@ -87,10 +90,7 @@ struct Sums {
     }
 };
 
-// Two values at once (fp32 pairs): d = x - m, w = e^d, l += w, u += w d
-struct Pairs {
-    uint64_t l, u;
-};
+// Two fp32 values in a register pair
 __device__ __forceinline__ uint64_t pair2(float a, float b) {
     uint64_t r;
     asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
