@@ -18,6 +18,7 @@ from . import _lib, ops
 _FORMATS = {"int8": _lib.JQ_KV_INT8, "e4m3": _lib.JQ_KV_E4M3}
 BLOCK_SIZES = (16, 32, 64, 128)
 HEAD_DIMS = (64, 128)          # of attend(); append() and read() take every multiple of 32 up to 256
+_TENSORS = ("keys", "values", "key_scales", "value_scales")
 _pack_strides = struct.Struct("=qq").pack              # int64_t[2]
 _pack_batch = struct.Struct("=QQQiiiiii").pack         # jq_kv_batch
 
@@ -31,10 +32,42 @@ class KVCache:
     sequence in order), ``lengths`` (int32 [sequences], tokens that a sequence holds, the new ones among them) and, where
     sequences have different numbers of new tokens, ``starts`` (int32 [sequences + 1]: the new tokens of sequence i are
     the rows starts[i] .. starts[i + 1] - 1; they sit at its end) with ``max_new``, which no sequence's number exceeds.
-    All three stay on the device; a step can be captured in a CUDA graph and replayed with other contents."""
+    All three stay on the device; a step can be captured in a CUDA graph and replayed with other contents.
+
+    The tensors may be replaced (and ``fmt`` with them), moved or resized in place between calls; a copy (``copy.deepcopy``) and
+    what comes back from a file have tensors of their own.  A captured step keeps the ones it was captured with."""
 
     def __init__(self, keys: torch.Tensor, values: torch.Tensor, key_scales: torch.Tensor, value_scales: torch.Tensor,
                  fmt: str = "int8"):
+        self.keys, self.values, self.key_scales, self.value_scales, self.fmt = keys, values, key_scales, value_scales, fmt
+        self._look()
+
+    def __setattr__(self, name, value):
+        object.__setattr__(self, name, value)
+        if name in _TENSORS or name == "fmt":
+            object.__setattr__(self, "_c", None)
+
+    def __getstate__(self):
+        return [getattr(self, name) for name in (*_TENSORS, "fmt")]
+
+    def __setstate__(self, state):
+        self.__init__(*state)
+
+    def _where(self) -> tuple:
+        """Addresses and sizes of the tensors: what a change in place shows in."""
+        k, v, ks, vs = self.keys, self.values, self.key_scales, self.value_scales
+        return (k.data_ptr(), v.data_ptr(), ks.data_ptr(), vs.data_ptr(), k.numel(), v.numel(), ks.numel(), vs.numel())
+
+    def _structure(self) -> bytes:
+        """jq_kv_cache of a call, of the tensors as they are now."""
+        if self._c is None or self._where() != self._at:
+            self._look()
+        return self._c
+
+    def _look(self) -> None:
+        """Looks the tensors over; what a call needs of them."""
+        self._c = None
+        keys, values, key_scales, value_scales, fmt = self.__getstate__()
         if fmt not in _FORMATS:
             raise ValueError(f"unknown cache format {fmt!r}")
         if keys.dim() != 4 or keys.shape != values.shape or keys.dtype != torch.uint8 or values.dtype != torch.uint8:
@@ -47,7 +80,6 @@ class KVCache:
             raise ValueError("the cache's tensors are contiguous")
         if any(t.device != keys.device for t in tensors):
             raise ValueError("the cache's tensors are on one device")
-        self.keys, self.values, self.key_scales, self.value_scales, self.fmt = keys, values, key_scales, value_scales, fmt
         self.blocks, self.kv_heads, self.block_size, self.head_dim = keys.shape
         if self.blocks == 0 or self.kv_heads == 0:
             raise ValueError("a cache has at least one block and one head")
@@ -57,10 +89,9 @@ class KVCache:
             raise ValueError("head_dim must be a multiple of 32 up to 256")
         self.device = keys.device
         self._cuda = keys.is_cuda
-        # (the structure of jq.h as bytes; the fields do not change)
-        self._c = bytes(_lib.jq_kv_cache(keys.data_ptr(), values.data_ptr(), key_scales.data_ptr(), value_scales.data_ptr(),
-                                         self.blocks, self.kv_heads, self.head_dim, self.block_size, _FORMATS[fmt], 0))
+        self._at = self._where()
         self._need = {}                # (tokens of a sequence at most, query heads) -> bytes of workspace
+        self._c = bytes(_lib.jq_kv_cache(*self._at[:4], self.blocks, self.kv_heads, self.head_dim, self.block_size, _FORMATS[fmt], 0))
 
     @classmethod
     def empty(cls, blocks: int, kv_heads: int, head_dim: int, *, block_size: int = 64, fmt: str = "int8",
@@ -134,13 +165,14 @@ class KVCache:
         the places that ``table`` and ``lengths`` give them.  A block's scale grows with its largest value, and codes that
         are there already are rounded to the new one: the result depends on what is appended in one call.  Infinities
         become the largest code, NaN 0.  A block is appended to by one sequence of a call; shared blocks are full."""
+        cache = self._structure()
         k, sk = self._rows(k, self.kv_heads, "k")
         v, sv = self._rows(v, self.kv_heads, "v")
         if k.shape != v.shape or k.dtype != v.dtype:
             raise RuntimeError("k and v have one shape and dtype")
         batch = self._batch(table, lengths, starts, k.shape[0], max_new)
         with ops._on(self.device):
-            st = _lib.load().jq_kv_append(self._c, batch, k.data_ptr(), v.data_ptr(), sk, sv, ops._DT[k.dtype],
+            st = _lib.load().jq_kv_append(cache, batch, k.data_ptr(), v.data_ptr(), sk, sv, ops._DT[k.dtype],
                                           ops._stream())
         if st:
             _lib.check(st, "jq_kv_append")
@@ -153,10 +185,11 @@ class KVCache:
             raise RuntimeError(f"unsupported dtype {dtype}")
         if last < 0:
             raise RuntimeError("last is a number of tokens")
+        cache = self._structure()
         batch = self._batch(table, lengths, None, 0, None)
         k, v = torch.empty((2, lengths.shape[0], last, self.kv_heads, self.head_dim), dtype=dtype, device=self.device).unbind()
         with ops._on(self.device):
-            st = _lib.load().jq_kv_read(self._c, batch, last, k.data_ptr(), v.data_ptr(), ops._DT[dtype], ops._stream())
+            st = _lib.load().jq_kv_read(cache, batch, last, k.data_ptr(), v.data_ptr(), ops._DT[dtype], ops._stream())
         if st:
             _lib.check(st, "jq_kv_read")
         return k, v
@@ -170,6 +203,7 @@ class KVCache:
         shape, dtype = q.shape, q.dtype
         if dtype is not torch.float16 and dtype is not torch.bfloat16:
             raise RuntimeError(f"unsupported query dtype {dtype}: fp16 or bf16")
+        cache = self._structure()
         if self.head_dim not in HEAD_DIMS:
             raise RuntimeError(f"attend() takes heads of {HEAD_DIMS}, the cache has {self.head_dim}")
         x, strides = self._rows(q, 0, "q")
@@ -194,10 +228,10 @@ class KVCache:
             if need is None:
                 if len(self._need) >= 1024:
                     self._need.clear()
-                need = self._need[most, heads] = lib.jq_kv_attend_workspace_bytes(self._c, batch, heads)
+                need = self._need[most, heads] = lib.jq_kv_attend_workspace_bytes(cache, batch, heads)
             stream = ops._stream()
             own, at, size = ops._parts_workspace(self.device, need, stream)
-            st = lib.jq_kv_attend(self._c, batch, x.data_ptr(), strides, heads, scale, min(window, 0x7fffffff), out.data_ptr(),
+            st = lib.jq_kv_attend(cache, batch, x.data_ptr(), strides, heads, scale, min(window, 0x7fffffff), out.data_ptr(),
                                   ops._addr(sums), ops._DT[dtype], at, size, stream)
             del own
         if st:

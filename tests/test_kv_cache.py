@@ -5,6 +5,8 @@ Bound of an attention output, relative to sum p |v| of the element: a weight is 
 exponent is off by at most D 2^-24 of the score's absolute products, 2^-23 of the score and 2^-21 (the exponential,
 the scales' logarithms), in the numerator and in the denominator; weights below fp16's normal range are off by 2^-25 of the
 largest one each; fp32 sums of `length` terms by length 2^-24; and the output is rounded once."""
+import copy
+import io
 import math
 
 import numpy as np
@@ -535,3 +537,80 @@ def test_the_python_layer_refuses():
             jq.KVCache(*args)
     with pytest.raises(ValueError):
         jq.KVCache.empty(4, 2, 48, device="cpu")
+
+
+TENSORS = ("keys", "values", "key_scales", "value_scales")
+
+
+def _through_a_file(cache):
+    file = io.BytesIO()
+    torch.save(cache, file)
+    file.seek(0)
+    return torch.load(file, weights_only=False)
+
+
+def _replaced(cache):
+    other = copy.copy(cache)
+    for name in TENSORS:
+        setattr(other, name, getattr(cache, name).clone())
+    return other
+
+
+def _replaced_in_place(cache):
+    other = jq.KVCache(*(getattr(cache, name)[:1].clone() for name in TENSORS), cache.fmt)
+    for name in TENSORS:
+        getattr(other, name).data = getattr(cache, name).clone()
+    return other
+
+
+COPIES = [copy.deepcopy, _through_a_file, _replaced, _replaced_in_place]
+
+
+@pytest.mark.parametrize("make", COPIES)
+def test_a_copy_names_its_own_memory(make):
+    cache = jq.KVCache.empty(5, 2, 64, block_size=16, fmt="e4m3", device="cpu")
+    other = make(cache)
+    for c in (cache, other):
+        seen = _lib.jq_kv_cache.from_buffer_copy(c._structure())
+        assert [seen.keys, seen.values, seen.key_scales, seen.value_scales] == [getattr(c, name).data_ptr() for name in TENSORS]
+        assert (seen.blocks, seen.kv_heads, seen.head_dim, seen.block_size, seen.fmt) == (5, 2, 64, 16, _lib.JQ_KV_E4M3)
+        assert (c.blocks, c.kv_heads, c.head_dim, c.block_size) == (5, 2, 64, 16)
+    assert all(getattr(cache, name).data_ptr() != getattr(other, name).data_ptr() for name in TENSORS)
+
+
+def test_replaced_tensors_are_looked_over():
+    cache = jq.KVCache.empty(5, 2, 64, block_size=16, device="cpu")
+    table, lens = torch.zeros(2, 3, dtype=torch.int32), torch.tensor([5, 9], dtype=torch.int32)
+    for name, value in (("keys", torch.zeros(5, 2, 16, 64)), ("value_scales", torch.ones(4, 2)), ("fmt", "fp8"), ("values", cache.values[:, :, :8])):
+        other = copy.copy(cache)
+        setattr(other, name, value)
+        with pytest.raises(ValueError):
+            other.read(table, lens, 3)
+    cache.keys.data = cache.keys[:3].clone()
+    with pytest.raises(ValueError):
+        cache.read(table, lens, 3)
+    cache.values, cache.key_scales, cache.value_scales = cache.values[:3].clone(), cache.key_scales[:3].clone(), cache.value_scales[:3].clone()
+    assert _lib.jq_kv_cache.from_buffer_copy(cache._structure()).blocks == cache.blocks == 3
+
+
+@gpu
+@pytest.mark.parametrize("make", COPIES)
+def test_a_copy_appends_and_attends_to_its_own_memory(make):
+    lengths, H, D = [100, 60], 2, 64
+    cache, table, dense = _filled(lengths, H, D, 16, "int8", 21)
+    kept = [getattr(cache, name).clone() for name in TENSORS]
+    other = make(cache)
+    table, lens = table.to(DEV), torch.tensor(lengths, dtype=torch.int32, device=DEV)
+    q = torch.randn(2, 4, D, device=DEV).half()
+    _check_attend(q, other.attend(q, table, lens), None, dense, lengths, [1, 1], 0)
+    k = torch.randn(2, H, D, device=DEV)
+    other.append(k, k, table, lens)
+    assert all(torch.equal(getattr(cache, name), was) for name, was in zip(TENSORS, kept))
+    assert not torch.equal(other.keys, cache.keys)
+    twin = jq.KVCache(*kept, "int8")
+    twin.append(k, k, table, lens)
+    assert all(torch.equal(getattr(other, name), getattr(twin, name)) for name in TENSORS)
+    want = twin.attend(q, table, lens)
+    del cache, twin, kept
+    assert torch.equal(other.attend(q, table, lens), want)
+    assert all(torch.equal(a, b) for a, b in zip(other.read(table, lens, 60), make(other).read(table, lens, 60)))
