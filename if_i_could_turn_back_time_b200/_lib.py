@@ -70,6 +70,7 @@ _SIGNATURES = {
     "jq_conv_rows": (c_int, [c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int,
                              c_int, c_int, c_int, c_void_p, c_size_t, c_void_p, c_void_p]),
     "jq_ta_status": (c_int, [c_void_p, c_int, c_void_p]),
+    "jq_status_word": (c_void_p, []),
     "jq_selftest_bounded_wait": (c_int, [c_void_p, ctypes.c_uint, c_void_p]),
     "jq_grouped_plan_bytes": (c_size_t, [c_int]),
     "jq_grouped_plan": (c_int, [c_int, c_void_p, c_int, c_int, c_void_p, c_size_t]),
@@ -87,6 +88,8 @@ _SIGNATURES = {
     "jq_kv_attend_workspace_bytes": (c_size_t, [c_void_p, c_void_p, c_int]),
     "jq_kv_attend": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int, ctypes.c_float, c_int, c_void_p, c_void_p, c_int,
                              c_void_p, c_size_t, c_void_p]),
+    "jq_kv_attend_status": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int, ctypes.c_float, c_int, c_void_p, c_void_p, c_int,
+                                    c_void_p, c_size_t, c_void_p, c_void_p]),
     "jq_token_logprobs_workspace_bytes": (c_size_t, [c_int, c_int]),
     "jq_token_logprobs": (c_int, [c_void_p, ctypes.c_int64, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p, c_int, c_void_p,
                                   c_void_p, c_void_p, c_size_t, c_void_p]),

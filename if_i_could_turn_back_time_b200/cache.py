@@ -230,12 +230,12 @@ class KVCache:
                     self._need.clear()
                 need = self._need[most, heads] = lib.jq_kv_attend_workspace_bytes(cache, batch, heads)
             stream = ops._stream()
-            own, at, size = ops._parts_workspace(self.device, need, stream)
-            st = lib.jq_kv_attend(cache, batch, x.data_ptr(), strides, heads, scale, min(window, 0x7fffffff), out.data_ptr(),
-                                  ops._addr(sums), ops._DT[dtype], at, size, stream)
+            own, at, size, status = ops._parts_workspace(self.device, need, stream)
+            st = lib.jq_kv_attend_status(cache, batch, x.data_ptr(), strides, heads, scale, min(window, 0x7fffffff), out.data_ptr(),
+                                         ops._addr(sums), ops._DT[dtype], at, size, status, stream)
             del own
         if st:
-            _lib.check(st, "jq_kv_attend")
+            _lib.check(st, "jq_kv_attend_status")
         if ops._checked:
             ops.check_status()
         return (out, sums) if lse else out

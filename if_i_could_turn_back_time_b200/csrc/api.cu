@@ -30,6 +30,25 @@ unsigned long long jq_context_id() {
     return get && get(nullptr, &id) == CUDA_SUCCESS ? id : 0;
 }
 
+// The status word of calls whose workspace does not outlast them, in a cache line of its own.  Its address belongs to the context, see
+// jq_noalloc_scratch (gemv.cu).
+static __device__ __align__(256) int jq_lasting_status[64];
+
+extern "C" int *jq_status_word(void) {
+    static struct { unsigned long long context; void *addr; } kept[8];
+    static std::mutex mu;
+    const unsigned long long id = jq_context_id();
+    std::lock_guard<std::mutex> lk(mu);
+    if (id && kept[id & 7].context == id) return reinterpret_cast<int *>(kept[id & 7].addr);
+    void *p = nullptr;
+    if (cudaGetSymbolAddress(&p, jq_lasting_status) != cudaSuccess) {
+        cudaGetLastError();                                    // (not left for the next launch to find)
+        return nullptr;
+    }
+    if (id) { kept[id & 7].context = id; kept[id & 7].addr = p; }
+    return reinterpret_cast<int *>(p);
+}
+
 extern "C" int jq_version(void) { return JQ_VERSION; }
 
 extern "C" const char *jq_strerror(int status) {

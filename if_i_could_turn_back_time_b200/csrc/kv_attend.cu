@@ -564,6 +564,12 @@ extern "C" size_t jq_kv_attend_workspace_bytes(const jq_kv_cache *c, const jq_kv
 extern "C" int jq_kv_attend(const jq_kv_cache *c, const jq_kv_batch *s, const void *q, const int64_t *stride_q, int q_heads,
                             float scale, int window, void *out, float *lse_or_null, int dtype, void *workspace,
                             size_t workspace_bytes, jq_stream_t stream) {
+    return jq_kv_attend_status(c, s, q, stride_q, q_heads, scale, window, out, lse_or_null, dtype, workspace, workspace_bytes, nullptr, stream);
+}
+
+extern "C" int jq_kv_attend_status(const jq_kv_cache *c, const jq_kv_batch *s, const void *q, const int64_t *stride_q, int q_heads,
+                                   float scale, int window, void *out, float *lse_or_null, int dtype, void *workspace,
+                                   size_t workspace_bytes, int *status_or_null, jq_stream_t stream) {
     const int bad = check_cache(c, s);
     if (bad) return bad;
     if (dtype != JQ_F16 && dtype != JQ_BF16) return JQ_ERR_BAD_DTYPE;
@@ -573,7 +579,7 @@ extern "C" int jq_kv_attend(const jq_kv_cache *c, const jq_kv_batch *s, const vo
     if ((long long)most_new(s) * (q_heads / c->kv_heads) > (1 << 30)) return JQ_ERR_BAD_SHAPE;
     if (!q || !out || !stride_q || !workspace) return JQ_ERR_NULL_PTR;
     if ((reinterpret_cast<uintptr_t>(q) & 1u) || !jq_aligned16(out) || (reinterpret_cast<uintptr_t>(lse_or_null) & 3u) ||
-        (reinterpret_cast<uintptr_t>(workspace) & 127u))
+        (reinterpret_cast<uintptr_t>(workspace) & 127u) || (reinterpret_cast<uintptr_t>(status_or_null) & 3u))
         return JQ_ERR_BAD_ALIGN;
     if (workspace_bytes < jq_kv_attend_workspace_bytes(c, s, q_heads)) return JQ_ERR_WORKSPACE;
     AttendArgs a{};
@@ -587,7 +593,7 @@ extern "C" int jq_kv_attend(const jq_kv_cache *c, const jq_kv_batch *s, const vo
     a.dtype = dtype;
     a.scale = scale * kLog2e;
     unsigned char *ws = reinterpret_cast<unsigned char *>(workspace);
-    a.status = reinterpret_cast<int *>(ws);
+    a.status = status_or_null ? status_or_null : reinterpret_cast<int *>(ws);
     a.counters = reinterpret_cast<int *>(ws + kJqHeader);
     a.parts = reinterpret_cast<float *>(ws + kJqData);
     const long long rows = (long long)most_new(s) * a.G;

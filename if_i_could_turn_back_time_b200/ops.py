@@ -183,7 +183,8 @@ def reserve_workspace(device, nbytes: int, kind: str = "ta") -> None:
 
 def check_status(raise_on_error: bool = True) -> int:
     """Read and clear the sticky status words of this device's workspaces on
-    the current stream (synchronises).  A kernel whose bounded wait expired
+    the current stream, and the word that captured attention over the cache
+    has on this device, whichever stream it replays on (synchronises).  A kernel whose bounded wait expired
     leaves JQ_ERR_TIMEOUT there and returns early with its outputs partly
     written; every later call keeps the word until it is read here."""
     lib = _lib.load()
@@ -192,6 +193,9 @@ def check_status(raise_on_error: bool = True) -> int:
         ws = _ws_cache().get((torch.cuda.current_device(), torch.cuda.current_stream().cuda_stream, kind))
         if ws is not None:
             worst = min(worst, lib.jq_ta_status(_ptr(ws), 1, _stream()))
+    word = lib.jq_status_word()
+    if word is not None:
+        worst = min(worst, lib.jq_ta_status(word, 1, _stream()))
     if worst and raise_on_error:
         raise _lib.JqError(worst, "device status")
     return worst
@@ -201,18 +205,21 @@ _PARTS_DATA = 1024 + 4 * 1024        # status word and counters of such a buffer
 
 
 def _parts_workspace(device, nbytes: int, stream: int):
-    """(tensor to keep, address, size) of the scratch of a call on the current stream whose last CTA adds up what the others
-    left: this thread's and stream's "parts" buffer, or, while a graph is captured, zeros of the call's own from the graph's
-    pool (graphs that were captured on one stream may replay on several).  The kernels leave the counters in it as they
-    found them, at zero."""
+    """(tensor to keep, address, size, status word) of the scratch of a call on the current stream whose last CTA adds up what
+    the others left: this thread's and stream's "parts" buffer, or, while a graph is captured, zeros of the call's own from the
+    graph's pool (graphs that were captured on one stream may replay on several).  The kernels leave the counters in it as
+    they found them, at zero.  The status word is the buffer's (None), or, as the graph's memory is another call's next, the
+    library's own."""
+    status = None
     if _capturing(stream):
+        status = _lib.load().jq_status_word()
         t = torch.empty(nbytes, dtype=torch.uint8, device=device)
         t[:_PARTS_DATA].zero_()
     else:
         t = _ws_cache().get((device.index, stream, "parts"))
         if t is None or t.numel() < nbytes:
             t = _workspace(device, nbytes, "parts")
-    return t, t.data_ptr(), t.numel()
+    return t, t.data_ptr(), t.numel(), status
 
 
 _ta_workspace_bytes = {}       # (K, rows) -> bytes
@@ -516,7 +523,7 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0) -> 
             if len(_logprobs_workspace_bytes) >= 4096:
                 _logprobs_workspace_bytes.clear()
             need = _logprobs_workspace_bytes[key] = lib.jq_token_logprobs_workspace_bytes(rows, vocab)
-        own, at, size = _parts_workspace(device, need, stream) if need else (None, None, 0)
+        own, at, size, _ = _parts_workspace(device, need, stream) if need else (None, None, 0, None)
         st = lib.jq_token_logprobs(x.data_ptr(), row, rows, vocab, _DT[dtype], tokens.data_ptr(), logprob.data_ptr(),
                                    entropy.data_ptr(), top, top_logprobs.data_ptr() if top else None,
                                    top_tokens.data_ptr() if top else None, at, size, stream)

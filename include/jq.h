@@ -266,6 +266,10 @@ int jq_gemm_ta(int fmt, const void *qweight, const void *scales, const void *cod
                int had_block, int x_dtype, int y_dtype, void *workspace, size_t workspace_bytes,
                jq_stream_t stream);
 int jq_ta_status(void *workspace, int clear, jq_stream_t stream);
+/* A status word of the library's own in the current context, zero at first and as sticky as the others, for calls whose
+ * workspace does not outlast them (captured ones, whose memory belongs to the graph): jq_ta_status reads it.  NULL without
+ * a device. */
+int *jq_status_word(void);
 
 /* Many activation rows (prompts, evaluation batches): the same operator as jq_gemv_* / jq_gemm_ta for any B >= 1 and
  * every K, g and alignment of the formats above, the F.linear(x, W_bar, bias) of
@@ -385,6 +389,11 @@ size_t jq_kv_attend_workspace_bytes(const jq_kv_cache *cache, const jq_kv_batch 
 int jq_kv_attend(const jq_kv_cache *cache, const jq_kv_batch *batch, const void *q, const int64_t *stride_q, int q_heads,
                  float scale, int window, void *out, float *lse_or_null, int dtype, void *workspace,
                  size_t workspace_bytes, jq_stream_t stream);
+/* The same with the status word elsewhere: a device int that is zero before its first use, for instance jq_status_word()
+ * (NULL: the workspace's). */
+int jq_kv_attend_status(const jq_kv_cache *cache, const jq_kv_batch *batch, const void *q, const int64_t *stride_q, int q_heads,
+                        float scale, int window, void *out, float *lse_or_null, int dtype, void *workspace,
+                        size_t workspace_bytes, int *status_or_null, jq_stream_t stream);
 
 /* Rows of logits [rows, vocab] of dtype, row_stride elements apart: for each row the log probability of its token, the entropy
  * (NULL: none) and the `top` (0 to 32) strongest tokens in falling order, the lowest index first among equals, with

@@ -8,6 +8,9 @@ largest one each; fp32 sums of `length` terms by length 2^-24; and the output is
 import copy
 import io
 import math
+import os
+import subprocess
+import sys
 
 import numpy as np
 import pytest
@@ -614,3 +617,73 @@ def test_a_copy_appends_and_attends_to_its_own_memory(make):
     del cache, twin, kept
     assert torch.equal(other.attend(q, table, lens), want)
     assert all(torch.equal(a, b) for a, b in zip(other.read(table, lens, 60), make(other).read(table, lens, 60)))
+
+
+def test_captured_calls_have_a_status_word_that_is_read(monkeypatch):
+    """What a captured call is given as its status word is what check_status() reads, and not a place in the graph's memory."""
+    lib, words = _lib.load(), {4096: -7}
+    monkeypatch.setattr(lib, "jq_status_word", lambda: 4096)
+    monkeypatch.setattr(lib, "jq_ta_status", lambda at, clear, stream: words.pop(at, 0))
+    monkeypatch.setattr(ops, "_capturing", lambda stream: True)
+    monkeypatch.setattr(ops, "_stream", lambda: 7)
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 0)
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda: type("Stream", (), {"cuda_stream": 7}))
+    own, at, size, status = ops._parts_workspace(torch.device("cpu"), 8192, 7)
+    assert own.data_ptr() == at and size == 8192 and bool((own[:ops._PARTS_DATA] == 0).all())
+    assert status == 4096
+    with pytest.raises(_lib.JqError):
+        ops.check_status()
+    assert ops.check_status() == 0
+
+
+@gpu
+@pytest.mark.parametrize("new", [1, 90])
+def test_a_wait_that_gives_up_in_a_replay_is_seen(new, monkeypatch):
+    """The word is raised as a kernel would raise it, by a wait that runs out; neither the graph's own zeroing nor what is captured
+    behind the call may clear it, and it is seen on a stream that the graph was not captured on."""
+    lengths, H, D = [300, 150], 2, 64
+    cache, table, _ = _filled(lengths, H, D, 32, "int8", 23)
+    q = torch.randn(2 * new, 4, D, device=DEV).half()
+    table, lens = table.to(DEV), torch.tensor(lengths, dtype=torch.int32, device=DEV)
+    want = cache.attend(q, table, lens)
+    lib, given = _lib.load(), []
+    real = lib.jq_kv_attend_status
+    monkeypatch.setattr(lib, "jq_kv_attend_status", lambda *a: given.append(a[-2]) or real(*a))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = cache.attend(q, table, lens)
+        behind = [torch.zeros(1 << 20, dtype=torch.uint8, device=DEV) + 1 for _ in range(4)]
+    graph.replay()
+    assert torch.equal(out, want) and ops.check_status(raise_on_error=False) == 0
+    assert given[0] and lib.jq_selftest_bounded_wait(given[0], 4096, None) == 0
+    graph.replay()
+    assert torch.equal(out, want) and all(bool((b == 1).all()) for b in behind)
+    with pytest.raises(_lib.JqError):
+        ops.check_status()
+    assert ops.check_status() == 0
+
+
+FIRST = """
+import sys
+import torch
+sys.path.insert(0, sys.argv[1])
+import if_i_could_turn_back_time_b200 as jq
+from if_i_could_turn_back_time_b200 import ops
+cache = jq.KVCache.empty(8, 2, 64, block_size=16)
+table = torch.arange(8, dtype=torch.int32, device="cuda").view(1, 8)
+lens = torch.tensor([100], dtype=torch.int32, device="cuda")
+q = torch.randn(1, 4, 64, device="cuda").half()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    out = cache.attend(q, table, lens)
+graph.replay()
+assert ops.check_status() == 0 and bool((out == 0).all())
+print("captured")
+"""
+
+
+@gpu
+def test_a_capture_that_is_the_librarys_first_call():
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([sys.executable, "-c", FIRST, root], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and r.stdout.strip() == "captured", r.stderr[-2000:]
