@@ -123,6 +123,8 @@ class KVCache:
             row = width
         elif row < width:
             raise RuntimeError("the table's rows lie behind one another")
+        if not n and tokens:
+            raise RuntimeError(f"{tokens} new tokens of no sequence")
         at = 0
         if starts is None:
             if n and tokens % n:
@@ -228,7 +230,9 @@ class KVCache:
             if need is None:
                 if len(self._need) >= 1024:
                     self._need.clear()
-                need = self._need[most, heads] = lib.jq_kv_attend_workspace_bytes(cache, batch, heads)
+                need = lib.jq_kv_attend_workspace_bytes(cache, batch, heads)
+                if need:                       # (0: refused, and so is the call below)
+                    self._need[most, heads] = need
             stream = ops._stream()
             own, at, size, status = ops._parts_workspace(self.device, need, stream)
             st = lib.jq_kv_attend_status(cache, batch, x.data_ptr(), strides, heads, scale, min(window, 0x7fffffff), out.data_ptr(),

@@ -309,7 +309,7 @@ int check_cache(const jq_kv_cache *c, const jq_kv_batch *s) {
     if (s->sequences < 0 || s->table_width <= 0 || s->table_stride < s->table_width || s->tokens < 0 ||
         (long long)s->table_width * c->block_size > 0x7fffff00LL)
         return JQ_ERR_BAD_SHAPE;
-    if (!s->starts && s->sequences && s->tokens % s->sequences) return JQ_ERR_BAD_SHAPE;
+    if (s->sequences ? !s->starts && s->tokens % s->sequences : s->tokens) return JQ_ERR_BAD_SHAPE;
     if (!jq_aligned16(c->keys) || !jq_aligned16(c->values) || (reinterpret_cast<uintptr_t>(c->key_scales) & 3u) ||
         (reinterpret_cast<uintptr_t>(c->value_scales) & 3u) || (reinterpret_cast<uintptr_t>(s->table) & 3u) ||
         (reinterpret_cast<uintptr_t>(s->lengths) & 3u) || (reinterpret_cast<uintptr_t>(s->starts) & 3u))

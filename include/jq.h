@@ -351,7 +351,8 @@ typedef struct jq_kv_cache {
 /* The sequences of a call.  The arrays are on the device and the host does not look at them: token t of sequence i lies in block
  * table[i * table_stride + t / block_size]; the sequence holds lengths[i] tokens (at most table_width * block_size are
  * looked at), of which the last n are new: the rows starts[i] .. starts[i + 1] - 1 of the call's tensors, or, where starts
- * is NULL, rows i n .. (i + 1) n - 1 with n = tokens / sequences.  max_new: no sequence has more new tokens
+ * is NULL, rows i n .. (i + 1) n - 1 with n = tokens / sequences (rows of no sequence are left as they are; without sequences
+ * there are no rows).  max_new: no sequence has more new tokens
  * (0: not known); it only sizes launches, and new tokens beyond it may be left out.  A table entry that names no block of the pool
  * is not followed: what would lie there is neither read (it counts as masked) nor written.  So is a sequence whose starts name no
  * rows of the call (a < 0, b > tokens, b <= a): it has no new tokens. */

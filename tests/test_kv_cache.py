@@ -687,3 +687,36 @@ def test_a_capture_that_is_the_librarys_first_call():
     root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
     r = subprocess.run([sys.executable, "-c", FIRST, root], capture_output=True, text=True, timeout=300)
     assert r.returncode == 0 and r.stdout.strip() == "captured", r.stderr[-2000:]
+
+
+def test_tokens_of_no_sequence_are_refused():
+    """Nothing would be written for them: the outputs would be what the memory held."""
+    import ctypes
+    lib, (c, b) = _lib.load(), _host_cache(sequences=0, tokens=4)
+    st, p, r = (ctypes.c_int64 * 2)(128, 64), 1 << 20, ctypes.byref
+    for starts in (None, p):
+        b.starts = starts
+        assert lib.jq_kv_append(r(c), r(b), p, p, st, st, 0, None) == -2
+        assert lib.jq_kv_attend(r(c), r(b), p, st, 4, 0.1, 0, p, None, 1, p, 1 << 40, None) == -2
+        assert lib.jq_kv_attend_workspace_bytes(r(c), r(b), 4) == 0
+    b.tokens = 0
+    assert lib.jq_kv_append(r(c), r(b), p, p, st, st, 0, None) == 0
+    cache = jq.KVCache.empty(4, 2, 64, block_size=16, device="cpu")
+    table, lens, q = torch.zeros(0, 3, dtype=torch.int32), torch.zeros(0, dtype=torch.int32), torch.zeros(2, 4, 64).half()
+    for starts in (None, torch.zeros(1, dtype=torch.int32)):
+        with pytest.raises(RuntimeError, match="no sequence"):
+            cache.attend(q, table, lens, starts)
+        with pytest.raises(RuntimeError, match="no sequence"):
+            cache.append(q[:, :2], q[:, :2], table, lens, starts)
+
+
+@gpu
+def test_a_refused_call_leaves_no_workspace_size_behind():
+    """A table of more tokens than positions have bits is refused by the library; the same heads and tokens with another table are not."""
+    cache = jq.KVCache.empty(4, 2, 64, block_size=128, device=DEV)
+    q = torch.zeros(1, 8, 64, device=DEV).half()
+    lens = torch.tensor([100], dtype=torch.int32, device=DEV)
+    with pytest.raises(_lib.JqError):
+        cache.attend(q, torch.zeros(1, 1 << 24, dtype=torch.int32, device=DEV), lens)
+    assert not cache._need
+    assert bool((cache.attend(q, torch.zeros(1, 1, dtype=torch.int32, device=DEV), lens) == 0).all())
