@@ -133,10 +133,12 @@ class KVCache:
             if starts.shape != (n + 1,) or not starts.is_contiguous() or starts.device != device:
                 raise RuntimeError(f"starts is a contiguous tensor [{n + 1}] on {device}")
             at = starts.data_ptr()
-        if max_new is None:
+        if max_new is None or max_new > tokens:
             max_new = tokens
         elif max_new < 0:
             raise RuntimeError("max_new is a number of tokens")
+        if max(tokens, row) > 0x7fffffff:
+            raise RuntimeError(f"{tokens} new tokens, table rows {row} apart: the library counts in 32 bits")
         if not self._cuda:
             raise RuntimeError("libjq operators run on CUDA tensors only (there is no CPU path)")
         return _pack_batch(table.data_ptr(), lengths.data_ptr(), at, n, width, row, tokens, max_new, 0)
@@ -185,7 +187,7 @@ class KVCache:
         head_dim], 0 before a sequence's first token."""
         if dtype not in ops._DT:
             raise RuntimeError(f"unsupported dtype {dtype}")
-        if last < 0:
+        if not 0 <= last <= 0x7fffffff:
             raise RuntimeError("last is a number of tokens")
         cache = self._structure()
         batch = self._batch(table, lengths, None, 0, None)

@@ -496,6 +496,8 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0) -> 
         raise RuntimeError(f"tokens {tuple(tokens.shape)} {tokens.dtype}: int64 of the logits' leading dims {tuple(lead)}")
     if not 0 <= top <= 32 or top > vocab:
         raise RuntimeError(f"top is {top}: 0 to 32 of the {vocab} tokens")
+    if vocab > 1 << 30 or tokens.numel() > 0x7fffffff:         # (the library's counts have 32 bits)
+        raise RuntimeError(f"{tokens.numel()} rows of {vocab} logits: at most 2^31 - 1 rows and a vocabulary of 2^30")
     _need_cuda(logits, tokens)
     device = logits.device
     if tokens.device != device:

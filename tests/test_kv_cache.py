@@ -720,3 +720,15 @@ def test_a_refused_call_leaves_no_workspace_size_behind():
         cache.attend(q, torch.zeros(1, 1 << 24, dtype=torch.int32, device=DEV), lens)
     assert not cache._need
     assert bool((cache.attend(q, torch.zeros(1, 1, dtype=torch.int32, device=DEV), lens) == 0).all())
+
+
+def test_counts_past_32_bits():
+    """A max_new that is larger than the call stands for all its tokens; what the library cannot count is refused."""
+    cache = jq.KVCache.empty(4, 2, 64, block_size=16, device="cpu")
+    cache._cuda = True                                  # (nothing is called)
+    table, lens = torch.zeros(2, 3, dtype=torch.int32), torch.tensor([5, 9], dtype=torch.int32)
+    assert _lib.jq_kv_batch.from_buffer_copy(cache._batch(table, lens, None, 6, 1 << 40)).max_new == 6
+    with pytest.raises(RuntimeError, match="32 bits"):
+        cache._batch(table, lens, None, 1 << 32, 5)
+    with pytest.raises(RuntimeError, match="last"):
+        cache.read(table, lens, 1 << 32)

@@ -175,3 +175,11 @@ def test_refusals():
                        ((x[:, :0], tokens), "one token"), ((x, tokens, 11), "top"), ((x, tokens, -1), "top")):
         with pytest.raises(RuntimeError, match=text):
             ops.token_logprobs(*args)
+
+
+@pytest.mark.parametrize("rows,vocab", [(2, (1 << 32) + 10), (2, (1 << 30) + 1), ((1 << 32) + 2, 10), (1 << 31, 3)])
+def test_sizes_past_32_bits_are_refused(rows, vocab):
+    """(The library's counts have 32 bits: a vocabulary of 2^32 + 10 would be one of 10.)"""
+    x, tokens = torch.zeros(1, 1).expand(rows, vocab), torch.zeros(1, dtype=torch.int64).expand(rows)
+    with pytest.raises(RuntimeError, match="rows of"):
+        ops.token_logprobs(x, tokens, 3)
