@@ -29,7 +29,7 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
 
 // A sequence's share of the work: row tiles x key heads pairs of `units` units each, pairs in the order (head, tile).
 struct Share {
-    int row0, n, len, lo, units, tiles;
+    int row0, n, len, see, lo, units, tiles;       // see: first key that any row sees; lo: the unit that it lies in
     long long total;
 };
 template <int ROWS>
@@ -37,9 +37,8 @@ __device__ __forceinline__ Share share_of(const AttendArgs &p, int i) {
     Share s;
     s.n = p.b.count(i, s.row0);
     s.len = p.b.length(i);
-    const int first = s.len - s.n;
-    s.lo = p.window > 0 ? max(0, first - p.window + 1) : 0;
-    s.lo &= ~(kUnit - 1);
+    s.see = first_seen(p, s.len - s.n);
+    s.lo = s.see & ~(kUnit - 1);
     s.units = max(1, (s.len - s.lo + kUnit - 1) / kUnit);      // (a row that sees nothing has its zeros written too)
     s.tiles = (int)(((long long)s.n * p.G + ROWS - 1) / ROWS);
     s.total = (long long)s.tiles * p.H * s.units;
@@ -176,7 +175,8 @@ __global__ void __launch_bounds__(warps_of(NT, WIDE) * 32, WIDE ? 1 : (NT > 2 ? 
 #pragma unroll
             for (int n = 0; n < NG; ++n) {
                 id[n] = -1;
-                if (st < own && key + 16 * n < k1) id[n] = p.b.block(seq, key + 16 * n);
+                // (16 keys that nobody sees are not looked at: their block may be another sequence's by now)
+                if (st < own && key + 16 * n < k1 && key + 16 * n + 16 > sh.see) id[n] = p.b.block(seq, key + 16 * n);
             }
         };
         auto scales = [&]() {

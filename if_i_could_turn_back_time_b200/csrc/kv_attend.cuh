@@ -32,6 +32,11 @@ __device__ __forceinline__ uint32_t pack_h2(float lo, float hi) {
 
 __device__ __forceinline__ float lse_of(float m, float l) { return l > 0.f ? (m + log2f(l)) * kLn2 : (l == 0.f ? -INFINITY : l); }
 
+// First key that a query at this position sees.
+__device__ __forceinline__ int first_seen(const AttendArgs &p, int position) {
+    return p.window > 0 && position >= p.window ? position - p.window + 1 : 0;
+}
+
 // Outputs from element `at` on: v times f, rounded once.
 __device__ __forceinline__ uint32_t pack_out(const AttendArgs &p, float a, float b) {
     if (p.dtype == JQ_F16) return pack_h2(a, b);

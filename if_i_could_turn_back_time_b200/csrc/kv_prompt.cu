@@ -81,15 +81,15 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
 
 // Keys that the rows of a tile see, rounded down to a unit at their beginning.
 struct Range {
-    int lo, hi, units;             // units: kPairCost and the key tiles
+    int see, lo, hi, units;        // see: lo before it was rounded; units: kPairCost and the key tiles
 };
 __device__ __forceinline__ Range range_of(const AttendArgs &p, int len, int n, int tile) {
     const int first = len - n;
     const int q0 = (int)((uint32_t)tile * kRows / (uint32_t)p.G), q1 = min(n - 1, (int)(((uint32_t)(tile + 1) * kRows - 1) / (uint32_t)p.G));
     Range r;
     r.hi = max(0, min(len, first + q1 + 1));
-    r.lo = p.window > 0 ? max(0, first + q0 - p.window + 1) : 0;
-    r.lo = min(r.lo, r.hi) & ~(kKeys - 1);
+    r.see = first_seen(p, first + q0);
+    r.lo = min(r.see, r.hi) & ~(kKeys - 1);
     r.units = kPairCost + max(1, (r.hi - r.lo + kKeys - 1) / kKeys);
     return r;
 }
@@ -134,7 +134,7 @@ struct Walk {
 
 // A segment, as the planning warp hands it to the others.
 struct Segment {
-    int tiles, key0, hi;           // key tiles, first key, end of the keys that its rows see
+    int tiles, key0, see, hi;      // key tiles, first key, begin and end of the keys that its rows see
     int seq, head, row0, n, len;   // row0, n: the sequence's rows of the call's tensors
     int flat0, rows;               // first of the rows (query, head of the group) among the sequence's, and how many
     int all, w0, w1, slot;         // the whole of a pair, or a part: CTAs that have one, and the place of this one's
@@ -545,13 +545,14 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
         uint32_t par = 1;                                  // (the first round finds every stage free)
         const uint32_t none = E4M3 ? 0u : 0x80808080u;     // code of 0
         while (const Segment *sg = next_segment()) {
-            const int tiles = sg->tiles, key0 = sg->key0 + 16 * cw, hi = sg->hi, head = sg->head, len = sg->len, seq = sg->seq;
+            const int tiles = sg->tiles, key0 = sg->key0 + 16 * cw, see = sg->see, hi = sg->hi, head = sg->head, len = sg->len, seq = sg->seq;
             int id = -1;
             float kc = -1.f, vl = 0.f, vi = 1.f;
             auto look_up = [&](int first) {                // lane l: block and scales of tile first + l
                 const int k = key0 + (first + lane) * kKeys;
                 id = -1;
-                if (first + lane < tiles && k < hi) id = p.b.block(seq, k);
+                // (16 keys that nobody sees are not looked at: their block may be another sequence's by now)
+                if (first + lane < tiles && k < hi && k + 16 > see) id = p.b.block(seq, k);
                 kc = -1.f;
                 vl = 0.f;
                 vi = 1.f;
@@ -702,6 +703,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
                     Segment &s = s_seg[count];
                     s.tiles = walk.u1 - walk.u0;
                     s.key0 = walk.range.lo + walk.u0 * kKeys;
+                    s.see = walk.range.see;
                     s.hi = walk.range.hi;
                     s.seq = walk.seq; s.head = walk.head; s.row0 = walk.row0; s.n = walk.n; s.len = walk.len;
                     s.flat0 = walk.tile * kRows;

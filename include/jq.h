@@ -378,7 +378,8 @@ int jq_kv_read(const jq_kv_cache *cache, const jq_kv_batch *batch, int last, voi
 /* Causal attention of the new tokens' queries over the cache, their own keys and values among it (append them first): a query at
  * position p = length - n + j sees the keys max(0, p - window + 1) .. p (window 0: 0 .. p),
  *   out = sum softmax(scale * q.k) v,   lse = ln sum exp(scale * q.k)   (fp32 [tokens, q_heads], or NULL);
- * a query that sees nothing gets 0 and -infinity.  q is [tokens, q_heads, head_dim] F16 or BF16 (strides as above), out the same shape,
+ * a query that sees nothing gets 0 and -infinity.  Blocks whose tokens lie before every query's window are not looked at and may
+ * hold anything.  q is [tokens, q_heads, head_dim] F16 or BF16 (strides as above), out the same shape,
  * contiguous and 16-byte aligned; query head h reads key head h / (q_heads / kv_heads).  head_dim 64 or 128.  scale > 0.
  * A row of q is brought into fp16's range by a power of two and rounded to fp16 (exact for F16, and for BF16 except
  * values 2^-29 of the row's largest and less); codes are exact in fp16; weights relative to the row's largest are rounded to fp16

@@ -732,3 +732,23 @@ def test_counts_past_32_bits():
         cache._batch(table, lens, None, 1 << 32, 5)
     with pytest.raises(RuntimeError, match="last"):
         cache.read(table, lens, 1 << 32)
+
+
+@gpu
+@pytest.mark.parametrize("new,G", [(1, 2), (5, 4), (40, 2)])
+@pytest.mark.parametrize("fmt,D", [("int8", 64), ("e4m3", 128)])
+def test_blocks_before_every_window_may_hold_anything(new, G, fmt, D):
+    """A sequence's blocks that no window reaches any more are another's, who has not filled them: codes and scales that are NaN."""
+    lengths, H, T, window = [320, 450], 2, 16, 100
+    cache, table, dense = _filled(lengths, H, D, T, fmt, 29)
+    bad = [b for b in range(cache.blocks) if b not in set(table.flatten().tolist())][0]
+    for what in ("keys", "values"):
+        getattr(cache, what)[bad] = 0x7F if fmt == "e4m3" else 0
+        getattr(cache, what[:-1] + "_scales")[bad] = math.nan
+    for i, length in enumerate(lengths):
+        first = length - new - window + 1
+        assert first % 64 >= 16                                    # (whole blocks before it in the 64 keys that it lies in)
+        table[i, :first // T] = bad
+    q = torch.randn(2 * new, H * G, D, generator=torch.Generator().manual_seed(9)).bfloat16().to(DEV)
+    got, lse = cache.attend(q, table.to(DEV), torch.tensor(lengths, dtype=torch.int32, device=DEV), window=window, lse=True)
+    _check_attend(q, got, lse, dense, lengths, [new] * 2, window)
