@@ -184,7 +184,7 @@ __global__ void __launch_bounds__(warps_of(NT, WIDE) * 32, WIDE ? 1 : (NT > 2 ? 
             for (int n = 0; n < NG; ++n) {
                 const size_t at = (size_t)max(id[n], 0) * p.H + h;
                 const float v = id[n] >= 0 ? p.vs[at] : 1.f;
-                kc[n] = id[n] >= 0 ? p.ks[at] * p.scale : 0.f;
+                kc[n] = id[n] >= 0 ? p.ks[at] : 0.f;
                 vl[n] = log2f(v);
                 vi[n] = __fdividef(1.f, v);
             }
@@ -257,7 +257,7 @@ __global__ void __launch_bounds__(warps_of(NT, WIDE) * 32, WIDE ? 1 : (NT > 2 ? 
             }
             amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
             amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
-            const int e = act_exponent(amax, false);
+            const int e = query_exponent(amax);
             const float down = __uint_as_float((uint32_t)(127 - e) << 23);
 #pragma unroll
             for (int c = 0; c < C; ++c) {
@@ -269,7 +269,7 @@ __global__ void __launch_bounds__(warps_of(NT, WIDE) * 32, WIDE ? 1 : (NT > 2 ? 
 #pragma unroll
             for (int k = 0; k < 2; ++k) {
                 const int r = nt * 8 + 2 * tq + k, ee = __shfl_sync(0xffffffffu, e, (2 * tq + k) * 4);
-                qs[nt][k] = __uint_as_float((uint32_t)(127 + ee) << 23);
+                qs[nt][k] = __uint_as_float((uint32_t)(127 + ee) << 23) * p.scale;
                 pos[nt][k] = r < rows ? sh.len - sh.n + (r0 + r) / p.G : -1;
             }
         }

@@ -32,6 +32,13 @@ __device__ __forceinline__ uint32_t pack_h2(float lo, float hi) {
 
 __device__ __forceinline__ float lse_of(float m, float l) { return l > 0.f ? (m + log2f(l)) * kLn2 : (l == 0.f ? -INFINITY : l); }
 
+// e with amax 2^-e in [2^14, 2^15), as far as 2^e and 2^-e are normal fp32 numbers: every finite row of bf16 is in fp16's range then
+// (a row of 2^-126 and less ends below 1).  0 for a row of zeros or with an infinity.
+__device__ __forceinline__ int query_exponent(float amax) {
+    const uint32_t bits = __float_as_uint(amax) & 0x7fffffffu;
+    return bits == 0 || bits >= 0x7f800000u ? 0 : max((int)(bits >> 23) - 127 - 14, -126);
+}
+
 // First key that a query at this position sees.
 __device__ __forceinline__ int first_seen(const AttendArgs &p, int position) {
     return p.window > 0 && position >= p.window ? position - p.window + 1 : 0;

@@ -146,7 +146,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
     constexpr int H = D / 2;                                 // values of a row that a thread loads, scales and stores
     extern __shared__ __align__(128) unsigned char smem[];
     __shared__ __align__(8) uint64_t bars[4 * kStages + 2 * 5];
-    __shared__ __align__(16) float s_scales[kScaleSlots][4][4];    // [.][group]: factor of the scores (negative: not there), log2(vs), 1 / vs
+    __shared__ __align__(16) float s_scales[kScaleSlots][4][4];    // [.][group]: scale of the keys (negative: not there), log2(vs), 1 / vs
     __shared__ float s_top[2][2][kRows];                     // [parity][half][row]
     __shared__ Segment s_seg[kSegments];
     __shared__ long long s_sum[8], s_at;
@@ -323,9 +323,9 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
                 pair_sync();
                 amax = fmaxf(amax, s_top[1][half ^ 1][row]);
                 pair_sync();
-                const int e = act_exponent(amax, false);
+                const int e = query_exponent(amax);
                 const float down = __uint_as_float((uint32_t)(127 - e) << 23);
-                qs = __uint_as_float((uint32_t)(127 + e) << 23);
+                qs = __uint_as_float((uint32_t)(127 + e) << 23) * p.scale;
 #pragma unroll
                 for (int c4 = 0; c4 < H / 32; ++c4) {
                     uint32_t h[16];
@@ -559,7 +559,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
                 if (id >= 0) {
                     const size_t at = (size_t)id * p.H + head;
                     const float v = p.vs[at];
-                    kc = p.ks[at] * p.scale;
+                    kc = p.ks[at];
                     vl = log2f(v);
                     vi = __fdividef(1.f, v);
                 }

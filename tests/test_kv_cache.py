@@ -752,3 +752,15 @@ def test_blocks_before_every_window_may_hold_anything(new, G, fmt, D):
     q = torch.randn(2 * new, H * G, D, generator=torch.Generator().manual_seed(9)).bfloat16().to(DEV)
     got, lse = cache.attend(q, table.to(DEV), torch.tensor(lengths, dtype=torch.int32, device=DEV), window=window, lse=True)
     _check_attend(q, got, lse, dense, lengths, [new] * 2, window)
+
+
+@gpu
+@pytest.mark.parametrize("new", [1, 90])
+@pytest.mark.parametrize("power", [120, -118])
+def test_queries_at_the_ends_of_their_type(new, power):
+    """Rows of bf16 whose largest value is near 2^123 or below 2^-116, with a scale that brings the scores back."""
+    lengths, H, D = [200], 1, 128
+    cache, table, dense = _filled(lengths, H, D, 16, "int8", 17)
+    q = torch.randn(new, 6, D, generator=torch.Generator().manual_seed(9)).mul(1.5 * 2.0 ** power).bfloat16().to(DEV)
+    got, lse = cache.attend(q, table.to(DEV), torch.tensor(lengths, dtype=torch.int32, device=DEV), scale=0.05 * 2.0 ** -power, lse=True)
+    _check_attend(q, got, lse, dense, lengths, [new], 0, 0.05 * 2.0 ** -power)
