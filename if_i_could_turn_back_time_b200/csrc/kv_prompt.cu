@@ -379,7 +379,8 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
                         m0 = max3(m0, s[c], s[c + 1]);
                         m1 = max3(m1, s[16 + c], s[17 + c]);
                     }
-                    const float f0 = fabsf(sc0.x) * qs, f1 = fabsf(sc1.x) * qs;
+                    // (never 0, which keys of zeros and tiny queries give: a masked score of -infinity times it would be NaN)
+                    const float f0 = fmaxf(fabsf(sc0.x) * qs, 1.17549435e-38f), f1 = fmaxf(fabsf(sc1.x) * qs, 1.17549435e-38f);
                     float top = fmaxf(fmaf(m0, f0, sc0.y), fmaf(m1, f1, sc1.y));
                     float(*const tops)[kRows] = s_top[it & 1];
                     tops[half][row] = top;

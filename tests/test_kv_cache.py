@@ -764,3 +764,18 @@ def test_queries_at_the_ends_of_their_type(new, power):
     q = torch.randn(new, 6, D, generator=torch.Generator().manual_seed(9)).mul(1.5 * 2.0 ** power).bfloat16().to(DEV)
     got, lse = cache.attend(q, table.to(DEV), torch.tensor(lengths, dtype=torch.int32, device=DEV), scale=0.05 * 2.0 ** -power, lse=True)
     _check_attend(q, got, lse, dense, lengths, [new], 0, 0.05 * 2.0 ** -power)
+
+
+@gpu
+@pytest.mark.parametrize("new", [1, 90])
+def test_keys_of_zeros_and_queries_of_nearly_zero(new):
+    """The factor of the scores (2^-67 of the keys' scale, 2^-113 of the query's) has no fp32 number: every visible key weighs the same."""
+    length, H, D = 150, 1, 64
+    cache = jq.KVCache.empty(10, H, D, block_size=16, device=DEV)
+    table, lens = torch.arange(10, dtype=torch.int32, device=DEV)[None], torch.tensor([length], dtype=torch.int32, device=DEV)
+    gen = torch.Generator().manual_seed(9)
+    cache.append(torch.zeros(length, H, D, device=DEV), torch.randn(length, H, D, generator=gen).to(DEV), table, lens)
+    k, v = cache.read(table, lens, length)
+    q = torch.randn(new, 3, D, generator=gen).mul(1e-30).bfloat16().to(DEV)
+    got, lse = cache.attend(q, table, lens, lse=True)
+    _check_attend(q, got, lse, {"keys": [k[0].transpose(0, 1).double()], "values": [v[0].transpose(0, 1).double()]}, [length], [new], 0)
