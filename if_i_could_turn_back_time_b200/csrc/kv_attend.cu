@@ -10,6 +10,7 @@ using namespace jqta;
 
 constexpr int kNear = 16;          // units: how far a boundary between CTAs moves to a pair's begin or end, at most half a CTA's share (see snap)
 constexpr int kUnit = 64;          // keys: what work is dealt out in
+constexpr float kLift = 14.f;      // a row's reference lies 2^14 below its largest weight, so that fp16 weights have eleven bits down to 2^-28 of it
 constexpr int kRing = 16384;       // bytes of a warp's ring: two stages of 32 keys at D = 128, three CTAs on an SM
 
 __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
@@ -323,7 +324,7 @@ __global__ void __launch_bounds__(warps_of(NT, WIDE) * 32, WIDE ? 1 : (NT > 2 ? 
                         mma16816(s[nt][n], a[1], qb[nt][c][1][0], qb[nt][c][1][1]);
                     }
                 }
-            // t = log2(weight of the key times its block's value scale); the sums are formed relative to the largest t
+            // t = log2(weight of the key times its block's value scale); the sums are formed relative to M, the largest t less kLift
             const bool masked = key + KEYS - 1 > pos_first || (p.window > 0 && key <= pos_last - p.window) || !there[0] || !there[NG - 1];
             uint32_t pb[NT][NG][2];
 #pragma unroll
@@ -331,7 +332,7 @@ __global__ void __launch_bounds__(warps_of(NT, WIDE) * 32, WIDE ? 1 : (NT > 2 ? 
                 float alpha[2];
 #pragma unroll
                 for (int k = 0; k < 2; ++k) {                  // row 2t + k; element 2 j + k: key (g, j)
-                    float m = M[nt][k];
+                    float m = -INFINITY;
 #pragma unroll
                     for (int n = 0; n < NG; ++n) {
                         const float f = kcs[n] * qs[nt][k];
@@ -349,6 +350,7 @@ __global__ void __launch_bounds__(warps_of(NT, WIDE) * 32, WIDE ? 1 : (NT > 2 ? 
                     m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 4));
                     m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
                     m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
+                    m = fmaxf(M[nt][k], m - kLift);
                     const float ref = m == -INFINITY ? 0.f : m;          // (nothing seen yet: every weight is 0)
                     alpha[k] = ex2(M[nt][k] - ref);
                     M[nt][k] = m;

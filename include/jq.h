@@ -381,9 +381,10 @@ int jq_kv_read(const jq_kv_cache *cache, const jq_kv_batch *batch, int last, voi
  * a query that sees nothing gets 0 and -infinity.  Blocks whose tokens lie before every query's window are not looked at and may
  * hold anything.  q is [tokens, q_heads, head_dim] F16 or BF16 (strides as above), out the same shape,
  * contiguous and 16-byte aligned; query head h reads key head h / (q_heads / kv_heads).  head_dim 64 or 128.  scale > 0.
- * A row of q is brought into fp16's range by a power of two and rounded to fp16 (exact except values 2^-28
- * of the row's largest and less); codes are exact in fp16; weights relative to the row's largest are rounded to fp16
- * for the second product; scores, maxima and sums are fp32.  The split of a long cache over CTAs is by its length and
+ * A row of q is brought into fp16's range by a power of two and rounded to fp16 (exact except values 2^-28 of the row's
+ * largest and less); codes are exact in fp16; for the second product weights, times their block's value scale, are rounded to
+ * fp16: to eleven bits where they are 2^-21 of the row's largest or more, by at most 2^-32 of it below; scores, maxima and
+ * sums are fp32.  The split of a long cache over CTAs is by its length and
  * the device alone and the parts are added in their order: results repeat bit for bit.
  * workspace: jq_kv_attend_workspace_bytes, 128-byte aligned, zero before its first use, one per stream.  Its first int is a status word
  * like that of jq_gemm_ta's workspace (jq_ta_status reads it).  Allocates nothing; may be captured in a graph. */

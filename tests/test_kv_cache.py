@@ -779,3 +779,40 @@ def test_keys_of_zeros_and_queries_of_nearly_zero(new):
     q = torch.randn(new, 3, D, generator=gen).mul(1e-30).bfloat16().to(DEV)
     got, lse = cache.attend(q, table, lens, lse=True)
     _check_attend(q, got, lse, {"keys": [k[0].transpose(0, 1).double()], "values": [v[0].transpose(0, 1).double()]}, [length], [new], 0)
+
+
+@gpu
+@pytest.mark.parametrize("new,D,fmt", [(1, 64, "int8"), (1, 128, "e4m3"), (5, 128, "int8"), (40, 64, "e4m3"), (40, 128, "int8")])
+def test_one_strong_token_before_a_long_text(new, D, fmt):
+    """An attention sink: the first token has nearly all the weight and a value that is nearly zero, so that what counts is the sum of
+    thousands of small weights.  The bound is the module's with 2^-32 of the largest weight in place of 2^-25 for those that are not rounded
+    to eleven bits, and fp32 sums of one term for 64 keys.  More sequences share the text than there are CTAs: one alone would be cut
+    into parts, with the strong token in one of them."""
+    length, T, H, S, gaps = 16384, 64, 1, 600 if new < 10 else 160, [11.0, 13.2, 14.284, 15.2, 16.1]
+    blocks = length // T
+    gen = torch.Generator().manual_seed(31)
+    top = 127.0 if fmt == "int8" else 448.0
+    keys, values = torch.zeros(blocks, T, D), torch.randint(64, 113, (blocks, T, D), generator=gen).float()
+    keys[0, 0, 0], values[0, 0] = top, 1.0
+    cache = jq.KVCache.empty(blocks, H, D, block_size=T, fmt=fmt, device=DEV)
+    dense = {}
+    for what, x in (("keys", keys), ("values", values)):
+        codes = x.add(128).to(torch.uint8) if fmt == "int8" else x.to(torch.float8_e4m3fn).view(torch.uint8)
+        laid = torch.empty(blocks, T * D, dtype=torch.uint8)
+        laid[:, torch.from_numpy(oracle.places(T, D, what).reshape(-1))] = codes.reshape(blocks, T * D)
+        getattr(cache, what).copy_(laid.view(blocks, H, T, D))
+        getattr(cache, what[:-1] + "_scales").fill_(2.0 ** -6)
+        real = torch.from_numpy(oracle.decode(codes.numpy(), fmt)).double() * 2.0 ** -6
+        dense[what] = real.reshape(length, D).to(DEV)
+    q = torch.zeros(new, len(gaps), D)
+    q[:, :, 0] = torch.tensor(gaps) / (top * 2.0 ** -6)
+    q = q.half().to(DEV)
+    table, lens = torch.arange(blocks, dtype=torch.int32, device=DEV).expand(S, blocks).contiguous(), torch.full((S,), length, dtype=torch.int32, device=DEV)
+    got, lse = cache.attend(q.expand(S, new, len(gaps), D), table, lens, scale=1.0, lse=True)
+    for h in range(len(gaps)):
+        ref, want, weight, size = oracle.attend(q[:, h], dense["keys"], dense["values"], length - new, 1.0, 0)
+        off = D * 2.0 ** -24 * size + 2.0 ** -23 * size + 2.0 ** -21 + length / 64 * 2.0 ** -24
+        bound = (2.0 ** -11 + 2 * off)[:, None] * weight + 2.0 ** -32 * length * dense["values"].max() + 2.0 ** -11 * ref.abs() + 2.0 ** -24
+        err = (got[:, :, h].double() - ref).abs().amax(0)
+        assert bool((err <= bound).all()), (gaps[h], (err / bound).max().item(), (err / ref).max().item())
+        assert bool(((lse[:, :, h].double() - want).abs() <= off + 2.0 ** -22 * want.abs()).all())
