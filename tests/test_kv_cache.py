@@ -816,3 +816,25 @@ def test_one_strong_token_before_a_long_text(new, D, fmt):
         err = (got[:, :, h].double() - ref).abs().amax(0)
         assert bool((err <= bound).all()), (gaps[h], (err / bound).max().item(), (err / ref).max().item())
         assert bool(((lse[:, :, h].double() - want).abs() <= off + 2.0 ** -22 * want.abs()).all())
+
+
+@gpu
+@pytest.mark.parametrize("pairs", ["few", "many"])
+@pytest.mark.parametrize("fmt", ["int8", "e4m3"])
+@pytest.mark.parametrize("D,new,G", [(64, 1, 7), (64, 3, 5), (64, 2, 9), (64, 9, 3), (64, 4, 8), (128, 2, 4), (128, 1, 16), (128, 8, 3), (128, 2, 9)])
+def test_every_tile_of_few_rows(D, new, G, fmt, pairs):
+    """Up to 24 rows (32 at 64 values) of a key head go through one kernel in tiles of 8, 16, 24 or 32 rows, with wide CTAs where pairs of a
+    sequence and a key head are at most half as many as SMs, with narrow ones where they are more."""
+    S, H = (5, 2) if pairs == "few" else (24, 4)
+    gen = torch.Generator().manual_seed(D + new + G)
+    lengths = [1 + (37 * i * i + 11 * i) % 400 for i in range(S)]
+    lengths[1], lengths[3] = 0, 1500
+    news = [max(0, new - i % 3) if i else new for i in range(S)]
+    cache, table, dense = _filled(lengths, H, D, 32 if G > 5 else 16, fmt, 37)
+    q = torch.randn(sum(news), H * G, D, generator=gen).mul(1.5).to(torch.float16 if G % 2 else torch.bfloat16).to(DEV)
+    args = (table.to(DEV), torch.tensor(lengths, dtype=torch.int32, device=DEV), _starts(news).to(DEV), new)
+    for window in (0, 130):
+        got, lse = cache.attend(q, *args, window=window, lse=True)
+        _check_attend(q, got, lse, dense, lengths, news, window)
+        assert torch.equal(cache.attend(q, *args, window=window), got)
+    assert ops.check_status(raise_on_error=False) == 0
