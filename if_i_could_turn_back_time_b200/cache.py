@@ -213,8 +213,8 @@ class KVCache:
         x, strides = self._rows(q, 0, "q")
         if scale is None:
             scale = 1.0 / math.sqrt(self.head_dim)
-        elif not 0.0 < scale < 3e38:
-            raise RuntimeError("scale must be above 0")
+        elif not 1.5e-45 <= scale <= 2.3e38:             # (above 0 and, times log2(e), finite in fp32)
+            raise RuntimeError("scale must be above 0 and a number of fp32")
         if window < 0:
             raise RuntimeError("window is a number of tokens, 0 for all")
         heads = shape[-2]

@@ -575,7 +575,7 @@ extern "C" int jq_kv_attend_status(const jq_kv_cache *c, const jq_kv_batch *s, c
     const int bad = check_cache(c, s);
     if (bad) return bad;
     if (dtype != JQ_F16 && dtype != JQ_BF16) return JQ_ERR_BAD_DTYPE;
-    if (q_heads <= 0 || q_heads % c->kv_heads || window < 0 || !(scale > 0.f) || scale > 3e38f) return JQ_ERR_BAD_SHAPE;
+    if (q_heads <= 0 || q_heads % c->kv_heads || window < 0 || !(scale > 0.f) || !(scale * kLog2e <= 3.4e38f)) return JQ_ERR_BAD_SHAPE;
     if (c->head_dim != 64 && c->head_dim != 128) return JQ_ERR_UNSUPPORTED;
     if (s->sequences == 0 || s->tokens == 0) return JQ_OK;
     if ((long long)most_new(s) * (q_heads / c->kv_heads) > (1 << 30)) return JQ_ERR_BAD_SHAPE;

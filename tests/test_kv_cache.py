@@ -838,3 +838,16 @@ def test_every_tile_of_few_rows(D, new, G, fmt, pairs):
         _check_attend(q, got, lse, dense, lengths, news, window)
         assert torch.equal(cache.attend(q, *args, window=window), got)
     assert ops.check_status(raise_on_error=False) == 0
+
+
+@pytest.mark.parametrize("scale", [2.5e38, 3e38, 1e-50])
+def test_scales_that_fp32_cannot_hold_are_refused(scale):
+    """(2.5e38 log2(e) is infinite: every output would be NaN.)"""
+    import ctypes
+    lib, (c, b) = _lib.load(), _host_cache()
+    st, p, r = (ctypes.c_int64 * 2)(128, 64), 1 << 20, ctypes.byref
+    assert lib.jq_kv_attend(r(c), r(b), p, st, 4, scale, 0, p, None, 1, p, 1024, None) == -2
+    cache = jq.KVCache.empty(4, 2, 64, block_size=16, device="cpu")
+    table, lens = torch.zeros(2, 3, dtype=torch.int32), torch.tensor([5, 9], dtype=torch.int32)
+    with pytest.raises(RuntimeError, match="scale"):
+        cache.attend(torch.zeros(2, 4, 64).half(), table, lens, scale=scale)
