@@ -47,11 +47,9 @@ class KVCache:
         if name in _TENSORS or name == "fmt":
             object.__setattr__(self, "_c", None)
 
-    def __getstate__(self):
-        return [getattr(self, name) for name in (*_TENSORS, "fmt")]
-
     def __setstate__(self, state):
-        self.__init__(*state)
+        self.__dict__.update(state)
+        self._look()
 
     def _where(self) -> tuple:
         """Addresses and sizes of the tensors: what a change in place shows in."""
@@ -67,7 +65,7 @@ class KVCache:
     def _look(self) -> None:
         """Looks the tensors over; what a call needs of them."""
         self._c = None
-        keys, values, key_scales, value_scales, fmt = self.__getstate__()
+        keys, values, key_scales, value_scales, fmt = self.keys, self.values, self.key_scales, self.value_scales, self.fmt
         if fmt not in _FORMATS:
             raise ValueError(f"unknown cache format {fmt!r}")
         if keys.dim() != 4 or keys.shape != values.shape or keys.dtype != torch.uint8 or values.dtype != torch.uint8:

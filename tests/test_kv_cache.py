@@ -851,3 +851,18 @@ def test_scales_that_fp32_cannot_hold_are_refused(scale):
     table, lens = torch.zeros(2, 3, dtype=torch.int32), torch.tensor([5, 9], dtype=torch.int32)
     with pytest.raises(RuntimeError, match="scale"):
         cache.attend(torch.zeros(2, 4, 64).half(), table, lens, scale=scale)
+
+
+class Layered(jq.KVCache):
+    def __init__(self, layer):
+        empty = jq.KVCache.empty(3, 2, 64, block_size=16, device="cpu")
+        super().__init__(*(getattr(empty, name) for name in TENSORS))
+        self.layer = layer
+
+
+@pytest.mark.parametrize("make", [copy.copy, copy.deepcopy, _through_a_file])
+def test_a_copy_is_what_the_cache_is(make):
+    other = make(Layered(7))
+    assert type(other) is Layered and other.layer == 7 and other.nbytes() == Layered(7).nbytes()
+    seen = _lib.jq_kv_cache.from_buffer_copy(other._c)
+    assert [seen.keys, seen.values, seen.key_scales, seen.value_scales] == [getattr(other, name).data_ptr() for name in TENSORS]
