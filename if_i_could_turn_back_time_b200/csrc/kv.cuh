@@ -2,11 +2,13 @@
 //
 // A block holds T tokens (16, 32, 64 or 128) of one key head: T * D codes of a byte each for the keys and as many for the
 // values, and one fp32 scale for each.  Codes lie in the order in which a warp's matrix instructions (m16n8k16) take
-// them as their B operand, so that a lane's 16 bytes are what it multiplies and nothing is shuffled or transposed:
+// them as their 16-row operand, K of S^T = K Q^T and V^T of O^T = V^T P^T, so that a lane's 16 bytes are what it multiplies and
+// no code is shuffled or transposed:
 //   groups of 16 tokens, in a group chunks of 32 values (512 bytes), in a chunk 32 places of 16 bytes;
 //   keys:   place (g, t) holds values 8t..8t+7 of the tokens k and k + 2, k = 4 (g / 2) + g % 2;
 //   values: place (g, t) holds tokens 4t..4t+3 of the values g, g + 8, g + 16, g + 24
-// (g = place / 4, t = place % 4).  The scores that a lane gets for its keys are then the A operand of the second product.
+// (g = place / 4, t = place % 4).  A lane gets the scores of the keys that its place names (kv_attend.cu); prompts turn the same 16 bytes
+// into operands in shared memory (kv_prompt.cu).
 #pragma once
 #include "tc.cuh"
 

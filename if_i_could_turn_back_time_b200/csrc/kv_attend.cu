@@ -1,6 +1,6 @@
 // Attention over the 8-bit cache, few query rows per key head (single tokens, drafts).
 //
-// Bound by reading the cache: 64 sequences of 257 to 8191 tokens, 8 key heads of 128, 556 MB: 100 us, 5.6 TB/s; one of 131071, 269 MB: 60 us.
+// Bound by reading the cache: 64 sequences of 257 to 8191 tokens, 8 key heads of 128, 556 MB: 104 us, 5.3 TB/s (107 under the power cap); one of 131071, 269 MB: 62 us.
 // One row of 517 tokens and 32 heads takes 8 us, a chain of global latencies: lengths, table, copies, the join of the parts.
 #include "kv_attend.cuh"
 

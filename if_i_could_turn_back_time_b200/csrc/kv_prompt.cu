@@ -8,9 +8,11 @@
 //   t = s ks scale log2(e) + log2(vs),  p = 2^(t - ref),  O = sum p v_code,  l = sum p / vs,  out = O / l,
 // and O is only rescaled when a row's largest t has grown by more than 2^8 since its reference was set (kLift, kGrowth).
 //
-// 1024 tokens behind 15360 cached ones, 64 query and 8 key heads of 128: 530 us, 1000 TFLOP/s; a prompt of 2048 tokens, 32 heads: 80 us.
+// 1024 tokens behind 15360 cached ones, 64 query and 8 key heads of 128: 540 us in a short burst, 573 once the power cap holds the clock
+// at 1.84 GHz (990 and 930 TFLOP/s); a prompt of 2048 tokens, 32 heads: 79 us.
 // A step of 64 keys takes about 2100 clocks, of which the tensor core needs 1150 and the exponentials' unit 1024; the rest is the
-// latency of a row's chain scores -> maxima -> weights -> tensor memory (one thread per row: 664 us; four warps a tile).
+// latency of a row's chain scores -> maxima -> weights -> tensor memory (one thread per row: 664 us; four warps a tile).  At 80 registers a
+// thread all instances spill a little: 36 bytes stored, 48 loaded.
 #include "kv_attend.cuh"
 
 namespace jqkv {
@@ -25,8 +27,8 @@ constexpr int kStages = 4;         // of the rings of key and value operands
 constexpr int kSegments = 32;      // planned at once
 constexpr int kPairCost = 6;       // what a pair costs besides its key tiles, in units of one: queries, outputs, hand-over
 // A row's reference is set 2^7 below its largest weight, and O rescaled when that has grown by more than 2^8: weights are fp16 numbers up to
-// 2^15, with eleven bits down to 2^-21 of the largest at least.  (Many small weights behind a strong token whose value is small are then as
-// good as the output's type; with the reference at the largest they were off by 0.2 to 6 %.  us of the two cases above with 2^7 and 2^8:
+// 2^15, with eleven bits down to 2^-21 of the largest at least.  (The sum of 16384 weights of e^-11 to e^-17 behind a strong token whose value
+// is small: off by 0.1 % at most with fp16 outputs, with the reference at the largest by 0.2 to 2.5 %.  us of the two cases above with 2^7 and 2^8:
 // 573 and 80; 2^10 and 2^5: 578 and 82; 2^14 and 2: 587 and 83; 0 and 2^8: 568 and 80.)
 constexpr float kLift = 7.f, kGrowth = 8.f;
 constexpr int kScaleSlots = 8;     // tiles whose scales are kept: at most five are in use (four operands ahead of the scores)

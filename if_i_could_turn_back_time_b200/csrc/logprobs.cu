@@ -17,7 +17,7 @@ struct Args {
     const long long *tokens;
     float *logprob, *entropy, *top_logprob;
     long long *top_token;
-    int rows, vocab, k, parts, chunk;          // chunk: elements of a part, a multiple of 2048
+    int rows, vocab, k, parts, chunk;          // chunk: elements of a part, a multiple of 512
     int *counters;                             // one per row
     float *sums;                               // three per part
     unsigned long long *lists;                 // 32 per part
@@ -30,7 +30,8 @@ __device__ __forceinline__ float ex2(float x) {
 }
 
 // A value and its index as a whole number: larger values first, the lower index first among equals (0 and -0 are equal; NaN is
-// above everything).
+// above everything, but only a NaN that has a large number beside it in its 16 bytes is looked at: the alternatives of a row with a
+// NaN are some of its tokens).
 __device__ __forceinline__ unsigned long long key_of(float x, uint32_t index) {
     uint32_t u = __float_as_uint(x + 0.f);
     if (x != x) u = 0x7fffffffu;
@@ -472,7 +473,7 @@ __global__ void __launch_bounds__(kThreads) logprobs_kernel(const __grid_constan
     }
 }
 
-constexpr int kStep = 2048;                    // elements that a part has at least
+constexpr int kStep = 2048;                    // a row has at most one part for so many elements (chunks are rounded to 512)
 
 // Parts of a row: as many as fill the chip where there are few rows, one where the rows fill it by themselves.  (Halves that would fill a
 // partly empty last wave cost more than it: 2047 rows of 32003 bf16 33 us whole, 46 us in halves; 1024 of 131072 fp32 108 and 115.)

@@ -481,7 +481,8 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0) -> 
     """Log probabilities of ``tokens`` (int64 [...]) under ``logits`` ([..., vocab]; fp32, fp16 or bf16, any row stride), the
     entropy of every row and its ``top`` (up to 32) strongest tokens, the lowest index first among equals.  One pass
     over the logits, sums in fp32.  Masked logits may be -inf or the type's lowest value; a row of nothing but -inf has
-    log probabilities -inf and entropy 0, a row with a NaN or +inf has NaN.  A negative token stands for none and gives
+    log probabilities -inf and entropy 0, a row with a NaN or +inf has NaN, and the
+    alternatives of a row with a NaN are any of its tokens.  A negative token stands for none and gives
     0, a token that the vocabulary does not have gives NaN.
 
     Replaces the log-softmax of an evaluation loop's loss (the reference's TestNetwork,

@@ -384,8 +384,9 @@ int jq_kv_read(const jq_kv_cache *cache, const jq_kv_batch *batch, int last, voi
  * A row of q is brought into fp16's range by a power of two and rounded to fp16 (exact except values 2^-28 of the row's
  * largest and less); codes are exact in fp16; for the second product weights, times their block's value scale, are rounded to
  * fp16: to eleven bits where they are 2^-21 of the row's largest or more, by at most 2^-32 of it below; scores, maxima and
- * sums are fp32.  The split of a long cache over CTAs is by its length and
- * the device alone and the parts are added in their order: results repeat bit for bit.
+ * sums are fp32.  A call's work is cut over the CTAs as one whole and
+ * the parts are added in their order: the same call (lengths, starts, max_new, window, heads, device) repeats bit for bit,
+ * whereas a sequence's last bits may differ with the sequences beside it and with max_new, which chooses the kernel.
  * workspace: jq_kv_attend_workspace_bytes, 128-byte aligned, zero before its first use, one per stream.  Its first int is a status word
  * like that of jq_gemm_ta's workspace (jq_ta_status reads it).  Allocates nothing; may be captured in a graph. */
 size_t jq_kv_attend_workspace_bytes(const jq_kv_cache *cache, const jq_kv_batch *batch, int q_heads);
@@ -402,7 +403,7 @@ int jq_kv_attend_status(const jq_kv_cache *cache, const jq_kv_batch *batch, cons
  * (NULL: none) and the `top` (0 to 32) strongest tokens in falling order, the lowest index first among equals, with
  * their log probabilities.  One pass over the row, sums in fp32.  Masked logits may be -infinity or the type's lowest value; a row
  * that has nothing else than -infinity has log probabilities -infinity and entropy 0; a row with a NaN or +infinity has
- * NaN.  A token below 0 stands for none (0 is stored), one at vocab or above gives NaN.  workspace (128-byte aligned, zero
+ * NaN, and with a NaN its strongest tokens are any of the vocabulary.  A token below 0 stands for none (0 is stored), one at vocab or above gives NaN.  workspace (128-byte aligned, zero
  * before its first use, one per stream; jq_token_logprobs_workspace_bytes, which may be 0) may be the one of
  * jq_kv_attend.  The reference's counterpart is the loss of its evaluation loop
  * (Python_Jenks_Test/Jenks_Tests/QuantNetworkTest.py:227-243). */
