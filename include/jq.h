@@ -384,9 +384,10 @@ int jq_kv_read(const jq_kv_cache *cache, const jq_kv_batch *batch, int last, voi
  * A row of q is brought into fp16's range by a power of two and rounded to fp16 (exact except values 2^-28 of the row's
  * largest and less); codes are exact in fp16; for the second product weights, times their block's value scale, are rounded to
  * fp16: to eleven bits where they are 2^-21 of the row's largest or more, by at most 2^-32 of it below; scores, maxima and
- * sums are fp32.  A call's work is cut over the CTAs as one whole and
- * the parts are added in their order: the same call (lengths, starts, max_new, window, heads, device) repeats bit for bit,
- * whereas a sequence's last bits may differ with the sequences beside it and with max_new, which chooses the kernel.
+ * sums are fp32 (lse is off by about 2^-20 besides the scores' own rounding: the value scales' logarithms pass through it).
+ * A call's work is cut over the CTAs as one whole and the parts are added in their order: the same call (lengths, starts,
+ * max_new, window, heads, device) repeats bit for bit, whereas a sequence's last bits may differ with the sequences beside
+ * it and with max_new, which chooses the kernel.
  * workspace: jq_kv_attend_workspace_bytes, 128-byte aligned, zero before its first use, one per stream.  Its first int is a status word
  * like that of jq_gemm_ta's workspace (jq_ta_status reads it).  Allocates nothing; may be captured in a graph. */
 size_t jq_kv_attend_workspace_bytes(const jq_kv_cache *cache, const jq_kv_batch *batch, int q_heads);
