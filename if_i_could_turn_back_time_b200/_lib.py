@@ -12,8 +12,10 @@ from ctypes import c_char_p, c_int, c_int32, c_size_t, c_void_p
 HERE = os.path.dirname(os.path.abspath(__file__))
 
 JQ_F32, JQ_F16, JQ_BF16 = 0, 1, 2
-JQ_FMT_E2M1, JQ_FMT_GF4 = 0, 1
+JQ_FMT_E2M1, JQ_FMT_GF4, JQ_FMT_INT8 = 0, 1, 2
 JQ_KV_INT8, JQ_KV_E4M3 = 0, 1
+JQ_NORM_RMS, JQ_NORM_LAYER = 0, 1
+JQ_INT8_MAX_K = 131071
 
 
 class JqError(RuntimeError):
@@ -44,6 +46,13 @@ class jq_kv_cache(ctypes.Structure):
 class jq_kv_batch(ctypes.Structure):
     _fields_ = [(n, c_void_p) for n in ("table", "lengths", "starts")] + [
         (n, c_int32) for n in ("sequences", "table_width", "table_stride", "tokens", "max_new", "reserved")]
+
+
+class jq_norm(ctypes.Structure):
+    _fields_ = [(n, c_void_p) for n in ("x", "residual", "weight", "bias", "post_weight", "post_bias", "gate", "h", "r", "codes", "scales")] + [
+        (n, ctypes.c_int64) for n in ("stride_x", "stride_residual", "stride_codes", "gate_outer", "gate_inner")] + [
+        (n, c_int32) for n in ("rows", "width", "gate_inner_rows", "gate_one", "post", "kind", "had_block", "x_dtype", "residual_dtype",
+                               "weight_dtype", "gate_dtype")] + [("scale", ctypes.c_float), ("eps", ctypes.c_float), ("reserved", c_int32)]
 
 
 _SIGNATURES = {
@@ -93,6 +102,14 @@ _SIGNATURES = {
     "jq_token_logprobs_workspace_bytes": (c_size_t, [c_int, c_int]),
     "jq_token_logprobs": (c_int, [c_void_p, ctypes.c_int64, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p, c_int, c_void_p,
                                   c_void_p, c_void_p, c_size_t, c_void_p]),
+    "jq_quantize_rows": (c_int, [c_void_p, ctypes.c_int64, c_int, c_int, c_int, c_int, c_void_p, ctypes.c_int64, c_void_p, c_void_p]),
+    "jq_dequantize_rows": (c_int, [c_void_p, ctypes.c_int64, c_void_p, c_int, c_int, c_void_p, c_int, c_void_p]),
+    "jq_int8_scratch_bytes": (c_size_t, [c_int, c_int]),
+    "jq_int8_linear": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_void_p,
+                               c_size_t, c_void_p, c_void_p]),
+    "jq_int8_matmul": (c_int, [c_void_p, c_void_p, c_void_p, ctypes.c_int64, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int,
+                               c_void_p, c_void_p]),
+    "jq_residual_norm": (c_int, [c_void_p, c_void_p]),
     "jq_pack_e2m1_host": (c_int, [c_void_p, c_int, c_int, c_int, c_void_p, c_void_p, c_int]),
     "jq_pack_gf4_host": (c_int, [c_void_p, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p, c_int]),
     "jq_rotate_weights_host": (c_int, [c_void_p, c_int, c_int, c_int, c_int]),

@@ -7,8 +7,8 @@ into ``nn.Sequential`` models whose Linear layers sit at keys like
 A packed checkpoint keeps every non-Linear entry as it is and replaces each
 2-D ``<prefix>.weight`` by
 
-    <prefix>.qweight   uint8 [N, stride/2]
-    <prefix>.scales    fp16  [N, K/g]        (absent when g == 0)
+    <prefix>.qweight   uint8 [N, stride/2]   (int8 [N, stride] for INT8)
+    <prefix>.scales    fp16  [N, K/g]        (absent when g == 0; fp32 [N] for INT8)
     <prefix>.codebook  fp16  [N, 16]         (GF4 only)
     <prefix>.meta      int32 [5] = (format id, group size, rotation block, N, K)
 
@@ -24,9 +24,9 @@ import torch.nn as nn
 
 from .linear import JenksQuantLinear
 from .pack import PackedWeight, pack_weight
-from .spec import QuantSpec
+from .spec import FORMATS, QuantSpec
 
-_FMT = {0: "e2m1", 1: "gf4"}
+_FMT = {number: name for name, number in FORMATS.items()}
 
 
 def pack_state_dict(state_dict: Dict[str, torch.Tensor], spec: QuantSpec,
@@ -37,8 +37,8 @@ def pack_state_dict(state_dict: Dict[str, torch.Tensor], spec: QuantSpec,
     the reference derives from them (Quantization_Experiments/utils.py:1507-1513)
     is implicit in the packed codes; with ``had_block`` the rotated weight has
     no zeros to keep.  A layer whose K is not a multiple of the group size or
-    rotation block cannot use ``spec``: it is packed as ungrouped GF4 instead,
-    with a warning, and its ``.meta`` records the format actually used."""
+    rotation block cannot use ``spec``: it is packed as ungrouped GF4 instead
+    (INT8: without the rotation), with a warning, and its ``.meta`` records the format actually used."""
     only = None if only is None else set(only)
     out: Dict[str, torch.Tensor] = {}
     for key, t in state_dict.items():
@@ -46,9 +46,10 @@ def pack_state_dict(state_dict: Dict[str, torch.Tensor], spec: QuantSpec,
         if prefix is not None and t.dim() == 2 and (only is None or prefix in only):
             g = spec.group_size
             fits = (not g or t.shape[1] % g == 0) and (not spec.had_block or t.shape[1] % spec.had_block == 0)
-            use = spec if fits else QuantSpec("gf4", 0, 0)
+            use = spec if fits else QuantSpec("int8" if spec.fmt == "int8" else "gf4", 0, 0)
             if not fits:
-                warnings.warn(f"{key}: K={t.shape[1]} does not fit {spec}; packed as ungrouped GF4 instead")
+                instead = "INT8 without rotation" if spec.fmt == "int8" else "ungrouped GF4"
+                warnings.warn(f"{key}: K={t.shape[1]} does not fit {spec}; packed as {instead} instead")
             pw = pack_weight(t, use, threads=threads)
             out[prefix + ".qweight"] = pw.qweight
             if pw.scales is not None:

@@ -28,8 +28,9 @@ from .spec import QuantSpec
 class JenksQuantConv2d(nn.Conv2d):
     def __init__(self, conv_module: nn.Conv2d, bitwidth: int = 4, mask: Optional[torch.Tensor] = None, *,
                  fmt: str = "gf4", group_size: int = 0, had_block: int = 0, threads: int = 0):
-        if bitwidth != 4:
-            raise ValueError("the packed formats are 4-bit; bitwidth must be 4")
+        bits = QuantSpec(fmt, 0 if fmt == "int8" else 32).bitwidth
+        if bitwidth != bits:
+            raise ValueError(f"format {fmt} has {bits} bits; bitwidth must be {bits}")
         if conv_module.groups != 1:
             raise ValueError("grouped convolutions are not supported")
         if isinstance(conv_module.padding, str):
@@ -44,7 +45,7 @@ class JenksQuantConv2d(nn.Conv2d):
             self.bias.data = conv_module.bias.data.clone()
         self.register_buffer("mask", mask if mask is not None else torch.ones_like(self.weight.data))
         kc = self.in_channels * self.kernel_size[0] * self.kernel_size[1]
-        if group_size and kc % group_size:
+        if group_size and kc % group_size and fmt != "int8":
             warnings.warn(f"reduction length {kc} is not a multiple of the group size {group_size}: "
                           "this layer is packed as ungrouped GF4")
             group_size, fmt = 0, "gf4"

@@ -9,7 +9,8 @@ broadcasting semantics, ``commit()``, attribute ``hard_quant``, buffer
 which swaps every ``nn.Linear`` of a model and derives the mask from the zero
 weights.  What differs is what sits underneath: the weight is stored as packed
 E2M1 or GF4 codes and the forward is one fused CUDA kernel instead of
-``F.linear`` on a dense fp32 matrix.
+``F.linear`` on a dense fp32 matrix; or, with ``bitwidth=8, fmt="int8"``, as
+8-bit integers that are multiplied with activations quantised by token.
 """
 from __future__ import annotations
 
@@ -26,9 +27,12 @@ from .spec import QuantSpec
 
 class JenksQuantLinear(nn.Linear):
     def __init__(self, linear_module: nn.Linear, bitwidth: int = 4, mask: Optional[torch.Tensor] = None, *,
-                 fmt: str = "gf4", group_size: int = 128, had_block: int = 0, threads: int = 0):
-        if bitwidth != 4:
-            raise ValueError("the packed formats are 4-bit; bitwidth must be 4")
+                 fmt: str = "gf4", group_size: Optional[int] = None, had_block: int = 0, threads: int = 0):
+        if group_size is None:
+            group_size = 0 if fmt == "int8" else 128
+        spec = QuantSpec(fmt, group_size, had_block)
+        if bitwidth != spec.bitwidth:
+            raise ValueError(f"format {fmt} has {spec.bitwidth} bits; bitwidth must be {spec.bitwidth}")
         super().__init__(linear_module.in_features, linear_module.out_features,
                          bias=(linear_module.bias is not None))
         self.weight.requires_grad = False
@@ -37,7 +41,7 @@ class JenksQuantLinear(nn.Linear):
             self.bias.requires_grad = False
             self.bias.data = linear_module.bias.data.clone()
         self.register_buffer("mask", mask if mask is not None else torch.ones_like(self.weight.data))
-        self.spec = QuantSpec(fmt, group_size, had_block)
+        self.spec = spec
         self.threads = threads
         self.hard_quant = False
         self.register_buffer("qweight", None)

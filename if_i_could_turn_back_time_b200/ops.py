@@ -1,4 +1,4 @@
-"""Operators over packed weights: thin, checked calls into libjq.so.
+"""Operators over packed weights and what stands around them: thin, checked calls into libjq.so.
 
 Everything here runs on the GPU through the C ABI; there is no eager or CPU
 fallback.  The fused linear is also registered as ``torch.ops.jq.linear`` so
@@ -7,6 +7,7 @@ that it composes with torch's dispatcher (fake tensors, export).
 from __future__ import annotations
 
 import ctypes
+import struct
 import threading
 import warnings
 from typing import List, NamedTuple, Optional, Sequence
@@ -44,6 +45,8 @@ def dequantize(pw: PackedWeight) -> torch.Tensor:
     """Dense fp32 [N, K] of a packed matrix (bit-exact definition of W_hat)."""
     lib = _lib.load()
     _need_cuda(pw.qweight, pw.scales, pw.codebook)
+    if pw.spec.fmt == "int8":
+        return QuantizedRows(pw.qweight[:, :pw.K], pw.scales, torch.float32, 0).dequantize()
     out = torch.empty((pw.N, pw.K), dtype=torch.float32, device=pw.qweight.device)
     with torch.cuda.device(out.device):
         if pw.spec.fmt == "e2m1":
@@ -312,8 +315,8 @@ def conv2d(x: torch.Tensor, pw: PackedWeight, bias: Optional[torch.Tensor], kern
     kh, kw, stride_h, stride_w, pad_h, pad_w, dil_h, dil_w = geo
     if C * kh * kw != pw.K:
         raise RuntimeError(f"x has {C} channels: fields of {C * kh * kw} values, packed weight has K={pw.K}")
-    if pw.spec.had_block:
-        raise RuntimeError("a rotated weight needs the fields laid out for the linear operator")
+    if pw.spec.had_block or pw.spec.fmt == "int8":
+        raise RuntimeError("a rotated or int8 weight needs the fields laid out for the linear operator")
     ho = (H + 2 * pad_h - dil_h * (kh - 1) - 1) // stride_h + 1
     wo = (W + 2 * pad_w - dil_w * (kw - 1) - 1) // stride_w + 1
     if ho <= 0 or wo <= 0:
@@ -362,7 +365,11 @@ def conv_gathers(fmt_id: int, K: int, g: int, positions: int) -> bool:
         2048        46 / 80        72 / 130       142 / 250
         3136        52 / 124       77 / 197       129 / 355
 
-    On the device alone 196 positions of 2304 values take 33 / 26, and of 1152 values 22 / 21."""
+    On the device alone 196 positions of 2304 values take 33 / 26, and of 1152 values 22 / 21.
+
+    The fields of an int8 layer are always unfolded: they become codes by position."""
+    if fmt_id == _lib.JQ_FMT_INT8:
+        return False
     few = ta_max_batch(fmt_id) if fmt_id == _lib.JQ_FMT_E2M1 and ta_eligible(fmt_id, K, g, positions) else 16
     return positions > few and (K <= 1536 or positions > 2048)
 
@@ -390,6 +397,8 @@ def _linear_rows(x2, qweight, scales, codebook, bias, fmt_id, N, K, g, had, out_
     lib = _lib.load()
     Bt = x2.shape[0]
     y = torch.empty((Bt, N), dtype=_OUT[out_id] or x2.dtype, device=x2.device)
+    if fmt_id == _lib.JQ_FMT_INT8:
+        return _linear_int8(x2, qweight, scales, bias, N, K, had, y)
     if many_rows(fmt_id, K, g, Bt):
         return _linear_many_rows(x2, qweight, scales, codebook, bias, fmt_id, N, K, g, had, y)
     if ta_eligible(fmt_id, K, g, Bt):
@@ -441,10 +450,14 @@ def _(x, qweight, scales, codebook, bias, fmt_id, N, K, group_size, had_block, o
     return x.new_empty((*x.shape[:-1], N), dtype=_OUT[out_id] or x.dtype)
 
 
-def linear(x: torch.Tensor, pw: PackedWeight, bias: Optional[torch.Tensor] = None,
+def linear(x, pw: PackedWeight, bias: Optional[torch.Tensor] = None,
            out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
     """``F.linear(rotate(x), W_hat, bias)`` without materialising W_hat; any
-    leading dims, last dim = K; output dtype = input dtype unless given."""
+    leading dims, last dim = K; output dtype = input dtype unless given.
+    An int8 weight multiplies x as ``quantize_rows`` gives it; several that
+    share an input take its ``QuantizedRows`` in x's place."""
+    if isinstance(x, QuantizedRows):
+        return _linear_quantized(x, pw, bias, out_dtype)
     if x.shape[-1] != pw.K:
         raise RuntimeError(f"last dim of x is {x.shape[-1]}, packed weight has K={pw.K}")
     if x.dtype not in _DT:
@@ -464,6 +477,285 @@ def linear(x: torch.Tensor, pw: PackedWeight, bias: Optional[torch.Tensor] = Non
     y = _linear_rows(x2, pw.qweight, pw.scales, pw.codebook, bias, pw.spec.fmt_id, pw.N, pw.K, pw.spec.group_size,
                      pw.spec.had_block, out_id)
     return y if flat else y.reshape(*x.shape[:-1], pw.N)
+
+
+class QuantizedRows(NamedTuple):
+    """Activations in 8-bit integers, a scale for each row: what ``quantize_rows`` and ``residual_norm`` make and ``linear``
+    multiplies with int8 weights."""
+    codes: torch.Tensor                   # int8 [..., K], rows a multiple of 16 bytes apart
+    scales: torch.Tensor                  # fp32 [...]; a row that had a NaN or an infinity has NaN
+    dtype: torch.dtype                    # of the values that the codes stand for, and of linear()'s outputs unless it is told
+    had_block: int = 0                    # 128: the values are rotated, as weights with this had_block need them
+
+    def dequantize(self, dtype: Optional[torch.dtype] = None) -> torch.Tensor:
+        """code * scale, of ``dtype`` or the rows' own; rotated rows as they are."""
+        dtype = dtype or self.dtype
+        if dtype not in _DT:
+            raise RuntimeError(f"unsupported dtype {dtype}")
+        codes, scales, K, stride = _codes_of(self)
+        out = torch.empty(self.codes.shape, dtype=dtype, device=codes.device)
+        if codes.shape[0]:
+            with _on(codes.device):
+                st = _lib.load().jq_dequantize_rows(codes.data_ptr(), stride, scales.data_ptr(), codes.shape[0], K, out.data_ptr(),
+                                                    _DT[dtype], _stream())
+            if st:
+                _lib.check(st, "jq_dequantize_rows")
+        return out
+
+
+def _row_stride(K: int) -> int:
+    return (K + 31) // 32 * 32
+
+
+def _codes_of(rows: QuantizedRows):
+    """(codes [n, K], scales [n], K, elements between rows of codes), looked over and laid out as the library takes them."""
+    codes, scales = rows.codes, rows.scales
+    if codes.dtype is not torch.int8 or codes.dim() == 0 or scales.dtype is not torch.float32 or scales.shape != codes.shape[:-1]:
+        raise RuntimeError(f"codes {tuple(codes.shape)} {codes.dtype}, scales {tuple(scales.shape)} {scales.dtype}: int8 [..., K] and fp32 [...]")
+    K = codes.shape[-1]
+    if not 0 < K <= _lib.JQ_INT8_MAX_K:
+        raise RuntimeError(f"rows of {K} codes: 1 to {_lib.JQ_INT8_MAX_K}")
+    _need_cuda(codes, scales)
+    if scales.device != codes.device:
+        raise RuntimeError(f"codes are on {codes.device}, scales on {scales.device}")
+    if codes.dim() != 2:
+        codes = codes.reshape(-1, K)
+    if codes.shape[0] > 0x7fffffff:
+        raise RuntimeError(f"{codes.shape[0]} rows: the library counts in 32 bits")
+    if scales.is_neg():
+        scales = scales.resolve_neg()
+    if not scales.is_contiguous():
+        scales = scales.contiguous()
+    stride, one = codes.stride()
+    if codes.shape[0] == 1:
+        stride = _row_stride(K)
+    if (one != 1 and K > 1) or stride % 16 or stride < K or codes.data_ptr() % 16:
+        stride = _row_stride(K)
+        laid = torch.empty((codes.shape[0], stride), dtype=torch.int8, device=codes.device)
+        laid[:, :K] = codes
+        codes = laid[:, :K]
+    return codes, scales, K, stride
+
+
+def _rows_of(x: torch.Tensor, what: str):
+    """x [..., K] as (tensor [n, K], elements between rows): rows of one stride, values adjacent."""
+    if x.dtype not in _DT:
+        raise RuntimeError(f"unsupported dtype {x.dtype} of {what}")
+    if x.is_neg():
+        x = x.resolve_neg()
+    if x.dim() != 2:
+        x = x.reshape(-1, x.shape[-1])
+    row, one = x.stride()
+    if (one != 1 and x.shape[1] > 1) or row < 0:
+        x = x.contiguous()
+        row = x.shape[1]
+    if x.shape[0] > 0x7fffffff:
+        raise RuntimeError(f"{x.shape[0]} rows of {what}: the library counts in 32 bits")
+    return x, row
+
+
+def quantize_rows(x: torch.Tensor, had_block: int = 0) -> QuantizedRows:
+    """x [..., K] (fp32, fp16 or bf16; any row stride) in 8-bit integers: scale = max(|x|, 2^-100) / 127 for each row, codes
+    x / scale to the nearest integer (ties to even).  With ``had_block`` 128 the row is rotated first, as weights of that
+    ``had_block`` need it.  A row with a NaN or an infinity has the scale NaN, so that what is computed from it is NaN.  One launch.
+
+    The activation's side of the reference's integer grid (QuantLinear, Python_Jenks_Test/Jenks_Tests/
+    Quantization_Experiments/layers.py:22-38, which quantises weights only)."""
+    if x.dim() == 0 or not 0 < x.shape[-1] <= _lib.JQ_INT8_MAX_K:
+        raise RuntimeError(f"x is {tuple(x.shape)}: rows of 1 to {_lib.JQ_INT8_MAX_K} values")
+    if had_block not in (0, 128) or (had_block and x.shape[-1] % had_block):
+        raise RuntimeError(f"had_block is {had_block}: 0, or 128 where rows are a multiple of it (here {x.shape[-1]})")
+    x2, row = _rows_of(x, "x")
+    _need_cuda(x)
+    K, lead, stride = x.shape[-1], x.shape[:-1], _row_stride(x.shape[-1])
+    codes = torch.empty((*lead, stride), dtype=torch.int8, device=x.device)
+    scales = torch.empty(lead, dtype=torch.float32, device=x.device)
+    if x2.shape[0]:
+        with _on(x.device):
+            st = _lib.load().jq_quantize_rows(x2.data_ptr(), row, x2.shape[0], K, had_block, _DT[x.dtype], codes.data_ptr(), stride,
+                                              scales.data_ptr(), _stream())
+        if st:
+            _lib.check(st, "jq_quantize_rows")
+    return QuantizedRows(codes if stride == K else codes[..., :K], scales, x.dtype, had_block)
+
+
+def _int8_weight(device, qweight, scales, bias, N, K):
+    """Refuses tensors that are not an int8 weight as the library takes it; the bias as it takes that."""
+    if qweight.dtype is not torch.int8 or qweight.shape != (N, _row_stride(K)) or not qweight.is_contiguous() or \
+            scales is None or scales.dtype is not torch.float32 or scales.shape != (N,) or not scales.is_contiguous():
+        raise RuntimeError(f"an int8 weight is int8 [{N}, {_row_stride(K)}] with fp32 scales [{N}], contiguous")
+    if qweight.device != device or scales.device != device or (bias is not None and bias.device != device):
+        raise RuntimeError(f"the activation is on {device}, the weight, its scales or the bias elsewhere")
+    if bias is None:
+        return None
+    if bias.shape != (N,):
+        raise RuntimeError(f"bias {tuple(bias.shape)}: [{N}]")
+    return bias if bias.is_contiguous() and not bias.is_neg() else bias.resolve_neg().contiguous()
+
+
+def _linear_int8(x2, qweight, scales, bias, N, K, had, y):
+    bias = _int8_weight(x2.device, qweight, scales, bias, N, K)
+    lib = _lib.load()
+    rows, stride = x2.shape[0], _row_stride(K)
+    part = max(256, MAX_ROWS_SCRATCH // stride // 256 * 256)
+    with _on(x2.device):
+        for b0 in range(0, rows, part):
+            b1 = min(rows, b0 + part)
+            xs, ys = (x2, y) if rows <= part else (x2[b0:b1], y[b0:b1])
+            own, scratch, size, status = _rows_scratch(x2.device, ((b1 - b0) * 4 + 255) // 256 * 256 + (b1 - b0) * stride)
+            st = lib.jq_int8_linear(qweight.data_ptr(), scales.data_ptr(), xs.data_ptr(), _addr(bias), ys.data_ptr(), N, K, b1 - b0, had,
+                                    _DT[x2.dtype], _DT[y.dtype], scratch, size, status, _stream())
+            if st:
+                _lib.check(st, "jq_int8_linear")
+            del own
+    if _checked:
+        check_status()
+    return y
+
+
+def _linear_quantized(x: QuantizedRows, pw: PackedWeight, bias, out_dtype) -> torch.Tensor:
+    if pw.spec.fmt != "int8":
+        raise RuntimeError(f"rows of 8-bit integers multiply int8 weights, not {pw.spec.fmt}")
+    codes, scales, K, stride = _codes_of(x)
+    if K != pw.K:
+        raise RuntimeError(f"rows of {K} codes, packed weight has K={pw.K}")
+    if x.had_block != pw.spec.had_block:
+        raise RuntimeError(f"rows with had_block {x.had_block}, packed weight has {pw.spec.had_block}")
+    dtype = out_dtype or x.dtype
+    if dtype not in _DT:
+        raise RuntimeError(f"unsupported output dtype {dtype}")
+    _need_cuda(pw.qweight, pw.scales, bias)
+    if bias is not None and bias.dtype != torch.float32:
+        bias = bias.float()
+    bias = _int8_weight(codes.device, pw.qweight, pw.scales, bias, pw.N, K)
+    y = torch.empty((*x.codes.shape[:-1], pw.N), dtype=dtype, device=codes.device)
+    if codes.shape[0]:
+        with _on(codes.device):
+            status = _workspace(codes.device, 1024, "ta").data_ptr()
+            st = _lib.load().jq_int8_matmul(pw.qweight.data_ptr(), pw.scales.data_ptr(), codes.data_ptr(), stride, scales.data_ptr(),
+                                            _addr(bias), y.data_ptr(), pw.N, K, codes.shape[0], _DT[dtype], status, _stream())
+        if st:
+            _lib.check(st, "jq_int8_matmul")
+        if _checked:
+            check_status()
+    return y
+
+
+class ResidualNorm(NamedTuple):
+    """What ``residual_norm`` returns, of x's shape."""
+    h: object                             # the next block's input: a tensor of x's dtype, or QuantizedRows
+    r: torch.Tensor                       # the residual stream behind the block
+
+
+NORM_MAX_WIDTH = 32768                    # a row stays in the registers of one block
+_NORM_KINDS = {"rms": _lib.JQ_NORM_RMS, "layer": _lib.JQ_NORM_LAYER}
+_pack_norm = struct.Struct("=QQQQQQQQQQQqqqqqiiiiiiiiiiiffi").pack        # jq_norm
+
+
+def residual_norm(x: torch.Tensor, residual: Optional[torch.Tensor] = None, weight: Optional[torch.Tensor] = None,
+                  bias: Optional[torch.Tensor] = None, *, post_weight: Optional[torch.Tensor] = None,
+                  post_bias: Optional[torch.Tensor] = None, gate: Optional[torch.Tensor] = None, scale: float = 1.0, eps: float = 1e-6,
+                  kind: str = "rms", quantize: bool = False, had_block: int = 0) -> ResidualNorm:
+    """What stands between a block's output ``x`` [..., width] and the next block's input, in one launch:
+
+        u = N(x) * post_weight + post_bias       (x itself where there is no post_weight)
+        r = residual + scale * (gate * u)
+        h = N(r) * weight + bias
+
+    with N(v) = v / sqrt(mean(v^2) + eps) (``kind`` "rms") or (v - mean(v)) / sqrt(var(v) + eps) ("layer"), everything in fp32
+    and rounded once: ``h`` to x's dtype, ``r`` to the residual's (x's or fp32).  h follows from r before its rounding.  The
+    weights and biases are [width] of one dtype; the gate has any shape that broadcasts to x's: a channel's, a sequence's, a token's.
+    With ``quantize`` h comes as ``QuantizedRows`` (rotated with ``had_block`` 128) for int8 linears, without passing through 16
+    bits.  Without residual, gate, scale and post_weight ``r`` is x.  Widths up to 32768.  Serving only: an input that asks for a gradient is
+    refused while gradients are recorded.
+
+    The reference has no norm (its models are the vision networks and the MLP of Python_Jenks_Test/Jenks_Tests/QuantNetworkTest.py)."""
+    shape, dtype, device = x.shape, x.dtype, x.device
+    if not shape or not 0 < shape[-1] <= NORM_MAX_WIDTH:
+        raise RuntimeError(f"x is {tuple(shape)}: rows of 1 to {NORM_MAX_WIDTH} values")
+    width = shape[-1]
+    if kind not in _NORM_KINDS:
+        raise RuntimeError(f"unknown kind of norm {kind!r}: rms or layer")
+    if had_block and (not quantize or had_block != 128 or width % 128):
+        raise RuntimeError(f"had_block is {had_block}: 0, or 128 with quantize where the width is a multiple of it (here {width})")
+    if post_bias is not None and post_weight is None:
+        raise RuntimeError("a post_bias comes with a post_weight")
+    if not eps >= 0 or not -3.4e38 <= scale <= 3.4e38 or eps > 3.4e38:
+        raise RuntimeError("scale is a finite number of fp32, eps one from 0 on")
+    vectors = [t for t in (weight, bias, post_weight, post_bias) if t is not None]
+    for t in vectors:
+        if t.shape != (width,) or t.dtype not in _DT or t.dtype != vectors[0].dtype:
+            raise RuntimeError(f"weights and biases are tensors [{width}] of one dtype; got {tuple(t.shape)} {t.dtype}")
+    if gate is not None and gate.dtype not in _DT:
+        raise RuntimeError(f"unsupported dtype {gate.dtype} of the gate")
+    if residual is not None and (residual.shape != shape or (residual.dtype != dtype and residual.dtype is not torch.float32)):
+        raise RuntimeError(f"residual {tuple(residual.shape)} {residual.dtype}: x's shape {tuple(shape)} and dtype, or fp32")
+    given = [t for t in (x, residual, gate) if t is not None] + vectors
+    _need_cuda(*given)
+    for t in given:
+        if t.device != device:
+            raise RuntimeError(f"x is on {device}, another tensor on {t.device}")
+    if torch.is_grad_enabled() and any(t.requires_grad for t in given):
+        raise RuntimeError("residual_norm has no backward pass: call it under torch.no_grad()")
+    x2, stride_x = _rows_of(x, "x")
+    stride_res = 0
+    if residual is not None:
+        residual, stride_res = _rows_of(residual, "the residual")
+    weight, bias, post_weight, post_bias = (None if t is None else t.resolve_neg().contiguous() for t in (weight, bias, post_weight, post_bias))
+    outer = inner = one = 0
+    each = 1
+    if gate is not None:
+        gate, outer, inner, each, one = _gate_of(gate.resolve_neg(), shape)
+    rows = x2.shape[0]
+    same = residual is None and gate is None and scale == 1.0 and post_weight is None
+    rdtype = dtype if residual is None else residual.dtype
+    r = x if same else torch.empty(shape, dtype=rdtype, device=device)
+    codes = scales = out = None
+    stride_q = 0
+    if quantize:
+        stride_q = _row_stride(width)
+        codes = torch.empty((*shape[:-1], stride_q), dtype=torch.int8, device=device)
+        scales = torch.empty(shape[:-1], dtype=torch.float32, device=device)
+        h = QuantizedRows(codes if stride_q == width else codes[..., :width], scales, dtype, had_block)
+    else:
+        h = out = torch.empty(shape, dtype=dtype, device=device)
+    if rows:
+        P = lambda t: 0 if t is None else t.data_ptr()                                                        # noqa: E731
+        packed = _pack_norm(x2.data_ptr(), P(residual), P(weight), P(bias), P(post_weight), P(post_bias), P(gate), P(out),
+                            0 if same else r.data_ptr(), P(codes), P(scales), stride_x, stride_res, stride_q, outer, inner, rows, width, each,
+                            one, post_weight is not None, _NORM_KINDS[kind], had_block, _DT[dtype], _DT[rdtype],
+                            _DT[vectors[0].dtype] if vectors else 0, 0 if gate is None else _DT[gate.dtype], scale, eps, 0)
+        with _on(device):
+            st = _lib.load().jq_residual_norm(packed, _stream())
+        if st:
+            _lib.check(st, "jq_residual_norm")
+    return ResidualNorm(h, r)
+
+
+def _gate_of(gate: torch.Tensor, shape):
+    """(gate, outer, inner, rows each, one value for a row) of a gate that broadcasts to shape: row i's values begin at
+    (i // each) * outer + (i % each) * inner."""
+    try:
+        g = gate.expand(shape)
+    except RuntimeError:
+        raise RuntimeError(f"a gate {tuple(gate.shape)} does not broadcast to {tuple(shape)}") from None
+    one = g.stride(-1) == 0 or shape[-1] == 1
+    if not one and g.stride(-1) != 1:
+        gate = gate.contiguous()
+        g = gate.expand(shape)
+    # leading dims with more than one row, from the last on: one stride for the rows of a group, another for the groups
+    dims = [(n, s) for n, s in zip(shape[:-1], g.stride()[:-1]) if n != 1]
+    steps = []
+    for n, s in reversed(dims):
+        if steps and s == steps[-1][0] * steps[-1][1]:
+            steps[-1] = (steps[-1][0] * n, steps[-1][1])
+        else:
+            steps.append((n, s))
+    if len(steps) > 2 or any(s < 0 for _, s in steps):
+        gate = (g if not one else g[..., :1]).contiguous()
+        return gate, gate.shape[-1], 0, 1, int(one)
+    each, inner = steps[0] if steps else (1, 0)
+    return gate, steps[1][1] if len(steps) > 1 else 0, inner, max(1, each), int(one)
 
 
 class TokenLogprobs(NamedTuple):
@@ -558,6 +850,8 @@ class GroupedGemv:
         if not weights:
             raise ValueError("no problems")
         spec0 = weights[0].spec
+        if spec0.fmt == "int8":
+            raise ValueError("a grouped launch takes the packed 4-bit formats")
         for w in weights:
             if w.spec.fmt != spec0.fmt:
                 raise ValueError("a grouped launch needs one weight format")

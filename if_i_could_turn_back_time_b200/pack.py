@@ -24,8 +24,8 @@ class PackedWeight:
     spec: QuantSpec
     N: int
     K: int
-    qweight: torch.Tensor                 # uint8 [N, stride/2]
-    scales: Optional[torch.Tensor]        # fp16 [N, K/g] or None
+    qweight: torch.Tensor                 # uint8 [N, stride/2], or int8 [N, stride] (int8)
+    scales: Optional[torch.Tensor]        # fp16 [N, K/g] or None, or fp32 [N] (int8)
     codebook: Optional[torch.Tensor]      # fp16 [N, 16] (gf4) or None
 
     def to(self, device) -> "PackedWeight":
@@ -109,11 +109,38 @@ def _pack_gf4_cuda(W: torch.Tensor, spec: QuantSpec, rotate: bool) -> PackedWeig
     return PackedWeight(spec, N, K, q, s, cb)
 
 
+def _pack_int8(W: torch.Tensor, spec: QuantSpec, threads: int, rotate: bool) -> PackedWeight:
+    """Codes and a scale for every row, by the rule of ``ops.quantize_rows``; on the CPU in torch operations of the same bits."""
+    N, K = W.shape
+    if not 0 < K <= _lib.JQ_INT8_MAX_K:
+        raise ValueError(f"K={K}: int8 takes rows of 1 to {_lib.JQ_INT8_MAX_K} values")
+    if spec.had_block and K % spec.had_block:
+        raise ValueError(f"K={K} is not a multiple of the rotation block {spec.had_block}")
+    q = torch.zeros((N, row_stride_codes(K)), dtype=torch.int8, device=W.device)
+    if W.is_cuda:
+        from . import ops
+        rows = ops.quantize_rows(W.detach(), spec.had_block if rotate else 0)
+        q[:, :K] = rows.codes
+        return PackedWeight(spec, N, K, q, rows.scales, None)
+    Wf = W.detach().to(torch.float32).contiguous()
+    if spec.had_block and rotate:
+        Wf = Wf.clone()
+        _lib.check(_lib.load().jq_rotate_weights_host(Wf.data_ptr(), N, K, spec.had_block, threads), "jq_rotate_weights_host")
+    size = Wf.abs().amax(1)
+    good = torch.isfinite(size)
+    scales = torch.where(good, size, 0.0).clamp_(min=2.0 ** -100) / torch.full_like(size, 127.0)
+    codes = torch.round(Wf / scales[:, None]).clamp_(-127, 127)
+    q[:, :K] = torch.where(good[:, None], codes, 0.0).to(torch.int8)
+    return PackedWeight(spec, N, K, q, torch.where(good, scales, torch.nan), None)
+
+
 def pack_weight(W: torch.Tensor, spec: QuantSpec, threads: int = 0, rotate: bool = True) -> PackedWeight:
     """Quantise and pack W [N, K].  With ``spec.had_block`` the weight is first
     multiplied on the right by the block Hadamard matrix (fp32), so that
     ``W x == (W H)(H x)`` once the operator rotates x."""
     lib = _lib.load()
+    if spec.fmt == "int8":
+        return _pack_int8(W, spec, threads, rotate)
     if W.is_cuda and spec.fmt == "e2m1" and _gpu_packable(W, spec):
         return _pack_e2m1_cuda(W, spec, rotate)
     if W.is_cuda and spec.fmt == "gf4" and W.shape[1] <= GF4_DEVICE_MAX_K:

@@ -71,6 +71,7 @@ extern "C" {
 /* weight formats */
 #define JQ_FMT_E2M1 0
 #define JQ_FMT_GF4 1
+#define JQ_FMT_INT8 2   /* 8-bit integers for weights and activations: the jq_int8_* entries below */
 
 /* ops for jq_workspace_bytes */
 #define JQ_OP_GEMV 0
@@ -412,6 +413,56 @@ size_t jq_token_logprobs_workspace_bytes(int rows, int vocab);
 int jq_token_logprobs(const void *logits, int64_t row_stride, int rows, int vocab, int dtype, const int64_t *tokens,
                       float *logprob, float *entropy_or_null, int top, float *top_logprob_or_null,
                       int64_t *top_token_or_null, void *workspace, size_t workspace_bytes, jq_stream_t stream);
+
+/* ---- linear layers in 8-bit integers, and the norms around a block ----
+ * Format INT8: a row of K values (a token's activation, or a channel's weights) is K signed codes and one fp32 scale, value =
+ * code * scale; rows of weights are jq_row_stride = K rounded up to a multiple of 32 codes apart, those of activations any multiple of 16;
+ * what lies between K and the stride is not read.  The codes' base is 16-byte aligned.  K is at most JQ_INT8_MAX_K, so that a sum of K
+ * products has 32 bits.  The counterpart of the reference is the per-row integer grid of QuantLinear
+ * (Python_Jenks_Test/Jenks_Tests/Quantization_Experiments/layers.py:22-38), which it multiplies out in fp32.
+ *
+ * jq_quantize_rows: x [rows, K] of x_dtype, rows row_stride elements apart (0: the same row again), rotated first where had_block is
+ * 128 (K % 128 == 0; the bits of jq_fwht_block):
+ *   scale = max(|x|, 2^-100) / 127,  code = x / scale to the nearest integer, ties to even  (both quotients rounded to fp32);
+ * a row with a NaN or an infinity has the scale NaN and codes 0.  One launch, as jq_dequantize_rows (out [rows, K] = code * scale). */
+#define JQ_INT8_MAX_K 131071
+int jq_quantize_rows(const void *x, int64_t row_stride, int rows, int K, int had_block, int x_dtype, void *codes,
+                     int64_t code_stride, float *scales, jq_stream_t stream);
+int jq_dequantize_rows(const void *codes, int64_t code_stride, const float *scales, int rows, int K, void *out, int dtype,
+                       jq_stream_t stream);
+/* y[B, N] = (sum of products of codes, exact, * the channel's scale) * the token's scale + bias, in fp32, rounded to y_dtype:
+ * the F.linear(x, W_bar, bias) of Quantization_Experiments/layers.py:38 with both operands in 8 bits.  jq_int8_linear quantises x
+ * [B, K] (row-major) into scratch (16-byte aligned, jq_int8_scratch_bytes), two launches; jq_int8_matmul takes rows of codes, one
+ * launch.  y is [B, N] row-major and overlaps no input.  The result does not depend on how the work is cut: a row's is the same whatever rows
+ * are beside it.  status_dev: as for jq_gemm_rows. */
+size_t jq_int8_scratch_bytes(int B, int K);
+int jq_int8_linear(const void *qweight, const float *scales, const void *x, const float *bias_or_null, void *y, int N, int K, int B,
+                   int had_block, int x_dtype, int y_dtype, void *scratch, size_t scratch_bytes, int *status_dev, jq_stream_t stream);
+int jq_int8_matmul(const void *qweight, const float *scales, const void *codes, int64_t code_stride, const float *row_scales,
+                   const float *bias_or_null, void *y, int N, int K, int B, int y_dtype, int *status_dev, jq_stream_t stream);
+
+/* The norms on both sides of a block with its gate, residual scale and sum, a row [width] at a time (width up to 32768):
+ *   u = N(x) * post_weight + post_bias  (post != 0; x otherwise),   r = residual + scale * (gate * u),   h = N(r) * weight + bias,
+ *   N(v) = v / sqrt(mean(v^2) + eps) (JQ_NORM_RMS) or (v - mean(v)) / sqrt(mean((v - mean(v))^2) + eps) (JQ_NORM_LAYER),
+ * all in fp32; h follows from r before its rounding.  residual, gate, weights and biases may be NULL (0, 1, 1, 0); r may be NULL where
+ * nobody wants it.  h is [rows, width] of x_dtype, or, where codes is given, h rotated (had_block 128) and quantised as by jq_quantize_rows into
+ * codes and scales.  r is [rows, width] of residual_dtype, which is x_dtype or F32.  x and residual have rows a stride apart, h and r are
+ * contiguous.  gate: row i's is at gate + (i / gate_inner_rows) gate_outer + (i % gate_inner_rows) gate_inner, `width` values, or one
+ * for the whole row (gate_one).  weight, bias, post_weight and post_bias are of weight_dtype.  h, r and codes overlap no input.  One launch.  The
+ * reference has no norm (its models are vision networks and an MLP, Python_Jenks_Test/Jenks_Tests/QuantNetworkTest.py). */
+#define JQ_NORM_RMS 0
+#define JQ_NORM_LAYER 1
+typedef struct jq_norm {
+    const void *x, *residual, *weight, *bias, *post_weight, *post_bias, *gate;
+    void *h, *r, *codes;
+    float *scales;
+    int64_t stride_x, stride_residual, stride_codes, gate_outer, gate_inner;
+    int32_t rows, width, gate_inner_rows, gate_one, post, kind, had_block;
+    int32_t x_dtype, residual_dtype, weight_dtype, gate_dtype;
+    float scale, eps;
+    int32_t reserved;      /* must be 0 */
+} jq_norm;
+int jq_residual_norm(const jq_norm *n, jq_stream_t stream);
 
 /* ---- host-side packers (CPU, multi-threaded; one-off, not the hot path) ----
  * Replace the grid/scale construction of QuantLinear.__init__

@@ -1,0 +1,435 @@
+"""Activations in 8-bit integers and their products with int8 weights.
+
+Codes and scales are held to their definition bit for bit.  A product's integer sum is exact; what follows is a conversion, a product and
+a fused multiply-add in fp32 and one rounding to the output's type, each off by at most half a step: 3 * 2^-24 of |sum * scales|,
+2^-24 of the result and eps / 2 of it (and half of the type's smallest step where the result is below its normal range)."""
+import copy
+import io
+import warnings
+
+import pytest
+import torch
+import torch.nn as nn
+import torch.nn.functional as F
+
+import if_i_could_turn_back_time_b200 as jq
+from if_i_could_turn_back_time_b200 import _lib, checkpoint, ops
+
+DEV = "cuda"
+gpu = pytest.mark.gpu
+DTYPES = (torch.float32, torch.float16, torch.bfloat16)
+
+
+def _codes(v):
+    """Codes and scales of fp32 rows [n, K], by their definition, on the CPU."""
+    v = v.cpu()
+    size = v.abs().amax(-1)
+    good = torch.isfinite(size)                                    # (NaN counts as the largest)
+    s = torch.where(good, size, 0.0).clamp(min=2.0 ** -100) / torch.full_like(size, 127.0)
+    q = torch.where(good[:, None], torch.round(v / s[:, None]).clamp(-127, 127), 0.0).to(torch.int8)
+    return q, torch.where(good, s, torch.nan)
+
+
+def _same(a, b):
+    return torch.equal(torch.isnan(a), torch.isnan(b)) and torch.equal(a.nan_to_num(0), b.nan_to_num(0))
+
+
+def _product(q, s, pw, bias, dtype):
+    """(result, bound) in 64 bits of codes [n, K] with their scales."""
+    total = q.double() @ pw.qweight[:, :pw.K].double().T           # (below 2^53: exact)
+    y = total * pw.scales.double() * s.double()[:, None]
+    part = y.abs()
+    if bias is not None:
+        y = y + bias.double()
+    fin = torch.finfo(dtype)
+    bound = 3 * 2.0 ** -24 * part + (2.0 ** -24 + fin.eps / 2) * (y.abs() + part * 2.0 ** -22) + fin.smallest_normal * fin.eps / 2
+    return y, bound
+
+
+def _near(got, want, bound):
+    assert got.shape == want.shape
+    off = (got.double() - want).abs()
+    assert bool((off <= bound).all()), (off / bound).max().item()
+
+
+def _weight(N, K, seed=0, had=0):
+    gen = torch.Generator(DEV).manual_seed(seed)
+    return jq.pack_weight(torch.randn(N, K, device=DEV, generator=gen) * (torch.rand(N, 1, device=DEV, generator=gen) + 0.5), jq.QuantSpec("int8", 0, had))
+
+
+# ------------------------------------------------------------------------------------------------------------ quantising
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,K", [(1, 1), (3, 7), (5, 8), (2, 31), (70, 100), (9, 256), (1, 1000), (400, 1000), (6, 1024), (400, 1032), (1, 8192), (301, 4100),
+                                    (500, 4096), (3, 32768), (2, 32776), (300, 11008), (2, 131071)])
+def test_codes_are_those_of_the_definition(rows, K, dtype):
+    gen = torch.Generator(DEV).manual_seed(rows + K)
+    x = torch.randn(rows, K, device=DEV, generator=gen)
+    x[:, ::13] *= 9
+    x = (x * torch.rand(rows, 1, device=DEV, generator=gen)).to(dtype)
+    got = ops.quantize_rows(x)
+    q, s = _codes(x.float())
+    assert got.codes.shape == (rows, K) and got.codes.stride(0) % 32 == 0 and got.dtype == dtype and got.had_block == 0
+    assert torch.equal(got.scales.cpu(), s) and torch.equal(got.codes.cpu(), q)
+    for out in DTYPES:
+        want = (q.float() * s[:, None]).to(out)
+        assert torch.equal(got.dequantize(out).cpu(), want)
+    assert got.dequantize().dtype == dtype
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,K", [(1, 128), (400, 128), (7, 384), (600, 1024), (3, 4096), (330, 11008), (2, 32768), (3, 33024)])
+def test_rotated_codes(rows, K, dtype):
+    """The rotation has the bits of ops.fwht_block."""
+    x = torch.randn(rows, K, device=DEV, generator=torch.Generator(DEV).manual_seed(K)).to(dtype)
+    x[:, 5] *= 30
+    got = ops.quantize_rows(x, had_block=128)
+    q, s = _codes(ops.fwht_block(x, 128))
+    assert got.had_block == 128 and torch.equal(got.scales.cpu(), s) and torch.equal(got.codes.cpu(), q)
+
+
+@gpu
+def test_quotients_at_the_border_of_two_codes():
+    """Values half a step from a code and their neighbours of fp32, at scales of many sizes: where the products with the reciprocals
+    on both sides of it disagree."""
+    size = torch.tensor([127.0, 254.0, 1.0, 3.3, 1e-20, 7e18, 2.0 ** -100, 126.99999, 0.1], device=DEV)
+    half = torch.arange(-126.5, 127, 1, device=DEV)
+    x = half * (size / 127)[:, None]
+    x = torch.cat([torch.nextafter(x, torch.full_like(x, -torch.inf)), x, torch.nextafter(x, torch.full_like(x, torch.inf)), size[:, None]], 1)
+    got = ops.quantize_rows(x)
+    q, s = _codes(x)
+    assert torch.equal(got.codes.cpu(), q) and torch.equal(got.scales.cpu(), s)
+
+
+@gpu
+@pytest.mark.parametrize("K", [24, 1003, 9000])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_rows_that_go_wrong(K, dtype):
+    x = torch.randn(400, K, device=DEV).to(dtype)
+    x[0] = 0
+    x[1, K // 2] = torch.nan
+    x[2, K - 1] = torch.inf
+    x[3, 0] = -torch.inf
+    x[4] = torch.finfo(dtype).max
+    x[5] = torch.finfo(dtype).tiny / 4
+    x[6] = torch.nan
+    x[7, 1:] = 0
+    for t in (x, x[:8]):
+        got = ops.quantize_rows(t)
+        q, s = _codes(t.float())
+        assert _same(got.scales.cpu(), s) and torch.equal(got.codes.cpu(), q)
+        assert torch.isnan(got.scales[[1, 2, 3, 6]]).all() and torch.isfinite(got.scales[[0, 4, 5, 7]]).all()
+        pw = _weight(40, K)
+        y = ops.linear(t, pw)
+        assert torch.isnan(y[[1, 2, 3, 6]]).all() and bool((y[0] == 0).all()) and torch.isfinite(y[[0, 5, 7]]).all() and torch.isfinite(y[8:]).all()
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_strides_and_leading_dims_of_rows(dtype):
+    raw = torch.randn(3, 40, 600, device=DEV).to(dtype)
+    for x in (raw[:, :, 1:257], raw[:, ::3, 8:520], raw[1, :, 3:300], raw.transpose(1, 2)[:, :, :40], raw[:1].expand(2, 40, 600), raw[0, 0, :77], raw[:, 0],
+              raw[:, :0], torch.randn(1, 600, device=DEV).expand(5, 600).to(dtype)):
+        got = ops.quantize_rows(x)
+        q, s = _codes(x.float().reshape(-1, x.shape[-1]))
+        assert got.codes.shape == x.shape and got.scales.shape == x.shape[:-1]
+        assert torch.equal(got.codes.reshape(-1, x.shape[-1]).cpu(), q) and torch.equal(got.scales.reshape(-1).cpu(), s)
+        assert got.dequantize().shape == x.shape
+
+
+# -------------------------------------------------------------------------------------------------------------- products
+
+ROWS = (1, 2, 15, 16, 17, 33, 64, 65, 129, 257, 700)
+
+
+@gpu
+@pytest.mark.parametrize("rows", ROWS)
+@pytest.mark.parametrize("N,K", [(1, 1), (7, 100), (300, 784), (128, 128), (129, 130), (1003, 4100), (4096, 512)])
+def test_linear_against_64_bits(rows, N, K):
+    gen = torch.Generator(DEV).manual_seed(rows + N + K)
+    pw = _weight(N, K)
+    x = torch.randn(rows, K, device=DEV, generator=gen)
+    x *= torch.rand(rows, 1, device=DEV, generator=gen) * 3
+    for i, dtype in enumerate(DTYPES):
+        bias = torch.randn(N, device=DEV, generator=gen) if (rows + i) % 2 else None
+        xs = x.to(dtype)
+        rows8 = ops.quantize_rows(xs)
+        y = ops.linear(xs, pw, bias)
+        _near(y, *_product(rows8.codes, rows8.scales, pw, bias, dtype))
+        assert y.dtype == dtype and torch.equal(ops.linear(rows8, pw, bias), y)
+        other = DTYPES[i - 1]
+        _near(ops.linear(xs, pw, bias, out_dtype=other), *_product(rows8.codes, rows8.scales, pw, bias, other))
+
+
+@gpu
+@pytest.mark.parametrize("rows,N,K", [(1, 11008, 4096), (3, 32003, 2048), (48, 8192, 8192), (1, 256, 131071), (300, 130, 131040), (2048, 4096, 1024),
+                                      (4097, 1000, 784), (1111, 2304, 3333), (9000, 640, 384), (3000, 9001, 640)])
+def test_linear_of_larger_sizes(rows, N, K):
+    pw = _weight(N, K)
+    x = torch.randn(rows, K, device=DEV, generator=torch.Generator(DEV).manual_seed(N)).bfloat16()
+    rows8 = ops.quantize_rows(x)
+    y = ops.linear(x, pw)
+    _near(y, *_product(rows8.codes, rows8.scales, pw, None, torch.bfloat16))
+    some = torch.tensor([0, rows - 1, rows // 2, rows // 3], device=DEV)         # a row's result does not depend on the rows beside it
+    assert torch.equal(ops.linear(x[some], pw), y[some])
+    assert ops.check_status() == 0
+
+
+@gpu
+def test_largest_sums_do_not_overflow():
+    """Codes of -128 (which no row of quantize_rows has) at the longest row: 2^31 - 2^14, still exact."""
+    K = _lib.JQ_INT8_MAX_K
+    q = torch.full((3, (K + 31) // 32 * 32), -128, dtype=torch.int8, device=DEV)
+    pw = jq.PackedWeight(jq.QuantSpec("int8", 0, 0), 3, K, q, torch.ones(3, device=DEV), None)
+    y = ops.linear(ops.QuantizedRows(q[:, :K], torch.ones(3, device=DEV), torch.float32), pw)
+    assert bool((y == float(16384 * K)).all())                     # 2^31 - 2^14: a number of fp32
+
+
+@gpu
+@pytest.mark.parametrize("rows", [1, 40, 400])
+def test_extreme_scales(rows):
+    """Neither product of the scales leaves fp32's range before the result does."""
+    x = torch.randn(rows, 256, device=DEV)
+    x[0] *= 1e36
+    w = torch.randn(64, 256, device=DEV)
+    w[:32] *= 1e-25
+    w[32:] *= 1e-36
+    pw = jq.pack_weight(w, jq.QuantSpec("int8", 0, 0))
+    rows8 = ops.quantize_rows(x)
+    y, bound = _product(rows8.codes, rows8.scales, pw, None, torch.float32)
+    _near(ops.linear(x, pw), y, bound + 2.0 ** -149 * 2)           # (a subnormal product and result are off by half of 2^-149 each)
+
+
+@gpu
+@pytest.mark.parametrize("rows", [1, 20, 300])
+def test_rotated_linear_undoes_the_weights_rotation(rows):
+    """W x = (W H)(H x): against the unquantised product, off by the rounding of both operands: half a step of 1/127 of a row's largest
+    value (about 4 times the typical one) each, independent over K: (4 / 127 / sqrt(12)) sqrt(2) = 0.013 of the result's size."""
+    K, N = 512, 96
+    w = torch.randn(N, K, device=DEV, generator=torch.Generator(DEV).manual_seed(1))
+    x = torch.randn(rows, K, device=DEV, generator=torch.Generator(DEV).manual_seed(2))
+    pw = jq.pack_weight(w, jq.QuantSpec("int8", 0, 128))
+    y = ops.linear(x, pw)
+    want = x.double() @ w.double().T
+    assert ((y - want).norm() / want.norm()).item() < 0.02
+    rows8 = ops.quantize_rows(x, 128)
+    _near(y, *_product(rows8.codes, rows8.scales, pw, None, torch.float32))
+
+
+@gpu
+def test_rows_of_codes_that_lie_otherwise():
+    pw = _weight(70, 200)
+    x = torch.randn(4, 6, 200, device=DEV)
+    rows8 = ops.quantize_rows(x)
+    want = ops.linear(x, pw)
+    assert want.shape == (4, 6, 70) and torch.equal(ops.linear(rows8, pw), want)
+    tight = rows8.codes.contiguous()                               # rows 200 bytes apart: not a multiple of 16
+    assert torch.equal(ops.linear(ops.QuantizedRows(tight, rows8.scales, torch.float32), pw), want)
+    turned = rows8.codes.transpose(0, 1), rows8.scales.transpose(0, 1)
+    assert torch.equal(ops.linear(ops.QuantizedRows(*turned, torch.float32), pw), want.transpose(0, 1))
+    shifted = torch.empty(24 * 224 + 1, dtype=torch.int8, device=DEV)[1:].view(24, 224)[:, :200]
+    shifted.copy_(rows8.codes.reshape(24, 200))
+    assert torch.equal(ops.linear(ops.QuantizedRows(shifted, rows8.scales.reshape(24), torch.float32), pw), want.reshape(24, 70))
+    one = ops.QuantizedRows(rows8.codes[:1, :1].expand(3, 1, 200), rows8.scales[:1, :1].expand(3, 1), torch.float32)
+    assert torch.equal(ops.linear(one, pw), want[:1, :1].expand(3, 1, 70))
+    assert torch.equal(one.dequantize(), rows8.dequantize()[:1, :1].expand(3, 1, 200))
+    assert ops.linear(ops.quantize_rows(x[:0]), pw).shape == (0, 6, 70) and ops.linear(x[:0], pw).shape == (0, 6, 70)
+    assert ops.linear(x[0, 0], pw).shape == (70,) and torch.equal(ops.linear(rows8, pw, out_dtype=torch.bfloat16), want.bfloat16())
+
+
+@gpu
+@pytest.mark.parametrize("rows", [1, 40, 500])
+def test_streams_graphs_and_calls_behind_one_another(rows):
+    pw, small = _weight(512, 640), _weight(64, 512, 3)
+    x = torch.randn(rows, 640, device=DEV).bfloat16()
+    want = ops.linear(ops.linear(x, pw), small)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        assert torch.equal(ops.linear(ops.linear(x, pw), small), want)
+        rows8 = ops.quantize_rows(x)
+        ops.linear(rows8, pw)
+    torch.cuda.current_stream().wait_stream(side)
+    held, graphs = x.clone(), []
+    for _ in range(2):                                             # two graphs captured one after the other, replayed on two streams
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            y = ops.linear(ops.linear(held, pw), small)
+            z = ops.linear(ops.quantize_rows(held), pw)
+        graphs.append((graph, y, z))
+    other = torch.randn(rows, 640, device=DEV).bfloat16()
+    held.copy_(other)
+    want, first = ops.linear(ops.linear(other, pw), small), ops.linear(other, pw)
+    side.wait_stream(torch.cuda.current_stream())
+    for _ in range(3):
+        graphs[0][0].replay()
+        with torch.cuda.stream(side):
+            graphs[1][0].replay()
+    torch.cuda.synchronize()
+    for _, y, z in graphs:
+        assert torch.equal(y, want) and torch.equal(z, first)
+    assert ops.check_status() == 0
+
+
+@gpu
+def test_memory_behind_and_beside_the_output_is_left_alone():
+    lib = _lib.load()
+    for rows, N in ((1, 7), (17, 130), (300, 257)):
+        pw = _weight(N, 100)
+        rows8 = ops.quantize_rows(torch.randn(rows, 100, device=DEV))
+        y = torch.full((rows * N + 64,), 7.0, device=DEV)
+        status = torch.zeros(1, dtype=torch.int32, device=DEV)
+        assert lib.jq_int8_matmul(pw.qweight.data_ptr(), pw.scales.data_ptr(), rows8.codes.data_ptr(), rows8.codes.stride(0), rows8.scales.data_ptr(), None,
+                                  y[32:].data_ptr(), N, 100, rows, 0, status.data_ptr(), None) == 0
+        assert bool((y[:32] == 7).all()) and bool((y[32 + rows * N:] == 7).all()) and status.item() == 0
+        assert torch.equal(y[32:32 + rows * N].view(rows, N), ops.linear(rows8, pw))
+
+
+# ---------------------------------------------------------------------------------------------------- layers and packing
+
+def test_packing_on_the_cpu():
+    w = torch.randn(5, 50)
+    w[0] = 0
+    w[1, ::2] = 0
+    w[2, 3] = torch.nan
+    pw = jq.pack_weight(w, jq.QuantSpec("int8", 0))
+    q, s = _codes(w)
+    assert pw.qweight.dtype == torch.int8 and pw.qweight.shape == (5, 64) and pw.codebook is None
+    assert torch.equal(pw.qweight[:, :50], q) and _same(pw.scales, s) and bool((pw.qweight[:, 50:] == 0).all())
+    assert bool((pw.qweight[1, :50:2] == 0).all()) and pw.nbytes() == 5 * 64 + 20
+    part = pw.rows(1, 3)
+    assert torch.equal(part.qweight, pw.qweight[1:3]) and part.N == 2
+    assert jq.algorithmic_bytes(jq.QuantSpec("int8", 0), 10, 100, 2, 2, 2) == 1000 + 40 + 400 + 40
+
+
+def test_refusals_of_specs_and_layers():
+    with pytest.raises(ValueError, match="group_size"):
+        jq.QuantSpec("int8", 32)
+    with pytest.raises(ValueError, match="bitwidth"):
+        jq.JenksQuantLinear(nn.Linear(64, 8), 4, fmt="int8")
+    with pytest.raises(ValueError, match="bitwidth"):
+        jq.JenksQuantLinear(nn.Linear(64, 8), 8)
+    with pytest.raises(ValueError, match="bitwidth"):
+        jq.JenksQuantConv2d(nn.Conv2d(3, 8, 3), 4, fmt="int8")
+    with pytest.raises(ValueError, match="rotation block"):
+        jq.pack_weight(torch.randn(4, 100), jq.QuantSpec("int8", 0, 128))
+    with pytest.raises(ValueError, match="1 to 131071"):
+        jq.pack_weight(torch.empty(1, 131072), jq.QuantSpec("int8", 0))
+    pw = jq.pack_weight(torch.randn(4, 100), jq.QuantSpec("int8", 0))
+    with pytest.raises(ValueError, match="4-bit"):
+        ops.GroupedGemv([pw], 1)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        ops.linear(torch.randn(2, 100), pw)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        ops.quantize_rows(torch.randn(2, 100))
+    with pytest.raises(RuntimeError, match="128"):
+        ops.quantize_rows(torch.randn(2, 100), 128)
+    with pytest.raises(RuntimeError, match="rows of 1"):
+        ops.quantize_rows(torch.randn(2, 0))
+    with pytest.raises(RuntimeError, match="dtype"):
+        ops.quantize_rows(torch.randn(2, 8).double())
+    with pytest.raises(RuntimeError, match="unfold|laid out"):
+        ops.conv2d(torch.randn(1, 4, 9, 9), jq.pack_weight(torch.randn(4, 36), jq.QuantSpec("int8", 0)), None, (3, 3), (1, 1), (0, 0), (1, 1))
+
+
+def test_refusals_of_the_library():
+    """Bad arguments are turned away before anything is launched; no GPU is needed."""
+    lib, p = _lib.load(), torch.zeros(4096, dtype=torch.uint8).data_ptr()
+    assert lib.jq_quantize_rows(None, 8, 1, 8, 0, 0, p, 32, p, None) == -1
+    for rows, K, had, stride in ((0, 8, 0, 32), (1, 0, 0, 32), (1, 131072, 0, 131072), (1, 100, 128, 128), (1, 128, 64, 128), (1, 40, 0, 32)):
+        assert lib.jq_quantize_rows(p, K, rows, K, had, 0, p, stride, p, None) == -2
+    assert lib.jq_quantize_rows(p, 8, 1, 8, 0, 3, p, 32, p, None) == -4
+    assert lib.jq_quantize_rows(p, 8, 1, 8, 0, 0, p + 8, 32, p, None) == -3 and lib.jq_quantize_rows(p, 8, 1, 8, 0, 0, p, 24, p, None) == -3
+    assert lib.jq_dequantize_rows(p, 24, p, 1, 8, p, 0, None) == -3 and lib.jq_dequantize_rows(p, 32, p, 1, 8, p, 5, None) == -4
+    assert lib.jq_int8_scratch_bytes(3, 100) == 256 + 3 * 128 and lib.jq_int8_scratch_bytes(0, 4) == 0
+    assert lib.jq_int8_linear(p, p, p, None, p, 4, 8, 1, 0, 0, 0, p, 8, p, None) == -6
+    assert lib.jq_int8_linear(p, p, None, None, p, 4, 8, 1, 0, 0, 0, p, 4096, p, None) == -1
+    assert lib.jq_int8_linear(p, p, p, None, p, 4, 131072, 1, 0, 0, 0, p, 4096, p, None) == -2
+    assert lib.jq_int8_linear(p + 8, p, p, None, p, 4, 8, 1, 0, 0, 0, p, 4096, p, None) == -3
+    assert lib.jq_int8_matmul(p, p, p, 24, p, None, p, 4, 8, 1, 0, p, None) == -3
+    assert lib.jq_int8_matmul(p, p, p, 32, p, None, p + 1, 4, 8, 1, 1, p, None) == -3
+    assert lib.jq_int8_matmul(p, p, p, 32, p, None, p, 4, 8, 1, 9, p, None) == -4
+    assert lib.jq_int8_matmul(p, p, p, 0, p, None, p, 4, 8, 1, 0, p, None) == -2
+    assert lib.jq_int8_matmul(p, p, p, 32, p, None, p, 4, 8, 1, 0, None, None) == -1
+
+
+@gpu
+def test_refusals_of_rows_and_weights():
+    pw, rot = _weight(8, 128), _weight(8, 128, had=128)
+    x = torch.randn(2, 128, device=DEV)
+    rows8 = ops.quantize_rows(x)
+    four = jq.pack_weight(torch.randn(8, 128), jq.QuantSpec("gf4", 128)).to(DEV)
+    for call, text in ((lambda: ops.linear(rows8, rot), "had_block"), (lambda: ops.linear(ops.quantize_rows(x, 128), pw), "had_block"),
+                       (lambda: ops.linear(rows8, four), "gf4"), (lambda: ops.linear(rows8, _weight(8, 64)), "K=64"),
+                       (lambda: ops.linear(rows8, pw, out_dtype=torch.float64), "dtype"),
+                       (lambda: ops.linear(x, pw, torch.zeros(9, device=DEV)), "bias"), (lambda: ops.linear(x, pw, torch.zeros(8)), "CUDA"),
+                       (lambda: ops.linear(rows8._replace(scales=rows8.scales[:1]), pw), "scales"),
+                       (lambda: ops.linear(rows8._replace(codes=rows8.codes.float()), pw), "int8"),
+                       (lambda: ops.linear(x, jq.PackedWeight(pw.spec, 8, 128, pw.qweight.float(), pw.scales, None)), "int8 weight"),
+                       (lambda: ops.linear(x, jq.PackedWeight(pw.spec, 8, 100, pw.qweight, pw.scales, None)), "K=100"),
+                       (lambda: ops.linear(x, jq.PackedWeight(pw.spec, 8, 128, pw.qweight, pw.scales.half(), None)), "fp32 scales"),
+                       (lambda: rows8.dequantize(torch.float64), "dtype"), (lambda: ops.linear(x.double(), pw), "dtype")):
+        with pytest.raises(RuntimeError, match=text):
+            call()
+
+
+@gpu
+@pytest.mark.parametrize("had", [0, 128])
+def test_packing_on_the_gpu_is_that_on_the_cpu(had):
+    w = torch.randn(37, 1152) * 0.1
+    a, b = jq.pack_weight(w, jq.QuantSpec("int8", 0, had)), jq.pack_weight(w.to(DEV), jq.QuantSpec("int8", 0, had))
+    assert torch.equal(a.qweight, b.qweight.cpu()) and torch.equal(a.scales, b.scales.cpu())
+    dense = ops.dequantize(b)
+    assert torch.equal(dense.cpu(), a.qweight[:, :1152].float() * a.scales[:, None])
+
+
+@gpu
+def test_layers_checkpoints_and_copies():
+    model = nn.Sequential(nn.Flatten(), nn.Linear(784, 300), nn.ReLU(), nn.Linear(300, 100), nn.ReLU(), nn.Linear(100, 10))
+    q = jq.quantize_module(model, 8, fmt="int8").to(DEV)
+    x = torch.randn(33, 1, 28, 28, device=DEV)
+
+    def plain(h, layers):
+        for m in layers:
+            if isinstance(m, jq.JenksQuantLinear):
+                q8, s = _codes(h)
+                h = (q8.to(DEV).float() * s.to(DEV)[:, None]).double() @ m.weight.double().T + m.bias.double()
+                h = h.float()
+            else:
+                h = m(h)
+        return h
+
+    y = q(x)
+    # fp32 between the layers: a hidden value off by 2^-22 may cross the border of two codes, a step of 1/127 of the largest in one of 100
+    assert ((y - plain(x, q)).abs().max() / y.abs().max()).item() < 0.02
+    for m in q:
+        if isinstance(m, jq.JenksQuantLinear):
+            m.commit()
+    assert torch.equal(q(x), y) and torch.equal(copy.deepcopy(q)(x), y)
+    state = checkpoint.pack_state_dict(model.state_dict(), jq.QuantSpec("int8", 0))
+    buf = io.BytesIO()
+    torch.save(state, buf)
+    buf.seek(0)
+    loaded = checkpoint.load_packed_into(copy.deepcopy(model), torch.load(buf)).to(DEV)
+    assert torch.equal(loaded(x), y) and loaded[1].spec == jq.QuantSpec("int8", 0, 0)
+    with warnings.catch_warnings(record=True) as told:
+        warnings.simplefilter("always")
+        state = checkpoint.pack_state_dict(model.state_dict(), jq.QuantSpec("int8", 0, 128))
+    assert len(told) == 3 and checkpoint.packed_weight_from(state, "1").spec == jq.QuantSpec("int8", 0, 0)
+
+
+@gpu
+def test_convolution_and_traced_call():
+    conv = nn.Conv2d(6, 20, 3, stride=2, padding=1)
+    q = jq.JenksQuantConv2d(conv, 8, fmt="int8").to(DEV)
+    x = torch.randn(5, 6, 21, 17, device=DEV)
+    y = q(x)
+    fields = F.unfold(x, 3, 1, 1, 2).transpose(1, 2)
+    q8, s = _codes(fields.reshape(-1, 54))
+    want, bound = _product(q8.to(DEV), s.to(DEV), q.packed, q.bias, torch.float32)
+    _near(y.flatten(2).transpose(1, 2).reshape(-1, 20), want, bound)
+    pw = _weight(48, 256)
+    z = torch.randn(7, 256, device=DEV)
+    assert torch.equal(torch.ops.jq.linear(z, pw.qweight, pw.scales, None, None, pw.spec.fmt_id, 48, 256, 0, 0, -1), ops.linear(z, pw))
