@@ -17,7 +17,7 @@ LIB = os.path.join(HERE, "libjq.so")
 
 CUDA_SOURCES = ["api.cu", "dequant.cu", "gemv.cu", "gemm_ta.cu", "gemm_rows.cu", "jenks2.cu", "pack_gpu.cu", "pack_gf4_gpu.cu",
                 "kv_cache.cu", "kv_attend.cu", "kv_prompt.cu", "logprobs.cu",
-                "rows8.cu", "gemm_int8.cu"]
+                "rows8.cu", "norms.cu", "gemm_int8.cu"]
 HOST_SOURCES = ["pack_host.cpp"]
 
 NVCC_FLAGS = [

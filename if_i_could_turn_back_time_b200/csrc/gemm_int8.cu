@@ -17,6 +17,7 @@ struct GemmArgs {
     void *y;
     int *status;
     int N, T, steps, split, y_dtype, vec, early;
+    int tiles_t, tiles_n, band;        // of a pair of CTAs
 };
 
 // K-major operand tile in shared memory, 128-byte swizzle: atoms of 8 rows x 128 bytes, 1024 bytes apart
@@ -54,7 +55,7 @@ __device__ __forceinline__ void store4(T *y, const float (&v)[4], int n, bool ve
 
 template <int NT> struct Few {
     static constexpr int kStage = (kTileN + NT) * kStep;
-    static constexpr int kStages = NT == 256 ? 4 : (NT == 128 ? 3 : (NT == 64 ? 4 : (NT == 32 ? 5 : 6)));
+    static constexpr int kStages = NT == 128 ? 3 : (NT == 64 ? 4 : (NT == 32 ? 5 : 6));
     static constexpr int kRing = kStage * kStages;
     static constexpr int kSmem = kRing + 1024 + 256;
     static constexpr int kCols = NT < 32 ? 32 : NT;
@@ -201,6 +202,335 @@ __global__ void __launch_bounds__(kThreads) gemm_int8_kernel(const __grid_consta
     }
 }
 
+// ---- many tokens: a pair of CTAs per tile ------------------------------------------------
+
+constexpr int kPairThreads = 320;      // 8 warps of outputs, a loader, an issuer
+constexpr int kPitch = 80;             // bytes between a warp's rows of outputs in shared memory (64 of them, spread over the banks)
+
+template <int BN> struct Pair {
+    static constexpr int kStage = (128 + BN / 2) * kStep;          // of each CTA: 128 tokens, half of the channels
+    static constexpr int kStages = BN == 256 ? 6 : 8;
+    static constexpr int kRing = kStage * kStages;
+    static constexpr int kOut = 8 * (32 * kPitch + BN * 4);        // a warp's outputs, and its BN / 2 columns' scales and biases
+    static_assert(kRing >= BN * 128 * 4, "a tile's sums pass through the ring where CTAs share its K range");
+    static constexpr int kSmem = kRing + kOut + 1024 + 256;
+};
+
+__device__ __forceinline__ uint32_t cta_rank() {
+    uint32_t r;
+    asm volatile("mov.u32 %0, %cluster_ctarank;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ uint32_t at_rank(uint32_t addr, uint32_t rank) {
+    uint32_t r;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+    return r;
+}
+// A box into this CTA's shared memory, counted on a barrier of either CTA of the pair
+__device__ __forceinline__ void tma_2d_pair(uint32_t dst, const void *tmap, int x, int y, uint32_t cluster_bar) {
+    asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%2, %3}], [%4];"
+                 ::"r"(dst), "l"(tmap), "r"(x), "r"(y), "r"(cluster_bar) : "memory");
+}
+__device__ __forceinline__ void mma_i8_pair(uint32_t elected, uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile("{ .reg .pred p, q; setp.ne.b32 p, %4, 0; setp.ne.b32 q, %5, 0;\n"
+                 "  @q tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p; }"
+                 ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(elected) : "memory");
+}
+// What has been issued so far is done: told to the barrier at this place of both CTAs
+__device__ __forceinline__ void commit_pair(uint32_t elected, uint32_t bar, uint32_t both) {
+    asm volatile("{ .reg .pred q; setp.ne.b32 q, %1, 0;\n"
+                 "  @q tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %2; }"
+                 ::"r"(bar), "r"(elected), "h"((uint16_t)both) : "memory");
+}
+__device__ __forceinline__ void arrive_cluster(uint32_t cluster_bar) {
+    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_bar) : "memory");
+}
+__device__ __forceinline__ float lds_f32(uint32_t a) { return __uint_as_float(lds32(a)); }
+
+template <class T> __device__ __forceinline__ uint32_t pack2(float a, float b);
+template <> __device__ __forceinline__ uint32_t pack2<__half>(float a, float b) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t *>(&h);
+}
+template <> __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float a, float b) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t *>(&h);
+}
+
+// 32 columns of a warp's 32 tokens (a token per lane): scaled, turned in shared memory 64 bytes of a row at a time, and written as rows
+template <class T>
+__device__ __forceinline__ void write32(const GemmArgs &p, const uint32_t (&r)[32], uint32_t out, uint32_t scales, uint32_t biases, float ts, int t0, int n0, int lane) {
+    constexpr int kCols = 64 / (int)sizeof(T);
+    T *const y = reinterpret_cast<T *>(p.y);
+#pragma unroll
+    for (int half = 0; half < 32 / kCols; ++half) {
+        float v[kCols];
+#pragma unroll
+        for (int c = 0; c < kCols; c += 4) {
+            const uint4 cs = lds128(scales + (half * kCols + c) * 4);
+            const uint32_t *s = &cs.x;
+            uint4 b4 = make_uint4(0, 0, 0, 0);
+            if (p.bias) b4 = lds128(biases + (half * kCols + c) * 4);
+            const uint32_t *b = &b4.x;
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+                v[c + k] = fmaf(__int2float_rn((int)r[half * kCols + c + k]) * __uint_as_float(s[k]), ts, __uint_as_float(b[k]));
+        }
+        __syncwarp();
+        const uint32_t row = out + lane * kPitch;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            uint32_t w[4];
+            if constexpr (sizeof(T) == 4) {
+#pragma unroll
+                for (int k = 0; k < 4; ++k) w[k] = __float_as_uint(v[4 * q + k]);
+            } else {
+#pragma unroll
+                for (int k = 0; k < 4; ++k) w[k] = pack2<T>(v[8 * q + 2 * k], v[8 * q + 2 * k + 1]);
+            }
+            asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(row + 16 * q), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
+        }
+        __syncwarp();
+        const int n = n0 + half * kCols;
+        if (p.vec) {                                   // rows of y are 16-byte aligned: four lanes write a row's 64 bytes
+            const int cn = n + (lane & 3) * (kCols / 4);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int t = i * 8 + (lane >> 2);
+                const uint4 u = lds128(out + t * kPitch + (lane & 3) * 16);
+                if (t0 + t < p.T && cn < p.N) *reinterpret_cast<uint4 *>(y + (size_t)(t0 + t) * p.N + cn) = u;
+            }
+        } else {
+            const int cn = n + lane % kCols;
+#pragma unroll 4
+            for (int i = 0; i < 32; i += 32 / kCols) {
+                const int t = i + lane / kCols;
+                T e;
+                if constexpr (sizeof(T) == 4) {
+                    e = lds_f32(out + t * kPitch + (lane % kCols) * 4);
+                } else {
+                    unsigned short u;
+                    asm volatile("ld.shared.u16 %0, [%1];" : "=h"(u) : "r"(out + t * kPitch + (lane % kCols) * 2));
+                    e = *reinterpret_cast<const T *>(&u);
+                }
+                if (t0 + t < p.T && cn < p.N) y[(size_t)(t0 + t) * p.N + cn] = e;
+            }
+        }
+    }
+}
+
+__device__ __forceinline__ uint32_t ld_cluster_u32(uint32_t cluster_addr) {
+    uint32_t v;
+    asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(cluster_addr) : "memory");
+    return v;
+}
+
+// Tiles of 256 tokens x BN channels on a pair of CTAs (cta_group::2): each holds the sums of its 128 tokens, and both read one another's
+// half of the weights, so that an SM's shared memory takes in half of the operand bytes per product.  Persistent; the sums of a tile are
+// scaled and written while the next one is multiplied.  Where there are few tiles, the pairs of a cluster share a tile's K range
+// instead (split > 1): their sums meet in distributed shared memory, a part of the columns in each.
+template <int BN>
+__global__ void __launch_bounds__(kPairThreads, 1)
+    gemm_int8_pair_kernel(const __grid_constant__ GemmArgs p, const __grid_constant__ CUtensorMap wmap, const __grid_constant__ CUtensorMap xmap) {
+    using C = Pair<BN>;
+    extern __shared__ __align__(1024) unsigned char smem_raw[];
+    __shared__ uint32_t s_tmem;
+    __shared__ int s_err;
+    const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
+    const uint32_t rank = cta_rank() & 1, leader = cta_rank() & ~1u;
+    const uint32_t ring = (smem_u32(smem_raw) + 1023u) & ~1023u, outs = ring + C::kRing, bars = outs + C::kOut;
+    auto full = [&](int s) { return bars + 8u * s; };                                  // (the leader's: both CTAs' boxes)
+    auto free_ = [&](int s) { return bars + 8u * (C::kStages + s); };
+    auto ready = [&](int a) { return bars + 8u * (2 * C::kStages + a); };              // sums complete
+    auto taken = [&](int a) { return bars + 8u * (2 * C::kStages + 2 + a); };          // (the leader's) read by both CTAs' warps
+    volatile int *err = &s_err;
+    if (tid == 0) {
+        s_err = 0;
+        for (int s = 0; s < C::kStages; ++s) { mbar_init(full(s), 1); mbar_init(free_(s), 1); }
+        for (int a = 0; a < 2; ++a) { mbar_init(ready(a), 1); mbar_init(taken(a), 16); }
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 9) {
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&s_tmem)), "r"(2 * BN) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    }
+    tc_fence_before();
+    cluster_sync();
+    tc_fence_after();
+    const uint32_t tmem = __shfl_sync(0xffffffffu, s_tmem, 0);
+    pdl_launch_dependents();
+
+    const int width = 2 * p.split, clusters = gridDim.x / width, first = blockIdx.x / width;     // (split > 1: a tile per cluster)
+    const int tiles = p.tiles_t * p.tiles_n;
+    const int part = (int)(leader >> 1);                   // of the K range
+    const int k_lo = p.steps * part / p.split, steps = p.steps * (part + 1) / p.split - k_lo;
+    // tiles in groups of `band` rows of tokens, which stay in the L2 while the weights pass by
+    auto place = [&](int tile, int &t0, int &n0) {
+        const int per = p.band * p.tiles_n, g = tile / per, in = tile - g * per;
+        const int rows = min(p.band, p.tiles_t - g * p.band);
+        t0 = (g * p.band + in % rows) * 256 + (int)rank * 128;
+        n0 = in / rows * BN;
+    };
+    const int quarter = warp & 3, side = warp >> 2;        // of an output warp: lanes of tensor memory, half of the columns
+    const uint32_t out = outs + warp * (32 * kPitch + BN * 4), scales = out + 32 * kPitch, biases = scales + BN * 2;
+    // scales and biases of `cols` columns from n on into the warp's shared memory; the scale of its lane's token
+    auto take_params = [&](int n, int cols) {
+        __syncwarp();
+        for (int c = lane; c < cols; c += 32) {
+            const float cs = n + c < p.N ? p.cs[n + c] : 0.f, b = n + c < p.N && p.bias ? p.bias[n + c] : 0.f;
+            asm volatile("st.shared.f32 [%0], %1;" ::"r"(scales + c * 4), "f"(cs) : "memory");
+            asm volatile("st.shared.f32 [%0], %1;" ::"r"(biases + c * 4), "f"(b) : "memory");
+        }
+        __syncwarp();
+    };
+    auto write = [&](const uint32_t (&r)[32], int c, float ts, int t0, int n0) {      // c: among the warp's columns
+        if (p.y_dtype == JQ_F32) write32<float>(p, r, out, scales + c * 4, biases + c * 4, ts, t0, n0 + c, lane);
+        else if (p.y_dtype == JQ_F16) write32<__half>(p, r, out, scales + c * 4, biases + c * 4, ts, t0, n0 + c, lane);
+        else write32<__nv_bfloat16>(p, r, out, scales + c * 4, biases + c * 4, ts, t0, n0 + c, lane);
+    };
+
+    if (warp == 8) {
+        if (lane == 0) {
+            const uint32_t stage_bytes = 2 * C::kStage;
+            int s = 0, ahead = 0;
+            uint32_t par = 1;                              // (the first round finds every stage free)
+            bool ok = true;
+            auto load_w = [&](int n0, int i, int s_) {
+                if (rank == 0) mbar_expect_tx(full(s_), stage_bytes);
+                tma_2d_pair(ring + s_ * C::kStage + 128 * kStep, &wmap, (k_lo + i) * kStep, n0 + (int)rank * (BN / 2), at_rank(full(s_), leader));
+            };
+            // Weights that no kernel of this call writes are asked for while the activation is still being quantised
+            if (p.early && first < tiles) {
+                int t0, n0;
+                place(first, t0, n0);
+                ahead = min(C::kStages, steps);
+                for (int i = 0; i < ahead; ++i) load_w(n0, i, i);
+            }
+            pdl_wait();
+            for (int tile = first; tile < tiles && ok; tile += clusters) {
+                int t0, n0;
+                place(tile, t0, n0);
+                for (int i = 0; i < steps; ++i) {
+                    if (ahead > 0) --ahead;
+                    else {
+                        if (!(ok = mbar_wait(free_(s), par, err))) break;
+                        load_w(n0, i, s);
+                    }
+                    tma_2d_pair(ring + s * C::kStage, &xmap, (k_lo + i) * kStep, t0, at_rank(full(s), leader));
+                    if (++s == C::kStages) { s = 0; par ^= 1; }
+                }
+            }
+        }
+        __syncwarp();
+    } else if (warp == 9) {
+        if (rank == 0) {
+            const uint32_t elected = elect_one();
+            constexpr uint32_t idesc = idesc_i8(256, BN);
+            const uint32_t both = 3u << leader;
+            auto wait = [&](uint32_t bar, uint32_t parity) -> bool { return __all_sync(0xffffffffu, mbar_wait(bar, parity, err)); };
+            int s = 0, a = 0;
+            uint32_t par = 0, a_par = 1;                   // (the first wait on free sums passes at once)
+            bool ok = true;
+            for (int tile = first; tile < tiles && ok; tile += clusters) {
+                if (!(ok = wait(taken(a), a_par))) break;
+                tc_fence_after();
+                const uint32_t d = tmem + a * BN;
+                for (int i = 0; i < steps; ++i) {
+                    if (!(ok = wait(full(s), par))) break;
+                    tc_fence_after();
+                    const uint64_t da = desc_sw128(ring + s * C::kStage), db = desc_sw128(ring + s * C::kStage + 128 * kStep);
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) mma_i8_pair(elected, d, da + 2 * k, db + 2 * k, idesc, i > 0 || k > 0);
+                    commit_pair(elected, free_(s), both);
+                    if (++s == C::kStages) { s = 0; par ^= 1; }
+                }
+                if (!ok) break;
+                commit_pair(elected, ready(a), both);
+                if (++a == 2) { a = 0; a_par ^= 1; }
+            }
+        }
+    } else if (p.split == 1) {
+        pdl_wait();
+        int a = 0;
+        uint32_t par = 0;
+        for (int tile = first; tile < tiles; tile += clusters) {
+            int t0, n0;
+            place(tile, t0, n0);
+            t0 += quarter * 32;
+            n0 += side * (BN / 2);
+            const float ts = t0 + lane < p.T ? p.ts[t0 + lane] : 0.f;
+            take_params(n0, BN / 2);
+            if (!__all_sync(0xffffffffu, mbar_wait(ready(a), par, err))) break;
+            tc_fence_after();
+            const uint32_t from = tmem + ((uint32_t)(quarter * 32) << 16) + a * BN + side * (BN / 2);
+            uint32_t r[2][32];
+            tmem_ld32(from, r[0]);
+#pragma unroll
+            for (int j = 0; j < BN / 64; ++j) {
+                tmem_wait_ld();
+                if (j + 1 < BN / 64) tmem_ld32(from + (j + 1) * 32, r[(j + 1) & 1]);
+                else {                                     // all of this warp's sums are in registers
+                    tc_fence_before();
+                    if (lane == 0) arrive_cluster(at_rank(taken(a), leader));
+                }
+                write(r[j & 1], j * 32, ts, t0, n0);
+            }
+            if (++a == 2) { a = 0; par ^= 1; }
+        }
+    } else {
+        // sums -> shared memory, [column][token]: every stage has been read once the last instruction is done
+        if (__all_sync(0xffffffffu, mbar_wait(ready(0), 0, err))) {
+            tc_fence_after();
+            const uint32_t to = ring + (quarter * 32 + lane) * 4;
+#pragma unroll 1
+            for (int c = side * (BN / 2); c < (side + 1) * (BN / 2); c += 32) {
+                uint32_t r[32];
+                tmem_ld32(tmem + ((uint32_t)(quarter * 32) << 16) + c, r);
+                tmem_wait_ld();
+#pragma unroll
+                for (int k = 0; k < 32; ++k) asm volatile("st.shared.u32 [%0], %1;" ::"r"(to + (c + k) * 512), "r"(r[k]) : "memory");
+            }
+        }
+    }
+    __syncwarp();
+    if (p.split > 1) {
+        cluster_sync();
+        if (warp < 8 && !*err) {
+            pdl_wait();
+            const int cols = BN / p.split / 2, c_lo = part * (BN / p.split) + side * cols;      // of this warp
+            int t0, n0;
+            place(first, t0, n0);
+            t0 += quarter * 32;
+            n0 += c_lo;
+            const float ts = t0 + lane < p.T ? p.ts[t0 + lane] : 0.f;
+            take_params(n0, cols);
+            for (int c = 0; c < cols; c += 32) {
+                uint32_t r[32];
+#pragma unroll
+                for (int k = 0; k < 32; ++k) r[k] = 0;
+#pragma unroll 1
+                for (int o = 0; o < p.split; ++o) {
+                    const uint32_t from = at_rank(ring + (quarter * 32 + lane) * 4, 2 * (uint32_t)o + rank) + (uint32_t)(c_lo + c) * 512;
+#pragma unroll
+                    for (int k = 0; k < 32; ++k) r[k] += ld_cluster_u32(from + k * 512);
+                }
+                write(r, c, ts, t0, n0);
+            }
+        }
+        __syncwarp();
+    }
+    if (*err) {   // a wait gave up: let the copies and products still in flight end before the pair's shared memory goes away
+        for (int i = 0; i < 400; ++i) __nanosleep(256);
+        if (lane == 0) atomicExch(p.status, *err);
+    }
+    tc_fence_before();
+    cluster_sync();
+    if (warp == 9) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(2 * BN) : "memory");
+    }
+}
+
 // ---- host side -------------------------------------------------------------------------
 
 static int encode(CUtensorMap *map, const void *base, int rows, int K, int64_t stride, int box_rows) {
@@ -213,11 +543,35 @@ static int encode(CUtensorMap *map, const void *base, int rows, int K, int64_t s
                ? JQ_OK : JQ_ERR_CUDA_BASE - (int)cudaErrorInvalidValue;
 }
 
-// CTAs that share a tile's K range: as many as give every SM about two CTAs with at least two stages each
-static int split_of(long long tiles, int steps, int sms) {
-    int s = 1;
-    while (s < 8 && tiles * s * 2 <= 2 * sms && steps >= 4 * s) s *= 2;
-    return s;
+struct Form { bool pair; int tile, split; };   // tile: tokens of a single CTA's tile, channels of a pair's
+
+static Form choose_form(int N, int T, int steps, int sms) {
+    Form best{false, 16, 1};
+    double least = 0;
+    auto offer = [&](bool pair, int tile, int split, double us) {
+        if (least == 0 || us < least) { best = Form{pair, tile, split}; least = us; }
+    };
+    for (int nt = 16; nt <= 128; nt *= 2) {
+        if ((T <= nt / 2 && nt > 16) || (nt < 64 && T > nt)) continue;
+        const long long tiles = (long long)((N + kTileN - 1) / kTileN) * ((T + nt - 1) / nt);
+        for (int s = 1; s <= 8; s = s == 4 ? 8 : s + 1) {
+            const long long ctas = tiles * s, room = s == 8 ? sms / 18 * 32 : 2 * sms;
+            if (s > steps || (s > 1 && ctas > room)) break;
+            const double turns = (double)(ctas / room * 2 + (ctas % room + sms - 1) / sms);       // CTAs that an SM has, one behind another
+            offer(false, nt, s, 3.0 + 0.0234 * nt + turns * ((steps + s - 1) / s) * (0.144 + 0.0012 * nt) + (s > 1 ? 0.0123 * nt : 0.0));
+        }
+    }
+    if (T > 64)
+        for (int bn = 256; bn >= 128; bn /= 2) {
+            const long long tiles = (long long)((N + bn - 1) / bn) * ((T + 255) / 256);
+            for (int s = 1; s <= bn / 64; s *= 2) {
+                const long long room = s == 1 ? sms / 2 : sms / 18 * (s == 2 ? 4 : 2);
+                if (s > steps || (s > 1 && tiles > room)) break;
+                const double waves = (double)((tiles + room - 1) / room);
+                offer(true, bn, s, 2.7 + bn / 128 * (1.0 + 0.65 * waves + (s > 1 ? 1.1 : 0.0)) + waves * ((steps + s - 1) / s) * (bn == 256 ? 0.286 : 0.2));
+            }
+        }
+    return best;
 }
 
 template <int NT>
@@ -227,7 +581,6 @@ static int launch(GemmArgs &a, const void *w, int64_t w_stride, const void *x, i
     if (!rc) rc = encode(&xmap, x, a.T, K, x_stride, NT);
     if (rc) return rc;
     const int tiles = (a.N + kTileN - 1) / kTileN, across = (a.T + NT - 1) / NT;
-    a.split = split_of((long long)tiles * across, a.steps, jq_sm_count());
     static jq_contexts done;
     auto kern = gemm_int8_kernel<NT>;
     JQ_CUDA_TRY(jq_allow_smem(reinterpret_cast<const void *>(kern), Few<NT>::kSmem, done));
@@ -248,6 +601,38 @@ static int launch(GemmArgs &a, const void *w, int64_t w_stride, const void *x, i
     return jq_launch_status();
 }
 
+template <int BN>
+static int launch_pair(GemmArgs &a, const void *w, int64_t w_stride, const void *x, int64_t x_stride, int K, cudaStream_t st) {
+    CUtensorMap wmap, xmap;
+    int rc = encode(&wmap, w, a.N, K, w_stride, BN / 2);
+    if (!rc) rc = encode(&xmap, x, a.T, K, x_stride, 128);
+    if (rc) return rc;
+    a.tiles_t = (a.T + 255) / 256;
+    a.tiles_n = (a.N + BN - 1) / BN;
+    a.band = 16;
+    a.vec = a.N * (a.y_dtype == JQ_F32 ? 4 : 2) % 16 == 0 && jq_aligned16(a.y);
+    static jq_contexts done;
+    auto kern = gemm_int8_pair_kernel<BN>;
+    JQ_CUDA_TRY(jq_allow_smem(reinterpret_cast<const void *>(kern), Pair<BN>::kSmem, done));
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = 2 * (unsigned)a.split;
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+    const long long tiles = (long long)a.tiles_t * a.tiles_n;
+    const int pairs = jq_sm_count() / 2;
+    cfg.gridDim = dim3(2 * (unsigned)(a.split > 1 ? tiles * a.split : (tiles < pairs ? tiles : pairs)));
+    cfg.blockDim = dim3(kPairThreads);
+    cfg.dynamicSmemBytes = Pair<BN>::kSmem;
+    cfg.stream = st;
+    cfg.attrs = attr;
+    cfg.numAttrs = 2;
+    JQ_CUDA_TRY(cudaLaunchKernelEx(&cfg, kern, a, wmap, xmap));
+    return jq_launch_status();
+}
+
 // early: the kernel in front of this one on the stream is one of this call, so that the weights are settled
 static int multiply(const void *w, const float *cs, const void *x, int64_t x_stride, const float *ts, const float *bias, void *y, int N, int K,
                     int T, int y_dtype, int *status, bool early, cudaStream_t st) {
@@ -256,11 +641,13 @@ static int multiply(const void *w, const float *cs, const void *x, int64_t x_str
     a.y_dtype = y_dtype; a.early = early;
     a.vec = N % 4 == 0 && (reinterpret_cast<uintptr_t>(y) & (y_dtype == JQ_F32 ? 15u : 7u)) == 0;
     const int64_t ws = jq_row_stride_codes(K);
-    if (T <= 16) return launch<16>(a, w, ws, x, x_stride, K, st);
-    if (T <= 32) return launch<32>(a, w, ws, x, x_stride, K, st);
-    if (T <= 64) return launch<64>(a, w, ws, x, x_stride, K, st);
-    if (T <= 128) return launch<128>(a, w, ws, x, x_stride, K, st);
-    return launch<256>(a, w, ws, x, x_stride, K, st);
+    const Form f = choose_form(N, T, a.steps, jq_sm_count());
+    a.split = f.split;
+    if (f.pair) return f.tile == 256 ? launch_pair<256>(a, w, ws, x, x_stride, K, st) : launch_pair<128>(a, w, ws, x, x_stride, K, st);
+    if (f.tile == 16) return launch<16>(a, w, ws, x, x_stride, K, st);
+    if (f.tile == 32) return launch<32>(a, w, ws, x, x_stride, K, st);
+    if (f.tile == 64) return launch<64>(a, w, ws, x, x_stride, K, st);
+    return launch<128>(a, w, ws, x, x_stride, K, st);
 }
 
 static int check(const void *w, const float *cs, const void *y, const int *status, int N, int K, int B, int y_dtype) {

@@ -78,29 +78,28 @@ __device__ __forceinline__ void load_any(const void *row, int dtype, int c, cons
     else widen(load_chunk(reinterpret_cast<const float *>(row), c, at, vec), v);
 }
 
-// Rotation of 128 neighbours: 16 lanes with eight of them each, in the order of stages (strides 1, 2, .., 64; sums in the lower place,
-// differences in the upper) of fwht128_warp, so that both give the same bits.
-__device__ __forceinline__ void rotate128(float (&v)[8], int lane) {
+// Rotation of 128 neighbours: 16 / A lanes with 8 A of them each, in the order of stages (strides 1, 2, .., 64; sums in the lower place,
+// differences in the upper) of fwht128_warp, so that both give the same bits.  Between lanes a stage is one shuffle and one fused
+// multiply-add with 1 or -1, which rounds as the sum or the difference does.  The shuffles bound it: four per value at A = 1, two at A = 4.
+template <int A>
+__device__ __forceinline__ void rotate128(float (&v)[A][8], int lane) {
 #pragma unroll
-    for (int m = 1; m < 8; m <<= 1)
+    for (int m = 1; m < 8 * A; m <<= 1)
 #pragma unroll
-        for (int j = 0; j < 8; ++j)
+        for (int j = 0; j < 8 * A; ++j)
             if (!(j & m)) {
-                const float a = v[j], b = v[j | m];
-                v[j] = a + b;
-                v[j | m] = a - b;
+                const float a = v[j >> 3][j & 7], b = v[(j | m) >> 3][(j | m) & 7];
+                v[j >> 3][j & 7] = a + b;
+                v[(j | m) >> 3][(j | m) & 7] = a - b;
             }
 #pragma unroll
-    for (int m = 1; m < 16; m <<= 1) {
-        const bool high = (lane & m) != 0;
+    for (int m = 1; m < 16 / A; m <<= 1) {
+        const float sign = (lane & m) ? -1.f : 1.f;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const float o = __shfl_xor_sync(0xffffffffu, v[j], m);
-            v[j] = high ? o - v[j] : v[j] + o;
-        }
+        for (int j = 0; j < 8 * A; ++j) v[j >> 3][j & 7] = fmaf(v[j >> 3][j & 7], sign, __shfl_xor_sync(0xffffffffu, v[j >> 3][j & 7], m));
     }
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] *= 0.08838834764831845f;
+    for (int j = 0; j < 8 * A; ++j) v[j >> 3][j & 7] *= 0.08838834764831845f;
 }
 
 // Bits of the largest |v|; NaN is above infinity.
@@ -109,6 +108,23 @@ __device__ __forceinline__ uint32_t largest_bits(const float (&v)[8]) {
 #pragma unroll
     for (int j = 0; j < 8; ++j) m = max(m, __float_as_uint(v[j]) & 0x7fffffffu);
     return m;
+}
+// The same of values as they lie
+__device__ __forceinline__ uint32_t largest_bits(const Raw8<float> &r) {
+    const uint32_t *u = &r.w[0].x, *w = &r.w[1].x;
+    uint32_t m = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) m = max(m, max(u[j] & 0x7fffffffu, w[j] & 0x7fffffffu));
+    return m;
+}
+template <class T>
+__device__ __forceinline__ uint32_t largest_pair(const Raw8<T> &r) {                     // two largest sizes, as bits of 16
+    const uint4 &w = r.w[0];
+    return __vmaxu2(__vmaxu2(w.x & 0x7fff7fffu, w.y & 0x7fff7fffu), __vmaxu2(w.z & 0x7fff7fffu, w.w & 0x7fff7fffu));
+}
+__device__ __forceinline__ uint32_t bits_of_pair(uint32_t m, __nv_bfloat16) { return max(m & 0xffffu, m >> 16) << 16; }
+__device__ __forceinline__ uint32_t bits_of_pair(uint32_t m, __half) {
+    return __float_as_uint(__half2float(__ushort_as_half((unsigned short)max(m & 0xffffu, m >> 16)))) & 0x7fffffffu;
 }
 
 // What turns values into codes.  The quotient lies between the products with a reciprocal 2^-21 too small and one as much too large,
@@ -140,9 +156,10 @@ struct Coder {
         const uint32_t r = __byte_perm(__byte_perm(n[0], n[1], 0x0040), __byte_perm(n[2], n[3], 0x0040), 0x5410);
         return good ? r : 0u;
     }
+    __device__ __forceinline__ uint2 eight(const float (&v)[8]) const { return make_uint2(four(v[0], v[1], v[2], v[3]), four(v[4], v[5], v[6], v[7])); }
     __device__ __forceinline__ void store(int8_t *row, int c, const Places &at, const float (&v)[8]) const {
         const int i = at.first(c);
-        const uint2 q = make_uint2(four(v[0], v[1], v[2], v[3]), four(v[4], v[5], v[6], v[7]));
+        const uint2 q = eight(v);
         if (at.next == 1) {
             if (i < at.width) *reinterpret_cast<uint2 *>(row + i) = q;
         } else {
@@ -177,5 +194,25 @@ template <bool kBlock> struct Joined {
         return __reduce_max_sync(0xffffffffu, (threadIdx.x & 31) < (blockDim.x >> 5) ? f[threadIdx.x & 31] : 0u);
     }
 };
+
+// ---- host side
+
+constexpr int kMostKept = 32768;       // longest row that a block keeps in registers: 1024 threads with four chunks of eight values
+
+struct Cut { int chunks, threads; };   // threads 0: a warp per row
+
+// A row's chunks over threads.  Up to 128 chunks a warp has them all and needs no barrier; longer rows have a block, with `many` chunks
+// per thread (loads in flight together, few warps at the barriers) unless rows are so few that latency counts: then one.
+inline Cut cut_of(int width, bool neighbours, int rows, int sms, int many) {
+    const int chunks = neighbours ? (width + 7) / 8 : (width + 255) / 256 * 32;
+    if (chunks <= 128 && (rows > 2 * sms || chunks <= 32)) return Cut{(chunks + 31) / 32, 0};
+    const int per = chunks > 2048 ? 4 : rows > 2 * sms || chunks > 1024 ? many : 1;
+    const int threads = ((chunks + per - 1) / per + 31) / 32 * 32;
+    return Cut{per, threads < 1024 ? threads : 1024};
+}
+
+inline bool aligned(const void *p, long long stride, int size) {
+    return jq_aligned16(p) && stride * size % 16 == 0;
+}
 
 }  // namespace jq8

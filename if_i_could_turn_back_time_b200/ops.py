@@ -493,11 +493,11 @@ class QuantizedRows(NamedTuple):
         if dtype not in _DT:
             raise RuntimeError(f"unsupported dtype {dtype}")
         codes, scales, K, stride = _codes_of(self)
-        out = torch.empty(self.codes.shape, dtype=dtype, device=codes.device)
-        if codes.shape[0]:
+        rows = codes.shape[0]
+        out = _new(self.codes.shape, dtype, codes.device)
+        if rows:
             with _on(codes.device):
-                st = _lib.load().jq_dequantize_rows(codes.data_ptr(), stride, scales.data_ptr(), codes.shape[0], K, out.data_ptr(),
-                                                    _DT[dtype], _stream())
+                st = _lib.load().jq_dequantize_rows(codes.data_ptr(), stride, scales.data_ptr(), rows, K, out.data_ptr(), _DT[dtype], _stream())
             if st:
                 _lib.check(st, "jq_dequantize_rows")
         return out
@@ -507,50 +507,61 @@ def _row_stride(K: int) -> int:
     return (K + 31) // 32 * 32
 
 
+def _new(shape, dtype, device, padded: int = 0) -> torch.Tensor:
+    """An uninitialised tensor; with ``padded`` its rows lie that many elements apart.  (torch.empty takes a microsecond longer.)"""
+    if len(shape) == 2:
+        return torch.empty_strided(shape, (padded or shape[1], 1), dtype=dtype, device=device)
+    if len(shape) == 1 or not padded:
+        return torch.empty(shape, dtype=dtype, device=device)
+    return torch.empty((*shape[:-1], padded), dtype=dtype, device=device)[..., :shape[-1]]
+
+
 def _codes_of(rows: QuantizedRows):
     """(codes [n, K], scales [n], K, elements between rows of codes), looked over and laid out as the library takes them."""
     codes, scales = rows.codes, rows.scales
-    if codes.dtype is not torch.int8 or codes.dim() == 0 or scales.dtype is not torch.float32 or scales.shape != codes.shape[:-1]:
+    shape = codes.shape
+    if codes.dtype is not torch.int8 or not shape or scales.dtype is not torch.float32 or scales.shape != shape[:-1]:
         raise RuntimeError(f"codes {tuple(codes.shape)} {codes.dtype}, scales {tuple(scales.shape)} {scales.dtype}: int8 [..., K] and fp32 [...]")
-    K = codes.shape[-1]
+    K = shape[-1]
     if not 0 < K <= _lib.JQ_INT8_MAX_K:
         raise RuntimeError(f"rows of {K} codes: 1 to {_lib.JQ_INT8_MAX_K}")
-    _need_cuda(codes, scales)
-    if scales.device != codes.device:
+    if not codes.is_cuda or not scales.is_cuda:
+        _need_cuda(codes, scales)
+    if scales.get_device() != codes.get_device():
         raise RuntimeError(f"codes are on {codes.device}, scales on {scales.device}")
-    if codes.dim() != 2:
+    if len(shape) != 2:
         codes = codes.reshape(-1, K)
-    if codes.shape[0] > 0x7fffffff:
-        raise RuntimeError(f"{codes.shape[0]} rows: the library counts in 32 bits")
+    n = codes.shape[0]
+    if n > 0x7fffffff:
+        raise RuntimeError(f"{n} rows: the library counts in 32 bits")
     if scales.is_neg():
         scales = scales.resolve_neg()
     if not scales.is_contiguous():
         scales = scales.contiguous()
     stride, one = codes.stride()
-    if codes.shape[0] == 1:
+    if n == 1:
         stride = _row_stride(K)
     if (one != 1 and K > 1) or stride % 16 or stride < K or codes.data_ptr() % 16:
         stride = _row_stride(K)
-        laid = torch.empty((codes.shape[0], stride), dtype=torch.int8, device=codes.device)
-        laid[:, :K] = codes
-        codes = laid[:, :K]
+        laid = _new((n, K), torch.int8, codes.device, stride)
+        laid.copy_(codes)
+        codes = laid
     return codes, scales, K, stride
 
 
 def _rows_of(x: torch.Tensor, what: str):
     """x [..., K] as (tensor [n, K], elements between rows): rows of one stride, values adjacent."""
-    if x.dtype not in _DT:
-        raise RuntimeError(f"unsupported dtype {x.dtype} of {what}")
     if x.is_neg():
         x = x.resolve_neg()
     if x.dim() != 2:
         x = x.reshape(-1, x.shape[-1])
+    n, K = x.shape
     row, one = x.stride()
-    if (one != 1 and x.shape[1] > 1) or row < 0:
+    if one != 1 and K > 1:
         x = x.contiguous()
-        row = x.shape[1]
-    if x.shape[0] > 0x7fffffff:
-        raise RuntimeError(f"{x.shape[0]} rows of {what}: the library counts in 32 bits")
+        row = K
+    if n > 0x7fffffff:
+        raise RuntimeError(f"{n} rows of {what}: the library counts in 32 bits")
     return x, row
 
 
@@ -561,22 +572,27 @@ def quantize_rows(x: torch.Tensor, had_block: int = 0) -> QuantizedRows:
 
     The activation's side of the reference's integer grid (QuantLinear, Python_Jenks_Test/Jenks_Tests/
     Quantization_Experiments/layers.py:22-38, which quantises weights only)."""
-    if x.dim() == 0 or not 0 < x.shape[-1] <= _lib.JQ_INT8_MAX_K:
-        raise RuntimeError(f"x is {tuple(x.shape)}: rows of 1 to {_lib.JQ_INT8_MAX_K} values")
-    if had_block not in (0, 128) or (had_block and x.shape[-1] % had_block):
-        raise RuntimeError(f"had_block is {had_block}: 0, or 128 where rows are a multiple of it (here {x.shape[-1]})")
-    x2, row = _rows_of(x, "x")
-    _need_cuda(x)
-    K, lead, stride = x.shape[-1], x.shape[:-1], _row_stride(x.shape[-1])
-    codes = torch.empty((*lead, stride), dtype=torch.int8, device=x.device)
-    scales = torch.empty(lead, dtype=torch.float32, device=x.device)
-    if x2.shape[0]:
-        with _on(x.device):
-            st = _lib.load().jq_quantize_rows(x2.data_ptr(), row, x2.shape[0], K, had_block, _DT[x.dtype], codes.data_ptr(), stride,
-                                              scales.data_ptr(), _stream())
+    shape, dtype = x.shape, x.dtype
+    K = shape[-1] if shape else 0
+    if not 0 < K <= _lib.JQ_INT8_MAX_K:
+        raise RuntimeError(f"x is {tuple(shape)}: rows of 1 to {_lib.JQ_INT8_MAX_K} values")
+    if had_block and (had_block != 128 or K % 128):
+        raise RuntimeError(f"had_block is {had_block}: 0, or 128 where rows are a multiple of it (here {K})")
+    if dtype not in _DT:
+        raise RuntimeError(f"unsupported dtype {dtype} of x")
+    if not x.is_cuda:
+        _need_cuda(x)
+    x, row = _rows_of(x, "x")
+    device, stride = x.device, _row_stride(K)
+    codes = _new(shape, torch.int8, device, stride)
+    scales = torch.empty(shape[:-1], dtype=torch.float32, device=device)
+    n = x.shape[0]
+    if n:
+        with _on(device):
+            st = _lib.load().jq_quantize_rows(x.data_ptr(), row, n, K, had_block, _DT[dtype], codes.data_ptr(), stride, scales.data_ptr(), _stream())
         if st:
             _lib.check(st, "jq_quantize_rows")
-    return QuantizedRows(codes if stride == K else codes[..., :K], scales, x.dtype, had_block)
+    return QuantizedRows(codes, scales, dtype, had_block)
 
 
 def _int8_weight(device, qweight, scales, bias, N, K):
@@ -594,15 +610,16 @@ def _int8_weight(device, qweight, scales, bias, N, K):
 
 
 def _linear_int8(x2, qweight, scales, bias, N, K, had, y):
-    bias = _int8_weight(x2.device, qweight, scales, bias, N, K)
+    device = x2.device
+    bias = _int8_weight(device, qweight, scales, bias, N, K)
     lib = _lib.load()
     rows, stride = x2.shape[0], _row_stride(K)
     part = max(256, MAX_ROWS_SCRATCH // stride // 256 * 256)
-    with _on(x2.device):
+    with _on(device):
         for b0 in range(0, rows, part):
             b1 = min(rows, b0 + part)
             xs, ys = (x2, y) if rows <= part else (x2[b0:b1], y[b0:b1])
-            own, scratch, size, status = _rows_scratch(x2.device, ((b1 - b0) * 4 + 255) // 256 * 256 + (b1 - b0) * stride)
+            own, scratch, size, status = _rows_scratch(device, ((b1 - b0) * 4 + 255) // 256 * 256 + (b1 - b0) * stride)
             st = lib.jq_int8_linear(qweight.data_ptr(), scales.data_ptr(), xs.data_ptr(), _addr(bias), ys.data_ptr(), N, K, b1 - b0, had,
                                     _DT[x2.dtype], _DT[y.dtype], scratch, size, status, _stream())
             if st:
@@ -614,26 +631,29 @@ def _linear_int8(x2, qweight, scales, bias, N, K, had, y):
 
 
 def _linear_quantized(x: QuantizedRows, pw: PackedWeight, bias, out_dtype) -> torch.Tensor:
-    if pw.spec.fmt != "int8":
-        raise RuntimeError(f"rows of 8-bit integers multiply int8 weights, not {pw.spec.fmt}")
+    spec = pw.spec
+    if spec.fmt != "int8":
+        raise RuntimeError(f"rows of 8-bit integers multiply int8 weights, not {spec.fmt}")
     codes, scales, K, stride = _codes_of(x)
     if K != pw.K:
         raise RuntimeError(f"rows of {K} codes, packed weight has K={pw.K}")
-    if x.had_block != pw.spec.had_block:
-        raise RuntimeError(f"rows with had_block {x.had_block}, packed weight has {pw.spec.had_block}")
+    if x.had_block != spec.had_block:
+        raise RuntimeError(f"rows with had_block {x.had_block}, packed weight has {spec.had_block}")
     dtype = out_dtype or x.dtype
     if dtype not in _DT:
         raise RuntimeError(f"unsupported output dtype {dtype}")
     _need_cuda(pw.qweight, pw.scales, bias)
     if bias is not None and bias.dtype != torch.float32:
         bias = bias.float()
-    bias = _int8_weight(codes.device, pw.qweight, pw.scales, bias, pw.N, K)
-    y = torch.empty((*x.codes.shape[:-1], pw.N), dtype=dtype, device=codes.device)
-    if codes.shape[0]:
-        with _on(codes.device):
-            status = _workspace(codes.device, 1024, "ta").data_ptr()
+    device, N = codes.device, pw.N
+    bias = _int8_weight(device, pw.qweight, pw.scales, bias, N, K)
+    y = _new((*x.codes.shape[:-1], N), dtype, device)
+    rows = codes.shape[0]
+    if rows:
+        with _on(device):
+            status = _workspace(device, 1024, "ta").data_ptr()
             st = _lib.load().jq_int8_matmul(pw.qweight.data_ptr(), pw.scales.data_ptr(), codes.data_ptr(), stride, scales.data_ptr(),
-                                            _addr(bias), y.data_ptr(), pw.N, K, codes.shape[0], _DT[dtype], status, _stream())
+                                            _addr(bias), y.data_ptr(), N, K, rows, _DT[dtype], status, _stream())
         if st:
             _lib.check(st, "jq_int8_matmul")
         if _checked:
@@ -670,61 +690,80 @@ def residual_norm(x: torch.Tensor, residual: Optional[torch.Tensor] = None, weig
     refused while gradients are recorded.
 
     The reference has no norm (its models are the vision networks and the MLP of Python_Jenks_Test/Jenks_Tests/QuantNetworkTest.py)."""
-    shape, dtype, device = x.shape, x.dtype, x.device
-    if not shape or not 0 < shape[-1] <= NORM_MAX_WIDTH:
+    shape, dtype = x.shape, x.dtype
+    width = shape[-1] if shape else 0
+    if not 0 < width <= NORM_MAX_WIDTH:
         raise RuntimeError(f"x is {tuple(shape)}: rows of 1 to {NORM_MAX_WIDTH} values")
-    width = shape[-1]
+    if dtype not in _DT:
+        raise RuntimeError(f"unsupported dtype {dtype} of x")
     if kind not in _NORM_KINDS:
         raise RuntimeError(f"unknown kind of norm {kind!r}: rms or layer")
     if had_block and (not quantize or had_block != 128 or width % 128):
         raise RuntimeError(f"had_block is {had_block}: 0, or 128 with quantize where the width is a multiple of it (here {width})")
     if post_bias is not None and post_weight is None:
         raise RuntimeError("a post_bias comes with a post_weight")
-    if not eps >= 0 or not -3.4e38 <= scale <= 3.4e38 or eps > 3.4e38:
+    if not (0 <= eps <= 3.4e38 and -3.4e38 <= scale <= 3.4e38):
         raise RuntimeError("scale is a finite number of fp32, eps one from 0 on")
-    vectors = [t for t in (weight, bias, post_weight, post_bias) if t is not None]
-    for t in vectors:
-        if t.shape != (width,) or t.dtype not in _DT or t.dtype != vectors[0].dtype:
+    given, at, wdtype, one = [x], [0, 0, 0, 0], None, (width,)
+    for i, t in enumerate((weight, bias, post_weight, post_bias)):
+        if t is None:
+            continue
+        if t.shape != one or t.dtype not in _DT or t.dtype is not (wdtype or t.dtype):
             raise RuntimeError(f"weights and biases are tensors [{width}] of one dtype; got {tuple(t.shape)} {t.dtype}")
-    if gate is not None and gate.dtype not in _DT:
-        raise RuntimeError(f"unsupported dtype {gate.dtype} of the gate")
-    if residual is not None and (residual.shape != shape or (residual.dtype != dtype and residual.dtype is not torch.float32)):
-        raise RuntimeError(f"residual {tuple(residual.shape)} {residual.dtype}: x's shape {tuple(shape)} and dtype, or fp32")
-    given = [t for t in (x, residual, gate) if t is not None] + vectors
-    _need_cuda(*given)
+        wdtype = t.dtype
+        if not t.is_contiguous() or t.is_neg():
+            t = t.resolve_neg().contiguous()
+        given.append(t)
+        at[i] = t.data_ptr()
+    rdtype = dtype
+    if residual is not None:
+        rdtype = residual.dtype
+        if residual.shape != shape or (rdtype is not dtype and rdtype is not torch.float32):
+            raise RuntimeError(f"residual {tuple(residual.shape)} {rdtype}: x's shape {tuple(shape)} and dtype, or fp32")
+        given.append(residual)
+    if gate is not None:
+        if gate.dtype not in _DT:
+            raise RuntimeError(f"unsupported dtype {gate.dtype} of the gate")
+        given.append(gate)
+    where, grad = x.get_device(), torch.is_grad_enabled()
     for t in given:
-        if t.device != device:
-            raise RuntimeError(f"x is on {device}, another tensor on {t.device}")
-    if torch.is_grad_enabled() and any(t.requires_grad for t in given):
-        raise RuntimeError("residual_norm has no backward pass: call it under torch.no_grad()")
+        if not t.is_cuda:
+            _need_cuda(t)
+        if t.get_device() != where:
+            raise RuntimeError(f"x is on {x.device}, another tensor on {t.device}")
+        if grad and t.requires_grad:
+            raise RuntimeError("residual_norm has no backward pass: call it under torch.no_grad()")
+    device = x.device
     x2, stride_x = _rows_of(x, "x")
-    stride_res = 0
+    res_at = stride_res = stride_q = out_at = r_at = codes_at = scales_at = 0
     if residual is not None:
         residual, stride_res = _rows_of(residual, "the residual")
-    weight, bias, post_weight, post_bias = (None if t is None else t.resolve_neg().contiguous() for t in (weight, bias, post_weight, post_bias))
-    outer = inner = one = 0
+        res_at = residual.data_ptr()
+    gate_at = outer = inner = flat = gdtype = 0
     each = 1
     if gate is not None:
-        gate, outer, inner, each, one = _gate_of(gate.resolve_neg(), shape)
-    rows = x2.shape[0]
-    same = residual is None and gate is None and scale == 1.0 and post_weight is None
-    rdtype = dtype if residual is None else residual.dtype
-    r = x if same else torch.empty(shape, dtype=rdtype, device=device)
-    codes = scales = out = None
-    stride_q = 0
+        gdtype = _DT[gate.dtype]
+        gate, outer, inner, each, flat = _gate_of(gate.resolve_neg(), shape)
+        gate_at = gate.data_ptr()
+    if residual is None and gate is None and scale == 1.0 and post_weight is None:
+        r = x
+    else:
+        r = _new(shape, rdtype, device)
+        r_at = r.data_ptr()
     if quantize:
         stride_q = _row_stride(width)
-        codes = torch.empty((*shape[:-1], stride_q), dtype=torch.int8, device=device)
+        codes = _new(shape, torch.int8, device, stride_q)
         scales = torch.empty(shape[:-1], dtype=torch.float32, device=device)
-        h = QuantizedRows(codes if stride_q == width else codes[..., :width], scales, dtype, had_block)
+        codes_at, scales_at = codes.data_ptr(), scales.data_ptr()
+        h = QuantizedRows(codes, scales, dtype, had_block)
     else:
-        h = out = torch.empty(shape, dtype=dtype, device=device)
+        h = _new(shape, dtype, device)
+        out_at = h.data_ptr()
+    rows = x2.shape[0]
     if rows:
-        P = lambda t: 0 if t is None else t.data_ptr()                                                        # noqa: E731
-        packed = _pack_norm(x2.data_ptr(), P(residual), P(weight), P(bias), P(post_weight), P(post_bias), P(gate), P(out),
-                            0 if same else r.data_ptr(), P(codes), P(scales), stride_x, stride_res, stride_q, outer, inner, rows, width, each,
-                            one, post_weight is not None, _NORM_KINDS[kind], had_block, _DT[dtype], _DT[rdtype],
-                            _DT[vectors[0].dtype] if vectors else 0, 0 if gate is None else _DT[gate.dtype], scale, eps, 0)
+        packed = _pack_norm(x2.data_ptr(), res_at, *at, gate_at, out_at, r_at, codes_at, scales_at, stride_x, stride_res, stride_q, outer, inner,
+                            rows, width, each, flat, post_weight is not None, _NORM_KINDS[kind], had_block, _DT[dtype], _DT[rdtype],
+                            _DT[wdtype] if wdtype else 0, gdtype, scale, eps, 0)
         with _on(device):
             st = _lib.load().jq_residual_norm(packed, _stream())
         if st:
