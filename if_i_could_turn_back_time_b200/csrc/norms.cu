@@ -14,25 +14,25 @@ struct NormArgs {
     int inner, gate_one;               // gate_one: one value for the whole row
     int rows, width;
     float scale, eps;
-    int layer, post, rotate, neighbours;
+    int layer, post, rotate;
     int wdtype, gdtype;                // types of the four vectors and of the gate
-    int vec_x, vec_res, vec_r, vec_h, vec_w, vec_g, wide_w, wide_g;
+    int wide_w, wide_g;                // fp32 rather than of x's type
 };
 
-// Eight values of a vector of T or of fp32, as they lie (weights: the same for every row, so that they come from the caches)
-template <class T> struct Weights {
-    uint4 a, b;
-    __device__ __forceinline__ void load(const void *p, bool wide, int i, int width) {
-        a = b = make_uint4(0, 0, 0, 0);
-        if (i >= width) return;
-        const uint4 *from = reinterpret_cast<const uint4 *>(reinterpret_cast<const unsigned char *>(p) + (size_t)i * (wide ? 4 : sizeof(T)));
-        a = from[0];
-        if (wide) b = from[1];
+// Eight values of a vector of T or of fp32 (weights, gates).  The piece that is enough for T is asked for ahead of its use (a gate's
+// with the row: 197 x 256 rows of 768 fp16, gated by image, 72 us without and 63 with; weights, which the caches have, behind the sums: asked for
+// ahead of them they cost registers, 8191 x 4096 bf16 45 us against 43); the second one of fp32 at its use.
+template <class T> struct Piece {
+    uint4 a;
+    __device__ __forceinline__ static const uint4 *at(const void *p, bool wide, int i) {
+        return reinterpret_cast<const uint4 *>(reinterpret_cast<const unsigned char *>(p) + (size_t)i * (wide ? 4 : sizeof(T)));
     }
-    __device__ __forceinline__ void get(bool wide, float (&v)[8]) const {
-        if (wide) {
+    __device__ __forceinline__ void ask(const void *p, bool wide, int i, int width) { a = i < width ? *at(p, wide, i) : make_uint4(0, 0, 0, 0); }
+    __device__ __forceinline__ void get(const void *p, bool wide, int i, int width, float (&v)[8]) const {
+        if (sizeof(T) == 4 || wide) {
             Raw8<float> r;
-            r.w[0] = a; r.w[1] = b;
+            r.w[0] = a;
+            r.w[1] = i < width ? at(p, true, i)[1] : make_uint4(0, 0, 0, 0);
             widen(r, v);
         } else if constexpr (sizeof(T) == 2) {
             Raw8<T> r;
@@ -45,8 +45,9 @@ template <class T> struct Weights {
 // A warp (kThreads 0) or a block per row, which stays in registers from the first read to the last write:
 //   u = N(x) post_weight + post_bias (or x),  r = residual + scale * (gate * u),  h = N(r) weight + bias,
 // N(v) = v / sqrt(mean(v^2) + eps), or of v - mean(v).  All in fp32; h follows from r as it was before its rounding.
-// kVec: every row and vector is of 16-byte pieces, and vectors are of T or fp32; the other form takes any width, alignment, stride and type.
-template <class T, class R, int kChunks, int kThreads, bool kVec>
+// kPieces: every row and vector is of 16-byte pieces, and vectors are of T or fp32; kPairs: rows are of pairs; kScattered: any width, alignment,
+// stride and type.
+template <class T, class R, int kChunks, int kThreads, Lay L>
 __global__ void __launch_bounds__(kThreads ? kThreads : 256) norm_kernel(const __grid_constant__ NormArgs p) {
     constexpr bool kBlock = kThreads != 0;
     __shared__ Shared sh;
@@ -55,36 +56,35 @@ __global__ void __launch_bounds__(kThreads ? kThreads : 256) norm_kernel(const _
     const int threads = kBlock ? blockDim.x : 32, me = kBlock ? threadIdx.x : lane;
     const int row = kBlock ? blockIdx.x : blockIdx.x * 8 + (threadIdx.x >> 5);
     if (row >= p.rows) return;
-    const Places at(p.width, kVec || p.neighbours);
     const T *x = reinterpret_cast<const T *>(p.x) + row * p.stride_x;
+    const auto first = [&](int j) { return first_of<L>(me + j * threads); };
     Joined<kBlock> joined(sh);
     const float each = 1.f / (float)p.width;
     float v[kChunks][8];
-    Raw8<R> res[kChunks];
+    Held<L, R> res[kChunks];
+    Piece<T> gates[kChunks];
+    const unsigned char *gate = reinterpret_cast<const unsigned char *>(p.gate);
+    if (gate) gate += ((row / p.inner) * p.gate_outer + (row % p.inner) * p.gate_inner) * (p.gdtype == JQ_F32 ? 4 : 2);
     {
-        Raw8<T> raw[kChunks];
+        Held<L, T> held[kChunks];
 #pragma unroll
-        for (int j = 0; j < kChunks; ++j) raw[j] = load_chunk(x, me + j * threads, at, kVec || p.vec_x);
+        for (int j = 0; j < kChunks; ++j) held[j].load(x, first(j), p.width);
         if (p.residual) {
             const R *from = reinterpret_cast<const R *>(p.residual) + row * p.stride_res;
 #pragma unroll
-            for (int j = 0; j < kChunks; ++j) res[j] = load_chunk(from, me + j * threads, at, kVec || p.vec_res);
+            for (int j = 0; j < kChunks; ++j) res[j].load(from, first(j), p.width);
+        }
+        if (L == kPieces && gate && !p.gate_one) {
+#pragma unroll
+            for (int j = 0; j < kChunks; ++j) gates[j].ask(gate, p.wide_g, first(j), p.width);
         }
 #pragma unroll
-        for (int j = 0; j < kChunks; ++j) widen(raw[j], v[j]);
+        for (int j = 0; j < kChunks; ++j) held[j].get(v[j]);
     }
     // whether element k of chunk j is one of the row
-    auto in = [&](int j, int k) { return kVec ? (me + j * threads) * 8 < p.width : at.first(me + j * threads) + k * at.next < at.width; };
-    auto vector = [&](const void *from, int j, float (&w)[8]) {           // of one of the four vectors
-        if constexpr (kVec) {
-            Weights<T> raw;
-            raw.load(from, p.wide_w, (me + j * threads) * 8, p.width);
-            raw.get(p.wide_w, w);
-        } else {
-            load_any(from, p.wdtype, me + j * threads, at, p.vec_w, w);
-        }
-    };
+    auto in = [&](int j, int k) { return inside<L>(first(j), k, p.width); };
     auto normed = [&](const void *weight, const void *bias) {
+        Piece<T> piece[kChunks];
         float s = 0.f;
         if (p.layer) {
             float mean = 0.f;
@@ -108,19 +108,29 @@ __global__ void __launch_bounds__(kThreads ? kThreads : 256) norm_kernel(const _
 #pragma unroll
             for (int k = 0; k < 8; ++k) v[j][k] *= s;
         if (weight) {
+            if (L == kPieces) {
+#pragma unroll
+                for (int j = 0; j < kChunks; ++j) piece[j].ask(weight, p.wide_w, first(j), p.width);
+            }
 #pragma unroll
             for (int j = 0; j < kChunks; ++j) {
                 float w[8];
-                vector(weight, j, w);
+                if constexpr (L == kPieces) piece[j].get(weight, p.wide_w, first(j), p.width, w);
+                else load_any<L>(weight, p.wdtype, first(j), p.width, w);
 #pragma unroll
                 for (int k = 0; k < 8; ++k) v[j][k] *= w[k];
             }
         }
         if (bias) {
+            if (L == kPieces) {
+#pragma unroll
+                for (int j = 0; j < kChunks; ++j) piece[j].ask(bias, p.wide_w, first(j), p.width);
+            }
 #pragma unroll
             for (int j = 0; j < kChunks; ++j) {
                 float b[8];
-                vector(bias, j, b);
+                if constexpr (L == kPieces) piece[j].get(bias, p.wide_w, first(j), p.width, b);
+                else load_any<L>(bias, p.wdtype, first(j), p.width, b);
 #pragma unroll
                 for (int k = 0; k < 8; ++k) v[j][k] += b[k];
             }
@@ -128,9 +138,7 @@ __global__ void __launch_bounds__(kThreads ? kThreads : 256) norm_kernel(const _
     };
     if (p.post) normed(p.post_weight, p.post_bias);
     float f = p.scale;
-    if (p.gate) {
-        const long long g0 = (long long)(row / p.inner) * p.gate_outer + (long long)(row % p.inner) * p.gate_inner;
-        const void *gate = reinterpret_cast<const unsigned char *>(p.gate) + g0 * (p.gdtype == JQ_F32 ? 4 : 2);
+    if (gate) {
         if (p.gate_one) {
             const float one = jq::load_act(gate, 0, p.gdtype);
 #pragma unroll
@@ -141,13 +149,8 @@ __global__ void __launch_bounds__(kThreads ? kThreads : 256) norm_kernel(const _
 #pragma unroll
             for (int j = 0; j < kChunks; ++j) {
                 float g[8];
-                if constexpr (kVec) {
-                    Weights<T> raw;
-                    raw.load(gate, p.wide_g, (me + j * threads) * 8, p.width);
-                    raw.get(p.wide_g, g);
-                } else {
-                    load_any(gate, p.gdtype, me + j * threads, at, p.vec_g, g);
-                }
+                if constexpr (L == kPieces) gates[j].get(gate, p.wide_g, first(j), p.width, g);
+                else load_any<L>(gate, p.gdtype, first(j), p.width, g);
 #pragma unroll
                 for (int k = 0; k < 8; ++k) v[j][k] *= g[k];
             }
@@ -157,7 +160,7 @@ __global__ void __launch_bounds__(kThreads ? kThreads : 256) norm_kernel(const _
     for (int j = 0; j < kChunks; ++j) {
         if (p.residual) {
             float old[8];
-            widen(res[j], old);
+            res[j].get(old);
 #pragma unroll
             for (int k = 0; k < 8; ++k) v[j][k] = old[k] + v[j][k] * f;
         } else {
@@ -168,10 +171,10 @@ __global__ void __launch_bounds__(kThreads ? kThreads : 256) norm_kernel(const _
     if (p.r) {
         R *r = reinterpret_cast<R *>(p.r) + (long long)row * p.width;
 #pragma unroll
-        for (int j = 0; j < kChunks; ++j) store_chunk(r, me + j * threads, at, kVec || p.vec_r, v[j]);
+        for (int j = 0; j < kChunks; ++j) store_chunk<L>(r, first(j), p.width, v[j]);
     }
     // (an infinite gate or root times the zeros behind the row's end is NaN)
-    if (p.post || p.gate) {
+    if (p.post || gate) {
 #pragma unroll
         for (int j = 0; j < kChunks; ++j)
 #pragma unroll
@@ -181,13 +184,13 @@ __global__ void __launch_bounds__(kThreads ? kThreads : 256) norm_kernel(const _
     if (!p.codes) {
         T *h = reinterpret_cast<T *>(p.h) + (long long)row * p.width;
 #pragma unroll
-        for (int j = 0; j < kChunks; ++j) store_chunk(h, me + j * threads, at, kVec || p.vec_h, v[j]);
+        for (int j = 0; j < kChunks; ++j) store_chunk<L>(h, first(j), p.width, v[j]);
         return;
     }
     uint32_t m = 0;
 #pragma unroll
     for (int j = 0; j < kChunks; ++j) {
-        if (p.rotate) {
+        if (L == kPieces && p.rotate) {
             float one[1][8];
 #pragma unroll
             for (int k = 0; k < 8; ++k) one[0][k] = v[j][k];
@@ -201,22 +204,28 @@ __global__ void __launch_bounds__(kThreads ? kThreads : 256) norm_kernel(const _
     if (me == 0) p.scales[row] = coder.told();
     int8_t *codes = p.codes + row * p.stride_q;
 #pragma unroll
-    for (int j = 0; j < kChunks; ++j) coder.store(codes, me + j * threads, at, v[j]);
+    for (int j = 0; j < kChunks; ++j) coder.template store_as<L>(codes, first(j), p.width, v[j]);
 }
 
 // ---- host side -------------------------------------------------------------------------
 
 template <class T, class R>
-static int launch_norm(const NormArgs &a, bool vec, cudaStream_t st) {
-    const Cut c = cut_of(a.width, a.neighbours, a.rows, jq_sm_count(), 2);
+static int launch_norm(const NormArgs &a, Lay l, cudaStream_t st) {
+    const int chunks = chunks_of(a.width, l);
+    Cut c = cut_of(chunks, a.rows, jq_sm_count(), 2);
+    // (rows by elements: four chunks of a warp's thread are some hundred registers, and a block of two warps is ahead)
+    if (l != kPieces && c.threads == 0 && c.chunks > 2) c = Cut{2, (chunks / 2 + 31) / 32 * 32};
     void (*k)(const NormArgs);
-    if (vec) {
-        if (c.threads == 0) k = c.chunks == 1 ? norm_kernel<T, R, 1, 0, true> : c.chunks == 2 ? norm_kernel<T, R, 2, 0, true> :
-                                c.chunks == 3 ? norm_kernel<T, R, 3, 0, true> : norm_kernel<T, R, 4, 0, true>;
-        else k = c.chunks == 1 ? norm_kernel<T, R, 1, 1024, true> : c.chunks == 2 ? norm_kernel<T, R, 2, 1024, true> : norm_kernel<T, R, 4, 1024, true>;
+    if (l == kPieces) {
+        if (c.threads == 0) k = c.chunks == 1 ? norm_kernel<T, R, 1, 0, kPieces> : c.chunks == 2 ? norm_kernel<T, R, 2, 0, kPieces> :
+                                c.chunks == 3 ? norm_kernel<T, R, 3, 0, kPieces> : norm_kernel<T, R, 4, 0, kPieces>;
+        else k = c.chunks == 1 ? norm_kernel<T, R, 1, 1024, kPieces> : c.chunks == 2 ? norm_kernel<T, R, 2, 1024, kPieces> : norm_kernel<T, R, 4, 1024, kPieces>;
+    } else if (l == kPairs) {
+        if (c.threads == 0) k = c.chunks == 1 ? norm_kernel<T, R, 1, 0, kPairs> : norm_kernel<T, R, 2, 0, kPairs>;
+        else k = c.chunks <= 2 ? norm_kernel<T, R, 2, 1024, kPairs> : norm_kernel<T, R, 4, 1024, kPairs>;
     } else {
-        if (c.threads == 0) k = norm_kernel<T, R, 4, 0, false>;
-        else k = c.chunks <= 2 ? norm_kernel<T, R, 2, 1024, false> : norm_kernel<T, R, 4, 1024, false>;
+        if (c.threads == 0) k = c.chunks == 1 ? norm_kernel<T, R, 1, 0, kScattered> : norm_kernel<T, R, 2, 0, kScattered>;
+        else k = c.chunks <= 2 ? norm_kernel<T, R, 2, 1024, kScattered> : norm_kernel<T, R, 4, 1024, kScattered>;
     }
     k<<<c.threads ? a.rows : (a.rows + 7) / 8, c.threads ? c.threads : 256, 0, st>>>(a);
     return jq_launch_status();
@@ -247,23 +256,20 @@ extern "C" int jq_residual_norm(const jq_norm *n, jq_stream_t stream) {
     a.rows = n->rows; a.width = W; a.scale = n->scale; a.eps = n->eps;
     a.layer = n->kind == JQ_NORM_LAYER; a.post = n->post; a.rotate = n->had_block != 0;
     a.wdtype = n->weight_dtype; a.gdtype = n->gate_dtype;
-    a.neighbours = W % 8 == 0;
-    bool vec = false;
-    if (a.neighbours) {
-        const int gs = n->gate_dtype == JQ_F32 ? 4 : 2;
-        const bool vectors = n->weight || n->bias || n->post_weight || n->post_bias;
-        a.vec_x = aligned(n->x, n->stride_x, xs);
-        a.vec_res = aligned(n->residual, n->stride_residual, rs);
-        a.vec_r = jq_aligned16(n->r); a.vec_h = jq_aligned16(n->h);
-        a.vec_w = jq_aligned16(n->weight) && jq_aligned16(n->bias) && jq_aligned16(n->post_weight) && jq_aligned16(n->post_bias);
-        a.vec_g = n->gate_one || (aligned(n->gate, n->gate_outer, gs) && n->gate_inner * gs % 16 == 0);
-        a.wide_w = n->weight_dtype == JQ_F32; a.wide_g = n->gate_dtype == JQ_F32;
-        vec = a.vec_x && a.vec_res && a.vec_r && a.vec_h && a.vec_w && a.vec_g && (!vectors || n->weight_dtype == n->x_dtype || a.wide_w) &&
-              (!n->gate || n->gate_one || n->gate_dtype == n->x_dtype || a.wide_g);
-        a.vec_g = a.vec_g && !n->gate_one;
-    }
+    a.wide_w = n->weight_dtype == JQ_F32;
+    a.wide_g = n->gate_dtype == JQ_F32;
+    const int gs = n->gate_dtype == JQ_F32 ? 4 : 2;
+    const bool vectors = n->weight || n->bias || n->post_weight || n->post_bias;
+    const bool vec = W % 8 == 0 && aligned(n->x, n->stride_x, xs) && aligned(n->residual, n->stride_residual, rs) && jq_aligned16(n->r) && jq_aligned16(n->h) &&
+                     jq_aligned16(n->weight) && jq_aligned16(n->bias) && jq_aligned16(n->post_weight) && jq_aligned16(n->post_bias) &&
+                     (!vectors || n->weight_dtype == n->x_dtype || a.wide_w) &&
+                     (!n->gate || n->gate_one || (aligned(n->gate, n->gate_outer, gs) && n->gate_inner * gs % 16 == 0 && (n->gate_dtype == n->x_dtype || a.wide_g)));
+    if (a.rotate && !vec) return JQ_ERR_BAD_ALIGN;
+    auto paired = [](const void *p, int64_t stride, int size) { return (reinterpret_cast<uintptr_t>(p) & (2 * size - 1)) == 0 && stride % 2 == 0; };
+    const bool pairs = W % 2 == 0 && paired(n->x, n->stride_x, xs) && paired(n->residual, n->stride_residual, rs) && paired(n->r, 0, rs) && paired(n->h, 0, xs);
+    const Lay lay = vec ? kPieces : pairs ? kPairs : kScattered;
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-    if (n->x_dtype == JQ_F32) return launch_norm<float, float>(a, vec, st);
-    if (n->x_dtype == JQ_F16) return n->residual_dtype == JQ_F32 ? launch_norm<__half, float>(a, vec, st) : launch_norm<__half, __half>(a, vec, st);
-    return n->residual_dtype == JQ_F32 ? launch_norm<__nv_bfloat16, float>(a, vec, st) : launch_norm<__nv_bfloat16, __nv_bfloat16>(a, vec, st);
+    if (n->x_dtype == JQ_F32) return launch_norm<float, float>(a, lay, st);
+    if (n->x_dtype == JQ_F16) return n->residual_dtype == JQ_F32 ? launch_norm<__half, float>(a, lay, st) : launch_norm<__half, __half>(a, lay, st);
+    return n->residual_dtype == JQ_F32 ? launch_norm<__nv_bfloat16, float>(a, lay, st) : launch_norm<__nv_bfloat16, __nv_bfloat16>(a, lay, st);
 }

@@ -8,68 +8,84 @@ struct QuantArgs {
     long long stride_x, stride_q;      // between rows
     int8_t *codes;
     float *scales;
-    int rows, width, rotate, neighbours, vec;
+    int rows, width, parts;            // parts: CTAs of a cluster that share a row
+    int inner;                         // around a row but the first and the last lie at least 16 elements of its neighbours
 };
 
-// How a thread's chunks lie and what becomes of them
+constexpr int kLong = 544;             // threads of a block of a cluster at most: eight of them hold JQ_INT8_MAX_K values
+
+// What becomes of a row
 enum Mode {
-    kStraight,    // rows of 16-byte pieces, not rotated: kept as they are, the maximum found in pairs of 16 bits
-    kRotated,     // rotated: a thread's chunks are neighbours, so that less of the rotation crosses lanes
-    kGeneral,     // any width, alignment and stride, rotated or not
-    kTiled        // the same for rows that a block does not keep, which are read twice
+    kStraight,    // rows of 16-byte pieces, kept as they are, the maximum found in pairs of 16 bits
+    kRotated,     // the same rows rotated: a thread's chunks are neighbours, so that less of the rotation crosses lanes
+    kAnywhere     // rows that begin anywhere
 };
 
-// A warp (kThreads 0) or a block per row, which stays in registers between its maximum and its codes.
+// A warp (kThreads 0), a block or a cluster of blocks per row, which stays in registers between its maximum and its codes.
+// 8191 x 11008 bf16: 53 us straight (5.1 TB/s), 68 rotated, where instructions bind (seven additions, two shuffles and four instructions of
+// encoding per value; with a thread's chunks apart and the stages' sums one by one 100).
 template <class T, int kChunks, int kThreads, Mode kMode>
-__global__ void __launch_bounds__(kThreads ? kThreads : 256) quantize_kernel(const __grid_constant__ QuantArgs p) {
+__global__ void __launch_bounds__(kThreads ? kThreads : 256, kThreads == 384 ? (kMode == kStraight ? 4 : 3) : 1) quantize_kernel(const __grid_constant__ QuantArgs p) {
     constexpr bool kBlock = kThreads != 0;
     __shared__ Shared sh;
+    __shared__ uint32_t s_top;
     jqta::pdl_launch_dependents();
     const int lane = threadIdx.x & 31;
-    const int threads = kBlock ? blockDim.x : 32, me = kBlock ? threadIdx.x : lane;
-    const int row = kBlock ? blockIdx.x : blockIdx.x * 8 + (threadIdx.x >> 5);
+    const int threads = kBlock ? blockDim.x : 32;
+    const int row = kBlock ? blockIdx.y : blockIdx.x * 8 + (threadIdx.x >> 5);
+    const int me = kBlock ? threadIdx.x : lane, part = kBlock ? blockIdx.x : 0;
     if (row >= p.rows) return;
     const T *x = reinterpret_cast<const T *>(p.x) + row * p.stride_x;
     int8_t *codes = p.codes + row * p.stride_q;
     Joined<kBlock> joined(sh);
+    // the row's maximum, over the CTAs that share it too; the scale told once
+    auto coder_of = [&](uint32_t m) {
+        m = joined.top(m);
+        if (kThreads == kLong) {
+            if (me == 0) s_top = m;
+            jqta::cluster_sync();
+            for (int r = 0; r < p.parts; ++r) {
+                uint32_t o;
+                asm volatile("{ .reg .b32 a; mapa.shared::cluster.u32 a, %1, %2; ld.shared::cluster.u32 %0, [a]; }" : "=r"(o) : "r"(jqta::smem_u32(&s_top)), "r"(r) : "memory");
+                m = max(m, o);
+            }
+            jqta::cluster_sync();                 // (nobody leaves while another reads)
+        }
+        const Coder coder(m);
+        if (me == 0 && part == 0) p.scales[row] = coder.told();
+        return coder;
+    };
     if constexpr (kMode == kStraight) {
-        const Places at(p.width, true);
-        Raw8<T> raw[kChunks];
+        const int c0 = part * threads * kChunks + me;
+        Held<kPieces, T> held[kChunks];
 #pragma unroll
-        for (int j = 0; j < kChunks; ++j) raw[j] = load_chunk(x, me + j * threads, at, true);
+        for (int j = 0; j < kChunks; ++j) held[j].load(x, (c0 + j * threads) * 8, p.width);
         uint32_t m = 0;
         if constexpr (sizeof(T) == 4) {
 #pragma unroll
-            for (int j = 0; j < kChunks; ++j) m = max(m, largest_bits(raw[j]));
+            for (int j = 0; j < kChunks; ++j) m = max(m, largest_bits(held[j].raw));
         } else {
 #pragma unroll
-            for (int j = 0; j < kChunks; ++j) m = __vmaxu2(m, largest_pair(raw[j]));
+            for (int j = 0; j < kChunks; ++j) m = __vmaxu2(m, largest_pair(held[j].raw));
             m = bits_of_pair(m, T());
         }
-        const Coder coder(joined.top(m));
-        if (me == 0) p.scales[row] = coder.told();
+        const Coder coder = coder_of(m);
 #pragma unroll
         for (int j = 0; j < kChunks; ++j) {
-            const int i = (me + j * threads) * 8;
             float v[8];
-            widen(raw[j], v);
-            if (i < p.width) *reinterpret_cast<uint2 *>(codes + i) = coder.eight(v);
+            held[j].get(v);
+            coder.template store_as<kPieces>(codes, (c0 + j * threads) * 8, p.width, v);
         }
     } else if constexpr (kMode == kRotated) {
-        const Places at(p.width, true);
+        const int c0 = (part * threads + me) * kChunks, i = c0 * 8;
         float v[kChunks][8];
-        Raw8<T> raw[kChunks];
+        Held<kPieces, T> held[kChunks];
 #pragma unroll
-        for (int j = 0; j < kChunks; ++j) raw[j] = load_chunk(x, me * kChunks + j, at, true);
+        for (int j = 0; j < kChunks; ++j) held[j].load(x, i + 8 * j, p.width);
 #pragma unroll
-        for (int j = 0; j < kChunks; ++j) widen(raw[j], v[j]);
+        for (int j = 0; j < kChunks; ++j) held[j].get(v[j]);
         rotate128<kChunks>(v, lane);
-        uint32_t m = 0;
-#pragma unroll
-        for (int j = 0; j < kChunks; ++j) m = max(m, largest_bits(v[j]));
-        const Coder coder(joined.top(m));
-        if (me == 0) p.scales[row] = coder.told();
-        const int i = me * kChunks * 8;
+        const Coder coder = coder_of(largest_rotated(v));
         if (i < p.width) {
             if constexpr (kChunks == 1) {
                 *reinterpret_cast<uint2 *>(codes + i) = coder.eight(v[0]);
@@ -82,32 +98,26 @@ __global__ void __launch_bounds__(kThreads ? kThreads : 256) quantize_kernel(con
             }
         }
     } else {
-        const Places at(p.width, p.neighbours);
-        const int tile = threads * kChunks, chunks = p.neighbours ? (p.width + 7) / 8 : (p.width + 255) / 256 * 32;
-        const int end = kMode == kTiled ? chunks : 1;
-        float v[kChunks][8];
-        auto read = [&](int c0) {
+        const int c0 = part * threads * kChunks + me;
+        const bool near = p.inner && row > 0 && row + 1 < p.rows;
+        Raw8<T> raw[kChunks];
 #pragma unroll
-            for (int j = 0; j < kChunks; ++j) {
-                float one[1][8];
-                widen(load_chunk(x, c0 + me + j * threads, at, p.vec), one[0]);
-                if (p.rotate) rotate128<1>(one, lane);
-#pragma unroll
-                for (int k = 0; k < 8; ++k) v[j][k] = one[0][k];
-            }
-        };
+        for (int j = 0; j < kChunks; ++j) raw[j] = load_anywhere(x, c0 + j * threads, p.width, near);
         uint32_t m = 0;
-        for (int c0 = 0; c0 < end; c0 += tile) {
-            read(c0);
+        if constexpr (sizeof(T) == 4) {
 #pragma unroll
-            for (int j = 0; j < kChunks; ++j) m = max(m, largest_bits(v[j]));
+            for (int j = 0; j < kChunks; ++j) m = max(m, largest_bits(raw[j]));
+        } else {
+#pragma unroll
+            for (int j = 0; j < kChunks; ++j) m = __vmaxu2(m, largest_pair(raw[j]));
+            m = bits_of_pair(m, T());
         }
-        const Coder coder(joined.top(m));
-        if (me == 0) p.scales[row] = coder.told();
-        for (int c0 = 0; c0 < end; c0 += tile) {
-            if (kMode == kTiled) read(c0);
+        const Coder coder = coder_of(m);
 #pragma unroll
-            for (int j = 0; j < kChunks; ++j) coder.store(codes, c0 + me + j * threads, at, v[j]);
+        for (int j = 0; j < kChunks; ++j) {
+            float v[8];
+            widen(raw[j], v);
+            coder.store(codes, (c0 + j * threads) * 8, p.width, v);
         }
     }
 }
@@ -117,73 +127,117 @@ struct DequantArgs {
     const float *scales;
     void *out;
     long long stride_q;
-    int rows, width, neighbours, vec, dtype, segments;
+    int rows, width, segments;
 };
 
 // A warp per 1024 values of a row.
-template <class T>
+template <class T, bool kVec>
 __global__ void __launch_bounds__(256) dequantize_kernel(const __grid_constant__ DequantArgs p) {
     const int lane = threadIdx.x & 31;
     const long long unit = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
     const long long row = unit / p.segments;
     if (row >= p.rows) return;
-    const int c0 = (int)(unit % p.segments) * 128 + lane;
-    const Places at(p.width, p.neighbours);
+    const int seg = (int)(unit % p.segments);
     const int8_t *codes = p.codes + row * p.stride_q;
     T *out = reinterpret_cast<T *>(p.out) + row * p.width;
     const float s = p.scales[row];
-    uint2 q[4];
+    if constexpr (kVec) {
+        uint2 q[4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        const int i = at.first(c0 + 32 * j);
-        q[j] = make_uint2(0, 0);
-        if (at.next == 1) {
-            if (i < at.width) q[j] = *reinterpret_cast<const uint2 *>(codes + i);
-        } else {
-            uint32_t w[2] = {0, 0};
-#pragma unroll
-            for (int k = 0; k < 8; ++k)
-                if (i + 32 * k < at.width) w[k >> 2] |= (uint32_t)(uint8_t)codes[i + 32 * k] << 8 * (k & 3);
-            q[j] = make_uint2(w[0], w[1]);
+        for (int j = 0; j < 4; ++j) {
+            const int i = (seg * 128 + 32 * j + lane) * 8;
+            q[j] = i < p.width ? *reinterpret_cast<const uint2 *>(codes + i) : make_uint2(0, 0);
         }
-    }
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        float v[8];
+        for (int j = 0; j < 4; ++j) {
+            float v[8];
 #pragma unroll
-        for (int k = 0; k < 8; ++k) v[k] = (float)(int8_t)((k < 4 ? q[j].x : q[j].y) >> 8 * (k & 3)) * s;
-        store_chunk(out, c0 + 32 * j, at, p.vec, v);
+            for (int k = 0; k < 8; ++k) v[k] = (float)(int8_t)((k < 4 ? q[j].x : q[j].y) >> 8 * (k & 3)) * s;
+            store_chunk<kPieces>(out, (seg * 128 + 32 * j + lane) * 8, p.width, v);
+        }
+    } else {
+        // chunks that are 16-byte pieces of the output: `off` elements behind, so that their codes lie across two words of eight
+        const int off = (int)((reinterpret_cast<uintptr_t>(out) / sizeof(T)) & 7);
+        auto eight = [&](int at) -> uint64_t { return at >= 0 && at + 8 <= p.width ? *reinterpret_cast<const uint64_t *>(codes + at) : 0ull; };
+#pragma unroll 2
+        for (int j = 0; j < 4; ++j) {
+            const int c = seg * 128 + 32 * j + lane, i = c * 8 - off;
+            if (i >= 0 && c * 8 + 8 <= p.width) {
+                uint64_t q = eight(c * 8);
+                if (off) q = q << 8 * off | eight(c * 8 - 8) >> (64 - 8 * off);
+                alignas(16) T e[8];
+#pragma unroll
+                for (int k = 0; k < 8; ++k) e[k] = (T)((float)(int8_t)(q >> 8 * k) * s);
+#pragma unroll
+                for (int k = 0; k < (int)sizeof(T) / 2; ++k)
+                    *reinterpret_cast<uint4 *>(reinterpret_cast<unsigned char *>(out + i) + 16 * k) = reinterpret_cast<const uint4 *>(e)[k];
+            } else if (i < p.width) {
+                for (int k = 0; k < 8; ++k)
+                    if (i + k >= 0 && i + k < p.width) out[i + k] = (T)((float)codes[i + k] * s);
+            }
+        }
     }
 }
 
 // ---- host side -------------------------------------------------------------------------
 
-template <class T>
-static int launch_quantize(const QuantArgs &a, cudaStream_t st) {
-    const int sms = jq_sm_count();
-    void (*k)(const QuantArgs);
-    Cut c;
-    if (a.vec && a.width <= kMostKept) {
-        c = cut_of(a.width, true, a.rows, sms, 4);
-        if (a.rotate) {
-            // (chunks that are neighbours: one, or four, which a row of 128 always fills)
-            if (c.threads == 0) c.chunks = c.chunks == 1 ? 1 : 4;
-            k = c.threads == 0 ? (c.chunks == 1 ? quantize_kernel<T, 1, 0, kRotated> : quantize_kernel<T, 4, 0, kRotated>)
-                               : (c.chunks == 1 ? quantize_kernel<T, 1, 1024, kRotated> : c.threads <= 512 ? quantize_kernel<T, 4, 512, kRotated> : quantize_kernel<T, 4, 1024, kRotated>);
-        } else {
-            k = c.threads == 0 ? (c.chunks == 1 ? quantize_kernel<T, 1, 0, kStraight> : c.chunks == 2 ? quantize_kernel<T, 2, 0, kStraight> :
-                                  c.chunks == 3 ? quantize_kernel<T, 3, 0, kStraight> : quantize_kernel<T, 4, 0, kStraight>)
-                               : (c.chunks == 1 ? quantize_kernel<T, 1, 1024, kStraight> : quantize_kernel<T, 4, 1024, kStraight>);
-        }
-    } else {
-        c = cut_of(a.width, a.neighbours, a.rows, sms, 4);
-        const int chunks = a.neighbours ? a.width / 8 : (a.width + 255) / 256 * 32;
-        if (c.threads == 0) k = quantize_kernel<T, 4, 0, kGeneral>;
-        else if (c.threads * c.chunks < chunks) k = quantize_kernel<T, 4, 1024, kTiled>;
-        else k = c.chunks == 1 ? quantize_kernel<T, 1, 1024, kGeneral> : quantize_kernel<T, 4, 1024, kGeneral>;
+static int launch_parts(void (*k)(const QuantArgs), const QuantArgs &a, const Cut &c, cudaStream_t st) {
+    if (a.parts == 1) {
+        k<<<c.threads ? dim3(1, a.rows) : dim3((a.rows + 7) / 8), c.threads ? c.threads : 256, 0, st>>>(a);
+        return jq_launch_status();
     }
-    k<<<c.threads ? a.rows : (a.rows + 7) / 8, c.threads ? c.threads : 256, 0, st>>>(a);
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = (unsigned)a.parts;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.gridDim = dim3((unsigned)a.parts, (unsigned)a.rows);
+    cfg.blockDim = dim3((unsigned)c.threads);
+    cfg.stream = st;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    JQ_CUDA_TRY(cudaLaunchKernelEx(&cfg, k, a));
     return jq_launch_status();
+}
+
+template <class T>
+static int launch_quantize(QuantArgs &a, bool vec, bool rotate, cudaStream_t st) {
+    const int sms = jq_sm_count(), chunks = chunks_of(a.width, kPieces);
+    Cut c = cut_of(chunks, a.rows, sms, 4);
+    void (*k)(const QuantArgs);
+    a.parts = 1;
+    if (chunks > 4096) {
+        // Longer rows than a block keeps go to clusters of eight blocks.  (Shorter ones in clusters, so that some blocks load while others
+        // compute, were slower: 4096 x 28672 bf16 rotated 143 us in clusters of three, 121 in blocks of 896 threads.)
+        a.parts = 8;
+        c = Cut{4, ((chunks + 31) / 32 + 31) / 32 * 32};
+        k = rotate ? quantize_kernel<T, 4, kLong, kRotated> : vec ? quantize_kernel<T, 4, kLong, kStraight> : quantize_kernel<T, 4, kLong, kAnywhere>;
+    } else if (rotate) {
+        if (c.threads == 0) c.chunks = c.chunks == 1 ? 1 : 4;
+        k = c.threads == 0 ? (c.chunks == 1 ? quantize_kernel<T, 1, 0, kRotated> : quantize_kernel<T, 4, 0, kRotated>)
+                           : (c.chunks == 1 ? quantize_kernel<T, 1, 1024, kRotated> : c.threads <= 384 ? quantize_kernel<T, 4, 384, kRotated> : quantize_kernel<T, 4, 1024, kRotated>);
+    } else if (vec) {
+        k = c.threads == 0 ? (c.chunks == 1 ? quantize_kernel<T, 1, 0, kStraight> : c.chunks == 2 ? quantize_kernel<T, 2, 0, kStraight> :
+                              c.chunks == 3 ? quantize_kernel<T, 3, 0, kStraight> : quantize_kernel<T, 4, 0, kStraight>)
+                           : (c.chunks == 1 ? quantize_kernel<T, 1, 1024, kStraight> : c.threads <= 384 ? quantize_kernel<T, 4, 384, kStraight> : quantize_kernel<T, 4, 1024, kStraight>);
+    } else {
+        k = c.threads == 0 ? (c.chunks == 1 ? quantize_kernel<T, 1, 0, kAnywhere> : c.chunks == 2 ? quantize_kernel<T, 2, 0, kAnywhere> : quantize_kernel<T, 4, 0, kAnywhere>)
+                           : (c.chunks == 1 ? quantize_kernel<T, 1, 1024, kAnywhere> : c.threads <= 384 ? quantize_kernel<T, 4, 384, kAnywhere> : quantize_kernel<T, 4, 1024, kAnywhere>);
+    }
+    if (c.threads && a.rows > 65535) {
+        // rows are the grid's second dimension: in parts of it
+        for (int r0 = 0; r0 < a.rows; r0 += 65535) {
+            QuantArgs b = a;
+            b.rows = a.rows - r0 < 65535 ? a.rows - r0 : 65535;
+            b.x = reinterpret_cast<const T *>(a.x) + r0 * a.stride_x;
+            b.codes += r0 * a.stride_q;
+            b.scales += r0;
+            const int rc = launch_parts(k, b, c, st);
+            if (rc) return rc;
+        }
+        return JQ_OK;
+    }
+    return launch_parts(k, a, c, st);
 }
 
 }  // namespace jq8
@@ -198,16 +252,17 @@ extern "C" int jq_quantize_rows(const void *x, int64_t row_stride, int rows, int
     if (x_dtype < 0 || x_dtype > 2) return JQ_ERR_BAD_DTYPE;
     if (!jq_aligned16(codes) || code_stride % 16) return JQ_ERR_BAD_ALIGN;
     const int size = x_dtype == JQ_F32 ? 4 : 2;
+    if (reinterpret_cast<uintptr_t>(x) & (size - 1)) return JQ_ERR_BAD_ALIGN;
     QuantArgs a{};
     a.x = x; a.stride_x = row_stride; a.stride_q = code_stride;
     a.codes = reinterpret_cast<int8_t *>(codes); a.scales = scales;
-    a.rows = rows; a.width = K; a.rotate = had_block != 0;
-    a.neighbours = K % 8 == 0;
-    a.vec = a.neighbours && aligned(x, row_stride, size);
+    a.rows = rows; a.width = K; a.inner = K >= 16 && row_stride >= K;
+    const bool vec = K % 8 == 0 && aligned(x, row_stride, size);
+    if (had_block && !vec) return JQ_ERR_BAD_ALIGN;
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-    if (x_dtype == JQ_F32) return launch_quantize<float>(a, st);
-    if (x_dtype == JQ_F16) return launch_quantize<__half>(a, st);
-    return launch_quantize<__nv_bfloat16>(a, st);
+    if (x_dtype == JQ_F32) return launch_quantize<float>(a, vec, had_block != 0, st);
+    if (x_dtype == JQ_F16) return launch_quantize<__half>(a, vec, had_block != 0, st);
+    return launch_quantize<__nv_bfloat16>(a, vec, had_block != 0, st);
 }
 
 extern "C" int jq_dequantize_rows(const void *codes, int64_t code_stride, const float *scales, int rows, int K, void *out, int dtype,
@@ -215,17 +270,18 @@ extern "C" int jq_dequantize_rows(const void *codes, int64_t code_stride, const 
     if (!codes || !scales || !out) return JQ_ERR_NULL_PTR;
     if (rows <= 0 || K <= 0 || code_stride < K) return JQ_ERR_BAD_SHAPE;
     if (dtype < 0 || dtype > 2) return JQ_ERR_BAD_DTYPE;
-    if (!jq_aligned16(codes) || code_stride % 16) return JQ_ERR_BAD_ALIGN;
+    if (!jq_aligned16(codes) || code_stride % 16 || (reinterpret_cast<uintptr_t>(out) & (dtype == JQ_F32 ? 3u : 1u))) return JQ_ERR_BAD_ALIGN;
     DequantArgs a{};
     a.codes = reinterpret_cast<const int8_t *>(codes); a.scales = scales; a.out = out; a.stride_q = code_stride;
-    a.rows = rows; a.width = K; a.neighbours = K % 8 == 0; a.dtype = dtype;
-    a.vec = a.neighbours && jq_aligned16(out);
-    a.segments = (K + 1023) / 1024;
+    a.rows = rows; a.width = K;
+    const bool vec = K % 8 == 0 && jq_aligned16(out);
+    a.segments = (K + (vec ? 0 : 7) + 1023) / 1024;
     const long long blocks = ((long long)rows * a.segments + 7) / 8;
     if (blocks > 0x7fffffff) return JQ_ERR_BAD_SHAPE;
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-    if (dtype == JQ_F32) dequantize_kernel<float><<<(unsigned)blocks, 256, 0, st>>>(a);
-    else if (dtype == JQ_F16) dequantize_kernel<__half><<<(unsigned)blocks, 256, 0, st>>>(a);
-    else dequantize_kernel<__nv_bfloat16><<<(unsigned)blocks, 256, 0, st>>>(a);
+    void (*const kernels[3][2])(const DequantArgs) = {{dequantize_kernel<float, false>, dequantize_kernel<float, true>},
+                                                      {dequantize_kernel<__half, false>, dequantize_kernel<__half, true>},
+                                                      {dequantize_kernel<__nv_bfloat16, false>, dequantize_kernel<__nv_bfloat16, true>}};
+    kernels[dtype][vec]<<<(unsigned)blocks, 256, 0, st>>>(a);
     return jq_launch_status();
 }

@@ -29,77 +29,197 @@ __device__ __forceinline__ void widen(const Raw8<__nv_bfloat16> &r, float (&v)[8
     for (int i = 0; i < 4; ++i) { v[2 * i] = __uint_as_float(u[i] << 16); v[2 * i + 1] = __uint_as_float(u[i] & 0xffff0000u); }
 }
 
-// Which elements of a row chunk c holds.  Rows whose width is a multiple of 8: eight neighbours.  Others: eight that are 32 apart, so
-// that a warp's one-element loads and stores lie side by side.
-struct Places {
-    int width, next;                   // next: between a chunk's elements
-    __device__ __forceinline__ Places(int width, bool neighbours) : width(width), next(neighbours ? 1 : 32) {}
-    __device__ __forceinline__ int first(int c) const { return next == 1 ? c * 8 : (c >> 5) * 256 + (c & 31); }
-};
+// A chunk is eight elements of a row, whose first one first_of() tells:
+//   kPieces     rows of 16-byte pieces: chunk c from 8 c on;
+//   kPairs      four pairs of neighbours 64 apart, so that a warp's two-element loads and stores lie side by side: rows of even length and place;
+//   kScattered  eight elements 32 apart: whatever else there is.
+// (For norms of rows that begin anywhere, chunks that are 16-byte pieces of memory, with a row's first and last one by elements, were slower up
+// to some thousand elements: 50000 x 197 bf16 30 us against 24.)
+enum Lay { kPieces, kPairs, kScattered };
+template <Lay L> __device__ __forceinline__ int first_of(int c) { return L == kPieces ? c * 8 : (c >> 5) * 256 + (L == kPairs ? 2 : 1) * (c & 31); }
+template <Lay L> __device__ __forceinline__ constexpr int place(int k) { return L == kPieces ? k : L == kPairs ? (k >> 1) * 64 + (k & 1) : k * 32; }
+// whether all of a chunk is the row's (the same for a warp's lanes where they lie side by side), and whether element k is
+template <Lay L> __device__ __forceinline__ bool whole(int i, int width) { return L == kPieces ? i < width : (i | 255) < width; }
+template <Lay L> __device__ __forceinline__ bool inside(int i, int k, int width) { return L == kPieces ? i < width : i + place<L>(k) < width; }
 
-// A chunk of a row; zeros behind its end.  vec: the row is 16-byte aligned and its chunks are neighbours.
-template <class T>
-__device__ __forceinline__ Raw8<T> load_chunk(const T *row, int c, const Places &at, bool vec) {
-    Raw8<T> r;
-    const int i = at.first(c);
-    if (vec) {
-        const bool in = i < at.width;
+template <class T> struct alignas(2 * sizeof(T)) PairOf { T a, b; };
+
+// A chunk between its load and its first use, zeros outside the row: as it lies, or, where it came in by elements, as fp32 (putting elements of 16
+// bits together again costs more than the registers)
+template <Lay L, class T> struct Held {
+    float e[8];
+    __device__ __forceinline__ void load(const T *row, int i, int width) {
+        const bool all = whole<L>(i, width);
+#pragma unroll
+        for (int k = 0; k < 8; k += L == kPairs ? 2 : 1) {
+            const T *at = row + i + place<L>(k);
+            const bool in = all || inside<L>(i, k, width);
+            if (L == kPairs) {
+                PairOf<T> p{(T)0.f, (T)0.f};
+                if (in) p = *reinterpret_cast<const PairOf<T> *>(at);
+                e[k] = (float)p.a;
+                e[k + 1] = (float)p.b;
+            } else {
+                e[k] = in ? (float)*at : 0.f;
+            }
+        }
+    }
+    __device__ __forceinline__ void get(float (&v)[8]) const {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) v[k] = e[k];
+    }
+};
+template <class T> struct Held<kPieces, T> {
+    Raw8<T> raw;
+    __device__ __forceinline__ void load(const T *row, int i, int width) {
+        const bool in = i < width;
 #pragma unroll
         for (int k = 0; k < (int)sizeof(T) / 2; ++k)
-            r.w[k] = in ? *reinterpret_cast<const uint4 *>(reinterpret_cast<const unsigned char *>(row + i) + 16 * k) : make_uint4(0, 0, 0, 0);
-    } else {
-        T *e = reinterpret_cast<T *>(&r);
-#pragma unroll
-        for (int k = 0; k < 8; ++k) e[k] = i + k * at.next < at.width ? row[i + k * at.next] : (T)0.f;
+            raw.w[k] = in ? *reinterpret_cast<const uint4 *>(reinterpret_cast<const unsigned char *>(row + i) + 16 * k) : make_uint4(0, 0, 0, 0);
     }
-    return r;
-}
-template <class T>
-__device__ __forceinline__ void store_chunk(T *row, int c, const Places &at, bool vec, const float (&v)[8]) {
-    const int i = at.first(c);
-    if (vec) {
-        if (i >= at.width) return;
-        Raw8<T> r;
-        T *e = reinterpret_cast<T *>(&r);
+    __device__ __forceinline__ void get(float (&v)[8]) const { widen(raw, v); }
+};
+template <Lay L, class T>
+__device__ __forceinline__ void store_chunk(T *row, int i, int width, const float (&v)[8]) {
+    if (L == kPieces) {
+        if (i >= width) return;
+        alignas(16) T e[8];
 #pragma unroll
         for (int k = 0; k < 8; ++k) e[k] = (T)v[k];
 #pragma unroll
-        for (int k = 0; k < (int)sizeof(T) / 2; ++k) *reinterpret_cast<uint4 *>(reinterpret_cast<unsigned char *>(row + i) + 16 * k) = r.w[k];
-    } else {
-#pragma unroll
-        for (int k = 0; k < 8; ++k)
-            if (i + k * at.next < at.width) row[i + k * at.next] = (T)v[k];
+        for (int k = 0; k < (int)sizeof(T) / 2; ++k) *reinterpret_cast<uint4 *>(reinterpret_cast<unsigned char *>(row + i) + 16 * k) = reinterpret_cast<const uint4 *>(e)[k];
+        return;
     }
+    const bool all = whole<L>(i, width);
+#pragma unroll
+    for (int k = 0; k < 8; k += L == kPairs ? 2 : 1)
+        if (all || inside<L>(i, k, width)) {
+            T *at = row + i + place<L>(k);
+            if (L == kPairs) *reinterpret_cast<PairOf<T> *>(at) = PairOf<T>{(T)v[k], (T)v[k + 1]};
+            else *at = (T)v[k];
+        }
 }
-// The same from a vector of any of the three types (weights: the same for every row, so that they come from the caches).
-__device__ __forceinline__ void load_any(const void *row, int dtype, int c, const Places &at, bool vec, float (&v)[8]) {
-    if (dtype == JQ_BF16) widen(load_chunk(reinterpret_cast<const __nv_bfloat16 *>(row), c, at, vec), v);
-    else if (dtype == JQ_F16) widen(load_chunk(reinterpret_cast<const __half *>(row), c, at, vec), v);
-    else widen(load_chunk(reinterpret_cast<const float *>(row), c, at, vec), v);
+
+// Chunk c, eight neighbours from 8 c on, of a row that begins anywhere: the 16-byte pieces of memory that hold it, shifted.
+// near: the memory around the row is its neighbours', so that pieces may be read whole at its ends.
+__device__ __forceinline__ void shift_words(uint32_t *w, int n, int by, bool yes) {
+    if (!yes) return;
+#pragma unroll
+    for (int k = 0; k < 12; ++k)
+        if (k + by < n) w[k] = w[k + by];
+}
+template <class T>
+__device__ __forceinline__ Raw8<T> load_anywhere(const T *row, int c, int width, bool near) {
+    constexpr int kPer = 16 / (int)sizeof(T), kWords = sizeof(T) == 4 ? 12 : 8;            // elements of a piece; words of the pieces
+    const int i = c * 8, off = (int)((reinterpret_cast<uintptr_t>(row) / sizeof(T)) & (kPer - 1)), begin = i - off;
+    Raw8<T> r;
+    uint32_t *out = &r.w[0].x;
+    if (i >= width) {
+#pragma unroll
+        for (int k = 0; k < (int)sizeof(T) / 2; ++k) r.w[k] = make_uint4(0, 0, 0, 0);
+        return r;
+    }
+    if (near || (begin >= 0 && begin + kWords * 4 / (int)sizeof(T) <= width)) {
+        uint4 piece[kWords / 4];
+#pragma unroll
+        for (int k = 0; k < kWords / 4; ++k)
+            piece[k] = k < kWords / 4 - 1 || off ? reinterpret_cast<const uint4 *>(row + begin)[k] : make_uint4(0, 0, 0, 0);
+        uint32_t w[kWords + 1];
+#pragma unroll
+        for (int k = 0; k < kWords / 4; ++k) { w[4 * k] = piece[k].x; w[4 * k + 1] = piece[k].y; w[4 * k + 2] = piece[k].z; w[4 * k + 3] = piece[k].w; }
+        w[kWords] = 0;
+        const int words = off * (int)sizeof(T) / 4;
+        shift_words(w, kWords, 2, words & 2);
+        shift_words(w, kWords, 1, words & 1);
+        if (sizeof(T) == 2) {
+            const int bits = 16 * (off & 1);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) out[k] = __funnelshift_r(w[k], w[k + 1], bits);
+        } else {
+            uint32_t *more = &r.w[sizeof(T) / 2 - 1].x;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) { out[k] = w[k]; more[k] = w[4 + k]; }
+        }
+        if (i + 8 > width) {
+#pragma unroll
+            for (int k = 1; k < 8; ++k)
+                if (i + k >= width) {
+                    if (sizeof(T) == 4) (k < 4 ? out[k & 3] : (&r.w[sizeof(T) / 2 - 1].x)[k & 3]) = 0;
+                    else out[k >> 1] &= k & 1 ? 0xffffu : 0u;
+                }
+        }
+    } else {
+        alignas(16) T e[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) e[k] = i + k < width ? row[i + k] : (T)0.f;
+#pragma unroll
+        for (int k = 0; k < (int)sizeof(T) / 2; ++k) r.w[k] = reinterpret_cast<const uint4 *>(e)[k];
+    }
+    return r;
+}
+
+// A chunk of a vector of any of the three types by elements (weights: the same for every row, so that they come from the caches)
+template <Lay L, class T>
+__device__ __forceinline__ void load_elements(const void *vector, int i, int width, float (&v)[8]) {
+    const T *from = reinterpret_cast<const T *>(vector);
+    const bool all = whole<L>(i, width);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[k] = all || inside<L>(i, k, width) ? (float)from[i + place<L>(k)] : 0.f;
+}
+template <Lay L>
+__device__ __forceinline__ void load_any(const void *vector, int dtype, int i, int width, float (&v)[8]) {
+    if (dtype == JQ_BF16) load_elements<L, __nv_bfloat16>(vector, i, width, v);
+    else if (dtype == JQ_F16) load_elements<L, __half>(vector, i, width, v);
+    else load_elements<L, float>(vector, i, width, v);
+}
+
+// Two fp32 operations in one instruction, each rounded as by itself
+struct Two { float x, y; };
+__device__ __forceinline__ Two add2(Two a, Two b) {
+    asm("{ .reg .b64 a, b; mov.b64 a, {%0, %1}; mov.b64 b, {%2, %3}; add.rn.f32x2 a, a, b; mov.b64 {%0, %1}, a; }" : "+f"(a.x), "+f"(a.y) : "f"(b.x), "f"(b.y));
+    return a;
+}
+__device__ __forceinline__ Two fma2(Two a, float f, Two c) {             // a * f + c
+    asm("{ .reg .b64 a, c, f; mov.b64 a, {%0, %1}; mov.b64 f, {%4, %4}; mov.b64 c, {%2, %3}; fma.rn.f32x2 a, a, f, c; mov.b64 {%0, %1}, a; }"
+        : "+f"(a.x), "+f"(a.y) : "f"(c.x), "f"(c.y), "f"(f));
+    return a;
 }
 
 // Rotation of 128 neighbours: 16 / A lanes with 8 A of them each, in the order of stages (strides 1, 2, .., 64; sums in the lower place,
-// differences in the upper) of fwht128_warp, so that both give the same bits.  Between lanes a stage is one shuffle and one fused
-// multiply-add with 1 or -1, which rounds as the sum or the difference does.  The shuffles bound it: four per value at A = 1, two at A = 4.
+// differences in the upper) of fwht128_warp, so that both give the same bits.  Differences, and sums between lanes, are fused multiply-adds
+// with 1 or -1, which round as the sum or the difference does, so that all stages but the first take two values at once.
+// The shuffles bound it: four per value at A = 1, two at A = 4.
 template <int A>
 __device__ __forceinline__ void rotate128(float (&v)[A][8], int lane) {
+    Two t[4 * A];
 #pragma unroll
-    for (int m = 1; m < 8 * A; m <<= 1)
+    for (int i = 0; i < 4 * A; ++i) {
+        const float a = v[i >> 2][2 * i & 7], b = v[i >> 2][(2 * i + 1) & 7];
+        t[i] = Two{a + b, a - b};
+    }
 #pragma unroll
-        for (int j = 0; j < 8 * A; ++j)
-            if (!(j & m)) {
-                const float a = v[j >> 3][j & 7], b = v[(j | m) >> 3][(j | m) & 7];
-                v[j >> 3][j & 7] = a + b;
-                v[(j | m) >> 3][(j | m) & 7] = a - b;
+    for (int m = 1; m < 4 * A; m <<= 1)
+#pragma unroll
+        for (int i = 0; i < 4 * A; ++i)
+            if (!(i & m)) {
+                const Two a = t[i], b = t[i | m];
+                t[i] = add2(a, b);
+                t[i | m] = fma2(b, -1.f, a);
             }
 #pragma unroll
     for (int m = 1; m < 16 / A; m <<= 1) {
         const float sign = (lane & m) ? -1.f : 1.f;
 #pragma unroll
-        for (int j = 0; j < 8 * A; ++j) v[j >> 3][j & 7] = fmaf(v[j >> 3][j & 7], sign, __shfl_xor_sync(0xffffffffu, v[j >> 3][j & 7], m));
+        for (int i = 0; i < 4 * A; ++i) {
+            const Two o{__shfl_xor_sync(0xffffffffu, t[i].x, m), __shfl_xor_sync(0xffffffffu, t[i].y, m)};
+            t[i] = fma2(t[i], sign, o);
+        }
     }
 #pragma unroll
-    for (int j = 0; j < 8 * A; ++j) v[j >> 3][j & 7] *= 0.08838834764831845f;
+    for (int i = 0; i < 4 * A; ++i) {
+        v[i >> 2][2 * i & 7] = t[i].x * 0.08838834764831845f;
+        v[i >> 2][(2 * i + 1) & 7] = t[i].y * 0.08838834764831845f;
+    }
 }
 
 // Bits of the largest |v|; NaN is above infinity.
@@ -108,6 +228,17 @@ __device__ __forceinline__ uint32_t largest_bits(const float (&v)[8]) {
 #pragma unroll
     for (int j = 0; j < 8; ++j) m = max(m, __float_as_uint(v[j]) & 0x7fffffffu);
     return m;
+}
+// The same of rotated values, a NaN or an infinity told by infinity: a block of 128 that holds one has no finite value left, and
+// where all are NaN the first one is.
+template <int A>
+__device__ __forceinline__ uint32_t largest_rotated(const float (&v)[A][8]) {
+    float m = 0.f;
+#pragma unroll
+    for (int j = 0; j < A; ++j)
+#pragma unroll
+        for (int k = 0; k < 8; ++k) m = fmaxf(m, fabsf(v[j][k]));
+    return v[0][0] != v[0][0] ? kInf : __float_as_uint(m);
 }
 // The same of values as they lie
 __device__ __forceinline__ uint32_t largest_bits(const Raw8<float> &r) {
@@ -157,16 +288,31 @@ struct Coder {
         return good ? r : 0u;
     }
     __device__ __forceinline__ uint2 eight(const float (&v)[8]) const { return make_uint2(four(v[0], v[1], v[2], v[3]), four(v[4], v[5], v[6], v[7])); }
-    __device__ __forceinline__ void store(int8_t *row, int c, const Places &at, const float (&v)[8]) const {
-        const int i = at.first(c);
+    // Codes of eight neighbours from i on
+    __device__ __forceinline__ void store(int8_t *row, int i, int width, const float (&v)[8]) const {
         const uint2 q = eight(v);
-        if (at.next == 1) {
-            if (i < at.width) *reinterpret_cast<uint2 *>(row + i) = q;
-        } else {
+        if (i + 8 <= width) *reinterpret_cast<uint2 *>(row + i) = q;
+        else
 #pragma unroll
             for (int k = 0; k < 8; ++k)
-                if (i + k * 32 < at.width) row[i + k * 32] = (int8_t)((k < 4 ? q.x : q.y) >> 8 * (k & 3));
+                if (i + k < width) row[i + k] = (int8_t)((k < 4 ? q.x : q.y) >> 8 * (k & 3));
+    }
+    // of a chunk that lies as L says
+    template <Lay L>
+    __device__ __forceinline__ void store_as(int8_t *row, int i, int width, const float (&v)[8]) const {
+        const uint2 q = eight(v);
+        if (L == kPieces) {
+            if (i < width) *reinterpret_cast<uint2 *>(row + i) = q;
+            return;
         }
+        const bool all = whole<L>(i, width);
+#pragma unroll
+        for (int k = 0; k < 8; k += L == kPairs ? 2 : 1)
+            if (all || inside<L>(i, k, width)) {
+                const uint32_t b = (k < 4 ? q.x : q.y) >> 8 * (k & 3);
+                if (L == kPairs) *reinterpret_cast<uint16_t *>(row + i + place<L>(k)) = (uint16_t)b;
+                else row[i + place<L>(k)] = (int8_t)b;
+            }
     }
 };
 
@@ -201,10 +347,11 @@ constexpr int kMostKept = 32768;       // longest row that a block keeps in regi
 
 struct Cut { int chunks, threads; };   // threads 0: a warp per row
 
+inline int chunks_of(int width, Lay l) { return l == kPieces ? (width + 7) / 8 : (width + 255) / 256 * 32; }
+
 // A row's chunks over threads.  Up to 128 chunks a warp has them all and needs no barrier; longer rows have a block, with `many` chunks
 // per thread (loads in flight together, few warps at the barriers) unless rows are so few that latency counts: then one.
-inline Cut cut_of(int width, bool neighbours, int rows, int sms, int many) {
-    const int chunks = neighbours ? (width + 7) / 8 : (width + 255) / 256 * 32;
+inline Cut cut_of(int chunks, int rows, int sms, int many) {
     if (chunks <= 128 && (rows > 2 * sms || chunks <= 32)) return Cut{(chunks + 31) / 32, 0};
     const int per = chunks > 2048 ? 4 : rows > 2 * sms || chunks > 1024 ? many : 1;
     const int threads = ((chunks + per - 1) / per + 31) / 32 * 32;

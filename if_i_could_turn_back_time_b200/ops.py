@@ -509,11 +509,19 @@ def _row_stride(K: int) -> int:
 
 def _new(shape, dtype, device, padded: int = 0) -> torch.Tensor:
     """An uninitialised tensor; with ``padded`` its rows lie that many elements apart.  (torch.empty takes a microsecond longer.)"""
-    if len(shape) == 2:
-        return torch.empty_strided(shape, (padded or shape[1], 1), dtype=dtype, device=device)
-    if len(shape) == 1 or not padded:
+    dims = len(shape)
+    if dims == 2:
+        strides = (padded or shape[1], 1)
+    elif dims == 3:
+        row = padded or shape[2]
+        strides = (shape[1] * row, row, 1)
+    elif dims == 1:
+        strides = (1,)
+    elif not padded:
         return torch.empty(shape, dtype=dtype, device=device)
-    return torch.empty((*shape[:-1], padded), dtype=dtype, device=device)[..., :shape[-1]]
+    else:
+        return torch.empty((*shape[:-1], padded), dtype=dtype, device=device)[..., :shape[-1]]
+    return torch.empty_strided(shape, strides, dtype=dtype, device=device)
 
 
 def _codes_of(rows: QuantizedRows):
@@ -549,19 +557,29 @@ def _codes_of(rows: QuantizedRows):
     return codes, scales, K, stride
 
 
-def _rows_of(x: torch.Tensor, what: str):
-    """x [..., K] as (tensor [n, K], elements between rows): rows of one stride, values adjacent."""
+def _rows_of(x: torch.Tensor, K: int, what: str):
+    """x [..., K] as rows of one stride with adjacent values: (tensor that has them, rows, elements between rows)."""
     if x.is_neg():
         x = x.resolve_neg()
-    if x.dim() != 2:
-        x = x.reshape(-1, x.shape[-1])
-    n, K = x.shape
-    row, one = x.stride()
-    if one != 1 and K > 1:
-        x = x.contiguous()
-        row = K
+    if x.is_contiguous():
+        n, row = x.numel() // K, K
+    else:
+        if x.dim() != 2:
+            x = x.reshape(-1, K)
+        n = x.shape[0]
+        row, one = x.stride()
+        if one != 1 and K > 1:
+            x = x.contiguous()
+            row = K
     if n > 0x7fffffff:
         raise RuntimeError(f"{n} rows of {what}: the library counts in 32 bits")
+    return x, n, row
+
+
+def _pieces(x: torch.Tensor, K: int, row: int):
+    """Rows (K a multiple of 128) that are to be rotated, of 16-byte pieces: a copy where they are not."""
+    if x.data_ptr() % 16 or row * x.element_size() % 16:
+        return x.clone(memory_format=torch.contiguous_format), K
     return x, row
 
 
@@ -582,11 +600,12 @@ def quantize_rows(x: torch.Tensor, had_block: int = 0) -> QuantizedRows:
         raise RuntimeError(f"unsupported dtype {dtype} of x")
     if not x.is_cuda:
         _need_cuda(x)
-    x, row = _rows_of(x, "x")
+    x, n, row = _rows_of(x, K, "x")
+    if had_block:
+        x, row = _pieces(x, K, row)
     device, stride = x.device, _row_stride(K)
     codes = _new(shape, torch.int8, device, stride)
-    scales = torch.empty(shape[:-1], dtype=torch.float32, device=device)
-    n = x.shape[0]
+    scales = _new(shape[:-1], torch.float32, device)
     if n:
         with _on(device):
             st = _lib.load().jq_quantize_rows(x.data_ptr(), row, n, K, had_block, _DT[dtype], codes.data_ptr(), stride, scales.data_ptr(), _stream())
@@ -704,17 +723,16 @@ def residual_norm(x: torch.Tensor, residual: Optional[torch.Tensor] = None, weig
         raise RuntimeError("a post_bias comes with a post_weight")
     if not (0 <= eps <= 3.4e38 and -3.4e38 <= scale <= 3.4e38):
         raise RuntimeError("scale is a finite number of fp32, eps one from 0 on")
-    given, at, wdtype, one = [x], [0, 0, 0, 0], None, (width,)
-    for i, t in enumerate((weight, bias, post_weight, post_bias)):
+    given, vectors, wdtype, one = [x], [weight, bias, post_weight, post_bias], None, (width,)
+    for i, t in enumerate(vectors):
         if t is None:
             continue
         if t.shape != one or t.dtype not in _DT or t.dtype is not (wdtype or t.dtype):
             raise RuntimeError(f"weights and biases are tensors [{width}] of one dtype; got {tuple(t.shape)} {t.dtype}")
         wdtype = t.dtype
         if not t.is_contiguous() or t.is_neg():
-            t = t.resolve_neg().contiguous()
+            vectors[i] = t = t.resolve_neg().contiguous()
         given.append(t)
-        at[i] = t.data_ptr()
     rdtype = dtype
     if residual is not None:
         rdtype = residual.dtype
@@ -734,17 +752,29 @@ def residual_norm(x: torch.Tensor, residual: Optional[torch.Tensor] = None, weig
         if grad and t.requires_grad:
             raise RuntimeError("residual_norm has no backward pass: call it under torch.no_grad()")
     device = x.device
-    x2, stride_x = _rows_of(x, "x")
+    x2, rows, stride_x = _rows_of(x, width, "x")
     res_at = stride_res = stride_q = out_at = r_at = codes_at = scales_at = 0
     if residual is not None:
-        residual, stride_res = _rows_of(residual, "the residual")
+        residual, _, stride_res = _rows_of(residual, width, "the residual")
         res_at = residual.data_ptr()
-    gate_at = outer = inner = flat = gdtype = 0
+    outer = inner = flat = gdtype = 0
     each = 1
     if gate is not None:
         gdtype = _DT[gate.dtype]
         gate, outer, inner, each, flat = _gate_of(gate.resolve_neg(), shape)
-        gate_at = gate.data_ptr()
+    if had_block:
+        # rows that are to be rotated, and the vectors with them, are of 16-byte pieces, and vectors of x's type or fp32
+        x2, stride_x = _pieces(x2, width, stride_x)
+        if residual is not None:
+            residual, stride_res = _pieces(residual, width, stride_res)
+            res_at = residual.data_ptr()
+        if any(t is not None and (t.data_ptr() % 16 or (wdtype is not dtype and wdtype is not torch.float32)) for t in vectors):
+            vectors, wdtype = [None if t is None else t.to(torch.float32, copy=True) for t in vectors], torch.float32
+        if gate is not None and not flat:
+            size = gate.element_size()
+            if gate.data_ptr() % 16 or outer * size % 16 or inner * size % 16 or (gate.dtype is not dtype and gate.dtype is not torch.float32):
+                gate = gate.expand(shape).to(torch.float32, copy=True).contiguous()
+                gdtype, outer, inner, each = _lib.JQ_F32, width, 0, 1
     if residual is None and gate is None and scale == 1.0 and post_weight is None:
         r = x
     else:
@@ -753,15 +783,14 @@ def residual_norm(x: torch.Tensor, residual: Optional[torch.Tensor] = None, weig
     if quantize:
         stride_q = _row_stride(width)
         codes = _new(shape, torch.int8, device, stride_q)
-        scales = torch.empty(shape[:-1], dtype=torch.float32, device=device)
+        scales = _new(shape[:-1], torch.float32, device)
         codes_at, scales_at = codes.data_ptr(), scales.data_ptr()
         h = QuantizedRows(codes, scales, dtype, had_block)
     else:
         h = _new(shape, dtype, device)
         out_at = h.data_ptr()
-    rows = x2.shape[0]
     if rows:
-        packed = _pack_norm(x2.data_ptr(), res_at, *at, gate_at, out_at, r_at, codes_at, scales_at, stride_x, stride_res, stride_q, outer, inner,
+        packed = _pack_norm(x2.data_ptr(), res_at, *[0 if t is None else t.data_ptr() for t in vectors], 0 if gate is None else gate.data_ptr(), out_at, r_at, codes_at, scales_at, stride_x, stride_res, stride_q, outer, inner,
                             rows, width, each, flat, post_weight is not None, _NORM_KINDS[kind], had_block, _DT[dtype], _DT[rdtype],
                             _DT[wdtype] if wdtype else 0, gdtype, scale, eps, 0)
         with _on(device):

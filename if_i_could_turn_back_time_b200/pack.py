@@ -119,7 +119,7 @@ def _pack_int8(W: torch.Tensor, spec: QuantSpec, threads: int, rotate: bool) -> 
     q = torch.zeros((N, row_stride_codes(K)), dtype=torch.int8, device=W.device)
     if W.is_cuda:
         from . import ops
-        rows = ops.quantize_rows(W.detach(), spec.had_block if rotate else 0)
+        rows = ops.quantize_rows(W.detach().float(), spec.had_block if rotate else 0)
         q[:, :K] = rows.codes
         return PackedWeight(spec, N, K, q, rows.scales, None)
     Wf = W.detach().to(torch.float32).contiguous()

@@ -424,7 +424,8 @@ int jq_token_logprobs(const void *logits, int64_t row_stride, int rows, int voca
  * jq_quantize_rows: x [rows, K] of x_dtype, rows row_stride elements apart (0: the same row again), rotated first where had_block is
  * 128 (K % 128 == 0; the bits of jq_fwht_block):
  *   scale = max(|x|, 2^-100) / 127,  code = x / scale to the nearest integer, ties to even  (both quotients rounded to fp32);
- * a row with a NaN or an infinity has the scale NaN and codes 0.  One launch, as jq_dequantize_rows (out [rows, K] = code * scale). */
+ * a row with a NaN or an infinity has the scale NaN and codes 0.  Rows that are rotated are of 16-byte pieces (x and row_stride).  One launch
+ * (for every 65535 rows, where a row has more than a warp), as jq_dequantize_rows (out [rows, K] = code * scale). */
 #define JQ_INT8_MAX_K 131071
 int jq_quantize_rows(const void *x, int64_t row_stride, int rows, int K, int had_block, int x_dtype, void *codes,
                      int64_t code_stride, float *scales, jq_stream_t stream);
@@ -448,7 +449,7 @@ int jq_int8_matmul(const void *qweight, const float *scales, const void *codes, 
  * nobody wants it.  h is [rows, width] of x_dtype, or, where codes is given, h rotated (had_block 128) and quantised as by jq_quantize_rows into
  * codes and scales.  r is [rows, width] of residual_dtype, which is x_dtype or F32.  x and residual have rows a stride apart, h and r are
  * contiguous.  gate: row i's is at gate + (i / gate_inner_rows) gate_outer + (i % gate_inner_rows) gate_inner, `width` values, or one
- * for the whole row (gate_one).  weight, bias, post_weight and post_bias are of weight_dtype.  h, r and codes overlap no input.  One launch.  The
+ * for the whole row (gate_one).  With had_block every tensor and stride is of 16-byte pieces, and the vectors are of x_dtype or F32.  weight, bias, post_weight and post_bias are of weight_dtype.  h, r and codes overlap no input.  One launch.  The
  * reference has no norm (its models are vision networks and an MLP, Python_Jenks_Test/Jenks_Tests/QuantNetworkTest.py). */
 #define JQ_NORM_RMS 0
 #define JQ_NORM_LAYER 1

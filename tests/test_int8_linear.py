@@ -62,7 +62,7 @@ def _weight(N, K, seed=0, had=0):
 @gpu
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("rows,K", [(1, 1), (3, 7), (5, 8), (2, 31), (70, 100), (9, 256), (1, 1000), (400, 1000), (6, 1024), (400, 1032), (1, 8192), (301, 4100),
-                                    (500, 4096), (3, 32768), (2, 32776), (300, 11008), (2, 131071)])
+                                    (500, 4096), (3, 32768), (2, 32776), (300, 11008), (400, 12296), (3, 28672), (2, 98304), (2, 131064), (2, 131071), (66000, 1100)])
 def test_codes_are_those_of_the_definition(rows, K, dtype):
     gen = torch.Generator(DEV).manual_seed(rows + K)
     x = torch.randn(rows, K, device=DEV, generator=gen)
@@ -80,7 +80,7 @@ def test_codes_are_those_of_the_definition(rows, K, dtype):
 
 @gpu
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("rows,K", [(1, 128), (400, 128), (7, 384), (600, 1024), (3, 4096), (330, 11008), (2, 32768), (3, 33024)])
+@pytest.mark.parametrize("rows,K", [(1, 128), (400, 128), (7, 384), (600, 1024), (3, 4096), (330, 11008), (300, 12416), (2, 32768), (3, 33024), (5, 130944)])
 def test_rotated_codes(rows, K, dtype):
     """The rotation has the bits of ops.fwht_block."""
     x = torch.randn(rows, K, device=DEV, generator=torch.Generator(DEV).manual_seed(K)).to(dtype)
@@ -88,6 +88,10 @@ def test_rotated_codes(rows, K, dtype):
     got = ops.quantize_rows(x, had_block=128)
     q, s = _codes(ops.fwht_block(x, 128))
     assert got.had_block == 128 and torch.equal(got.scales.cpu(), s) and torch.equal(got.codes.cpu(), q)
+    wide = torch.empty(rows, K + 3, dtype=dtype, device=DEV)[:, 3:]                  # rows that are not of 16-byte pieces
+    wide.copy_(x)
+    again = ops.quantize_rows(wide, 128)
+    assert torch.equal(again.scales, got.scales) and torch.equal(again.codes, got.codes)
 
 
 @gpu
@@ -342,6 +346,7 @@ def test_refusals_of_the_library():
         assert lib.jq_quantize_rows(p, K, rows, K, had, 0, p, stride, p, None) == -2
     assert lib.jq_quantize_rows(p, 8, 1, 8, 0, 3, p, 32, p, None) == -4
     assert lib.jq_quantize_rows(p, 8, 1, 8, 0, 0, p + 8, 32, p, None) == -3 and lib.jq_quantize_rows(p, 8, 1, 8, 0, 0, p, 24, p, None) == -3
+    assert lib.jq_quantize_rows(p + 4, 128, 1, 128, 128, 0, p, 128, p, None) == -3 and lib.jq_quantize_rows(p, 130, 2, 128, 128, 0, p, 128, p, None) == -3
     assert lib.jq_dequantize_rows(p, 24, p, 1, 8, p, 0, None) == -3 and lib.jq_dequantize_rows(p, 32, p, 1, 8, p, 5, None) == -4
     assert lib.jq_int8_scratch_bytes(3, 100) == 256 + 3 * 128 and lib.jq_int8_scratch_bytes(0, 4) == 0
     assert lib.jq_int8_linear(p, p, p, None, p, 4, 8, 1, 0, 0, 0, p, 8, p, None) == -6

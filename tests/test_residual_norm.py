@@ -134,6 +134,20 @@ def test_gates_of_every_shape(width):
 
 
 @gpu
+def test_rotated_rows_of_every_layout():
+    """Rows that are to be rotated are copied where they are not of 16-byte pieces, vectors where they are of another 16-bit type."""
+    x, res, (w, b, pw, pb) = _inputs((6, 50, 256), torch.float16)
+    same = ops.residual_norm(x, res, w, b, post_weight=pw, gate=pb, quantize=True, had_block=128)
+    wide = lambda t: torch.empty(*t.shape[:-1], t.shape[-1] + 3, dtype=t.dtype, device=DEV)[..., 3:].copy_(t)                  # noqa: E731
+    for args in ((wide(x), wide(res), wide(w), wide(b), wide(pw), wide(pb)), (x, wide(res), w, b, pw, pb), (x, res, w, b, pw, wide(pb.expand(6, 50, 256))),
+                 (x, res, wide(w), b, pw, pb), (x.transpose(0, 1).contiguous().transpose(0, 1), res, w, b, pw, pb)):
+        got = ops.residual_norm(args[0], args[1], args[2], args[3], post_weight=args[4], gate=args[5], quantize=True, had_block=128)
+        assert torch.equal(got.r, same.r) and torch.equal(got.h.codes, same.h.codes) and torch.equal(got.h.scales, same.h.scales)
+    _check(x, res, w.bfloat16(), b.bfloat16(), gate=pb.bfloat16(), had=128)
+    _check(x, res, w.float(), gate=pb.bfloat16().view(1, 1, 256).expand(6, 1, 256), had=128)
+
+
+@gpu
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_strides_leading_dims_and_alignment(dtype):
     raw = torch.randn(3, 50, 700, device=DEV).to(dtype)
@@ -268,6 +282,7 @@ def test_refusals_of_the_library():
     assert lib.jq_residual_norm(None, None) == -1 and call(x=None) == -1 and call(h=None) == -1 and call(codes=p) == -1
     assert call(rows=0) == -2 and call(width=0) == -2 and call(width=32769) == -2 and call(had_block=128) == -2 and call(gate=p, gate_inner_rows=0) == -2
     assert call(codes=p, scales=p, stride_codes=48) == -2 and call(codes=p, scales=p, stride_codes=72) == -3 and call(codes=p + 4, scales=p, stride_codes=64) == -3
+    assert call(codes=p, scales=p, stride_codes=128, width=128, had_block=128, x=p + 4) == -3
     assert call(x_dtype=3) == -4 and call(residual_dtype=1) == -4 and call(weight_dtype=-1) == -4 and call(kind=2) == -5
 
 
