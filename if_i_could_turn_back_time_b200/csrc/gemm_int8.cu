@@ -18,6 +18,7 @@ struct GemmArgs {
     int *status;
     int N, T, steps, split, y_dtype, vec, early;
     int tiles_t, tiles_n, band;        // of a pair of CTAs
+    int piece;                         // bytes that rows of y are multiples of: 16, 8, 4 or 2
 };
 
 // K-major operand tile in shared memory, 128-byte swizzle: atoms of 8 rows x 128 bytes, 1024 bytes apart
@@ -245,7 +246,6 @@ __device__ __forceinline__ void commit_pair(uint32_t elected, uint32_t bar, uint
 __device__ __forceinline__ void arrive_cluster(uint32_t cluster_bar) {
     asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_bar) : "memory");
 }
-__device__ __forceinline__ float lds_f32(uint32_t a) { return __uint_as_float(lds32(a)); }
 
 template <class T> __device__ __forceinline__ uint32_t pack2(float a, float b);
 template <> __device__ __forceinline__ uint32_t pack2<__half>(float a, float b) {
@@ -257,11 +257,40 @@ template <> __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float a, fl
     return *reinterpret_cast<const uint32_t *>(&h);
 }
 
+// 64 bytes of 32 rows from a warp's shared memory into rows of y, in pieces of W bytes that rows of y are multiples of
+template <int W>
+__device__ __forceinline__ void store_rows(const GemmArgs &p, uint32_t out, int t0, int nb, int row_bytes, int lane) {
+    constexpr int kLanes = 64 / W, kRows = 32 / kLanes;
+    const int b = nb + lane % kLanes * W;
+    const uint32_t from = out + lane / kLanes * kPitch + lane % kLanes * W;
+    unsigned char *y = reinterpret_cast<unsigned char *>(p.y) + (size_t)(t0 + lane / kLanes) * row_bytes + b;
+    const int left = p.T - t0 - lane / kLanes;
+#pragma unroll 8
+    for (int i = 0; i < 32; i += kRows) {
+        const bool in = i < left && b < row_bytes;
+        if constexpr (W == 16) {
+            const uint4 u = lds128(from + i * kPitch);
+            if (in) *reinterpret_cast<uint4 *>(y) = u;
+        } else if constexpr (W == 8) {
+            uint2 u;
+            asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(u.x), "=r"(u.y) : "r"(from + i * kPitch));
+            if (in) *reinterpret_cast<uint2 *>(y) = u;
+        } else if constexpr (W == 4) {
+            const uint32_t u = lds32(from + i * kPitch);
+            if (in) *reinterpret_cast<uint32_t *>(y) = u;
+        } else {
+            unsigned short u;
+            asm volatile("ld.shared.u16 %0, [%1];" : "=h"(u) : "r"(from + i * kPitch));
+            if (in) *reinterpret_cast<unsigned short *>(y) = u;
+        }
+        y += (size_t)kRows * row_bytes;
+    }
+}
+
 // 32 columns of a warp's 32 tokens (a token per lane): scaled, turned in shared memory 64 bytes of a row at a time, and written as rows
 template <class T>
 __device__ __forceinline__ void write32(const GemmArgs &p, const uint32_t (&r)[32], uint32_t out, uint32_t scales, uint32_t biases, float ts, int t0, int n0, int lane) {
     constexpr int kCols = 64 / (int)sizeof(T);
-    T *const y = reinterpret_cast<T *>(p.y);
 #pragma unroll
     for (int half = 0; half < 32 / kCols; ++half) {
         float v[kCols];
@@ -291,31 +320,11 @@ __device__ __forceinline__ void write32(const GemmArgs &p, const uint32_t (&r)[3
             asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(row + 16 * q), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
         }
         __syncwarp();
-        const int n = n0 + half * kCols;
-        if (p.vec) {                                   // rows of y are 16-byte aligned: four lanes write a row's 64 bytes
-            const int cn = n + (lane & 3) * (kCols / 4);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int t = i * 8 + (lane >> 2);
-                const uint4 u = lds128(out + t * kPitch + (lane & 3) * 16);
-                if (t0 + t < p.T && cn < p.N) *reinterpret_cast<uint4 *>(y + (size_t)(t0 + t) * p.N + cn) = u;
-            }
-        } else {
-            const int cn = n + lane % kCols;
-#pragma unroll 4
-            for (int i = 0; i < 32; i += 32 / kCols) {
-                const int t = i + lane / kCols;
-                T e;
-                if constexpr (sizeof(T) == 4) {
-                    e = lds_f32(out + t * kPitch + (lane % kCols) * 4);
-                } else {
-                    unsigned short u;
-                    asm volatile("ld.shared.u16 %0, [%1];" : "=h"(u) : "r"(out + t * kPitch + (lane % kCols) * 2));
-                    e = *reinterpret_cast<const T *>(&u);
-                }
-                if (t0 + t < p.T && cn < p.N) y[(size_t)(t0 + t) * p.N + cn] = e;
-            }
-        }
+        const int nb = (n0 + half * kCols) * (int)sizeof(T), row_bytes = p.N * (int)sizeof(T);
+        if (p.piece == 16) store_rows<16>(p, out, t0, nb, row_bytes, lane);
+        else if (p.piece == 8) store_rows<8>(p, out, t0, nb, row_bytes, lane);
+        else if (p.piece == 4) store_rows<4>(p, out, t0, nb, row_bytes, lane);
+        else if constexpr (sizeof(T) == 2) store_rows<2>(p, out, t0, nb, row_bytes, lane);
     }
 }
 
@@ -384,6 +393,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
         __syncwarp();
     };
     auto write = [&](const uint32_t (&r)[32], int c, float ts, int t0, int n0) {      // c: among the warp's columns
+        if (t0 >= p.T || n0 + c >= p.N) return;
         if (p.y_dtype == JQ_F32) write32<float>(p, r, out, scales + c * 4, biases + c * 4, ts, t0, n0 + c, lane);
         else if (p.y_dtype == JQ_F16) write32<__half>(p, r, out, scales + c * 4, biases + c * 4, ts, t0, n0 + c, lane);
         else write32<__nv_bfloat16>(p, r, out, scales + c * 4, biases + c * 4, ts, t0, n0 + c, lane);
@@ -545,30 +555,40 @@ static int encode(CUtensorMap *map, const void *base, int rows, int K, int64_t s
 
 struct Form { bool pair; int tile, split; };   // tile: tokens of a single CTA's tile, channels of a pair's
 
-static Form choose_form(int N, int T, int steps, int sms) {
+// Which kernel, tile and split of K, by a model of the time in us: what a launch, a tile's outputs, a stage of 128 values of K and an exchange
+// between CTAs take.  Its constants are fitted to 1600 timed calls (17 numbers of tokens up to 10000, 14 matrices from 100 x 300 to
+// 32000 x 2048 and 28672 x 8192, every form): the choice is 1.0 % behind the best form on average, 15 % at most.  Both sides of its turns, us:
+//   4096 x 4096         T = 64    single CTAs of 64 tokens, K in eight parts 9.5    pairs of 128 channels 11.0
+//                       T = 256   single 14.1 (128 tokens, four parts)              pairs of 128 channels, two parts 11.0, one 11.5
+//                       T = 1024  single 19.9                                       pairs of 128 18.6, of 256 17.1
+//   28672 x 8192        T = 64    single 44                                         pairs of 256 52
+//                       T = 200   single 82                                         pairs of 256 55
+//   100 x 300           T = 512   single, 32 tokens 4.1                             pairs of 128 5.3
+static Form choose_form(int N, int K, int T, int steps, int sms) {
     Form best{false, 16, 1};
     double least = 0;
     auto offer = [&](bool pair, int tile, int split, double us) {
         if (least == 0 || us < least) { best = Form{pair, tile, split}; least = us; }
     };
     for (int nt = 16; nt <= 128; nt *= 2) {
-        if ((T <= nt / 2 && nt > 16) || (nt < 64 && T > nt)) continue;
+        // (tiles of 32 tokens for more than 32 only where the weights are next to nothing)
+        if ((T <= nt / 2 && nt > 16) || (T > nt && (nt < 32 || (nt == 32 && (long long)N * K >= 600000)))) continue;
         const long long tiles = (long long)((N + kTileN - 1) / kTileN) * ((T + nt - 1) / nt);
         for (int s = 1; s <= 8; s = s == 4 ? 8 : s + 1) {
-            const long long ctas = tiles * s, room = s == 8 ? sms / 18 * 32 : 2 * sms;
-            if (s > steps || (s > 1 && ctas > room)) break;
+            const long long ctas = tiles * s, room = s == 8 ? sms / 18 * 32 : 2 * sms;      // (clusters of eight: two in the 16 or 18 SMs of a GPC, twice)
+            if (s > steps || (ctas > room && (s > 1 || T > 64))) break;
             const double turns = (double)(ctas / room * 2 + (ctas % room + sms - 1) / sms);       // CTAs that an SM has, one behind another
-            offer(false, nt, s, 3.0 + 0.0234 * nt + turns * ((steps + s - 1) / s) * (0.144 + 0.0012 * nt) + (s > 1 ? 0.0123 * nt : 0.0));
+            offer(false, nt, s, 2.16 + 0.030 * nt + turns * ((steps + s - 1) / s) * (0.2045 + 0.0008 * nt) + (s > 1 ? 0.034 * nt : 0.0));
         }
     }
     if (T > 64)
         for (int bn = 256; bn >= 128; bn /= 2) {
             const long long tiles = (long long)((N + bn - 1) / bn) * ((T + 255) / 256);
-            for (int s = 1; s <= bn / 64; s *= 2) {
+            for (int s = 1; s <= bn / 64; s *= 2) {                                            // (32 columns for each of a CTA's output warps at least)
                 const long long room = s == 1 ? sms / 2 : sms / 18 * (s == 2 ? 4 : 2);
                 if (s > steps || (s > 1 && tiles > room)) break;
                 const double waves = (double)((tiles + room - 1) / room);
-                offer(true, bn, s, 2.7 + bn / 128 * (1.0 + 0.65 * waves + (s > 1 ? 1.1 : 0.0)) + waves * ((steps + s - 1) / s) * (bn == 256 ? 0.286 : 0.2));
+                offer(true, bn, s, 2.78 + bn / 128 * (0.22 + 1.25 * waves + (s > 1 ? 2.68 : 0.0)) + waves * ((steps + s - 1) / s) * (bn == 256 ? 0.294 : 0.207));
             }
         }
     return best;
@@ -610,7 +630,8 @@ static int launch_pair(GemmArgs &a, const void *w, int64_t w_stride, const void 
     a.tiles_t = (a.T + 255) / 256;
     a.tiles_n = (a.N + BN - 1) / BN;
     a.band = 16;
-    a.vec = a.N * (a.y_dtype == JQ_F32 ? 4 : 2) % 16 == 0 && jq_aligned16(a.y);
+    const uintptr_t rows = reinterpret_cast<uintptr_t>(a.y) | (uintptr_t)a.N * (a.y_dtype == JQ_F32 ? 4 : 2);
+    a.piece = rows % 16 == 0 ? 16 : rows % 8 == 0 ? 8 : rows % 4 == 0 ? 4 : 2;
     static jq_contexts done;
     auto kern = gemm_int8_pair_kernel<BN>;
     JQ_CUDA_TRY(jq_allow_smem(reinterpret_cast<const void *>(kern), Pair<BN>::kSmem, done));
@@ -641,7 +662,7 @@ static int multiply(const void *w, const float *cs, const void *x, int64_t x_str
     a.y_dtype = y_dtype; a.early = early;
     a.vec = N % 4 == 0 && (reinterpret_cast<uintptr_t>(y) & (y_dtype == JQ_F32 ? 15u : 7u)) == 0;
     const int64_t ws = jq_row_stride_codes(K);
-    const Form f = choose_form(N, T, a.steps, jq_sm_count());
+    const Form f = choose_form(N, K, T, a.steps, jq_sm_count());
     a.split = f.split;
     if (f.pair) return f.tile == 256 ? launch_pair<256>(a, w, ws, x, x_stride, K, st) : launch_pair<128>(a, w, ws, x, x_stride, K, st);
     if (f.tile == 16) return launch<16>(a, w, ws, x, x_stride, K, st);
@@ -652,7 +673,7 @@ static int multiply(const void *w, const float *cs, const void *x, int64_t x_str
 
 static int check(const void *w, const float *cs, const void *y, const int *status, int N, int K, int B, int y_dtype) {
     if (!w || !cs || !y || !status) return JQ_ERR_NULL_PTR;
-    if (N <= 0 || K <= 0 || B <= 0 || K > JQ_INT8_MAX_K) return JQ_ERR_BAD_SHAPE;
+    if (N <= 0 || K <= 0 || B <= 0 || K > JQ_INT8_MAX_K || N > (1 << 28)) return JQ_ERR_BAD_SHAPE;
     if ((B + 255) / 256 > 65535) return JQ_ERR_BAD_SHAPE;
     if (y_dtype < 0 || y_dtype > 2) return JQ_ERR_BAD_DTYPE;
     const uintptr_t off = reinterpret_cast<uintptr_t>(y) & (y_dtype == JQ_F32 ? 3u : 1u);
