@@ -1,6 +1,7 @@
-"""A small decoder of packed 4-bit layers that answers with alternatives: the prompt goes through in one pass, then token by token.
+"""A small decoder of packed 4-bit or 8-bit layers that answers with alternatives: the prompt goes through in one pass, then token by token.
 
-Its matrices are ``JenksQuantLinear`` layers, what its attention reads lies in a ``KVCache`` of 8 bits per layer, and every
+Its matrices are ``JenksQuantLinear`` layers, the sums and norms between its blocks ``ops.residual_norm`` (with int8 weights it writes
+the rows of 8-bit integers that several products share), what its attention reads lies in a ``KVCache`` of 8 bits per layer, and every
 position's log probability, entropy and strongest alternatives come from ``ops.token_logprobs``.  Weights are random: what
 it shows is how the calls fit together, with sequences of different lengths in one batch.
 
@@ -28,13 +29,16 @@ class Layer(nn.Module):
         self.k, self.v = (nn.Linear(hidden, kv_heads * self.dim, bias=False) for _ in range(2))
         self.up, self.down = nn.Linear(hidden, ffn, bias=False), nn.Linear(ffn, hidden, bias=False)
 
-    def forward(self, x, cache, table, lengths, starts, max_new):
-        h = F.rms_norm(x, x.shape[-1:])
+    def forward(self, x, block, cache, table, lengths, starts, max_new):
+        """(residual stream, what the last block adds to it) -> the same behind this layer."""
+        int8 = getattr(self.q, "spec", None) is not None and self.q.spec.fmt == "int8"
+        h, x = ops.residual_norm(x, quantize=int8) if block is None else ops.residual_norm(block, x, quantize=int8)
         q = self.q(h).view(-1, self.heads, self.dim)
         k, v = self.k(h).view(-1, self.kv_heads, self.dim), self.v(h).view(-1, self.kv_heads, self.dim)
         cache.append(k, v, table, lengths, starts, max_new)
-        x = x + self.o(cache.attend(q, table, lengths, starts, max_new).view(x.shape))
-        return x + self.down(F.silu(self.up(F.rms_norm(x, x.shape[-1:]))))
+        block = self.o(cache.attend(q, table, lengths, starts, max_new).view(x.shape))
+        h, x = ops.residual_norm(block, x, quantize=int8)
+        return x, self.down(F.silu(self.up(h)))
 
 
 class Decoder(nn.Module):
@@ -46,15 +50,15 @@ class Decoder(nn.Module):
 
     def forward(self, tokens, caches, table, lengths, starts, max_new):
         """Logits of the new tokens [tokens], which the sequences' lengths count already."""
-        x = self.embed(tokens)
+        x, block = self.embed(tokens), None
         for layer, cache in zip(self.layers, caches):
-            x = layer(x, cache, table, lengths, starts, max_new)
-        return self.head(F.rms_norm(x, x.shape[-1:]))
+            x, block = layer(x, block, cache, table, lengths, starts, max_new)
+        return self.head(ops.residual_norm(block, x).h)
 
 
 def packed(model, fmt="gf4"):
-    """The model with every Linear as packed 4-bit weights, on the GPU in bf16."""
-    model = jq.quantize_module(model, 4, fmt=fmt, group_size=128 if fmt == "gf4" else 32).to("cuda")
+    """The model with every Linear as packed 4-bit weights (or int8 ones), on the GPU in bf16."""
+    model = jq.quantize_module(model, 8 if fmt == "int8" else 4, fmt=fmt, group_size={"gf4": 128, "e2m1": 32, "int8": 0}[fmt]).to("cuda")
     for m in model.modules():
         if isinstance(m, jq.JenksQuantLinear):
             m.commit()
@@ -98,7 +102,7 @@ def main(argv=None):
     ap = argparse.ArgumentParser(description=__doc__, formatter_class=argparse.RawDescriptionHelpFormatter)
     for name, default in (("layers", 2), ("hidden", 512), ("heads", 8), ("kv-heads", 2), ("ffn", 1024), ("vocab", 4000), ("new", 8)):
         ap.add_argument("--" + name, type=int, default=default)
-    ap.add_argument("--weights", choices=("gf4", "e2m1"), default="gf4")
+    ap.add_argument("--weights", choices=("gf4", "e2m1", "int8"), default="gf4")
     ap.add_argument("--cache", choices=("int8", "e4m3"), default="int8")
     a = ap.parse_args(argv)
     torch.manual_seed(0)

@@ -674,7 +674,6 @@ static int multiply(const void *w, const float *cs, const void *x, int64_t x_str
 static int check(const void *w, const float *cs, const void *y, const int *status, int N, int K, int B, int y_dtype) {
     if (!w || !cs || !y || !status) return JQ_ERR_NULL_PTR;
     if (N <= 0 || K <= 0 || B <= 0 || K > JQ_INT8_MAX_K || N > (1 << 28)) return JQ_ERR_BAD_SHAPE;
-    if ((B + 255) / 256 > 65535) return JQ_ERR_BAD_SHAPE;
     if (y_dtype < 0 || y_dtype > 2) return JQ_ERR_BAD_DTYPE;
     const uintptr_t off = reinterpret_cast<uintptr_t>(y) & (y_dtype == JQ_F32 ? 3u : 1u);
     return !jq_aligned16(w) || (reinterpret_cast<uintptr_t>(cs) & 3u) || off ? JQ_ERR_BAD_ALIGN : JQ_OK;

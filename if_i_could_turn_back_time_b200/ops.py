@@ -396,7 +396,7 @@ def _on(device):
 def _linear_rows(x2, qweight, scales, codebook, bias, fmt_id, N, K, g, had, out_id=-1):
     lib = _lib.load()
     Bt = x2.shape[0]
-    y = torch.empty((Bt, N), dtype=_OUT[out_id] or x2.dtype, device=x2.device)
+    y = _new((Bt, N), _OUT[out_id] or x2.dtype, x2.device)
     if fmt_id == _lib.JQ_FMT_INT8:
         return _linear_int8(x2, qweight, scales, bias, N, K, had, y)
     if many_rows(fmt_id, K, g, Bt):
