@@ -45,6 +45,9 @@ template <class T> struct Piece {
 // A warp (kThreads 0) or a block per row, which stays in registers from the first read to the last write:
 //   u = N(x) post_weight + post_bias (or x),  r = residual + scale * (gate * u),  h = N(r) weight + bias,
 // N(v) = v / sqrt(mean(v^2) + eps), or of v - mean(v).  All in fp32; h follows from r as it was before its rounding.
+// Bound by memory: 8191 x 4096 with both norms and an fp32 stream 69 us (5.8 TB/s), 50432 x 768 fp16 with a gate for each image 63 (4.9), 50000 x
+// 197 23, 4000 x 5025 44 (3.6: one-element loads).  Two chunks a thread and code without paths that a call does not take are what did it (four chunks,
+// every alignment and type in one kernel: 104, 72, 69 and 79; instructions waited for the instruction cache).
 // kPieces: every row and vector is of 16-byte pieces, and vectors are of T or fp32; kPairs: rows are of pairs; kScattered: any width, alignment,
 // stride and type.
 template <class T, class R, int kChunks, int kThreads, Lay L>

@@ -22,8 +22,9 @@ enum Mode {
 };
 
 // A warp (kThreads 0), a block or a cluster of blocks per row, which stays in registers between its maximum and its codes.
-// 8191 x 11008 bf16: 53 us straight (5.1 TB/s), 68 rotated, where instructions bind (seven additions, two shuffles and four instructions of
-// encoding per value; with a thread's chunks apart and the stages' sums one by one 100).
+// 8191 x 11008 bf16: 53 us straight (5.1 TB/s), 68 rotated, where instructions bind (17 per value: seven additions, two shuffles, four of
+// encoding; issue slots 65 % busy, the L1 71 %; with a thread's chunks apart and the stages' sums one by one 100), 95 at 11007 values, where pieces
+// are read twice and shifted (by elements 167).  64 x 8192: 2.8 us, nearly all of it the launch and two barriers.
 template <class T, int kChunks, int kThreads, Mode kMode>
 __global__ void __launch_bounds__(kThreads ? kThreads : 256, kThreads == 384 ? (kMode == kStraight ? 4 : 3) : 1) quantize_kernel(const __grid_constant__ QuantArgs p) {
     constexpr bool kBlock = kThreads != 0;
