@@ -128,6 +128,7 @@ __global__ void __launch_bounds__(kThreads) gemm_int8_kernel(const __grid_consta
     } else if (warp == 5) {
         const uint32_t elected = elect_one();
         constexpr uint32_t idesc = idesc_i8(kTileN, NT);
+        pdl_wait();                                        // (the bounded waits do not count the kernel in front of this one)
         int s = 0;
         uint32_t par = 0;
         bool ok = true;
@@ -443,6 +444,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
             const uint32_t elected = elect_one();
             constexpr uint32_t idesc = idesc_i8(256, BN);
             const uint32_t both = 3u << leader;
+            pdl_wait();                                    // (the bounded waits do not count the kernel in front of this one)
             auto wait = [&](uint32_t bar, uint32_t parity) -> bool { return __all_sync(0xffffffffu, mbar_wait(bar, parity, err)); };
             int s = 0, a = 0;
             uint32_t par = 0, a_par = 1;                   // (the first wait on free sums passes at once)
@@ -562,7 +564,7 @@ static int encode(CUtensorMap *map, const void *base, int rows, int K, int64_t s
 struct Form { bool pair; int tile, split; };   // tile: tokens of a single CTA's tile, channels of a pair's
 
 // Which kernel, tile and split of K, by a model of the time in us: what a launch, a tile's outputs, a stage of 128 values of K and an exchange
-// between CTAs take.  Its constants are fitted to 1600 timed calls (17 numbers of tokens up to 10000, 14 matrices from 100 x 300 to
+// between CTAs take.  Its constants are fitted to 2524 timed calls (18 numbers of tokens up to 10000, 14 matrices from 100 x 300 to
 // 32000 x 2048 and 28672 x 8192, every form): the choice is 1.0 % behind the best form on average, 15 % at most.  Both sides of its turns, us:
 //   4096 x 4096         T = 64    single CTAs of 64 tokens, K in eight parts 9.5    pairs of 128 channels 11.0
 //                       T = 256   single 14.1 (128 tokens, four parts)              pairs of 128 channels, two parts 11.0, one 11.5

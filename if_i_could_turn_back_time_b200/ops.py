@@ -628,8 +628,21 @@ def _int8_weight(device, qweight, scales, bias, N, K):
     return bias if bias.is_contiguous() and not bias.is_neg() else bias.resolve_neg().contiguous()
 
 
+def _int8_scratch(lib, device, nbytes: int):
+    """(tensor to keep, scratch address, size, status word) of an int8 call.  While a graph is captured both outlast the call without
+    a buffer of the stream's: scratch from the graph's pool, the library's own status word."""
+    if _capturing(_stream()):
+        own = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+        return own, _addr(own), nbytes, lib.jq_status_word()
+    if not nbytes:
+        return None, None, 0, _workspace(device, 1024, "ta").data_ptr()
+    return _rows_scratch(device, nbytes)
+
+
 def _linear_int8(x2, qweight, scales, bias, N, K, had, y):
     device = x2.device
+    if had and x2.data_ptr() % 16:                         # (rows that are to be rotated are read in 16-byte pieces)
+        x2 = x2.clone()
     bias = _int8_weight(device, qweight, scales, bias, N, K)
     lib = _lib.load()
     rows, stride = x2.shape[0], _row_stride(K)
@@ -638,7 +651,7 @@ def _linear_int8(x2, qweight, scales, bias, N, K, had, y):
         for b0 in range(0, rows, part):
             b1 = min(rows, b0 + part)
             xs, ys = (x2, y) if rows <= part else (x2[b0:b1], y[b0:b1])
-            own, scratch, size, status = _rows_scratch(device, ((b1 - b0) * 4 + 255) // 256 * 256 + (b1 - b0) * stride)
+            own, scratch, size, status = _int8_scratch(lib, device, ((b1 - b0) * 4 + 255) // 256 * 256 + (b1 - b0) * stride)
             st = lib.jq_int8_linear(qweight.data_ptr(), scales.data_ptr(), xs.data_ptr(), _addr(bias), ys.data_ptr(), N, K, b1 - b0, had,
                                     _DT[x2.dtype], _DT[y.dtype], scratch, size, status, _stream())
             if st:
@@ -670,8 +683,9 @@ def _linear_quantized(x: QuantizedRows, pw: PackedWeight, bias, out_dtype) -> to
     rows = codes.shape[0]
     if rows:
         with _on(device):
-            status = _workspace(device, 1024, "ta").data_ptr()
-            st = _lib.load().jq_int8_matmul(pw.qweight.data_ptr(), pw.scales.data_ptr(), codes.data_ptr(), stride, scales.data_ptr(),
+            lib = _lib.load()
+            status = _int8_scratch(lib, device, 0)[3]
+            st = lib.jq_int8_matmul(pw.qweight.data_ptr(), pw.scales.data_ptr(), codes.data_ptr(), stride, scales.data_ptr(),
                                             _addr(bias), y.data_ptr(), N, K, rows, _DT[dtype], status, _stream())
         if st:
             _lib.check(st, "jq_int8_matmul")
@@ -705,7 +719,8 @@ def residual_norm(x: torch.Tensor, residual: Optional[torch.Tensor] = None, weig
     and rounded once: ``h`` to x's dtype, ``r`` to the residual's (x's or fp32).  h follows from r before its rounding.  The
     weights and biases are [width] of one dtype; the gate has any shape that broadcasts to x's: a channel's, a sequence's, a token's.
     With ``quantize`` h comes as ``QuantizedRows`` (rotated with ``had_block`` 128) for int8 linears, without passing through 16
-    bits.  Without residual, gate, scale and post_weight ``r`` is x.  Widths up to 32768.  Serving only: an input that asks for a gradient is
+    bits.  Without residual, gate, scale and post_weight ``r`` is x.  Widths up to 32768; a row of values above some 10^18, the
+    sum of whose squares leaves fp32, is normed to zeros, as by fp32 operations one by one.  Serving only: an input that asks for a gradient is
     refused while gradients are recorded.
 
     The reference has no norm (its models are the vision networks and the MLP of Python_Jenks_Test/Jenks_Tests/QuantNetworkTest.py)."""

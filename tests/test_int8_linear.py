@@ -246,6 +246,46 @@ def test_rotated_linear_undoes_the_weights_rotation(rows):
 
 
 @gpu
+@pytest.mark.parametrize("rows", [1, 33, 300])
+def test_rotated_linear_of_values_anywhere(rows):
+    """A contiguous activation that does not begin at a 16-byte boundary."""
+    pw = _weight(72, 256, had=128)
+    flat = torch.randn(rows * 256 + 1, device=DEV).bfloat16()
+    x = flat[1:].view(rows, 256)
+    assert torch.equal(ops.linear(x, pw), ops.linear(x.clone(), pw)) and torch.equal(ops.linear(x, _weight(72, 256)), ops.linear(x.clone(), _weight(72, 256)))
+
+
+@gpu
+def test_captured_before_any_other_call():
+    """A thread and stream that have no scratch buffer yet: the captured calls' own outlast them."""
+    import threading
+    pw = _weight(200, 384)
+    x = torch.randn(300, 384, device=DEV)
+    rows8, found = ops.quantize_rows(x), []
+    want = ops.linear(x, pw)
+    torch.cuda.synchronize()
+
+    def work():
+        stream = torch.cuda.Stream()
+        with torch.cuda.stream(stream):
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph, stream=stream):
+                a, b = ops.linear(x, pw), ops.linear(rows8, pw)
+            more = ops.linear(x[:3], pw)
+            for _ in range(2):
+                a.zero_()
+                b.zero_()
+                graph.replay()
+            stream.synchronize()
+            found.extend([a.clone(), b.clone(), more.clone(), ops.check_status(raise_on_error=False)])
+
+    t = threading.Thread(target=work)
+    t.start()
+    t.join()
+    assert torch.equal(found[0], want) and torch.equal(found[1], want) and torch.equal(found[2], want[:3]) and found[3] == 0
+
+
+@gpu
 def test_rows_of_codes_that_lie_otherwise():
     pw = _weight(70, 200)
     x = torch.randn(4, 6, 200, device=DEV)
