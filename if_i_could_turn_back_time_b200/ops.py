@@ -396,9 +396,9 @@ def _on(device):
 def _linear_rows(x2, qweight, scales, codebook, bias, fmt_id, N, K, g, had, out_id=-1):
     lib = _lib.load()
     Bt = x2.shape[0]
-    y = _new((Bt, N), _OUT[out_id] or x2.dtype, x2.device)
     if fmt_id == _lib.JQ_FMT_INT8:
-        return _linear_int8(x2, qweight, scales, bias, N, K, had, y)
+        return _linear_int8(x2, qweight, scales, bias, N, K, had, _OUT[out_id] or x2.dtype)
+    y = _new((Bt, N), _OUT[out_id] or x2.dtype, x2.device)
     if many_rows(fmt_id, K, g, Bt):
         return _linear_many_rows(x2, qweight, scales, codebook, bias, fmt_id, N, K, g, had, y)
     if ta_eligible(fmt_id, K, g, Bt):
@@ -470,6 +470,8 @@ def linear(x, pw: PackedWeight, bias: Optional[torch.Tensor] = None,
         # through the dispatcher so that tracing sees one opaque op with a fake implementation
         return torch.ops.jq.linear(x, pw.qweight, pw.scales, pw.codebook, bias, pw.spec.fmt_id, pw.N, pw.K,
                                    pw.spec.group_size, pw.spec.had_block, out_id)
+    if pw.spec.fmt == "int8":
+        return _linear_int8(x, pw.qweight, pw.scales, bias, pw.N, pw.K, pw.spec.had_block, out_dtype or x.dtype)
     flat = x.dim() == 2
     x2 = x if flat else x.reshape(-1, pw.K)
     if not x2.is_contiguous():
@@ -492,8 +494,7 @@ class QuantizedRows(NamedTuple):
         dtype = dtype or self.dtype
         if dtype not in _DT:
             raise RuntimeError(f"unsupported dtype {dtype}")
-        codes, scales, K, stride = _codes_of(self)
-        rows = codes.shape[0]
+        codes, scales, rows, K, stride = _codes_of(self)
         out = _new(self.codes.shape, dtype, codes.device)
         if rows:
             with _on(codes.device):
@@ -525,7 +526,7 @@ def _new(shape, dtype, device, padded: int = 0) -> torch.Tensor:
 
 
 def _codes_of(rows: QuantizedRows):
-    """(codes [n, K], scales [n], K, elements between rows of codes), looked over and laid out as the library takes them."""
+    """(codes [n, K], scales [n], n, K, elements between rows of codes), looked over and laid out as the library takes them."""
     codes, scales = rows.codes, rows.scales
     shape = codes.shape
     if codes.dtype is not torch.int8 or not shape or scales.dtype is not torch.float32 or scales.shape != shape[:-1]:
@@ -533,19 +534,17 @@ def _codes_of(rows: QuantizedRows):
     K = shape[-1]
     if not 0 < K <= _lib.JQ_INT8_MAX_K:
         raise RuntimeError(f"rows of {K} codes: 1 to {_lib.JQ_INT8_MAX_K}")
-    if not codes.is_cuda or not scales.is_cuda:
+    index = codes.get_device()
+    if index < 0 or scales.get_device() != index:
         _need_cuda(codes, scales)
-    if scales.get_device() != codes.get_device():
         raise RuntimeError(f"codes are on {codes.device}, scales on {scales.device}")
     if len(shape) != 2:
         codes = codes.reshape(-1, K)
     n = codes.shape[0]
     if n > 0x7fffffff:
         raise RuntimeError(f"{n} rows: the library counts in 32 bits")
-    if scales.is_neg():
-        scales = scales.resolve_neg()
-    if not scales.is_contiguous():
-        scales = scales.contiguous()
+    if scales.is_neg() or not scales.is_contiguous():
+        scales = scales.resolve_neg().contiguous()
     stride, one = codes.stride()
     if n == 1:
         stride = _row_stride(K)
@@ -554,7 +553,7 @@ def _codes_of(rows: QuantizedRows):
         laid = _new((n, K), torch.int8, codes.device, stride)
         laid.copy_(codes)
         codes = laid
-    return codes, scales, K, stride
+    return codes, scales, n, K, stride
 
 
 def _rows_of(x: torch.Tensor, K: int, what: str):
@@ -614,59 +613,75 @@ def quantize_rows(x: torch.Tensor, had_block: int = 0) -> QuantizedRows:
     return QuantizedRows(codes, scales, dtype, had_block)
 
 
-def _int8_weight(device, qweight, scales, bias, N, K):
-    """Refuses tensors that are not an int8 weight as the library takes it; the bias as it takes that."""
-    if qweight.dtype is not torch.int8 or qweight.shape != (N, _row_stride(K)) or not qweight.is_contiguous() or \
-            scales is None or scales.dtype is not torch.float32 or scales.shape != (N,) or not scales.is_contiguous():
+def _int8_weight(index, qweight, scales, bias, N, K):
+    """Refuses tensors that are not an int8 weight as the library takes it, on that device; the bias as it takes that."""
+    if scales is None or qweight.dtype is not torch.int8 or scales.dtype is not torch.float32 or qweight.shape != (N, _row_stride(K)) or \
+            scales.shape != (N,) or not qweight.is_contiguous() or not scales.is_contiguous():
         raise RuntimeError(f"an int8 weight is int8 [{N}, {_row_stride(K)}] with fp32 scales [{N}], contiguous")
-    if qweight.device != device or scales.device != device or (bias is not None and bias.device != device):
-        raise RuntimeError(f"the activation is on {device}, the weight, its scales or the bias elsewhere")
+    if qweight.get_device() != index or scales.get_device() != index:
+        raise RuntimeError(f"the activation is on cuda:{index}, the weight or its scales elsewhere")
     if bias is None:
         return None
     if bias.shape != (N,):
         raise RuntimeError(f"bias {tuple(bias.shape)}: [{N}]")
+    if bias.get_device() != index:
+        raise RuntimeError(f"the activation is on cuda:{index}, the bias on {bias.device}")
+    if bias.dtype is not torch.float32:
+        bias = bias.float()
     return bias if bias.is_contiguous() and not bias.is_neg() else bias.resolve_neg().contiguous()
 
 
-def _int8_scratch(lib, device, nbytes: int):
+def _int8_scratch(lib, device, index: int, stream: int, nbytes: int):
     """(tensor to keep, scratch address, size, status word) of an int8 call.  While a graph is captured both outlast the call without
     a buffer of the stream's: scratch from the graph's pool, the library's own status word."""
-    if _capturing(_stream()):
+    if _capturing(stream):
         own = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
         return own, _addr(own), nbytes, lib.jq_status_word()
-    if not nbytes:
-        return None, None, 0, _workspace(device, 1024, "ta").data_ptr()
-    return _rows_scratch(device, nbytes)
+    ws = _ws_cache().get((index, stream, "ta"))
+    if ws is None:
+        ws = _workspace(device, 1024, "ta")
+    at, size = ws.data_ptr(), ws.numel()
+    if size >= 1024 + nbytes:
+        return None, at + 1024, size - 1024, at
+    own = torch.empty(nbytes, dtype=torch.uint8, device=device)
+    return own, own.data_ptr(), nbytes, at
 
 
-def _linear_int8(x2, qweight, scales, bias, N, K, had, y):
-    device = x2.device
-    if had and x2.data_ptr() % 16:                         # (rows that are to be rotated are read in 16-byte pieces)
-        x2 = x2.clone()
-    bias = _int8_weight(device, qweight, scales, bias, N, K)
-    lib = _lib.load()
-    rows, stride = x2.shape[0], _row_stride(K)
+def _linear_int8(x, qweight, scales, bias, N, K, had, dtype):
+    """[..., N] of x [..., K], which is quantised first."""
+    index = x.get_device()
+    if index != torch._C._cuda_getDevice():
+        with torch.cuda.device(index):
+            return _linear_int8(x, qweight, scales, bias, N, K, had, dtype)
+    bias = _int8_weight(index, qweight, scales, bias, N, K)
+    if x.is_neg() or not x.is_contiguous():
+        x = x.resolve_neg().contiguous()
+    if had and x.data_ptr() % 16:                          # (rows that are to be rotated are read in 16-byte pieces)
+        x = x.clone()
+    shape, device = x.shape, x.device
+    y = _new((*shape[:-1], N), dtype, device)
+    rows, stride = x.numel() // K, _row_stride(K)
+    lib, raw = _lib.load(), torch._C._cuda_getCurrentRawStream(index)
     part = max(256, MAX_ROWS_SCRATCH // stride // 256 * 256)
-    with _on(device):
-        for b0 in range(0, rows, part):
-            b1 = min(rows, b0 + part)
-            xs, ys = (x2, y) if rows <= part else (x2[b0:b1], y[b0:b1])
-            own, scratch, size, status = _int8_scratch(lib, device, ((b1 - b0) * 4 + 255) // 256 * 256 + (b1 - b0) * stride)
-            st = lib.jq_int8_linear(qweight.data_ptr(), scales.data_ptr(), xs.data_ptr(), _addr(bias), ys.data_ptr(), N, K, b1 - b0, had,
-                                    _DT[x2.dtype], _DT[y.dtype], scratch, size, status, _stream())
-            if st:
-                _lib.check(st, "jq_int8_linear")
-            del own
+    for b0 in range(0, rows, part):
+        n = min(rows - b0, part)
+        own, scratch, size, status = _int8_scratch(lib, device, index, raw, (n * 4 + 255) // 256 * 256 + n * stride)
+        st = lib.jq_int8_linear(qweight.data_ptr(), scales.data_ptr(), x.data_ptr() + b0 * K * x.element_size() if b0 else x.data_ptr(), _addr(bias),
+                                y.data_ptr() + b0 * N * y.element_size() if b0 else y.data_ptr(), N, K, n, had, _DT[x.dtype], _DT[dtype], scratch,
+                                size, status, raw)
+        if st:
+            _lib.check(st, "jq_int8_linear")
+        del own
     if _checked:
         check_status()
     return y
 
 
 def _linear_quantized(x: QuantizedRows, pw: PackedWeight, bias, out_dtype) -> torch.Tensor:
-    spec = pw.spec
+    spec, N = pw.spec, pw.N
     if spec.fmt != "int8":
         raise RuntimeError(f"rows of 8-bit integers multiply int8 weights, not {spec.fmt}")
-    codes, scales, K, stride = _codes_of(x)
+    codes, scales, rows, K, stride = _codes_of(x)
     if K != pw.K:
         raise RuntimeError(f"rows of {K} codes, packed weight has K={pw.K}")
     if x.had_block != spec.had_block:
@@ -675,18 +690,17 @@ def _linear_quantized(x: QuantizedRows, pw: PackedWeight, bias, out_dtype) -> to
     if dtype not in _DT:
         raise RuntimeError(f"unsupported output dtype {dtype}")
     _need_cuda(pw.qweight, pw.scales, bias)
-    if bias is not None and bias.dtype != torch.float32:
-        bias = bias.float()
-    device, N = codes.device, pw.N
-    bias = _int8_weight(device, pw.qweight, pw.scales, bias, N, K)
+    index = codes.get_device()
+    if index != torch._C._cuda_getDevice():
+        with torch.cuda.device(index):
+            return _linear_quantized(x, pw, bias, out_dtype)
+    bias = _int8_weight(index, pw.qweight, pw.scales, bias, N, K)
+    device = codes.device
     y = _new((*x.codes.shape[:-1], N), dtype, device)
-    rows = codes.shape[0]
     if rows:
-        with _on(device):
-            lib = _lib.load()
-            status = _int8_scratch(lib, device, 0)[3]
-            st = lib.jq_int8_matmul(pw.qweight.data_ptr(), pw.scales.data_ptr(), codes.data_ptr(), stride, scales.data_ptr(),
-                                            _addr(bias), y.data_ptr(), N, K, rows, _DT[dtype], status, _stream())
+        lib, raw = _lib.load(), torch._C._cuda_getCurrentRawStream(index)
+        st = lib.jq_int8_matmul(pw.qweight.data_ptr(), pw.scales.data_ptr(), codes.data_ptr(), stride, scales.data_ptr(), _addr(bias), y.data_ptr(),
+                                N, K, rows, _DT[dtype], _int8_scratch(lib, device, index, raw, 0)[3], raw)
         if st:
             _lib.check(st, "jq_int8_matmul")
         if _checked:
