@@ -21,12 +21,16 @@ enum Mode {
     kAnywhere     // rows that begin anywhere
 };
 
+// Blocks that an SM is to hold.  Both sides, us: 8191 x 11008 rotated, 74 with four and 68 with three; 8191 x 11007, 82 and 96; 20000 x 1024 rotated, a
+// warp per row, 16 with four and 18 unbounded.
+constexpr int blocks_of(int threads, bool rotated) { return threads == 0 ? 4 : threads == 384 ? (rotated ? 3 : 4) : threads == 512 ? 2 : 1; }
+
 // A warp (kThreads 0), a block or a cluster of blocks per row, which stays in registers between its maximum and its codes.
 // 8191 x 11008 bf16: 53 us straight (5.1 TB/s), 68 rotated, where instructions bind (17 per value: seven additions, two shuffles, four of
-// encoding; issue slots 65 % busy, the L1 71 %; with a thread's chunks apart and the stages' sums one by one 100), 95 at 11007 values, where pieces
+// encoding; issue slots 65 % busy, the L1 71 %; with a thread's chunks apart and the stages' sums one by one 100), 82 at 11007 values, where pieces
 // are read twice and shifted (by elements 167).  64 x 8192: 2.8 us, nearly all of it the launch and two barriers.
 template <class T, int kChunks, int kThreads, Mode kMode>
-__global__ void __launch_bounds__(kThreads ? kThreads : 256, kThreads == 384 ? (kMode == kStraight ? 4 : 3) : 1) quantize_kernel(const __grid_constant__ QuantArgs p) {
+__global__ void __launch_bounds__(kThreads ? kThreads : 256, blocks_of(kThreads, kMode == kRotated)) quantize_kernel(const __grid_constant__ QuantArgs p) {
     constexpr bool kBlock = kThreads != 0;
     __shared__ Shared sh;
     __shared__ uint32_t s_top;
@@ -214,9 +218,12 @@ static int launch_quantize(QuantArgs &a, bool vec, bool rotate, cudaStream_t st)
         c = Cut{4, ((chunks + 31) / 32 + 31) / 32 * 32};
         k = rotate ? quantize_kernel<T, 4, kLong, kRotated> : vec ? quantize_kernel<T, 4, kLong, kStraight> : quantize_kernel<T, 4, kLong, kAnywhere>;
     } else if (rotate) {
-        if (c.threads == 0) c.chunks = c.chunks == 1 ? 1 : 4;
-        k = c.threads == 0 ? (c.chunks == 1 ? quantize_kernel<T, 1, 0, kRotated> : quantize_kernel<T, 4, 0, kRotated>)
+        k = c.threads == 0 ? (c.chunks == 1 ? quantize_kernel<T, 1, 0, kRotated> : c.chunks == 2 ? quantize_kernel<T, 2, 0, kRotated> : quantize_kernel<T, 4, 0, kRotated>)
                            : (c.chunks == 1 ? quantize_kernel<T, 1, 1024, kRotated> : c.threads <= 384 ? quantize_kernel<T, 4, 384, kRotated> : quantize_kernel<T, 4, 1024, kRotated>);
+    } else if (vec && sizeof(T) == 2 && chunks > 1536 && a.rows > 2 * sms) {
+        // (eight chunks a thread, so that an SM holds two blocks: 4096 x 28672 bf16 71 us, in one block of 896 threads 97)
+        c = Cut{8, ((chunks + 7) / 8 + 31) / 32 * 32};
+        k = quantize_kernel<T, 8, 512, kStraight>;
     } else if (vec) {
         k = c.threads == 0 ? (c.chunks == 1 ? quantize_kernel<T, 1, 0, kStraight> : c.chunks == 2 ? quantize_kernel<T, 2, 0, kStraight> :
                               c.chunks == 3 ? quantize_kernel<T, 3, 0, kStraight> : quantize_kernel<T, 4, 0, kStraight>)
