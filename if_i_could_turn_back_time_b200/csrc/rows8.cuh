@@ -229,16 +229,16 @@ __device__ __forceinline__ uint32_t largest_bits(const float (&v)[8]) {
     for (int j = 0; j < 8; ++j) m = max(m, __float_as_uint(v[j]) & 0x7fffffffu);
     return m;
 }
-// The same of rotated values, a NaN or an infinity told by infinity: a block of 128 that holds one has no finite value left, and
-// where all are NaN the first one is.
+// The same of rotated values, by a maximum that keeps a NaN: one may come up beside finite values where the rotation's sums leave fp32's range
+// (infinities of one sign that meet), with no infinity left in the block.
 template <int A>
 __device__ __forceinline__ uint32_t largest_rotated(const float (&v)[A][8]) {
     float m = 0.f;
 #pragma unroll
     for (int j = 0; j < A; ++j)
 #pragma unroll
-        for (int k = 0; k < 8; ++k) m = fmaxf(m, fabsf(v[j][k]));
-    return v[0][0] != v[0][0] ? kInf : __float_as_uint(m);
+        for (int k = 0; k < 8; ++k) asm("max.NaN.f32 %0, %0, %1;" : "+f"(m) : "f"(fabsf(v[j][k])));
+    return __float_as_uint(m) & 0x7fffffffu;
 }
 // The same of values as they lie
 __device__ __forceinline__ uint32_t largest_bits(const Raw8<float> &r) {

@@ -527,3 +527,49 @@ def test_the_example_decoder_with_int8_weights():
         assert len(p) == 1 or (scored[at:at + len(p) - 1] - want[:len(p) - 1]).abs().max().item() < 0.2
         at += len(p)
         assert (logprobs[i, :, 0] - want[len(p) - 1:]).abs().max().item() < 0.2
+
+
+# ------------------------------------------------------------------------------------------- rotations that leave fp32's range
+
+def _overflowing(rows, K, dtype):
+    """Rows of which some have a NaN or an infinity, and some leave fp32's range only within the rotation."""
+    x = torch.randn(rows, K, device=DEV, generator=torch.Generator(DEV).manual_seed(K)).to(dtype)
+    top = min(torch.finfo(dtype).max, 3e38)
+    signs = torch.tensor([1, -1, 1, -1, 1, -1, -1, 1], device=DEV, dtype=torch.float32)
+    x[0] = 0
+    x[0, :8] = (top * signs).to(dtype)                              # odd places end as NaN, even ones as 0, none as an infinity
+    x[1] = (top * signs).to(dtype).repeat(K // 8)
+    x[2, K // 2] = torch.nan
+    x[3, K - 1] = torch.inf
+    x[4, 0], x[4, 1] = torch.inf, -torch.inf
+    x[5] = top
+    x[6] = 0
+    x[6, K - 8:] = (top * signs).to(dtype)                          # the last block only
+    x[7, ::2] = -top
+    return x
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,K", [(8, 128), (400, 256), (400, 512), (8, 1024), (400, 1024), (9, 4096), (400, 4096), (8, 16384), (400, 16384), (8, 33024)])
+def test_rotated_rows_that_go_wrong(rows, K, dtype):
+    """What the rotation makes of a row decides: a NaN or an infinity among its values, also one that only the rotation's sums make of
+    finite values, gives the scale NaN and codes 0, and the product's row is NaN."""
+    x = _overflowing(rows, K, dtype)
+    got = ops.quantize_rows(x, 128)
+    q, s = _codes(ops.fwht_block(x, 128))
+    assert _same(got.scales.cpu(), s) and torch.equal(got.codes.cpu(), q)
+    lost = [2, 3, 4] if dtype == torch.float16 else [0, 1, 2, 3, 4, 5, 6, 7]
+    assert torch.isnan(got.scales[lost]).all() and torch.isfinite(got.scales[8:]).all()
+    if K <= 4096:
+        y = ops.linear(x, _weight(40, K, had=128))
+        assert torch.isnan(y[lost]).all() and torch.isfinite(y[8:]).all()
+
+
+@gpu
+@pytest.mark.parametrize("K", [128, 1024])
+def test_rotated_weights_that_go_wrong_are_packed_as_on_the_cpu(K):
+    w = _overflowing(12, K, torch.float32)
+    spec = jq.QuantSpec("int8", 0, 128)
+    a, b = jq.pack_weight(w.cpu(), spec), jq.pack_weight(w, spec)
+    assert _same(a.scales, b.scales.cpu()) and torch.equal(a.qweight, b.qweight.cpu()) and torch.isnan(a.scales[:8]).all()

@@ -300,3 +300,16 @@ def test_refusals_on_the_gpu():
         ops.residual_norm(x, gate=torch.ones(1, 2, 64, device=DEV))
     with pytest.raises(RuntimeError, match="CUDA"):
         ops.residual_norm(x, gate=torch.ones(64))
+
+
+@gpu
+@pytest.mark.parametrize("width", [128, 1024, 8192])
+def test_rotations_that_leave_the_range(width):
+    """Normed values whose rotation leaves fp32's range: the row's scale is NaN, as by quantising the rotated values."""
+    signs = torch.tensor([1, -1, 1, -1, 1, -1, -1, 1], device=DEV, dtype=torch.float32)
+    x = torch.ones(5, width, device=DEV)
+    x[3] = torch.nan
+    for weight, lost in ((3e38 * signs.repeat(width // 8), [0, 1, 2, 3, 4]), (torch.full((width,), 3e38, device=DEV), [0, 1, 2, 3, 4]), (signs.repeat(width // 8), [3])):
+        rows = ops.residual_norm(x, weight=weight, quantize=True, had_block=128).h
+        assert torch.isnan(rows.scales[lost]).all() and bool((rows.codes[lost] == 0).all())
+        assert int(torch.isnan(rows.scales).sum()) == len(lost)
