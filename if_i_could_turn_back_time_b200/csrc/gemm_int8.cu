@@ -497,6 +497,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
         }
     } else {
         // sums -> shared memory, [column][token]: every stage has been read once the last instruction is done
+        pdl_wait();
         if (__all_sync(0xffffffffu, mbar_wait(ready(0), 0, err))) {
             tc_fence_after();
             const uint32_t to = ring + (quarter * 32 + lane) * 4;
@@ -514,7 +515,6 @@ __global__ void __launch_bounds__(kPairThreads, 1)
     if (p.split > 1) {
         cluster_sync();
         if (warp < 8 && !*err) {
-            pdl_wait();
             const int cols = BN / p.split / 2, c_lo = part * (BN / p.split) + side * cols;      // of this warp
             int t0, n0;
             place(first, t0, n0);

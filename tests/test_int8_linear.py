@@ -573,3 +573,56 @@ def test_rotated_weights_that_go_wrong_are_packed_as_on_the_cpu(K):
     spec = jq.QuantSpec("int8", 0, 128)
     a, b = jq.pack_weight(w.cpu(), spec), jq.pack_weight(w, spec)
     assert _same(a.scales, b.scales.cpu()) and torch.equal(a.qweight, b.qweight.cpu()) and torch.isnan(a.scales[:8]).all()
+
+
+# A kernel that lets what is behind it start at once and ends `ns` nanoseconds later, or after 4 million pauses
+_PAUSE = b"""
+.version 8.0
+.target sm_90
+.address_size 64
+.visible .entry pause(.param .u64 ns) {
+    .reg .u64 want, begin, now;
+    .reg .u32 i;
+    .reg .pred p;
+    ld.param.u64 want, [ns];
+    griddepcontrol.launch_dependents;
+    mov.u64 begin, %globaltimer;
+    mov.u32 i, 0;
+again:
+    nanosleep.u32 1000;
+    mov.u64 now, %globaltimer;
+    sub.u64 now, now, begin;
+    setp.ge.u64 p, now, want;
+    @p bra done;
+    add.u32 i, i, 1;
+    setp.lt.u32 p, i, 4000000;
+    @p bra again;
+done:
+    ret;
+}
+"""
+
+
+@gpu
+@pytest.mark.parametrize("rows,N,K", [(1, 256, 4096), (40, 300, 256), (256, 4096, 4096), (300, 512, 16384), (2000, 1000, 512)])
+def test_products_behind_a_kernel_that_lasts(rows, N, K):
+    """A product that starts while the kernel in front of it runs on for a second: its bounded waits (a quarter of a second) begin behind
+    that kernel, in the forms that share K too (4096 x 4096 of 256 rows)."""
+    import ctypes
+    pw = _weight(N, K)
+    rows8 = ops.quantize_rows(torch.randn(rows, K, device=DEV))
+    want = ops.linear(rows8, pw)
+    cuda, module, entry = ctypes.CDLL("libcuda.so.1"), ctypes.c_void_p(), ctypes.c_void_p()
+    assert cuda.cuModuleLoadData(ctypes.byref(module), ctypes.c_char_p(_PAUSE)) == 0
+    try:
+        assert cuda.cuModuleGetFunction(ctypes.byref(entry), module, b"pause") == 0
+        ns = ctypes.c_uint64(10 ** 9)
+        args = (ctypes.c_void_p * 1)(ctypes.cast(ctypes.byref(ns), ctypes.c_void_p))
+        stream = ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
+        torch.cuda.synchronize()
+        assert cuda.cuLaunchKernel(entry, 1, 1, 1, 32, 1, 1, 0, stream, args, None) == 0
+        y = ops.linear(rows8, pw)
+        torch.cuda.synchronize()
+        assert ops.check_status(raise_on_error=False) == 0 and torch.equal(y, want)
+    finally:
+        cuda.cuModuleUnload(module)
