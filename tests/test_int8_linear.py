@@ -626,3 +626,31 @@ def test_products_behind_a_kernel_that_lasts(rows, N, K):
         assert ops.check_status(raise_on_error=False) == 0 and torch.equal(y, want)
     finally:
         cuda.cuModuleUnload(module)
+
+
+@gpu
+@pytest.mark.parametrize("rows,N,K", [(1, 64, 256), (40, 64, 256), (400, 64, 256), (300, 4096, 4096), (2000, 2001, 256), (3000, 4096, 384)])
+def test_scales_whose_product_with_the_sum_leaves_the_range(rows, N, K):
+    """Channels so large that the sum times their scale is no number of fp32, tokens so small that the result is one.  Such channels
+    have one rounding more than others, the third of 2^-24 that the bound counts."""
+    gen = torch.Generator(DEV).manual_seed(N)
+    x = torch.randn(rows, K, device=DEV, generator=gen) * 1e-28
+    x[rows // 2] *= 1e-20                                           # below the least scale: codes 0
+    w = torch.randn(N, K, device=DEV, generator=gen)
+    w[::3] *= 1e36
+    w[1::3] *= 1e25
+    w[-1] = 3e38
+    bias = torch.randn(N, device=DEV, generator=gen)
+    pw = jq.pack_weight(w, jq.QuantSpec("int8", 0, 0))
+    rows8 = ops.quantize_rows(x)
+    for b in (None, bias):
+        y, bound = _product(rows8.codes, rows8.scales, pw, b, torch.float32)
+        assert y.abs().max().item() < 1e38
+        _near(ops.linear(rows8, pw, b), y, bound)
+    w[2], w[5] = torch.nan, torch.inf
+    rows8.scales[rows // 2] = torch.nan
+    pw = jq.pack_weight(w, jq.QuantSpec("int8", 0, 0))
+    y = ops.linear(rows8, pw)
+    good = torch.ones(N, dtype=torch.bool, device=DEV)
+    good[[2, 5]] = False
+    assert torch.isnan(y[:, [2, 5]]).all() and torch.isnan(y[rows // 2]).all() and torch.isfinite(y[:rows // 2][:, good]).all()
