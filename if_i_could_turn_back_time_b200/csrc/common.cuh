@@ -22,6 +22,9 @@ static inline int jq_launch_status() {
     return e == cudaSuccess ? JQ_OK : JQ_ERR_CUDA_BASE - (int)e;
 }
 
+// whether an array of elements of `size` bytes may begin there (null: it is not given)
+static inline bool jq_whole(const void *p, int size) { return (reinterpret_cast<uintptr_t>(p) & (size - 1)) == 0; }
+
 static inline bool jq_aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
 // Number of the calling thread's current CUDA context, from 1 on and never given twice by the driver; 0 if there is none or the

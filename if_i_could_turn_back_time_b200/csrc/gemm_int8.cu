@@ -719,12 +719,11 @@ static int multiply(const void *w, const float *cs, const void *x, int64_t x_str
     return launch<128>(a, w, ws, x, x_stride, K, st);
 }
 
-static int check(const void *w, const float *cs, const void *y, const int *status, int N, int K, int B, int y_dtype) {
+static int check(const void *w, const float *cs, const float *bias, const void *y, const int *status, int N, int K, int B, int y_dtype) {
     if (!w || !cs || !y || !status) return JQ_ERR_NULL_PTR;
     if (N <= 0 || K <= 0 || B <= 0 || K > JQ_INT8_MAX_K || N > (1 << 28)) return JQ_ERR_BAD_SHAPE;
     if (y_dtype < 0 || y_dtype > 2) return JQ_ERR_BAD_DTYPE;
-    const uintptr_t off = reinterpret_cast<uintptr_t>(y) & (y_dtype == JQ_F32 ? 3u : 1u);
-    return !jq_aligned16(w) || (reinterpret_cast<uintptr_t>(cs) & 3u) || off ? JQ_ERR_BAD_ALIGN : JQ_OK;
+    return jq_aligned16(w) && jq_whole(cs, 4) && jq_whole(bias, 4) && jq_whole(y, y_dtype == JQ_F32 ? 4 : 2) && jq_whole(status, 4) ? JQ_OK : JQ_ERR_BAD_ALIGN;
 }
 
 static size_t scale_room(int rows) { return ((size_t)rows * 4 + 255) / 256 * 256; }
@@ -741,7 +740,7 @@ extern "C" size_t jq_int8_scratch_bytes(int B, int K) {
 extern "C" int jq_int8_linear(const void *qweight, const float *scales, const void *x, const float *bias, void *y, int N, int K, int B,
                               int had_block, int x_dtype, int y_dtype, void *scratch, size_t scratch_size, int *status, jq_stream_t stream) {
     if (!x || !scratch) return JQ_ERR_NULL_PTR;
-    int rc = check(qweight, scales, y, status, N, K, B, y_dtype);
+    int rc = check(qweight, scales, bias, y, status, N, K, B, y_dtype);
     if (rc) return rc;
     if (scratch_size < jq_int8_scratch_bytes(B, K)) return JQ_ERR_WORKSPACE;
     if (!jq_aligned16(scratch)) return JQ_ERR_BAD_ALIGN;
@@ -755,9 +754,9 @@ extern "C" int jq_int8_linear(const void *qweight, const float *scales, const vo
 extern "C" int jq_int8_matmul(const void *qweight, const float *scales, const void *codes, int64_t code_stride, const float *row_scales,
                               const float *bias, void *y, int N, int K, int B, int y_dtype, int *status, jq_stream_t stream) {
     if (!codes || !row_scales) return JQ_ERR_NULL_PTR;
-    const int rc = check(qweight, scales, y, status, N, K, B, y_dtype);
+    const int rc = check(qweight, scales, bias, y, status, N, K, B, y_dtype);
     if (rc) return rc;
     if (code_stride < K) return JQ_ERR_BAD_SHAPE;
-    if (!jq_aligned16(codes) || code_stride % 16) return JQ_ERR_BAD_ALIGN;
+    if (!jq_aligned16(codes) || code_stride % 16 || !jq_whole(row_scales, 4)) return JQ_ERR_BAD_ALIGN;
     return multiply(qweight, scales, codes, code_stride, row_scales, bias, y, N, K, B, y_dtype, status, false, reinterpret_cast<cudaStream_t>(stream));
 }

@@ -261,7 +261,12 @@ extern "C" int jq_residual_norm(const jq_norm *n, jq_stream_t stream) {
     if (n->residual_dtype != n->x_dtype && n->residual_dtype != JQ_F32) return JQ_ERR_BAD_DTYPE;
     if (n->codes && (!jq_aligned16(n->codes) || n->stride_codes % 16)) return JQ_ERR_BAD_ALIGN;
     if (n->codes && n->stride_codes < n->width) return JQ_ERR_BAD_SHAPE;
+    if (n->reserved) return JQ_ERR_BAD_SHAPE;
     const int W = n->width, xs = n->x_dtype == JQ_F32 ? 4 : 2, rs = n->residual_dtype == JQ_F32 ? 4 : 2;
+    const int ws = n->weight_dtype == JQ_F32 ? 4 : 2, gs = n->gate_dtype == JQ_F32 ? 4 : 2;
+    if (!jq_whole(n->x, xs) || !jq_whole(n->h, xs) || !jq_whole(n->residual, rs) || !jq_whole(n->r, rs) || !jq_whole(n->weight, ws) || !jq_whole(n->bias, ws) ||
+        !jq_whole(n->post_weight, ws) || !jq_whole(n->post_bias, ws) || !jq_whole(n->gate, gs) || (n->codes && !jq_whole(n->scales, 4)))
+        return JQ_ERR_BAD_ALIGN;
     NormArgs a{};
     a.x = n->x; a.residual = n->residual; a.r = n->r; a.h = n->h; a.codes = reinterpret_cast<int8_t *>(n->codes); a.scales = n->scales;
     a.weight = n->weight; a.bias = n->bias; a.post_weight = n->post_weight; a.post_bias = n->post_bias; a.gate = n->gate;
@@ -272,7 +277,6 @@ extern "C" int jq_residual_norm(const jq_norm *n, jq_stream_t stream) {
     a.wdtype = n->weight_dtype; a.gdtype = n->gate_dtype;
     a.wide_w = n->weight_dtype == JQ_F32;
     a.wide_g = n->gate_dtype == JQ_F32;
-    const int gs = n->gate_dtype == JQ_F32 ? 4 : 2;
     const bool vectors = n->weight || n->bias || n->post_weight || n->post_bias;
     const bool vec = W % 8 == 0 && aligned(n->x, n->stride_x, xs) && aligned(n->residual, n->stride_residual, rs) && jq_aligned16(n->r) && jq_aligned16(n->h) &&
                      jq_aligned16(n->weight) && jq_aligned16(n->bias) && jq_aligned16(n->post_weight) && jq_aligned16(n->post_bias) &&

@@ -260,7 +260,7 @@ extern "C" int jq_quantize_rows(const void *x, int64_t row_stride, int rows, int
     if (x_dtype < 0 || x_dtype > 2) return JQ_ERR_BAD_DTYPE;
     if (!jq_aligned16(codes) || code_stride % 16) return JQ_ERR_BAD_ALIGN;
     const int size = x_dtype == JQ_F32 ? 4 : 2;
-    if (reinterpret_cast<uintptr_t>(x) & (size - 1)) return JQ_ERR_BAD_ALIGN;
+    if (!jq_whole(x, size) || !jq_whole(scales, 4)) return JQ_ERR_BAD_ALIGN;
     QuantArgs a{};
     a.x = x; a.stride_x = row_stride; a.stride_q = code_stride;
     a.codes = reinterpret_cast<int8_t *>(codes); a.scales = scales;
@@ -278,7 +278,7 @@ extern "C" int jq_dequantize_rows(const void *codes, int64_t code_stride, const 
     if (!codes || !scales || !out) return JQ_ERR_NULL_PTR;
     if (rows <= 0 || K <= 0 || code_stride < K) return JQ_ERR_BAD_SHAPE;
     if (dtype < 0 || dtype > 2) return JQ_ERR_BAD_DTYPE;
-    if (!jq_aligned16(codes) || code_stride % 16 || (reinterpret_cast<uintptr_t>(out) & (dtype == JQ_F32 ? 3u : 1u))) return JQ_ERR_BAD_ALIGN;
+    if (!jq_aligned16(codes) || code_stride % 16 || !jq_whole(scales, 4) || !jq_whole(out, dtype == JQ_F32 ? 4 : 2)) return JQ_ERR_BAD_ALIGN;
     DequantArgs a{};
     a.codes = reinterpret_cast<const int8_t *>(codes); a.scales = scales; a.out = out; a.stride_q = code_stride;
     a.rows = rows; a.width = K;

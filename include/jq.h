@@ -417,7 +417,8 @@ int jq_token_logprobs(const void *logits, int64_t row_stride, int rows, int voca
 /* ---- linear layers in 8-bit integers, and the norms around a block ----
  * Format INT8: a row of K values (a token's activation, or a channel's weights) is K signed codes and one fp32 scale, value =
  * code * scale; rows of weights are jq_row_stride = K rounded up to a multiple of 32 codes apart, those of activations any multiple of 16;
- * what lies between K and the stride is not read.  The codes' base is 16-byte aligned.  K is at most JQ_INT8_MAX_K, so that a sum of K
+ * what lies between K and the stride is not read.  The codes' base is 16-byte aligned; every other array of the entries below, the norm's among
+ * them, begins at a multiple of its element's size (JQ_ERR_BAD_ALIGN otherwise).  K is at most JQ_INT8_MAX_K, so that a sum of K
  * products has 32 bits.  The counterpart of the reference is the per-row integer grid of QuantLinear
  * (Python_Jenks_Test/Jenks_Tests/Quantization_Experiments/layers.py:22-38), which it multiplies out in fp32.
  *

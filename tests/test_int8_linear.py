@@ -654,3 +654,20 @@ def test_scales_whose_product_with_the_sum_leaves_the_range(rows, N, K):
     good = torch.ones(N, dtype=torch.bool, device=DEV)
     good[[2, 5]] = False
     assert torch.isnan(y[:, [2, 5]]).all() and torch.isnan(y[rows // 2]).all() and torch.isfinite(y[:rows // 2][:, good]).all()
+
+
+def test_arrays_off_their_elements_boundary_are_refused():
+    """Scales, biases, outputs and status words that a kernel would access at a misaligned address; no GPU is needed."""
+    lib, p = _lib.load(), torch.zeros(8192, dtype=torch.uint8).data_ptr()
+    assert p % 16 == 0
+    for dtype, off in ((0, 1), (0, 2), (1, 1), (2, 1)):
+        assert lib.jq_quantize_rows(p + off, 8, 1, 8, 0, dtype, p, 32, p, None) == -3
+        assert lib.jq_dequantize_rows(p, 32, p, 1, 8, p + off, dtype, None) == -3
+        assert lib.jq_int8_linear(p, p, p + off, None, p, 4, 8, 1, 0, dtype, 0, p, 4096, p, None) == -3
+        assert lib.jq_int8_matmul(p, p, p, 32, p, None, p + off, 4, 8, 1, dtype, p, None) == -3
+    for off in (1, 2, 3):
+        assert lib.jq_quantize_rows(p, 8, 1, 8, 0, 0, p, 32, p + off, None) == -3 and lib.jq_dequantize_rows(p, 32, p + off, 1, 8, p, 0, None) == -3
+        for at in range(4):                                        # the channels' scales, the rows', the bias, the status word
+            cs, ts, bias, status = (p + off if i == at else p for i in range(4))
+            assert lib.jq_int8_matmul(p, cs, p, 32, ts, bias, p, 4, 8, 1, 0, status, None) == -3
+            assert at == 1 or lib.jq_int8_linear(p, cs, p, bias, p, 4, 8, 1, 0, 0, 0, p, 4096, status, None) == -3

@@ -313,3 +313,25 @@ def test_rotations_that_leave_the_range(width):
         rows = ops.residual_norm(x, weight=weight, quantize=True, had_block=128).h
         assert torch.isnan(rows.scales[lost]).all() and bool((rows.codes[lost] == 0).all())
         assert int(torch.isnan(rows.scales).sum()) == len(lost)
+
+
+def test_arrays_off_their_elements_boundary_are_refused():
+    import ctypes
+    lib, p = _lib.load(), torch.zeros(4096, dtype=torch.uint8).data_ptr()
+    assert p % 16 == 0
+
+    def call(**change):
+        n = _lib.jq_norm(x=p, residual=p, h=p, r=p, stride_x=8, stride_residual=8, rows=1, width=8, gate_inner_rows=1, scale=1.0, eps=1e-6)
+        for k, v in change.items():
+            setattr(n, k, v)
+        return lib.jq_residual_norm(ctypes.byref(n), None)
+
+    arrays = {"x": "x_dtype", "h": "x_dtype", "residual": "residual_dtype", "r": "residual_dtype", "weight": "weight_dtype", "bias": "weight_dtype",
+              "post_weight": "weight_dtype", "post_bias": "weight_dtype", "gate": "gate_dtype"}
+    for name in arrays:
+        for off in (1, 2, 3):
+            assert call(**{name: p + off}) == -3
+        for dtype in (1, 2):
+            assert call(**{"x_dtype": dtype, "residual_dtype": dtype, arrays[name]: dtype, name: p + 1}) == -3
+    assert call(codes=p, scales=p + 2, stride_codes=16) == -3
+    assert call(reserved=1) == -2
