@@ -16,6 +16,7 @@ JQ_FMT_E2M1, JQ_FMT_GF4, JQ_FMT_INT8 = 0, 1, 2
 JQ_KV_INT8, JQ_KV_E4M3 = 0, 1
 JQ_NORM_RMS, JQ_NORM_LAYER = 0, 1
 JQ_INT8_MAX_K = 131071
+JQ_INT8_MAX_ROWS = 0x7fffff00
 
 
 class JqError(RuntimeError):

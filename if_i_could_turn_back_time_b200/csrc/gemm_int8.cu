@@ -721,7 +721,7 @@ static int multiply(const void *w, const float *cs, const void *x, int64_t x_str
 
 static int check(const void *w, const float *cs, const float *bias, const void *y, const int *status, int N, int K, int B, int y_dtype) {
     if (!w || !cs || !y || !status) return JQ_ERR_NULL_PTR;
-    if (N <= 0 || K <= 0 || B <= 0 || K > JQ_INT8_MAX_K || N > (1 << 28)) return JQ_ERR_BAD_SHAPE;
+    if (N <= 0 || K <= 0 || B <= 0 || B > JQ_INT8_MAX_ROWS || K > JQ_INT8_MAX_K || N > (1 << 28)) return JQ_ERR_BAD_SHAPE;
     if (y_dtype < 0 || y_dtype > 2) return JQ_ERR_BAD_DTYPE;
     return jq_aligned16(w) && jq_whole(cs, 4) && jq_whole(bias, 4) && jq_whole(y, y_dtype == JQ_F32 ? 4 : 2) && jq_whole(status, 4) ? JQ_OK : JQ_ERR_BAD_ALIGN;
 }
@@ -733,7 +733,7 @@ static size_t scale_room(int rows) { return ((size_t)rows * 4 + 255) / 256 * 256
 using namespace jq8;
 
 extern "C" size_t jq_int8_scratch_bytes(int B, int K) {
-    if (B <= 0 || K <= 0) return 0;
+    if (B <= 0 || K <= 0 || K > JQ_INT8_MAX_K) return 0;
     return scale_room(B) + (size_t)B * jq_row_stride_codes(K);
 }
 

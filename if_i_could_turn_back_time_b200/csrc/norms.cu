@@ -251,7 +251,7 @@ using namespace jq8;
 
 extern "C" int jq_residual_norm(const jq_norm *n, jq_stream_t stream) {
     if (!n || !n->x || (!n->h && !n->codes) || (n->codes && !n->scales)) return JQ_ERR_NULL_PTR;
-    if (n->rows <= 0 || n->width <= 0 || n->width > kMostKept || n->stride_x < 0 || n->stride_residual < 0) return JQ_ERR_BAD_SHAPE;
+    if (n->rows <= 0 || n->rows > JQ_INT8_MAX_ROWS || n->width <= 0 || n->width > kMostKept || n->stride_x < 0 || n->stride_residual < 0) return JQ_ERR_BAD_SHAPE;
     if (n->kind != JQ_NORM_RMS && n->kind != JQ_NORM_LAYER) return JQ_ERR_UNSUPPORTED;
     if (n->had_block != 0 && (n->had_block != 128 || n->width % 128 || !n->codes)) return JQ_ERR_BAD_SHAPE;
     if (n->gate && n->gate_inner_rows <= 0) return JQ_ERR_BAD_SHAPE;

@@ -234,9 +234,9 @@ static int launch_quantize(QuantArgs &a, bool vec, bool rotate, cudaStream_t st)
     }
     if (c.threads && a.rows > 65535) {
         // rows are the grid's second dimension: in parts of it
-        for (int r0 = 0; r0 < a.rows; r0 += 65535) {
+        for (long long r0 = 0; r0 < a.rows; r0 += 65535) {
             QuantArgs b = a;
-            b.rows = a.rows - r0 < 65535 ? a.rows - r0 : 65535;
+            b.rows = a.rows - r0 < 65535 ? (int)(a.rows - r0) : 65535;
             b.x = reinterpret_cast<const T *>(a.x) + r0 * a.stride_x;
             b.codes += r0 * a.stride_q;
             b.scales += r0;
@@ -255,7 +255,7 @@ using namespace jq8;
 extern "C" int jq_quantize_rows(const void *x, int64_t row_stride, int rows, int K, int had_block, int x_dtype, void *codes,
                                 int64_t code_stride, float *scales, jq_stream_t stream) {
     if (!x || !codes || !scales) return JQ_ERR_NULL_PTR;
-    if (rows <= 0 || K <= 0 || K > JQ_INT8_MAX_K || code_stride < K || row_stride < 0) return JQ_ERR_BAD_SHAPE;
+    if (rows <= 0 || rows > JQ_INT8_MAX_ROWS || K <= 0 || K > JQ_INT8_MAX_K || code_stride < K || row_stride < 0) return JQ_ERR_BAD_SHAPE;
     if (had_block != 0 && (had_block != 128 || K % 128)) return JQ_ERR_BAD_SHAPE;
     if (x_dtype < 0 || x_dtype > 2) return JQ_ERR_BAD_DTYPE;
     if (!jq_aligned16(codes) || code_stride % 16) return JQ_ERR_BAD_ALIGN;
@@ -276,7 +276,7 @@ extern "C" int jq_quantize_rows(const void *x, int64_t row_stride, int rows, int
 extern "C" int jq_dequantize_rows(const void *codes, int64_t code_stride, const float *scales, int rows, int K, void *out, int dtype,
                                   jq_stream_t stream) {
     if (!codes || !scales || !out) return JQ_ERR_NULL_PTR;
-    if (rows <= 0 || K <= 0 || code_stride < K) return JQ_ERR_BAD_SHAPE;
+    if (rows <= 0 || rows > JQ_INT8_MAX_ROWS || K <= 0 || K > JQ_INT8_MAX_K || code_stride < K) return JQ_ERR_BAD_SHAPE;
     if (dtype < 0 || dtype > 2) return JQ_ERR_BAD_DTYPE;
     if (!jq_aligned16(codes) || code_stride % 16 || !jq_whole(scales, 4) || !jq_whole(out, dtype == JQ_F32 ? 4 : 2)) return JQ_ERR_BAD_ALIGN;
     DequantArgs a{};

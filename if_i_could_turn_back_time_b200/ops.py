@@ -541,7 +541,7 @@ def _codes_of(rows: QuantizedRows):
     if len(shape) != 2:
         codes = codes.reshape(-1, K)
     n = codes.shape[0]
-    if n > 0x7fffffff:
+    if n > _lib.JQ_INT8_MAX_ROWS:
         raise RuntimeError(f"{n} rows: the library counts in 32 bits")
     if scales.is_neg() or not scales.is_contiguous():
         scales = scales.resolve_neg().contiguous()
@@ -570,7 +570,7 @@ def _rows_of(x: torch.Tensor, K: int, what: str):
         if one != 1 and K > 1:
             x = x.contiguous()
             row = K
-    if n > 0x7fffffff:
+    if n > _lib.JQ_INT8_MAX_ROWS:
         raise RuntimeError(f"{n} rows of {what}: the library counts in 32 bits")
     return x, n, row
 

@@ -428,6 +428,7 @@ int jq_token_logprobs(const void *logits, int64_t row_stride, int rows, int voca
  * a row with a NaN or an infinity has the scale NaN and codes 0.  Rows that are rotated are of 16-byte pieces (x and row_stride).  One launch
  * (for every 65535 rows, where a row has more than a warp), as jq_dequantize_rows (out [rows, K] = code * scale). */
 #define JQ_INT8_MAX_K 131071
+#define JQ_INT8_MAX_ROWS 0x7fffff00   /* of a call, the norm's too: what is counted from there on leaves 32 bits (JQ_ERR_BAD_SHAPE) */
 int jq_quantize_rows(const void *x, int64_t row_stride, int rows, int K, int had_block, int x_dtype, void *codes,
                      int64_t code_stride, float *scales, jq_stream_t stream);
 int jq_dequantize_rows(const void *codes, int64_t code_stride, const float *scales, int rows, int K, void *out, int dtype,

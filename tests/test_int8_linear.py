@@ -671,3 +671,16 @@ def test_arrays_off_their_elements_boundary_are_refused():
             cs, ts, bias, status = (p + off if i == at else p for i in range(4))
             assert lib.jq_int8_matmul(p, cs, p, 32, ts, bias, p, 4, 8, 1, 0, status, None) == -3
             assert at == 1 or lib.jq_int8_linear(p, cs, p, bias, p, 4, 8, 1, 0, 0, 0, p, 4096, status, None) == -3
+
+
+def test_sizes_that_leave_32_bits_are_refused():
+    """Rows whose count the kernels' arithmetic could not hold, and rows of codes longer than the format has; no GPU is needed."""
+    lib, p = _lib.load(), torch.zeros(4096, dtype=torch.uint8).data_ptr()
+    for rows in (_lib.JQ_INT8_MAX_ROWS + 1, 2 ** 31 - 1):
+        assert lib.jq_quantize_rows(p, 0, rows, 8, 0, 0, p, 32, p, None) == -2 and lib.jq_dequantize_rows(p, 32, p, rows, 8, p, 0, None) == -2
+        assert lib.jq_int8_matmul(p, p, p, 32, p, None, p, 4, 8, rows, 0, p, None) == -2
+        assert lib.jq_int8_linear(p, p, p, None, p, 4, 8, rows, 0, 0, 0, p, 1 << 60, p, None) == -2
+        with pytest.raises(RuntimeError, match="32 bits"):
+            ops._rows_of(torch.zeros(1, 8).expand(rows, 8), 8, "x")
+    for K in (_lib.JQ_INT8_MAX_K + 1, 2 ** 31 - 1):
+        assert lib.jq_dequantize_rows(p, 1 << 32, p, 1, K, p, 0, None) == -2 and lib.jq_int8_scratch_bytes(1, K) == 0

@@ -335,3 +335,11 @@ def test_arrays_off_their_elements_boundary_are_refused():
             assert call(**{"x_dtype": dtype, "residual_dtype": dtype, arrays[name]: dtype, name: p + 1}) == -3
     assert call(codes=p, scales=p + 2, stride_codes=16) == -3
     assert call(reserved=1) == -2
+
+
+def test_rows_that_leave_32_bits_are_refused():
+    import ctypes
+    p = torch.zeros(4096, dtype=torch.uint8).data_ptr()
+    for rows in (_lib.JQ_INT8_MAX_ROWS + 1, 2 ** 31 - 1):
+        n = _lib.jq_norm(x=p, h=p, rows=rows, width=8, gate_inner_rows=1, scale=1.0, eps=1e-6)
+        assert _lib.load().jq_residual_norm(ctypes.byref(n), None) == -2
