@@ -110,6 +110,7 @@ _SIGNATURES = {
                                c_size_t, c_void_p, c_void_p]),
     "jq_int8_matmul": (c_int, [c_void_p, c_void_p, c_void_p, ctypes.c_int64, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int,
                                c_void_p, c_void_p]),
+    "jq_int8_form": (c_int, [c_int, c_int, c_int, c_void_p, c_void_p, c_void_p]),
     "jq_residual_norm": (c_int, [c_void_p, c_void_p]),
     "jq_pack_e2m1_host": (c_int, [c_void_p, c_int, c_int, c_int, c_void_p, c_void_p, c_int]),
     "jq_pack_gf4_host": (c_int, [c_void_p, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p, c_int]),

@@ -737,6 +737,14 @@ extern "C" size_t jq_int8_scratch_bytes(int B, int K) {
     return scale_room(B) + (size_t)B * jq_row_stride_codes(K);
 }
 
+extern "C" int jq_int8_form(int N, int K, int B, int *pair, int *tile, int *split) {
+    if (!pair || !tile || !split) return JQ_ERR_NULL_PTR;
+    if (N <= 0 || K <= 0 || B <= 0 || B > JQ_INT8_MAX_ROWS || K > JQ_INT8_MAX_K || N > (1 << 28)) return JQ_ERR_BAD_SHAPE;
+    const Form f = choose_form(N, K, B, (K + kStep - 1) / kStep, jq_sm_count());
+    *pair = f.pair; *tile = f.tile; *split = f.split;
+    return JQ_OK;
+}
+
 extern "C" int jq_int8_linear(const void *qweight, const float *scales, const void *x, const float *bias, void *y, int N, int K, int B,
                               int had_block, int x_dtype, int y_dtype, void *scratch, size_t scratch_size, int *status, jq_stream_t stream) {
     if (!x || !scratch) return JQ_ERR_NULL_PTR;

@@ -443,6 +443,9 @@ int jq_int8_linear(const void *qweight, const float *scales, const void *x, cons
                    int had_block, int x_dtype, int y_dtype, void *scratch, size_t scratch_bytes, int *status_dev, jq_stream_t stream);
 int jq_int8_matmul(const void *qweight, const float *scales, const void *codes, int64_t code_stride, const float *row_scales,
                    const float *bias_or_null, void *y, int N, int K, int B, int y_dtype, int *status_dev, jq_stream_t stream);
+/* How the product of these sizes is cut on the current device (host only; one of 148 SMs where there is none): pair 0, tiles of `tile` tokens x 128
+ * channels on a CTA each, or 1, of 256 tokens x `tile` channels on a pair of CTAs; `split` of them share a tile's K. */
+int jq_int8_form(int N, int K, int B, int *pair, int *tile, int *split);
 
 /* The norms on both sides of a block with its gate, residual scale and sum, a row [width] at a time (width up to 32768):
  *   u = N(x) * post_weight + post_bias  (post != 0; x otherwise),   r = residual + scale * (gate * u),   h = N(r) * weight + bias,

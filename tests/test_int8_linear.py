@@ -684,3 +684,69 @@ def test_sizes_that_leave_32_bits_are_refused():
             ops._rows_of(torch.zeros(1, 8).expand(rows, 8), 8, "x")
     for K in (_lib.JQ_INT8_MAX_K + 1, 2 ** 31 - 1):
         assert lib.jq_dequantize_rows(p, 1 << 32, p, 1, K, p, 0, None) == -2 and lib.jq_int8_scratch_bytes(1, K) == 0
+
+
+# Rows, N and K of two products for each form that the rule may take: (pair, tile, split) -> odd N, and rows of y of 16 bytes
+FORMS = {
+    (0, 16, 1): ((2, 133, 205), (2, 132, 202)), (0, 16, 2): ((2, 6285, 657), (3, 6300, 668)), (0, 16, 3): ((3, 131, 513), (4, 132, 520)),
+    (0, 16, 4): ((3, 133, 391), (4, 132, 394)), (0, 16, 8): ((2, 131, 915), (3, 132, 911)), (0, 32, 1): ((19, 137, 212), (17, 132, 206)),
+    (0, 32, 2): ((397, 385, 1219), (398, 400, 1229)), (0, 32, 3): ((134, 402, 1035), (294, 160, 1025)), (0, 32, 4): ((17, 131, 777), (19, 136, 774)),
+    (0, 32, 8): ((17, 131, 936), (21, 132, 921)), (0, 64, 1): ((34, 666, 905), (33, 584, 1060)), (0, 64, 2): ((521, 649, 3212), (511, 780, 3315)),
+    (0, 64, 3): ((449, 522, 2230), (258, 948, 2191)), (0, 64, 4): ((270, 398, 1806), (264, 396, 1863)), (0, 64, 8): ((34, 393, 1572), (33, 376, 1631)),
+    (0, 128, 1): ((71, 18998, 205), (65, 20332, 203)), (0, 128, 2): ((85, 8439, 14591), (120, 8516, 14510)), (0, 128, 3): ((75, 4838, 7733), (85, 4868, 7903)),
+    (0, 128, 4): ((342, 1033, 16203), (265, 1164, 17033)), (0, 128, 8): ((265, 389, 21122), (210, 560, 21015)), (1, 128, 1): ((68, 666, 904), (69, 488, 1245)),
+    (1, 128, 2): ((331, 1033, 3592), (275, 1180, 3402)), (1, 256, 1): ((10016, 131, 209), (196, 9600, 205)), (1, 256, 2): ((520, 1398, 15160), (332, 2068, 14862)),
+    (1, 256, 4): ((442, 1182, 17757), (390, 1308, 17729))}
+
+
+def _form(N, K, rows):
+    import ctypes
+    found = [ctypes.c_int() for _ in range(3)]
+    assert _lib.load().jq_int8_form(N, K, rows, *(ctypes.byref(v) for v in found)) == 0
+    return tuple(v.value for v in found)
+
+
+def test_the_products_below_reach_every_form():
+    """On a device of 148 SMs, as where there is none; the kernels, tiles and splits are all that the rule can choose from."""
+    if torch.cuda.is_available() and torch.cuda.get_device_properties(0).multi_processor_count != 148:
+        pytest.skip("another number of SMs")
+    every = {(0, tile, split) for tile in (16, 32, 64, 128) for split in (1, 2, 3, 4, 8)} | {(1, 128, 1), (1, 128, 2), (1, 256, 1), (1, 256, 2), (1, 256, 4)}
+    assert set(FORMS) == every
+    for form, cases in FORMS.items():
+        assert [_form(N, K, rows) for rows, N, K in cases] == [form, form]
+    for bad in ((0, 8, 1), (8, 0, 1), (8, 8, 0), (8, _lib.JQ_INT8_MAX_K + 1, 1), (8, 8, _lib.JQ_INT8_MAX_ROWS + 1), ((1 << 28) + 1, 8, 1)):
+        with pytest.raises(AssertionError):
+            _form(*bad)
+    assert _lib.load().jq_int8_form(8, 8, 1, None, None, None) == -1
+
+
+@gpu
+@pytest.mark.parametrize("form", sorted(FORMS))
+def test_every_form_against_64_bits(form):
+    for i, (rows, N, K) in enumerate(FORMS[form]):
+        gen = torch.Generator(DEV).manual_seed(N + K)
+        pw = _weight(N, K)
+        x = torch.randn(rows, K, device=DEV, generator=gen) * (torch.rand(rows, 1, device=DEV, generator=gen) + 0.1)
+        bias = torch.randn(N, device=DEV, generator=gen)
+        for dtype in DTYPES:
+            xs, b = x.to(dtype), bias if (i == 0) == (dtype == torch.bfloat16) else None
+            rows8 = ops.quantize_rows(xs)
+            y = ops.linear(xs, pw, b)
+            _near(y, *_product(rows8.codes, rows8.scales, pw, b, dtype))
+            assert torch.equal(ops.linear(rows8, pw, b), y)
+        # captured, replayed on another stream; and into memory whose surroundings stay as they are
+        graph, side = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+        with torch.cuda.graph(graph):
+            again, direct = ops.linear(xs, pw, b), ops.linear(rows8, pw, b)
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            graph.replay()
+        side.synchronize()
+        assert torch.equal(again, y) and torch.equal(direct, y)
+        room = torch.full((rows * N + 64,), 7.0, dtype=dtype, device=DEV)
+        status = torch.zeros(1, dtype=torch.int32, device=DEV)
+        assert _lib.load().jq_int8_matmul(pw.qweight.data_ptr(), pw.scales.data_ptr(), rows8.codes.data_ptr(), rows8.codes.stride(0), rows8.scales.data_ptr(),
+                                          ops._addr(b), room[32:].data_ptr(), N, K, rows, _lib.JQ_BF16, status.data_ptr(), None) == 0
+        assert bool((room[:32] == 7).all()) and bool((room[32 + rows * N:] == 7).all()) and status.item() == 0
+        assert torch.equal(room[32:32 + rows * N].view(rows, N), y)
+    assert ops.check_status(raise_on_error=False) == 0
