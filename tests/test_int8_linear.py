@@ -750,3 +750,81 @@ def test_every_form_against_64_bits(form):
         assert bool((room[:32] == 7).all()) and bool((room[32 + rows * N:] == 7).all()) and status.item() == 0
         assert torch.equal(room[32:32 + rows * N].view(rows, N), y)
     assert ops.check_status(raise_on_error=False) == 0
+
+
+@gpu
+@pytest.mark.parametrize("had", [0, 128])
+@pytest.mark.parametrize("dtype,out", [(torch.bfloat16, None), (torch.float32, None), (torch.float16, torch.float32), (torch.float32, torch.bfloat16)])
+def test_activations_in_parts(monkeypatch, had, dtype, out):
+    """Rows beyond what a call's scratch holds go in parts of a multiple of 256, each into its own rows of the output."""
+    pw = _weight(130, 384, had=had)
+    x, bias = torch.randn(700, 384, device=DEV).to(dtype), torch.randn(130, device=DEV)
+    want = ops.linear(x, pw, bias, out_dtype=out)
+    calls, linear = [], _lib.load().jq_int8_linear
+    monkeypatch.setattr(_lib.load(), "jq_int8_linear", lambda *a: calls.append(a[7]) or linear(*a))
+    monkeypatch.setattr(ops, "MAX_ROWS_SCRATCH", 300 * 384)
+    graph = torch.cuda.CUDAGraph()
+    for leading in ((700,), (7, 100)):
+        assert torch.equal(ops.linear(x.view(*leading, 384), pw, bias, out_dtype=out), want.view(*leading, 130))
+    with torch.cuda.graph(graph):
+        y = ops.linear(x, pw, bias, out_dtype=out)
+    assert calls == [256, 256, 188] * 3
+    other = torch.randn(700, 384, device=DEV).to(dtype)
+    x.copy_(other)
+    for _ in range(2):
+        y.zero_()
+        graph.replay()
+    monkeypatch.undo()
+    assert torch.equal(y, ops.linear(other, pw, bias, out_dtype=out)) and ops.check_status(raise_on_error=False) == 0
+
+
+@gpu
+def test_rows_sharded_over_ranks():
+    """A world of one, and the slices that two ranks would have, side by side."""
+    import torch.distributed as dist
+    from if_i_could_turn_back_time_b200 import dist as sharded
+    pw, x, bias = _weight(96, 200), torch.randn(5, 200, device=DEV), torch.randn(96)
+    want = ops.linear(x, pw, bias.to(DEV))
+    two = [sharded.shard_rows(pw, rank, 2) for rank in range(2)]
+    assert torch.equal(torch.cat([ops.linear(x, part, bias[48 * i:48 * i + 48].to(DEV)) for i, part in enumerate(two)], -1), want)
+    dist.init_process_group("gloo", store=dist.HashStore(), rank=0, world_size=1)
+    try:
+        layer = sharded.RowShardedLinear(jq.PackedWeight(pw.spec, 96, 200, pw.qweight.cpu(), pw.scales.cpu(), None), bias, device=DEV)
+        assert torch.equal(layer(x), want)
+    finally:
+        dist.destroy_process_group()
+
+
+@gpu
+def test_linear_under_torch_compile():
+    """One opaque operation in the traced graph, the same bits."""
+    pw, x, bias = _weight(72, 200), torch.randn(3, 5, 200, device=DEV).bfloat16(), torch.randn(72, device=DEV)
+    traced = []
+
+    def backend(graph, _):
+        traced.append([str(n.target) for n in graph.graph.nodes if n.op == "call_function"])
+        return graph.forward
+
+    for out in (None, torch.float32):
+        call = torch.compile(lambda t: ops.linear(t, pw, bias, out_dtype=out) + 1, backend=backend, fullgraph=True)
+        assert torch.equal(call(x), ops.linear(x, pw, bias, out_dtype=out) + 1)
+    layer = jq.JenksQuantLinear(nn.Linear(200, 72), 8, fmt="int8").to(DEV)
+    layer.commit()
+    assert torch.equal(torch.compile(layer, backend=backend, fullgraph=True)(x), layer(x))
+    assert len(traced) == 3 and all(sum("jq.linear" in n for n in names) == 1 for names in traced)
+
+
+@gpu
+@pytest.mark.parametrize("rotate", [0, 128])
+def test_a_norm_its_codes_and_their_products_repeat_themselves(rotate):
+    """Every pass over the same inputs gives the same bits."""
+    x, residual = (torch.randn(512, 1024, device=DEV).bfloat16() for _ in range(2))
+    weights = [_weight(n, 1024, n, rotate) for n in (1024, 256, 256)]
+
+    def chain():
+        h, r = ops.residual_norm(x, residual, quantize=True, had_block=rotate)
+        return [h.codes, h.scales, r] + [ops.linear(h, w) for w in weights]
+
+    first = chain()
+    for _ in range(50):
+        assert all(torch.equal(a, b) for a, b in zip(chain(), first))
