@@ -54,7 +54,7 @@ __device__ __forceinline__ float scaled_large(int sum, float cs, float ts, float
 template <class T>
 __device__ __forceinline__ void store4(T *y, const float (&v)[4], int n, bool vec) {
     if (vec && n >= 4) {
-        T r[4] = {(T)v[0], (T)v[1], (T)v[2], (T)v[3]};
+        alignas(16) const T r[4] = {(T)v[0], (T)v[1], (T)v[2], (T)v[3]};
         if (sizeof(T) == 4) *reinterpret_cast<uint4 *>(y) = *reinterpret_cast<const uint4 *>(r);
         else *reinterpret_cast<uint2 *>(y) = *reinterpret_cast<const uint2 *>(r);
         return;
