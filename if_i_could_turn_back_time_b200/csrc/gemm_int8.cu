@@ -365,8 +365,9 @@ __device__ __forceinline__ uint32_t ld_cluster_u32(uint32_t cluster_addr) {
 // scaled and written while the next one is multiplied.  Where there are few tiles, the pairs of a cluster share a tile's K range
 // instead (split > 1): their sums meet in distributed shared memory, a part of the columns in each.
 // Bound by the tensor core: a stage of 128 values takes 520 to 560 clocks (512 are its products') with 256 channels, 400 to 450 (256) with 128,
-// which ask the L2 for 24 KB in that time.  8192 x 8192 x 28672: 1131 us, 3.4 POP/s, twice what the measured peak of bf16 is, with the board's power
-// cap active; 2048 x 4096 x 11008: 61 us, 344 tiles on 74 pairs being 4.65 waves.  (Single CTAs of 128 x 256: 2098 and 121.)
+// which ask the L2 for 24 KB in that time.  8192 x 8192 x 28672: 1100 us in a few calls (3.5 POP/s, 1.06 of twice the measured bf16 rate),
+// 1270 in calls one behind another for seconds, when the power cap holds the clock down (3.0 POP/s, 0.92 of that rate, 1.11 of twice the bf16 rate
+// measured the same way); 2048 x 4096 x 11008: 60 and 70 us, 344 tiles on 74 pairs being 4.65 waves.  (Single CTAs of 128 x 256: 2098 and 121.)
 template <int BN>
 __global__ void __launch_bounds__(kPairThreads, 1)
     gemm_int8_pair_kernel(const __grid_constant__ GemmArgs p, const __grid_constant__ CUtensorMap wmap, const __grid_constant__ CUtensorMap xmap) {
@@ -606,12 +607,12 @@ struct Form { bool pair; int tile, split; };   // tile: tokens of a single CTA's
 // Which kernel, tile and split of K, by a model of the time in us: what a launch, a tile's outputs, a stage of 128 values of K and an exchange
 // between CTAs take.  Its constants are fitted to 2524 timed calls (18 numbers of tokens up to 10000, 14 matrices from 100 x 300 to
 // 32000 x 2048 and 28672 x 8192, every form): the choice is 1.0 % behind the best form on average, 15 % at most.  Both sides of its turns, us:
-//   4096 x 4096         T = 64    single CTAs of 64 tokens, K in eight parts 9.5    pairs of 128 channels 11.0
-//                       T = 256   single 14.1 (128 tokens, four parts)              pairs of 128 channels, two parts 11.0, one 11.5
-//                       T = 1024  single 19.9                                       pairs of 128 18.6, of 256 17.1
-//   28672 x 8192        T = 64    single 44                                         pairs of 256 52
-//                       T = 200   single 82                                         pairs of 256 55
-//   100 x 300           T = 512   single, 32 tokens 4.1                             pairs of 128 5.3
+//   4096 x 4096         T = 64    single CTAs of 64 tokens, K in four parts 9.6     pairs of 128 channels, two parts 10.5, one 10.9
+//                       T = 256   single 14.0 (128 tokens, four parts)              pairs of 128 channels, two parts 11.0, one 11.5
+//                       T = 1024  single 20.1                                       pairs of 128 18.7, of 256 16.5
+//   28672 x 8192        T = 64    single 44                                         pairs of 256 53
+//                       T = 200   single 84                                         pairs of 256 57
+//   100 x 300           T = 512   single, 32 tokens 4.1                             pairs of 128 5.4
 static Form choose_form(int N, int K, int T, int steps, int sms) {
     Form best{false, 16, 1};
     double least = 0;
@@ -619,7 +620,8 @@ static Form choose_form(int N, int K, int T, int steps, int sms) {
         if (least == 0 || us < least) { best = Form{pair, tile, split}; least = us; }
     };
     for (int nt = 16; nt <= 128; nt *= 2) {
-        // (tiles of 32 tokens for more than 32 only where the weights are next to nothing)
+        // (tiles of 32 tokens for more than 32 only where the weights are next to nothing: 300 x 784, T = 200, 4.7 and in tiles of 64 5.1; between that
+        // and the bound nothing was timed)
         if ((T <= nt / 2 && nt > 16) || (T > nt && (nt < 32 || (nt == 32 && (long long)N * K >= 600000)))) continue;
         const long long tiles = (long long)((N + kTileN - 1) / kTileN) * ((T + nt - 1) / nt);
         for (int s = 1; s <= 8; s = s == 4 ? 8 : s + 1) {

@@ -45,7 +45,7 @@ template <class T> struct Piece {
 // Blocks that an SM is to hold: more of them hide more of a row's chain of loads and sums, as long as what no longer fits in registers stays little.
 // us at 3 / 4 / unbounded (2 or 3): 50432 x 768 fp16, three chunks a thread - / 54 / 63; bf16 with an fp32 stream 74 / - / 80; 50000 x 500, two chunks
 // - / 37 / 48; 20000 x 1024, four chunks: bf16 with its stream of 16 bits 46 at 4 and 34 unbounded, of 32 bits 47 at 3 and 43, fp32 56 at 3 and 59.
-// Blocks of 256 threads, 8191 x 4096 with both norms and an fp32 stream: 74 at 4, 78 at 5, 79 unbounded (calls one behind another).
+// Blocks of 256 threads, 8191 x 4096 with both norms and an fp32 stream, calls one behind another on inputs that take turns: 74 at 4, 78 at 5, 79 unbounded.
 constexpr int resident(int threads, int chunks, int x_size, int r_size) {
     if (threads) return threads == 256 ? 4 : 1;
     if (chunks < 3) return 4;
@@ -56,8 +56,9 @@ constexpr int resident(int threads, int chunks, int x_size, int r_size) {
 // A warp (kThreads 0) or a block per row, which stays in registers from the first read to the last write:
 //   u = N(x) post_weight + post_bias (or x),  r = residual + scale * (gate * u),  h = N(r) weight + bias,
 // N(v) = v / sqrt(mean(v^2) + eps), or of v - mean(v).  All in fp32; h follows from r as it was before its rounding.
-// Bound by memory: 8191 x 4096 with both norms and an fp32 stream 69 us (5.8 TB/s), 50432 x 768 fp16 with a gate for each image 54 (5.8), 50000 x
-// 197 23, 4000 x 5025 44 (3.6: one-element loads).  Two chunks a thread and code without paths that a call does not take are what did it (four chunks,
+// Bound by memory: 8191 x 4096 with both norms and an fp32 stream 68 us in a graph (5.9 TB/s), 70 to 74 in calls one behind another; with codes in
+// place of h 72, rotated 79; one norm in bf16 44, 47 and 56 (codes: 5.0 and 4.2 TB/s; the rotation has four shuffles a value here).  50432 x 768
+// fp16 with a gate for each image 54 (5.8), 50000 x 197 23, 4000 x 5025 44 (3.6: one-element loads).  Two chunks a thread and code without paths that a call does not take are what did it (four chunks,
 // every alignment and type in one kernel: 104, 72, 69 and 79; instructions waited for the instruction cache).
 // kPieces: every row and vector is of 16-byte pieces, and vectors are of T or fp32; kPairs: rows are of pairs; kScattered: any width, alignment,
 // stride and type.

@@ -436,8 +436,9 @@ int jq_dequantize_rows(const void *codes, int64_t code_stride, const float *scal
 /* y[B, N] = (sum of products of codes, exact, * the channel's scale) * the token's scale + bias, in fp32, rounded to y_dtype:
  * the F.linear(x, W_bar, bias) of Quantization_Experiments/layers.py:38 with both operands in 8 bits.  jq_int8_linear quantises x
  * [B, K] (row-major) into scratch (16-byte aligned, jq_int8_scratch_bytes), two launches; jq_int8_matmul takes rows of codes, one
- * launch.  y is [B, N] row-major and overlaps no input.  The result does not depend on how the work is cut: a row's is the same whatever rows
- * are beside it.  status_dev: as for jq_gemm_rows. */
+ * launch.  y is [B, N] row-major and overlaps no input.  With scales as the packers make them no product in between leaves fp32's range where
+ * the result does not.  The result does not depend on how the work is cut: a row's is the same whatever rows are beside it.  status_dev: as for
+ * jq_gemm_rows. */
 size_t jq_int8_scratch_bytes(int B, int K);
 int jq_int8_linear(const void *qweight, const float *scales, const void *x, const float *bias_or_null, void *y, int N, int K, int B,
                    int had_block, int x_dtype, int y_dtype, void *scratch, size_t scratch_bytes, int *status_dev, jq_stream_t stream);
